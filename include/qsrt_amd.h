@@ -420,6 +420,82 @@ int qsrt_ldlq_targets(float *tiles, const double *W, const double *L, const floa
 int qsrt_ldlq_commit(float *Q, int16_t *encoded, const float *recon, const uint16_t *states, const int32_t *slot,
                      int B, int64_t K, int64_t N, int64_t sQ, int64_t sE, int64_t blk, void *stream);
 
+/*
+ * A packed matrix, or one for each of several keys (a layer's experts), as
+ * the products below read it: W = diag(suh) H_L X H_R diag(svh) of shape
+ * [rows, cols], labels X from the payload's record-major words.  Record r
+ * covers 128 channels of the rate axis (0: rows, 1: columns), tiles in
+ * row-major order of its strip; records[r] = first word of the record << 3 |
+ * its rate K (2, 3 or 4), records of one rate that follow one another
+ * without a gap.  Key e reads words + e key_stride, records + e
+ * record_stride and its scales likewise (FP16, as stored; stride 0: one for
+ * all keys).  words 4-byte aligned, scales 8-byte aligned, strides in
+ * elements, rows and cols multiples of 128.
+ */
+typedef struct qsrt_packed_matrix {
+    const int16_t *words;
+    int64_t key_stride;
+    const int64_t *records;
+    int64_t record_stride;
+    const void *suh;
+    int64_t suh_stride;
+    const void *svh;
+    int64_t svh_stride;
+    int64_t rows;
+    int64_t cols;
+    int rate_axis;
+    int rates; /* bit K is set where a record has rate K */
+} qsrt_packed_matrix;
+
+/*
+ * Router of a mixture-of-experts layer: logits x w^T ([tokens, hidden] by
+ * [experts, hidden], both bf16 (dtype 0) or both f16 (1), FP32 sums), scores
+ * by softmax over the experts (scoring 0) or sigmoid (1), the k experts of
+ * each token with the largest key -- score + bias with a bias (f32
+ * [experts]), else the logit; ties to the lowest index, NaN as -inf -- in
+ * falling order of key, and their scores (without bias) as weights, divided
+ * by their sum where `normalize`, times `scale`.  weights f32 and ids int32
+ * [tokens, k].  hidden and both leading dimensions multiples of 8, rows
+ * 16-byte aligned; experts <= 1024, k <= min(64, experts).
+ */
+size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t experts);
+int qsrt_route(const void *x, int64_t x_ld, const void *weight, int64_t weight_ld, int dtype, int64_t tokens,
+               int64_t hidden, int64_t experts, int k, const float *bias, int scoring, int normalize, float scale,
+               float *weights, int32_t *ids, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * Experts of a layer for a few tokens, straight from their payloads:
+ *   out[t] = sum_j weights[t, j] act(x_t W1_e, x_t W3_e) W2_e,  e = ids[t, j]
+ * with act(g, u) = silu(g) u (activation 0) or 4 tanh(g/4) sigmoid(g) 25
+ * tanh(u/25) (1).  w1, w3 [hidden, inter] and w2 [inter, hidden] per expert;
+ * luts[K - 2] is the device label table of rate K (16-byte aligned, only
+ * rates that occur are read; `luts` itself is host memory).  An id outside
+ * [0, experts) contributes nothing.  x and out bf16 (dtype 0) or f16 (1),
+ * rows 8-byte aligned; sums are FP32 and rounded once.  Needs
+ * qsrt_packed_moe_workspace_bytes bytes of workspace.
+ */
+size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3,
+                                       const qsrt_packed_matrix *w2, int64_t experts, int64_t tokens, int k);
+int qsrt_packed_moe(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, const qsrt_packed_matrix *w2,
+                    const uint8_t *const *luts, int64_t experts, int activation, const void *x, int64_t x_ld, int dtype,
+                    int64_t tokens, int k, const int32_t *ids, const float *weights, void *out, int64_t out_ld, void *ws,
+                    size_t ws_bytes, void *stream);
+
+/*
+ * A packed projection with low-rank adapters, each row its own or none:
+ *   out[t] = x_t W + scale[a] (x_t A_a^T) B_a^T,  a = ids[t]
+ * A [adapters, rank, rows of W] and B [adapters, cols of W, rank] in x's
+ * type, rank a multiple of 16 up to 128 (zero-padded), 16-byte aligned; an
+ * id outside [0, adapters) has no adapter.  adapters = 0 leaves them out (a,
+ * b, scale and ids may be NULL).  x rows 16-byte aligned, out rows 8-byte
+ * aligned.  Needs qsrt_adapter_linear_workspace_bytes bytes of workspace.
+ */
+size_t qsrt_adapter_linear_workspace_bytes(const qsrt_packed_matrix *w, int64_t rows, int64_t adapters, int64_t rank);
+int qsrt_adapter_linear(const qsrt_packed_matrix *w, const uint8_t *const *luts, const void *a, const void *b,
+                        const float *scale, int64_t adapters, int64_t rank, const void *x, int64_t x_ld, int dtype,
+                        int64_t rows, const int32_t *ids, void *out, int64_t out_ld, void *ws, size_t ws_bytes,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -111,7 +111,44 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_void_p, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     ),
+    "qsrt_route_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "qsrt_route": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p, _c_int, _c_int,
+         ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p],
+    ),
+    "qsrt_packed_moe_workspace_bytes": (_c_size, [_c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_int]),
+    "qsrt_packed_moe": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_int,
+         _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
+    ),
+    "qsrt_adapter_linear_workspace_bytes": (_c_size, [_c_void_p, _c_i64, _c_i64, _c_i64]),
+    "qsrt_adapter_linear": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64,
+         _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
+    ),
 }
+
+
+class PackedMatrixStruct(ctypes.Structure):
+    """``qsrt_packed_matrix`` of ``include/qsrt_amd.h``."""
+
+    _fields_ = [
+        ("words", _c_void_p),
+        ("key_stride", _c_i64),
+        ("records", _c_void_p),
+        ("record_stride", _c_i64),
+        ("suh", _c_void_p),
+        ("suh_stride", _c_i64),
+        ("svh", _c_void_p),
+        ("svh_stride", _c_i64),
+        ("rows", _c_i64),
+        ("cols", _c_i64),
+        ("rate_axis", _c_int),
+        ("rates", _c_int),
+    ]
 
 
 class DecodeJob(ctypes.Structure):

@@ -1,0 +1,1037 @@
+// Products of a few rows with packed trellis matrices, and what stands around them in a mixture-of-experts layer.
+#include <algorithm>
+
+#include "packed.h"
+#include "qsrt_amd.h"
+
+using namespace qsrt;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// The product: part sums of xr X, decoded on the way
+// ---------------------------------------------------------------------------
+
+struct ProductArgs {
+    const int16_t* words[2];
+    int64_t key_stride[2];        // words between the matrices of two keys
+    const int64_t* records[2];    // per record: first word << 3 | bits
+    int64_t record_stride[2];     // 0: one table for every key
+    const char* x[2];             // rotated rows
+    int x_div;                    // row of order entry o: o / x_div
+    const GroupHead* head;        // null: chunks are runs of kRows rows of `rows`
+    const Chunk* chunks;
+    const int* order;
+    int which;                    // head->parts[which]
+    int parts;                    // without a head
+    const uint8_t* lut[2];
+    int lut_bits[2];
+    int luts;
+    int pass;                     // this launch's parts follow `pass` times as many
+    float* part;                  // [passes * parts][nmat][rows][cols]
+    int nmat, axis, kb, nb;       // 128-channel blocks of both axes
+    int rows;
+};
+
+typedef const __attribute__((address_space(1))) uint32_t* gu32;
+
+// Eight successive positions of a tile, 8 i8 .. 8 i8 + 7, are the rows 2g + {0, 1, 8, 9} of columns i8 / 4 and i8 / 4 + 8
+// (g = i8 % 4): one window of 16 + 7 K bits of the tile's stream, two dwords.  w0 holds its bits 0..31, w1 its bits 16..47.
+template <int K>
+__device__ __forceinline__ uint32_t state_of(uint32_t w0, uint32_t w1, int j) {
+    return 16 + j * K <= 32 ? (w0 >> (16 - j * K)) & 0xFFFFu : (w1 >> (32 - j * K)) & 0xFFFFu;
+}
+
+// `strips` strips of 32 payload rows by 128 columns at `tiles`, times G groups of 16 rows.  Lane 16 g + m decodes tile
+// column 2 t + m / 8 of every pair t; MFMA 2 t + u has its columns m % 8 + 8 u as rows.
+template <int K, int G>
+__device__ __forceinline__ void multiply_strips(const char* tiles, int64_t tile_row_bytes, int strips,
+                                                const char* const (&x)[G], const uint8_t* lut, int lane,
+                                                f32x4 (&acc)[G][8]) {
+    const int m = lane & 15, g = lane >> 4;
+    int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;
+    if (b0 < 0) b0 += 256 * K;
+    const int d0 = b0 >> 5, d1 = (d0 + 1) % (8 * K);
+    const uint32_t sh = b0 & 31, rsh = 32u - sh;  // sh is never 0 at K = 2, 3, 4
+    const uint32_t o0 = 4 * d0 + (m >> 3) * 32 * K, o1 = 4 * d1 + (m >> 3) * 32 * K;
+    uint32_t lo[8], hi[8];
+    bf16x8 xn[G][2];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char* p = tiles + (2 * s + h) * tile_row_bytes;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                lo[4 * h + t] = *(gu32)(p + o0 + t * 64 * K);
+                hi[4 * h + t] = *(gu32)(p + o1 + t * 64 * K);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                xn[q][p] = *(const __attribute__((address_space(1))) bf16x8*)(x[q] + s * kStripBytes + p * 64);
+    };
+    fetch(0);
+    for (int s = 0; s < strips; ++s) {
+        uint32_t w0[8], w1[8];
+        bf16x8 b[G][2];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            w0[t] = __builtin_amdgcn_alignbit(lo[t], hi[t], rsh);
+            w1[t] = K > 2 ? __builtin_amdgcn_alignbit(w0[t], hi[t] << sh, 16) : 0u;
+        }
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            b[q][0] = xn[q][0];
+            b[q][1] = xn[q][1];
+        }
+        if (s + 1 < strips) fetch(s + 1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            uint32_t label[2][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) label[h][j] = lut[state_of<K>(w0[4 * h + t], w1[4 * h + t], j)];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                u32x4 a;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t two = label[q >> 1][4 * u + 2 * (q & 1)] | (label[q >> 1][4 * u + 2 * (q & 1) + 1] << 8);
+                    a[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
+                }
+                const bf16x8 av = __builtin_bit_cast(bf16x8, a);
+#pragma unroll
+                for (int q = 0; q < G; ++q) {
+                    acc[q][2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[q][0], acc[q][2 * t + u], 0, 0, 0);
+                    acc[q][2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[q][1], acc[q][2 * t + u], 0, 0, 0);
+                }
+            }
+        }
+    }
+}
+
+template <int G, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lut_s[];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int i = w; i < p.luts * 64; i += kWaves)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(p.lut[i >> 6] + 1024 * (i & 63) + 16 * lane),
+            (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
+    __builtin_amdgcn_s_waitcnt(0);  // the builtin's writes to LDS are not ordered by the barrier alone
+    __syncthreads();
+
+    constexpr int kRows = 16 * G;
+    const int n = lane & 15, g = lane >> 4;
+    const int chunks = p.head ? p.head->chunks : (p.rows + kRows - 1) / kRows;
+    const int parts = p.head ? p.head->parts[p.which] : p.parts;
+    const int64_t items = static_cast<int64_t>(chunks) * p.nmat * p.nb * parts;
+    const int64_t row_bytes = static_cast<int64_t>(p.kb) * 4 * kStripBytes;
+    const int64_t cols = 128 * static_cast<int64_t>(p.nb);
+    const int strips = 4 * p.kb;
+
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + w; item < items;
+         item += static_cast<int64_t>(gridDim.x) * kWaves) {
+        int rest = static_cast<int>(item / parts);
+        const int part = static_cast<int>(item - static_cast<int64_t>(rest) * parts);
+        const int cb = rest % p.nb;
+        rest /= p.nb;
+        const int mat = rest % p.nmat;
+        const int ci = rest / p.nmat;
+        Chunk c{0, ci * kRows, 0, 0};
+        if (p.head) {
+            c = p.chunks[ci];
+            c.key = __builtin_amdgcn_readfirstlane(c.key);
+            c.first = __builtin_amdgcn_readfirstlane(c.first);
+            c.count = __builtin_amdgcn_readfirstlane(c.count);
+        } else {
+            c.count = min(kRows, p.rows - c.first);
+        }
+        int row[G];
+        const char* x[G];
+#pragma unroll
+        for (int q = 0; q < G; ++q) {  // lanes past the last row repeat it; their sums are not stored
+            const int at = c.first + min(16 * q + n, c.count - 1);
+            row[q] = p.head ? p.order[at] : at;
+            x[q] = (mat ? p.x[1] : p.x[0]) + (row[q] / p.x_div) * row_bytes + 16 * g;
+        }
+        f32x4 acc[G][8];
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int t = 0; t < 8; ++t) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        const char* words = reinterpret_cast<const char*>((mat ? p.words[1] : p.words[0]) +
+                                                          c.key * (mat ? p.key_stride[1] : p.key_stride[0]));
+        const int64_t* records =
+            (mat ? p.records[1] : p.records[0]) + c.key * (mat ? p.record_stride[1] : p.record_stride[0]);
+        int s = static_cast<int>(static_cast<int64_t>(strips) * part / parts);
+        const int end = static_cast<int>(static_cast<int64_t>(strips) * (part + 1) / parts);
+        while (s < end) {  // runs of one rate
+            const int r = p.axis ? cb : s >> 2;
+            const uint64_t rec = static_cast<uint64_t>(records[r]);
+            const int bits = __builtin_amdgcn_readfirstlane(static_cast<int>(rec & 7));
+            const int64_t first = static_cast<int64_t>(
+                (static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rec >> 32))) << 32 |
+                 __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rec))) >> 3);
+            int stop = end;
+            if (!p.axis) {  // records of one rate that follow one another are one strip of tiles
+                int r1 = r + 1;
+                while (4 * r1 < end && __builtin_amdgcn_readfirstlane(static_cast<int>(records[r1] & 7)) == bits) ++r1;
+                stop = min(end, 4 * r1);
+            }
+            const int64_t tile = 32 * bits;
+            const int64_t tile_row = p.axis ? 8 * tile : 8 * p.nb * tile;
+            const char* tiles = words + 2 * first + (p.axis ? 2 * s * tile_row : 2 * (s - 4 * r) * tile_row + 8 * cb * tile);
+            const int slot = bits == p.lut_bits[0] ? 0 : (p.luts > 1 && bits == p.lut_bits[1]) ? 1 : -1;
+            if (slot >= 0) {
+                const uint8_t* lut = lut_s + 65536 * slot;
+                const char* xs[G];
+#pragma unroll
+                for (int q = 0; q < G; ++q) xs[q] = x[q] + s * kStripBytes;
+                if (bits == 2)
+                    multiply_strips<2, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
+                else if (bits == 3)
+                    multiply_strips<3, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
+                else
+                    multiply_strips<4, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
+            }
+            s = stop;
+        }
+        // MFMA rows 4 g .. 4 g + 3: columns 16 (2 t + g / 2) + 8 u + 4 (g % 2) + 0..3 of row n
+        float* out = p.part + (static_cast<int64_t>(p.pass * parts + part) * p.nmat + mat) * p.rows * cols + 128 * cb +
+                     16 * (g >> 1) + 4 * (g & 1);
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            if (16 * q + n >= c.count) continue;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                *reinterpret_cast<f32x4*>(out + row[q] * cols + 32 * (t >> 1) + 8 * (t & 1)) = acc[q][t];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows into the payload's basis
+// ---------------------------------------------------------------------------
+
+struct RotateArgs {
+    const void* x;  // [rows][ld]
+    int64_t ld;
+    const _Float16* suh[2];
+    int64_t suh_stride[2];
+    const int* ids;  // null: one scale vector for all; else row r of the result is row r / x_div of x at scale ids[r]
+    int x_div;
+    char* out[2];
+    int rows, kb, nmat;
+};
+
+// One wave for 16 rows of 128 channels of one matrix.
+template <typename T>
+__global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int kb = static_cast<int>(wave % p.kb);
+    const int64_t rest = wave / p.kb;
+    const int mat = static_cast<int>(rest % p.nmat);
+    const int64_t r0 = rest / p.nmat * 16;
+    if (r0 >= p.rows) return;
+    const int row = static_cast<int>(min(r0 + n, static_cast<int64_t>(p.rows) - 1));
+    const int id = p.ids ? p.ids[row] : 0;
+    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + max(id, 0) * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
+    const T* x = static_cast<const T*>(p.x) + (row / p.x_div) * p.ld + 128 * kb;
+    float v[32];
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+        const t4 xv = *reinterpret_cast<const t4*>(x + 16 * a + 4 * g);
+        const f16x4 sv = *reinterpret_cast<const f16x4*>(suh + 16 * a + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * a + i] = static_cast<float>(xv[i]) * static_cast<float>(sv[i]);
+    }
+    hadamard128(v, lane);
+    if (r0 + n >= p.rows) return;
+    char* block = (mat ? p.out[1] : p.out[0]) + (static_cast<int64_t>(row) * p.kb + kb) * 4 * kStripBytes;
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+        store_pieces(block, a, g, v[4 * a] * kHadamardScale, v[4 * a + 1] * kHadamardScale, v[4 * a + 2] * kHadamardScale,
+                     v[4 * a + 3] * kHadamardScale);
+}
+
+// ---------------------------------------------------------------------------
+// Between the two products of an expert
+// ---------------------------------------------------------------------------
+
+struct MiddleArgs {
+    const float* part;  // [passes * parts][2][pairs][inter]
+    const GroupHead* head;
+    const int* ids;
+    const _Float16* svh[2];
+    int64_t svh_stride[2];
+    const _Float16* suh;  // of the second product
+    int64_t suh_stride;
+    char* out;
+    int pairs, ib, passes, act;
+};
+
+__device__ __forceinline__ float activate(float g, float u, int act) {
+    const float s = 1.0f / (1.0f + expf(-g));
+    return act == 0 ? g * s * u : 4.0f * tanhf(0.25f * g) * s * (25.0f * tanhf(0.04f * u));
+}
+
+// One wave for 128 middle channels of one (token, expert) pair.  Lane n < 8 sums the gate's parts n, n + 8, ..., lane
+// n >= 8 the up's.
+__global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int ib = static_cast<int>(wave % p.ib);
+    const int pair = static_cast<int>(wave / p.ib);
+    if (pair >= p.pairs) return;
+    const int id = __builtin_amdgcn_readfirstlane(p.ids[pair]);
+    if (id < 0) return;
+    const int64_t inter = 128 * static_cast<int64_t>(p.ib);
+    const int parts = p.passes * p.head->parts[0];
+    const int mat = n >> 3;
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    for (int s = n & 7; s < parts; s += 8) {
+        const float* src = p.part + ((static_cast<int64_t>(s) * 2 + mat) * p.pairs + pair) * inter + 128 * ib + 4 * g;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * a + i] += x[i];
+        }
+    }
+#pragma unroll
+    for (int h = 1; h < 8; h <<= 1)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += __shfl_xor(v[j], h);
+    hadamard128(v, lane);
+    const _Float16* svh = (mat ? p.svh[1] + id * p.svh_stride[1] : p.svh[0] + id * p.svh_stride[0]) + 128 * ib + 4 * g;
+    const _Float16* suh = p.suh + id * p.suh_stride + 128 * ib + 4 * g;
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+        const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 16 * a);
+        const f16x4 su = *reinterpret_cast<const f16x4*>(suh + 16 * a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float mine = v[4 * a + i] * kHadamardScale * static_cast<float>(sv[i]);
+            const float other = __shfl_xor(mine, 8);
+            v[4 * a + i] = activate(mat ? other : mine, mat ? mine : other, p.act) * static_cast<float>(su[i]);
+        }
+    }
+    hadamard128(v, lane);
+    if (n) return;
+    char* block = p.out + (static_cast<int64_t>(pair) * p.ib + ib) * 4 * kStripBytes;
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+        store_pieces(block, a, g, v[4 * a] * kHadamardScale, v[4 * a + 1] * kHadamardScale, v[4 * a + 2] * kHadamardScale,
+                     v[4 * a + 3] * kHadamardScale);
+}
+
+// ---------------------------------------------------------------------------
+// The layer's sum over a token's experts
+// ---------------------------------------------------------------------------
+
+struct CombineArgs {
+    const float* part;  // [passes * parts][pairs][hidden]
+    const GroupHead* head;
+    const int* ids;
+    const float* weights;
+    const _Float16* svh;
+    int64_t svh_stride;
+    void* out;
+    int64_t ld;
+    int tokens, k, hb, passes;
+};
+
+// One wave for 128 channels of one token.  With one svh for all experts the weighted part sums are rotated once; with one
+// for each, an expert at a time.  Lanes n split the parts of an expert.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const CombineArgs p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int hb = static_cast<int>(wave % p.hb);
+    const int64_t token = wave / p.hb;
+    if (token >= p.tokens) return;
+    const int64_t hidden = 128 * static_cast<int64_t>(p.hb);
+    const int64_t pairs = static_cast<int64_t>(p.tokens) * p.k;
+    const int parts = p.passes * p.head->parts[1];
+    float y[32], v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = 0.f;
+    auto add_pair = [&](int64_t pair, float wt, float(&to)[32], int first, int step) {
+        for (int s = first; s < parts; s += step) {
+            const float* src = p.part + (s * pairs + pair) * hidden + 128 * hb + 4 * g;
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[4 * a + i] += wt * x[i];
+            }
+        }
+    };
+    auto over_lanes = [&](float(&to)[32]) {
+#pragma unroll
+        for (int h = 1; h < 16; h <<= 1)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) to[j] += __shfl_xor(to[j], h);
+    };
+    auto scaled = [&](float(&to)[32], const _Float16* svh) {
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+            const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 128 * hb + 4 * g + 16 * a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[4 * a + i] *= kHadamardScale * static_cast<float>(sv[i]);
+        }
+    };
+    if (p.svh_stride == 0) {
+        // (pair, part) couples over the 16 lanes
+        const int total = p.k * parts;
+        for (int c = n; c < total; c += 16) {
+            const int64_t pair = token * p.k + c / parts;
+            if (p.ids[pair] < 0) continue;
+            add_pair(pair, p.weights[pair], y, c % parts, parts);
+        }
+        over_lanes(y);
+        hadamard128(y, lane);
+        scaled(y, p.svh);
+    } else {
+        for (int j = 0; j < p.k; ++j) {
+            const int64_t pair = token * p.k + j;
+            const int id = __builtin_amdgcn_readfirstlane(p.ids[pair]);
+            if (id < 0) continue;
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = 0.f;
+            add_pair(pair, 1.0f, v, n, 16);
+            over_lanes(v);
+            hadamard128(v, lane);
+            scaled(v, p.svh + id * p.svh_stride);
+            const float wt = p.weights[pair];
+#pragma unroll
+            for (int q = 0; q < 32; ++q) y[q] += wt * v[q];
+        }
+    }
+    if (n) return;
+    T* out = static_cast<T*>(p.out) + token * p.ld + 128 * hb + 4 * g;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+        *reinterpret_cast<t4*>(out + 16 * a) = t4{static_cast<T>(y[4 * a]), static_cast<T>(y[4 * a + 1]),
+                                                  static_cast<T>(y[4 * a + 2]), static_cast<T>(y[4 * a + 3])};
+}
+
+// ---------------------------------------------------------------------------
+// Low-rank adapters
+// ---------------------------------------------------------------------------
+
+constexpr int kMaxRank = 128;
+
+struct ShrinkArgs {
+    const void* x;
+    int64_t ld;
+    const void* a;  // [adapters][rank][k]
+    const GroupHead* head;
+    const Chunk* chunks;
+    const int* order;
+    float* out;  // [parts][rows][rank]
+    int rows, k, rank, parts;
+};
+
+// x A_a^T of 16 rows of one adapter over a part of the K axis; a wave each.  Products of the inputs are exact, sums FP32.
+template <typename T>
+__global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int64_t nw = static_cast<int64_t>(gridDim.x) * 4;
+    const int64_t items = static_cast<int64_t>(p.head->chunks) * p.parts;
+    const int steps = p.k / 32, tiles = p.rank / 16;
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+         item < items; item += nw) {
+        const int ci = static_cast<int>(item / p.parts), part = static_cast<int>(item % p.parts);
+        const Chunk c = p.chunks[ci];
+        const int key = __builtin_amdgcn_readfirstlane(c.key);
+        if (key < 0) continue;
+        const int row = p.order[c.first + min(n, c.count - 1)];
+        const T* x = static_cast<const T*>(p.x) + row * p.ld + 8 * g;
+        const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + n) * p.k + 8 * g;
+        f32x4 acc[kMaxRank / 16];
+#pragma unroll
+        for (int t = 0; t < kMaxRank / 16; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.parts);
+        for (int s = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts); s < s1; ++s) {
+            const t8 xv = *reinterpret_cast<const t8*>(x + 32 * s);
+#pragma unroll
+            for (int t = 0; t < kMaxRank / 16; ++t) {
+                if (t >= tiles) break;
+                const t8 av = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * s);
+                if constexpr (__is_same(T, __bf16))
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, xv, acc[t], 0, 0, 0);
+                else
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, xv, acc[t], 0, 0, 0);
+            }
+        }
+        if (n >= c.count) continue;
+        float* out = p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank + 4 * g;
+#pragma unroll
+        for (int t = 0; t < kMaxRank / 16; ++t) {
+            if (t >= tiles) break;
+            *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
+        }
+    }
+}
+
+struct FinishArgs {
+    const float* part;  // [parts][rows][cols]
+    int parts;
+    const GroupHead* head;  // null: no adapters, chunks are runs of 16 rows
+    const Chunk* chunks;
+    const int* order;
+    const _Float16* svh;
+    const float* low;  // [low_parts][rows][rank]
+    int low_parts;
+    const void* b;  // [adapters][cols][rank]
+    const float* scale;
+    int rank;
+    void* out;
+    int64_t ld;
+    int rows, nb;
+};
+
+// Sum of the parts, back into the output's basis, plus the adapter's second product; a wave for 16 rows by 128 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nb = static_cast<int>(wave % p.nb);
+    const int ci = static_cast<int>(wave / p.nb);
+    if (ci >= (p.head ? p.head->chunks : (p.rows + 15) / 16)) return;
+    Chunk c{-1, 16 * ci, 0, 0};
+    if (p.head)
+        c = p.chunks[ci];
+    else
+        c.count = min(16, p.rows - c.first);
+    const int64_t cols = 128 * static_cast<int64_t>(p.nb);
+    // the lanes beyond the chunk's rows (in powers of two) share the parts
+    int width = 1;
+    while (width < c.count) width <<= 1;
+    const int mine = n & (width - 1), sub = n / width, subs = 16 / width;
+    const int at = c.first + min(mine, c.count - 1);
+    const int row = p.head ? p.order[at] : at;
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    for (int s = sub; s < p.parts; s += subs) {
+        const float* src = p.part + (static_cast<int64_t>(s) * p.rows + row) * cols + 128 * nb + 4 * g;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * a + i] += x[i];
+        }
+    }
+    for (int h = width; h < 16; h <<= 1)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += __shfl_xor(v[j], h);
+    hadamard128(v, lane);
+    const _Float16* svh = p.svh + 128 * nb + 4 * g;
+    f32x4 acc[8];
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+        const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 16 * a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[a][i] = v[4 * a + i] * kHadamardScale * static_cast<float>(sv[i]);
+    }
+    const int key = __builtin_amdgcn_readfirstlane(c.key);
+    if (key >= 0) {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        const float scale = p.scale[key];
+        const T* b = static_cast<const T*>(p.b) + (static_cast<int64_t>(key) * cols + 128 * nb + n) * p.rank + 8 * g;
+        const float* low = p.low + static_cast<int64_t>(row) * p.rank + 8 * g;
+        for (int r = 0; r < p.rank; r += 32) {
+            const bool in = r + 8 * g < p.rank;  // the rank is a multiple of 16
+            float xv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xv[j] = 0.f;
+            if (in) {
+                for (int s = 0; s < p.low_parts; ++s) {
+                    const float* src = low + static_cast<int64_t>(s) * p.rows * p.rank + r;
+                    const f32x4 x0 = *reinterpret_cast<const f32x4*>(src), x1 = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        xv[j] += x0[j];
+                        xv[4 + j] += x1[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xv[j] *= scale;
+            const t8 zero = {};
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+                const t8 bv = in ? *reinterpret_cast<const t8*>(b + static_cast<int64_t>(16 * a) * p.rank + r) : zero;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(static_cast<float>(bv[j]), xv[j], acc[a], 0, 0, 0);
+            }
+        }
+    }
+    if (n >= c.count) return;
+    T* out = static_cast<T*>(p.out) + row * p.ld + 128 * nb + 4 * g;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+        *reinterpret_cast<t4*>(out + 16 * a) = t4{static_cast<T>(acc[a][0]), static_cast<T>(acc[a][1]),
+                                                  static_cast<T>(acc[a][2]), static_cast<T>(acc[a][3])};
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one product, unless one part alone takes more
+
+template <int G>
+struct Shape {
+    static constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
+};
+
+template <int G>
+int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
+    constexpr int kWaves = Shape<G>::kWaves;
+    const size_t lds = static_cast<size_t>(65536) * args.luts;
+    if (args.luts > 1)
+        QSRT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<G, kWaves>),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, 131072));
+    hipLaunchKernelGGL((product_kernel<G, kWaves>), dim3(cus), dim3(64 * kWaves), lds, stream, args);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
+int waves_of(int groups, int cus) { return cus * (groups == 1 ? 16 : 8); }
+
+// All passes of a product: the tables of at most two rates fit LDS at once.
+int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
+    int set[3], n = 0;
+    for (int b = 2; b <= 4; ++b)
+        if (rates >> b & 1) set[n++] = b;
+    for (int first = 0, pass = 0; first < n; first += 2, ++pass) {
+        args.pass = pass;
+        args.luts = std::min(2, n - first);
+        for (int j = 0; j < args.luts; ++j) {
+            args.lut_bits[j] = set[first + j];
+            args.lut[j] = luts[set[first + j] - 2];
+        }
+        const int rc = groups == 1   ? launch_product_g<1>(args, cus, stream)
+                       : groups == 2 ? launch_product_g<2>(args, cus, stream)
+                                     : launch_product_g<4>(args, cus, stream);
+        if (rc != kOk) return rc;
+    }
+    return kOk;
+}
+
+int passes_of(int rates) { return __builtin_popcount(rates & 0x1C) > 2 ? 2 : 1; }
+
+const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts) {
+    if (!m || !m->words || !m->records || !m->suh || !m->svh) return "null pointer in a matrix";
+    if (m->rows <= 0 || m->cols <= 0 || m->rows % 128 || m->cols % 128) return "rows and cols must be multiples of 128";
+    if (m->rows > (1 << 22) || m->cols > (1 << 22)) return "matrix too large";
+    if (m->rate_axis != 0 && m->rate_axis != 1) return "rate_axis must be 0 (rows) or 1 (columns)";
+    if ((m->rates & 0x1C) == 0 || (m->rates & ~0x1C)) return "rates must name K2, K3 or K4";
+    if (m->key_stride < 0 || m->record_stride < 0 || m->suh_stride < 0 || m->svh_stride < 0) return "negative stride";
+    if (reinterpret_cast<uintptr_t>(m->words) % 4 || m->key_stride % 2) return "words must be 4-byte aligned";
+    if (reinterpret_cast<uintptr_t>(m->suh) % 8 || reinterpret_cast<uintptr_t>(m->svh) % 8 || m->suh_stride % 4 ||
+        m->svh_stride % 4)
+        return "scales must be 8-byte aligned";
+    for (int b = 2; b <= 4; ++b)
+        if ((m->rates >> b & 1) && (!luts || !luts[b - 2] || reinterpret_cast<uintptr_t>(luts[b - 2]) % 16))
+            return "a rate's label table is missing or not 16-byte aligned";
+    return nullptr;
+}
+
+const char* rows_fault(const void* p, int64_t ld, int64_t cols, int align) {
+    if (!p) return "null rows";
+    if (ld < cols || ld % (align / 2) || reinterpret_cast<uintptr_t>(p) % align) return "rows are not aligned";
+    return nullptr;
+}
+
+struct Carve {
+    char* base;
+    size_t used = 0;
+    template <typename T>
+    T* take(int64_t n) {
+        T* p = reinterpret_cast<T*>(base + used);
+        used += (static_cast<size_t>(n) * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+int part_limit(int64_t row_floats, int strips) {
+    const int64_t fit = kMaxPartBytes / (row_floats * 4);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(fit, strips), 64)));
+}
+
+struct MoeSpace {
+    GroupHead* head;
+    Chunk* chunks;
+    int *order, *clean;
+    char *x[2], *mid;
+    float* part;
+    int max_parts[2], passes[2], groups;
+    size_t bytes;
+};
+
+MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inter, int64_t experts, int rates13, int rates2,
+                   bool shared) {
+    MoeSpace s;
+    const int64_t pairs = tokens * k;
+    s.groups = pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;  // groups of 16 rows a wave multiplies at once
+    Carve c{static_cast<char*>(ws)};
+    s.head = c.take<GroupHead>(1);
+    s.chunks = c.take<Chunk>(pairs);
+    s.order = c.take<int>(pairs);
+    s.clean = c.take<int>(pairs);
+    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>((shared ? tokens : pairs) * hidden * 4);
+    s.mid = c.take<char>(pairs * inter * 4);
+    s.passes[0] = passes_of(rates13);
+    s.passes[1] = passes_of(rates2);
+    s.max_parts[0] = part_limit(2 * pairs * inter * s.passes[0], static_cast<int>(hidden / 32));
+    s.max_parts[1] = part_limit(pairs * hidden * s.passes[1], static_cast<int>(inter / 32));
+    s.part = c.take<float>(std::max(s.max_parts[0] * s.passes[0] * 2 * pairs * inter,
+                                    s.max_parts[1] * s.passes[1] * pairs * hidden));
+    s.bytes = c.used;
+    return s;
+}
+
+void set_matrix(ProductArgs& a, int i, const qsrt_packed_matrix* m) {
+    a.words[i] = m->words;
+    a.key_stride[i] = m->key_stride;
+    a.records[i] = m->records;
+    a.record_stride[i] = m->record_stride;
+    a.axis = m->rate_axis;
+    a.kb = static_cast<int>(m->rows / 128);
+    a.nb = static_cast<int>(m->cols / 128);
+}
+
+unsigned blocks_of(int64_t waves) { return static_cast<unsigned>((waves + 3) / 4); }
+
+const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                      const uint8_t* const* luts, int64_t experts, int64_t tokens, int k) {
+    for (const qsrt_packed_matrix* m : {w1, w3, w2})
+        if (const char* e = matrix_fault(m, luts)) return e;
+    if (w1->rows != w3->rows || w1->cols != w3->cols || w2->rows != w1->cols || w2->cols != w1->rows ||
+        w1->rate_axis != w3->rate_axis)
+        return "w1, w3 [hidden, inter] and w2 [inter, hidden] do not match";
+    if ((w1->suh_stride == 0) != (w3->suh_stride == 0)) return "w1 and w3 must both share their suh, or neither";
+    if (experts < 1 || experts > kMaxKeys) return "experts must be 1 .. 8191";
+    if (k < 1 || tokens < 0 || tokens * k > (1 << 20)) return "tokens * k must be at most 2^20";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
+                                                  const qsrt_packed_matrix* w2, int64_t experts, int64_t tokens, int k) {
+    if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0) return 0;
+    return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates,
+                     w1->suh_stride == 0).bytes;
+}
+
+extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                               const uint8_t* const* luts, int64_t experts, int activation, const void* x, int64_t x_ld,
+                               int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
+                               int64_t out_ld, void* ws, size_t ws_bytes, void* stream_) {
+    if (const char* e = moe_fault(w1, w3, w2, luts, experts, tokens, k)) return fail(kBadArgument, "qsrt_packed_moe: %s", e);
+    if (tokens == 0) return kOk;
+    const int64_t hidden = w1->rows, inter = w1->cols, pairs = tokens * k;
+    if (dtype != 0 && dtype != 1) return fail(kBadArgument, "qsrt_packed_moe: dtype must be 0 (bf16) or 1 (f16)");
+    if (activation != 0 && activation != 1) return fail(kBadArgument, "qsrt_packed_moe: unknown activation");
+    if (const char* e = rows_fault(x, x_ld, hidden, 8)) return fail(kBadArgument, "qsrt_packed_moe: x: %s", e);
+    if (const char* e = rows_fault(out, out_ld, hidden, 8)) return fail(kBadArgument, "qsrt_packed_moe: out: %s", e);
+    if (!ids || !weights) return fail(kBadArgument, "qsrt_packed_moe: null routing");
+    const bool shared = w1->suh_stride == 0;
+    const int rates13 = w1->rates | w3->rates;
+    const MoeSpace s = moe_space(ws, tokens, k, hidden, inter, experts, rates13, w2->rates, shared);
+    if (!ws || ws_bytes < s.bytes) return fail(kWorkspaceTooSmall, "qsrt_packed_moe: needs %zu workspace bytes", s.bytes);
+    int cus = 0;
+    if (const int rc = current_cu_count(&cus)) return rc;
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+
+    GroupArgs ga{};
+    ga.ids = ids;
+    ga.n = static_cast<int>(pairs);
+    ga.keys = static_cast<int>(experts);
+    ga.none = false;
+    ga.chunk_rows = 16 * s.groups;
+    ga.head = s.head;
+    ga.chunks = s.chunks;
+    ga.order = s.order;
+    ga.clean = s.clean;
+    ga.units[0] = 2 * static_cast<int>(inter / 128);
+    ga.units[1] = static_cast<int>(hidden / 128);
+    ga.strips[0] = static_cast<int>(hidden / 32);
+    ga.strips[1] = static_cast<int>(inter / 32);
+    for (int i = 0; i < 2; ++i) ga.max_parts[i] = s.max_parts[i];
+    ga.waves = waves_of(s.groups, cus);
+    if (const int rc = launch_group(ga, stream)) return rc;
+
+    RotateArgs ra{};
+    ra.x = x;
+    ra.ld = x_ld;
+    ra.suh[0] = reinterpret_cast<const _Float16*>(w1->suh);
+    ra.suh[1] = reinterpret_cast<const _Float16*>(w3->suh);
+    ra.suh_stride[0] = w1->suh_stride;
+    ra.suh_stride[1] = w3->suh_stride;
+    ra.ids = shared ? nullptr : s.clean;
+    ra.x_div = shared ? 1 : k;
+    ra.out[0] = s.x[0];
+    ra.out[1] = s.x[1];
+    ra.rows = static_cast<int>(shared ? tokens : pairs);
+    ra.kb = static_cast<int>(hidden / 128);
+    ra.nmat = 2;
+    const dim3 rgrid(blocks_of((ra.rows + 15) / 16 * static_cast<int64_t>(ra.kb) * 2));
+    if (dtype == 0)
+        hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
+    else
+        hipLaunchKernelGGL(rotate_rows_kernel<_Float16>, rgrid, dim3(256), 0, stream, ra);
+    QSRT_HIP_TRY(hipGetLastError());
+
+    ProductArgs pa{};
+    set_matrix(pa, 0, w1);
+    set_matrix(pa, 1, w3);
+    pa.x[0] = s.x[0];
+    pa.x[1] = s.x[1];
+    pa.x_div = shared ? k : 1;
+    pa.head = s.head;
+    pa.chunks = s.chunks;
+    pa.order = s.order;
+    pa.which = 0;
+    pa.part = s.part;
+    pa.nmat = 2;
+    pa.rows = static_cast<int>(pairs);
+    if (const int rc = launch_product(pa, s.groups, rates13, luts, cus, stream)) return rc;
+
+    MiddleArgs ma{};
+    ma.part = s.part;
+    ma.head = s.head;
+    ma.ids = s.clean;
+    ma.svh[0] = reinterpret_cast<const _Float16*>(w1->svh);
+    ma.svh[1] = reinterpret_cast<const _Float16*>(w3->svh);
+    ma.svh_stride[0] = w1->svh_stride;
+    ma.svh_stride[1] = w3->svh_stride;
+    ma.suh = reinterpret_cast<const _Float16*>(w2->suh);
+    ma.suh_stride = w2->suh_stride;
+    ma.out = s.mid;
+    ma.pairs = static_cast<int>(pairs);
+    ma.ib = static_cast<int>(inter / 128);
+    ma.passes = s.passes[0];
+    ma.act = activation;
+    hipLaunchKernelGGL(middle_kernel, dim3(blocks_of(pairs * ma.ib)), dim3(256), 0, stream, ma);
+    QSRT_HIP_TRY(hipGetLastError());
+
+    ProductArgs pb{};
+    set_matrix(pb, 0, w2);
+    pb.x[0] = s.mid;
+    pb.x_div = 1;
+    pb.head = s.head;
+    pb.chunks = s.chunks;
+    pb.order = s.order;
+    pb.which = 1;
+    pb.part = s.part;
+    pb.nmat = 1;
+    pb.rows = static_cast<int>(pairs);
+    if (const int rc = launch_product(pb, s.groups, w2->rates, luts, cus, stream)) return rc;
+
+    CombineArgs ca{};
+    ca.part = s.part;
+    ca.head = s.head;
+    ca.ids = s.clean;
+    ca.weights = weights;
+    ca.svh = reinterpret_cast<const _Float16*>(w2->svh);
+    ca.svh_stride = w2->svh_stride;
+    ca.out = out;
+    ca.ld = out_ld;
+    ca.tokens = static_cast<int>(tokens);
+    ca.k = k;
+    ca.hb = static_cast<int>(hidden / 128);
+    ca.passes = s.passes[1];
+    const dim3 cgrid(blocks_of(tokens * ca.hb));
+    if (dtype == 0)
+        hipLaunchKernelGGL(combine_kernel<__bf16>, cgrid, dim3(256), 0, stream, ca);
+    else
+        hipLaunchKernelGGL(combine_kernel<_Float16>, cgrid, dim3(256), 0, stream, ca);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
+namespace {
+
+struct LinearSpace {
+    GroupHead* head;
+    Chunk* chunks;
+    int *order, *clean;
+    char* x;
+    float *low, *part;
+    int low_parts, parts, passes, groups;
+    size_t bytes;
+};
+
+LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates, int64_t adapters, int64_t rank, int cus) {
+    LinearSpace s;
+    Carve c{static_cast<char*>(ws)};
+    s.groups = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    s.passes = passes_of(rates);
+    const int64_t chunks = (rows + 16 * s.groups - 1) / (16 * s.groups);
+    const int strips = static_cast<int>(k / 32);
+    const int limit = part_limit(rows * n * s.passes, strips);
+    int64_t best = INT64_MAX;
+    s.parts = 1;
+    for (int p = 1; p <= limit; ++p) {  // as choose_parts
+        const int64_t rounds = (chunks * (n / 128) * p + waves_of(s.groups, cus) - 1) / waves_of(s.groups, cus);
+        const int64_t cost = rounds * ((strips + p - 1) / p + 2);
+        if (cost < best) {
+            best = cost;
+            s.parts = p;
+        }
+    }
+    s.low_parts = 1;
+    if (adapters) {
+        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1);  // chunks of one adapter's rows
+        s.low_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / most, k / 256)));
+        s.head = c.take<GroupHead>(1);
+        s.chunks = c.take<Chunk>(rows);
+        s.order = c.take<int>(rows);
+        s.clean = c.take<int>(rows);
+        s.low = c.take<float>(s.low_parts * rows * rank);
+    } else {
+        s.head = nullptr;
+        s.chunks = nullptr;
+        s.order = s.clean = nullptr;
+        s.low = nullptr;
+    }
+    s.x = c.take<char>(rows * k * 4);
+    s.part = c.take<float>(static_cast<int64_t>(s.parts) * s.passes * rows * n);
+    s.bytes = c.used;
+    return s;
+}
+
+}  // namespace
+
+extern "C" size_t qsrt_adapter_linear_workspace_bytes(const qsrt_packed_matrix* w, int64_t rows, int64_t adapters,
+                                                      int64_t rank) {
+    int cus = 0;
+    if (!w || rows <= 0 || w->rows <= 0 || w->cols <= 0 || current_cu_count(&cus)) return 0;
+    return linear_space(nullptr, rows, w->rows, w->cols, w->rates, adapters, rank, cus).bytes;
+}
+
+extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* const* luts, const void* a, const void* b,
+                                   const float* scale, int64_t adapters, int64_t rank, const void* x, int64_t x_ld,
+                                   int dtype, int64_t rows, const int32_t* ids, void* out, int64_t out_ld, void* ws,
+                                   size_t ws_bytes, void* stream_) {
+    if (const char* e = matrix_fault(w, luts)) return fail(kBadArgument, "qsrt_adapter_linear: %s", e);
+    if (rows < 0 || rows > (1 << 20)) return fail(kBadArgument, "qsrt_adapter_linear: at most 2^20 rows");
+    if (dtype != 0 && dtype != 1) return fail(kBadArgument, "qsrt_adapter_linear: dtype must be 0 (bf16) or 1 (f16)");
+    if (adapters < 0 || adapters > kMaxKeys) return fail(kBadArgument, "qsrt_adapter_linear: at most %d adapters", kMaxKeys);
+    if (adapters && (!a || !b || !scale || !ids || rank < 16 || rank > kMaxRank || rank % 16 ||
+                     reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(b) % 16))
+        return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a, b of a rank 16, 32 .. 128, scales and ids");
+    if (rows == 0) return kOk;
+    const int64_t k = w->rows, n = w->cols;
+    if (const char* e = rows_fault(x, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
+    if (const char* e = rows_fault(out, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
+    int cus = 0;
+    if (const int rc = current_cu_count(&cus)) return rc;
+    const LinearSpace s = linear_space(ws, rows, k, n, w->rates, adapters, rank, cus);
+    if (!ws || ws_bytes < s.bytes) return fail(kWorkspaceTooSmall, "qsrt_adapter_linear: needs %zu workspace bytes", s.bytes);
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+
+    RotateArgs ra{};
+    ra.x = x;
+    ra.ld = x_ld;
+    ra.suh[0] = reinterpret_cast<const _Float16*>(w->suh);
+    ra.x_div = 1;
+    ra.out[0] = s.x;
+    ra.rows = static_cast<int>(rows);
+    ra.kb = static_cast<int>(k / 128);
+    ra.nmat = 1;
+    const dim3 rgrid(blocks_of((rows + 15) / 16 * ra.kb));
+    if (dtype == 0)
+        hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
+    else
+        hipLaunchKernelGGL(rotate_rows_kernel<_Float16>, rgrid, dim3(256), 0, stream, ra);
+    QSRT_HIP_TRY(hipGetLastError());
+
+    if (adapters) {
+        GroupArgs ga{};
+        ga.ids = ids;
+        ga.n = static_cast<int>(rows);
+        ga.keys = static_cast<int>(adapters);
+        ga.none = true;
+        ga.chunk_rows = 16;
+        ga.head = s.head;
+        ga.chunks = s.chunks;
+        ga.order = s.order;
+        ga.clean = s.clean;
+        if (const int rc = launch_group(ga, stream)) return rc;
+        ShrinkArgs sa{};
+        sa.x = x;
+        sa.ld = x_ld;
+        sa.a = a;
+        sa.head = s.head;
+        sa.chunks = s.chunks;
+        sa.order = s.order;
+        sa.out = s.low;
+        sa.rows = static_cast<int>(rows);
+        sa.k = static_cast<int>(k);
+        sa.rank = static_cast<int>(rank);
+        sa.parts = s.low_parts;
+        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1) * s.low_parts;
+        const dim3 sgrid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most), 8 * cus)));
+        if (dtype == 0)
+            hipLaunchKernelGGL(shrink_kernel<__bf16>, sgrid, dim3(256), 0, stream, sa);
+        else
+            hipLaunchKernelGGL(shrink_kernel<_Float16>, sgrid, dim3(256), 0, stream, sa);
+        QSRT_HIP_TRY(hipGetLastError());
+    }
+
+    ProductArgs pa{};
+    set_matrix(pa, 0, w);
+    pa.x[0] = s.x;
+    pa.x_div = 1;
+    pa.parts = s.parts;
+    pa.part = s.part;
+    pa.nmat = 1;
+    pa.rows = static_cast<int>(rows);
+    if (const int rc = launch_product(pa, s.groups, w->rates, luts, cus, stream)) return rc;
+
+    FinishArgs fa{};
+    fa.part = s.part;
+    fa.parts = s.parts * s.passes;
+    fa.head = s.head;
+    fa.chunks = s.chunks;
+    fa.order = s.order;
+    fa.svh = reinterpret_cast<const _Float16*>(w->svh);
+    fa.low = s.low;
+    fa.low_parts = s.low_parts;
+    fa.b = b;
+    fa.scale = scale;
+    fa.rank = static_cast<int>(rank);
+    fa.out = out;
+    fa.ld = out_ld;
+    fa.rows = static_cast<int>(rows);
+    fa.nb = static_cast<int>(n / 128);
+    const int64_t most = adapters ? std::min(rows, (rows + 15) / 16 + adapters + 1) : (rows + 15) / 16;
+    const dim3 fgrid(blocks_of(most * fa.nb));
+    if (dtype == 0)
+        hipLaunchKernelGGL(finish_kernel<__bf16>, fgrid, dim3(256), 0, stream, fa);
+    else
+        hipLaunchKernelGGL(finish_kernel<_Float16>, fgrid, dim3(256), 0, stream, fa);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}

@@ -1,0 +1,160 @@
+"""A mixture-of-experts layer for a few tokens, straight from its packed payloads.
+
+``route_tokens`` chooses each token's experts, ``PackedExperts`` multiplies by them and ``PackedMoELayer`` is both
+(``qsrt_route`` and ``qsrt_packed_moe`` in ``include/qsrt_amd.h``).  Nothing waits for the device: which experts are
+chosen is known there alone.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows
+
+SCORING = {"softmax": 0, "sigmoid": 1}
+ACTIVATIONS = {"swiglu": 0, "situ": 1}
+MAX_EXPERTS = 1024
+MAX_CHOSEN = 64
+
+
+def _checked_router(weight: torch.Tensor, k: int, bias, scoring: str) -> tuple:
+    if weight.dim() != 2 or not weight.is_cuda or weight.dtype not in TYPES:
+        raise ValueError("the router's weight must be bfloat16 or float16 [experts, hidden] on a CUDA device")
+    e, h = weight.shape
+    if not 1 <= e <= MAX_EXPERTS or h == 0 or h % 8:
+        raise ValueError(f"the router takes 1 .. {MAX_EXPERTS} experts and a multiple of 8 channels")
+    if isinstance(k, bool) or not isinstance(k, int) or not 1 <= k <= min(MAX_CHOSEN, e):
+        raise ValueError(f"k must be 1 .. {min(MAX_CHOSEN, e)}")
+    if scoring not in SCORING:
+        raise ValueError(f"scoring must be one of {tuple(SCORING)}")
+    if bias is not None and (bias.shape != (e,) or bias.dtype != torch.float32 or bias.device != weight.device):
+        raise ValueError("bias must be float32 [experts] on the router's device")
+    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < h or weight.data_ptr() % 16:
+        weight = weight.contiguous().clone()
+    return weight, None if bias is None else bias.contiguous()
+
+
+def _route(x, weight, k, bias, scoring, normalize, scale):
+    e, h = weight.shape
+    if x.dtype != weight.dtype:
+        raise ValueError("x must be of the router's type")
+    x = checked_rows(x, h, weight.device)
+    t = x.shape[0]
+    weights = torch.empty((t, k), dtype=torch.float32, device=x.device)
+    ids = torch.empty((t, k), dtype=torch.int32, device=x.device)
+    if t == 0:
+        return weights, ids
+    ws = torch.empty((t, e), dtype=torch.float32, device=x.device)
+    _native.check(
+        _native.lib().qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
+                                 k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize),
+                                 float(scale), weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), 4 * ws.numel(),
+                                 _native.stream_handle(x.device)),
+        "qsrt_route",
+    )
+    return weights, ids
+
+
+def route_tokens(x: torch.Tensor, weight: torch.Tensor, k: int, *, bias: torch.Tensor | None = None,
+                 scoring: str = "softmax", normalize: bool = True, scale: float = 1.0):
+    """The ``k`` experts of each row of ``x [T, hidden]``: ``(weights float32 [T, k], ids int32 [T, k])``.
+
+    Scores are the softmax or the sigmoid of ``x weight^T`` (``weight [experts, hidden]``, of ``x``'s type).  The largest
+    ``score + bias`` (without a bias: the largest logits) are chosen, ties to the lowest index, NaN last, and returned in
+    falling order; their weights are the scores without the bias, divided by their sum where ``normalize``, times
+    ``scale``."""
+
+    weight, bias = _checked_router(weight, k, bias, scoring)
+    return _route(x, weight, k, bias, scoring, normalize, scale)
+
+
+class PackedExperts:
+    """The experts of one layer: ``w1`` and ``w3 [hidden, inter]`` (gate and up) and ``w2 [inter, hidden]`` (down), each a
+    dict of the stacked payloads of all experts: ``trellis`` int16 ``[experts, words]``, ``suh``/``svh`` float16 (one
+    vector for the layer or ``[experts, ...]``), ``record_bits`` (one rate, one schedule, or one for each expert) and
+    ``rate_axis`` (default: columns for w1 and w3, rows for w2, as stored)."""
+
+    def __init__(self, w1: dict, w3: dict, w2: dict, luts_by_bits: dict, *, activation: str = "swiglu"):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+        self.experts = int(w1["trellis"].shape[0])
+        self.w1, self.w3, self.w2 = (
+            PackedMatrix(w["trellis"], w["suh"], w["svh"], w["record_bits"], rate_axis=w.get("rate_axis", axis),
+                         keys=self.experts)
+            for w, axis in ((w1, "n"), (w3, "n"), (w2, "k")))
+        self.hidden, self.inter, self.device = self.w1.k, self.w1.n, self.w1.device
+        if ((self.w3.k, self.w3.n) != (self.hidden, self.inter) or (self.w2.k, self.w2.n) != (self.inter, self.hidden)
+                or self.w3.device != self.device or self.w2.device != self.device):
+            raise ValueError("w1, w3 [hidden, inter] and w2 [inter, hidden] do not match")
+        if (self.w1.suh.dim() == 1) != (self.w3.suh.dim() == 1):
+            raise ValueError("w1 and w3 must both share their suh, or neither")
+        self.luts = LabelTables(luts_by_bits, self.w1.rates | self.w3.rates | self.w2.rates, self.device)
+        self.activation = ACTIVATIONS[activation]
+
+    @classmethod
+    def from_experts(cls, experts: list, record_bits, luts_by_bits: dict, *, activation: str = "swiglu",
+                     device="cuda:0") -> "PackedExperts":
+        """From a list of ``{"w1", "w3", "w2"}`` dicts as a layer file's reader returns them (``read_expert``)."""
+
+        def stack(name):
+            def scale(part):
+                all_ = torch.stack([e[name][part].reshape(-1) for e in experts])
+                return (all_[0] if bool((all_ == all_[0]).all()) else all_).to(device)
+
+            return {"trellis": torch.stack([e[name]["trellis"].reshape(-1) for e in experts]).to(device),
+                    "suh": scale("suh"), "svh": scale("svh"), "record_bits": record_bits}
+
+        if not experts:
+            raise ValueError("a layer needs at least one expert")
+        w1, w3, w2 = (stack(name) for name in ("w1", "w3", "w2"))
+        if w1["suh"].dim() != w3["suh"].dim():  # both shared or neither
+            for w in (w1, w3):
+                w["suh"] = w["suh"].expand(len(experts), -1).contiguous()
+        return cls(w1, w3, w2, luts_by_bits, activation=activation)
+
+    def __call__(self, x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, *,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """``out[t] = sum_j weights[t, j] act(x_t W1_e, x_t W3_e) W2_e`` with ``e = ids[t, j]``; an id outside
+        ``[0, experts)`` (-1) contributes nothing.  ``x [T, hidden]`` bf16 or f16, ``weights`` float32 and ``ids`` int32
+        ``[T, k]``."""
+
+        x = checked_rows(x, self.hidden, self.device)
+        out = checked_out(out, x, self.hidden)
+        if (ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape[1] < 1 or weights.shape != ids.shape
+                or ids.dtype != torch.int32 or weights.dtype != torch.float32 or ids.device != self.device
+                or weights.device != self.device):
+            raise ValueError("weights float32 and ids int32 must be [T, k] on the payload's device")
+        t, k = ids.shape
+        if t == 0:
+            return out
+        ids, weights = ids.contiguous(), weights.contiguous()
+        lib = _native.lib()
+        ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(self.w1.ref, self.w3.ref, self.w2.ref, self.experts, t, k),
+                         dtype=torch.uint8, device=self.device)
+        _native.check(
+            lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
+                                x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
+                                out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                                _native.stream_handle(self.device)),
+            "qsrt_packed_moe",
+        )
+        return out
+
+
+class PackedMoELayer:
+    """Router and packed experts of one layer; calling it on ``x [T, hidden]`` returns ``(y, weights, ids)``."""
+
+    def __init__(self, router: torch.Tensor, experts: PackedExperts, k: int, *, bias: torch.Tensor | None = None,
+                 scoring: str = "softmax", normalize: bool = True, scale: float = 1.0):
+        self.router, self.bias = _checked_router(router, k, bias, scoring)
+        if self.router.shape != (experts.experts, experts.hidden) or self.router.device != experts.device:
+            raise ValueError("the router's weight must be [experts, hidden] on the experts' device")
+        self.experts, self.k, self.scoring, self.normalize, self.scale = experts, k, scoring, normalize, scale
+
+    def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None):
+        weights, ids = _route(x, self.router, self.k, self.bias, self.scoring, self.normalize, self.scale)
+        return self.experts(x, weights, ids, out=out), weights, ids
+
+
+__all__ = ["PackedExperts", "PackedMoELayer", "route_tokens"]
