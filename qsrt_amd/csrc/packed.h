@@ -13,62 +13,63 @@ namespace qsrt {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // Rotated rows in memory: a row of K channels is K / 32 strips of 128 bytes, one for 32 payload rows: the strip's 32 hi
 // pieces, then its 32 lo pieces, both in the order in which a lane of the product takes them: for lane group g = 0..3 the
 // eight channels 16 h + {2g, 2g + 1, 2g + 8, 2g + 9}, h = 0, 1 (the rows that a trellis window of a tile covers).
 constexpr int kStripBytes = 128;
 
-// A wave holds 128 channels of 16 rows as v[4 a + i] = channel 16 a + 4 g + i of row n, lane = 16 g + n.
-// Unnormalised 128-point Sylvester Hadamard of every row: stages over a and i in registers, over g across lanes.
-__device__ __forceinline__ void hadamard128(float (&v)[32], int lane) {
-#pragma unroll
-    for (int h = 1; h < 32; h <<= 1) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if (j & h) continue;
-            const float x = v[j], y = v[j + h];
-            v[j] = x + y;
-            v[j + h] = x - y;
-        }
-    }
-#pragma unroll
-    for (int h = 16; h < 64; h <<= 1) {
-        const bool upper = (lane & h) != 0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float o = __shfl_xor(v[j], h);
-            v[j] = upper ? o - v[j] : v[j] + o;
-        }
-    }
-}
-
 constexpr float kHadamardScale = 0.08838834764831845f;  // 128^-1/2
 
-// Channels 16 a + 4 g .. + 3 of a rotated row, split and stored in the product's order.  rho = 4 g + i lies in lane group
-// (rho % 8) / 2 of its tile, at place (rho & 1) + 2 (rho / 8) of four.
-__device__ __forceinline__ void store_pieces(char* block, int a, int g, float v0, float v1, float v2, float v3) {
-    const float v[4] = {v0, v1, v2, v3};
-    __bf16 hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        hi[i] = static_cast<__bf16>(v[i]);
-        lo[i] = static_cast<__bf16>(v[i] - static_cast<float>(hi[i]));
+template <int kControl>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, 0xF, 0xF, true));
+}
+
+// One butterfly stage between lanes that differ in bit h: lower + upper in the lower, lower - upper in the upper one.
+// `sign` is -1 in the upper lane.  Bits 0..3 stay within a row of 16 lanes (data-parallel moves), 16 and 32 are swaps.
+template <int h>
+__device__ __forceinline__ float stage(float v, float sign) {
+    if constexpr (h == 1) return __builtin_fmaf(sign, v, dpp<0xB1>(v));              // quad_perm 1 0 3 2
+    if constexpr (h == 2) return __builtin_fmaf(sign, v, dpp<0x4E>(v));              // quad_perm 2 3 0 1
+    if constexpr (h == 4) return __builtin_fmaf(sign, v, dpp<0x1B>(dpp<0x141>(v)));  // half mirror, then quad_perm 3 2 1 0
+    if constexpr (h == 8) return __builtin_fmaf(sign, v, dpp<0x128>(v));             // row rotated by 8
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto both = h == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                              : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t lower = both[0], upper = both[1];
+    return __builtin_fmaf(sign, __builtin_bit_cast(float, upper), __builtin_bit_cast(float, lower));
+}
+
+// Unnormalised 128-point Sylvester Hadamard over a wave that holds channels 2 lane and 2 lane + 1.  The 2 x 2 exact
+// stages cost 7 x 2 VALU instructions and no LDS; short code matters here, as the kernels around a product run it once.
+__device__ __forceinline__ void hadamard128(float& a, float& b, int lane) {
+    const float x = a, y = b;
+    a = x + y;
+    b = x - y;
+#define QSRT_STAGE(h)                                \
+    {                                                \
+        const float sign = (lane & h) ? -1.f : 1.f;  \
+        a = stage<h>(a, sign);                       \
+        b = stage<h>(b, sign);                       \
     }
-    char* strip = block + (a >> 1) * kStripBytes;
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {  // channel pairs (0, 1) and (2, 3)
-        const int group = 2 * (g & 1) + p, place = 2 * (g >> 1) + 4 * (a & 1);
-        char* dst = strip + group * 16 + place * 2;
-        *reinterpret_cast<bf16x2*>(dst) = bf16x2{hi[2 * p], hi[2 * p + 1]};
-        *reinterpret_cast<bf16x2*>(dst + 64) = bf16x2{lo[2 * p], lo[2 * p + 1]};
-    }
+    QSRT_STAGE(1) QSRT_STAGE(2) QSRT_STAGE(4) QSRT_STAGE(8) QSRT_STAGE(16) QSRT_STAGE(32)
+#undef QSRT_STAGE
+}
+
+// Channels 2 lane, 2 lane + 1 of a rotated row's block of 128, split and stored in the product's order: channel rho of a
+// tile's 16 lies in lane group (rho % 8) / 2, at place (rho & 1) + 2 (rho / 8) of the tile's four.
+__device__ __forceinline__ void store_pieces(char* block, int lane, float a, float b) {
+    const __bf16 h0 = static_cast<__bf16>(a), h1 = static_cast<__bf16>(b);
+    const bf16x2 lo = {static_cast<__bf16>(a - static_cast<float>(h0)), static_cast<__bf16>(b - static_cast<float>(h1))};
+    const int tile = lane >> 3, pair = lane & 7;  // channels 2 pair, 2 pair + 1 of the tile
+    char* dst = block + (tile >> 1) * kStripBytes + (pair & 3) * 16 + (tile & 1) * 8 + (pair >> 2) * 4;
+    *reinterpret_cast<bf16x2*>(dst) = bf16x2{h0, h1};
+    *reinterpret_cast<bf16x2*>(dst + 64) = lo;
 }
 
 // Rows of one key (an expert, an adapter) in groups that one wave multiplies at once.
@@ -88,6 +89,7 @@ struct GroupHead {
 __device__ __forceinline__ int choose_parts(int64_t units, int strips, int max_parts, int waves, int lane) {
     int64_t best = INT64_MAX;
     for (int s = lane + 1; s <= min(max_parts, strips); s += 64) {
+        if (units * s >= int64_t(1) << 31) break;  // the product counts its items in 32 bits
         const int64_t rounds = (units * s + waves - 1) / waves;
         const int64_t cost = rounds * ((strips + s - 1) / s + 2) << 16 | s;  // ties: the fewest parts
         best = cost < best ? cost : best;

@@ -1,5 +1,6 @@
 // Products of a few rows with packed trellis matrices, and what stands around them in a mixture-of-experts layer.
 #include <algorithm>
+#include <type_traits>
 
 #include "packed.h"
 #include "qsrt_amd.h"
@@ -33,74 +34,92 @@ struct ProductArgs {
     int rows;
 };
 
-typedef const __attribute__((address_space(1))) uint32_t* gu32;
+typedef const __attribute__((address_space(1))) bf16x8* gbf8;
 
-// Eight successive positions of a tile, 8 i8 .. 8 i8 + 7, are the rows 2g + {0, 1, 8, 9} of columns i8 / 4 and i8 / 4 + 8
-// (g = i8 % 4): one window of 16 + 7 K bits of the tile's stream, two dwords.  w0 holds its bits 0..31, w1 its bits 16..47.
-template <int K>
-__device__ __forceinline__ uint32_t state_of(uint32_t w0, uint32_t w1, int j) {
-    return 16 + j * K <= 32 ? (w0 >> (16 - j * K)) & 0xFFFFu : (w1 >> (32 - j * K)) & 0xFFFFu;
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// `strips` strips of 32 payload rows by 128 columns at `tiles`, times G groups of 16 rows.  Lane 16 g + m decodes tile
-// column 2 t + m / 8 of every pair t; MFMA 2 t + u has its columns m % 8 + 8 u as rows.
-template <int K, int G>
-__device__ __forceinline__ void multiply_strips(const char* tiles, int64_t tile_row_bytes, int strips,
-                                                const char* const (&x)[G], const uint8_t* lut, int lane,
+// The label tables come to LDS while a wave looks up its first item and asks for its first words; one barrier a wave.
+struct Tables {
+    bool ready = false;
+    __device__ __forceinline__ void wait() {
+        if (ready) return;
+        __builtin_amdgcn_s_waitcnt(0);  // the direct loads to LDS are not ordered by the barrier alone
+        __syncthreads();
+        ready = true;
+    }
+};
+
+// `strips` strips of 32 payload rows by 128 columns at `tiles`, of rate K, times G groups of 16 rows.  Eight successive
+// positions of a tile, 8 i8 .. 8 i8 + 7, are the rows 2g + {0, 1, 8, 9} of columns i8 / 4 and i8 / 4 + 8 (g = i8 % 4): one
+// window of 16 + 7 K bits of the tile's stream, two dwords.  Lane 16 g + m reads it in tile column 2 t + m / 8 of each pair
+// t, for i8 = 4 (m % 8) + g; MFMA 2 t + u has its columns m % 8 + 8 u as rows.  K is a value and not a template argument:
+// the same instructions with other shifts, where a body for each rate made the compiler keep a second set of sums.
+template <int G>
+__device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_bytes, int strips, int K,
+                                                const char* (&x)[G], const uint8_t* lut, int lane, Tables& tables,
                                                 f32x4 (&acc)[G][8]) {
     const int m = lane & 15, g = lane >> 4;
     int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;
     if (b0 < 0) b0 += 256 * K;
-    const int d0 = b0 >> 5, d1 = (d0 + 1) % (8 * K);
+    const int d0 = b0 >> 5, d1 = d0 + 1 == 8 * K ? 0 : d0 + 1;
     const uint32_t sh = b0 & 31, rsh = 32u - sh;  // sh is never 0 at K = 2, 3, 4
     const uint32_t o0 = 4 * d0 + (m >> 3) * 32 * K, o1 = 4 * d1 + (m >> 3) * 32 * K;
+    const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(tiles), 0, (2 * strips - 1) * tile_row_bytes + 256 * K, 0x00027000);
     uint32_t lo[8], hi[8];
-    bf16x8 xn[G][2];
-    auto fetch = [&](int s) {
+    auto fetch = [&](int s, int t) {  // the pair's windows of both tile rows
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const char* p = tiles + (2 * s + h) * tile_row_bytes;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                lo[4 * h + t] = *(gu32)(p + o0 + t * 64 * K);
-                hi[4 * h + t] = *(gu32)(p + o1 + t * 64 * K);
-            }
+            const int at = (2 * s + h) * tile_row_bytes + t * 64 * K;
+            lo[2 * t + h] = __builtin_amdgcn_raw_buffer_load_b32(src, o0, at, 0);
+            hi[2 * t + h] = __builtin_amdgcn_raw_buffer_load_b32(src, o1, at, 0);
         }
-#pragma unroll
-        for (int q = 0; q < G; ++q)
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-                xn[q][p] = *(const __attribute__((address_space(1))) bf16x8*)(x[q] + s * kStripBytes + p * 64);
     };
-    fetch(0);
-    for (int s = 0; s < strips; ++s) {
-        uint32_t w0[8], w1[8];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) fetch(0, t);
+    tables.wait();
+    int s = 0;
+    do {
         bf16x8 b[G][2];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            w0[t] = __builtin_amdgcn_alignbit(lo[t], hi[t], rsh);
-            w1[t] = K > 2 ? __builtin_amdgcn_alignbit(w0[t], hi[t] << sh, 16) : 0u;
-        }
-#pragma unroll
         for (int q = 0; q < G; ++q) {
-            b[q][0] = xn[q][0];
-            b[q][1] = xn[q][1];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) b[q][p] = *(gbf8)(x[q] + p * 64);
+            x[q] += kStripBytes;
         }
-        if (s + 1 < strips) fetch(s + 1);
+        uint32_t next[16];
+        auto gather = [&](int t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // bits 0..31 of the window, and 4 K .. 4 K + 31: four labels in each
+                const uint32_t w0 = __builtin_amdgcn_alignbit(lo[2 * t + h], hi[2 * t + h], rsh);
+                const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[2 * t + h] << sh, 32 - 4 * K);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) next[8 * h + j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+            }
+            fetch(min(s + 1, strips - 1), t);  // the last strip asks for itself again: no branch, so that waits stay exact
+        };
+        gather(0);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            uint32_t label[2][8];
+            uint32_t label[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) label[h][j] = lut[state_of<K>(w0[4 * h + t], w1[4 * h + t], j)];
+            for (int j = 0; j < 16; ++j) label[j] = next[j];
+            if (t < 3) gather(t + 1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 u32x4 a;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint32_t two = label[q >> 1][4 * u + 2 * (q & 1)] | (label[q >> 1][4 * u + 2 * (q & 1) + 1] << 8);
-                    a[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
+                    const int j = 8 * (q >> 1) + 4 * u + 2 * (q & 1);
+                    a[q] = __builtin_bit_cast(
+                        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                      __builtin_amdgcn_perm(label[j + 1], label[j], 0x0C0C0400u), 1.0f, false));
                 }
                 const bf16x8 av = __builtin_bit_cast(bf16x8, a);
 #pragma unroll
@@ -109,55 +128,55 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int64_t tile_
                     acc[q][2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[q][1], acc[q][2 * t + u], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);  // two pairs' labels in registers at most
         }
-    }
+    } while (++s < strips);
 }
 
-template <int G, int kWaves>
+template <int G, int kWaves, int kTables>
 __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs p) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lut_s[];
+    __shared__ __attribute__((aligned(16))) uint8_t lut_s[65536 * kTables];
     const int lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int i = w; i < p.luts * 64; i += kWaves)
+    const int w = uniform(static_cast<int>(threadIdx.x >> 6));
+    for (int i = w; i < kTables * 64; i += kWaves)
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(p.lut[i >> 6] + 1024 * (i & 63) + 16 * lane),
+            (const __attribute__((address_space(1))) void*)((i < 64 ? p.lut[0] : p.lut[1]) + 1024 * (i & 63) + 16 * lane),
             (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
-    __builtin_amdgcn_s_waitcnt(0);  // the builtin's writes to LDS are not ordered by the barrier alone
-    __syncthreads();
+    Tables tables;
 
     constexpr int kRows = 16 * G;
     const int n = lane & 15, g = lane >> 4;
-    const int chunks = p.head ? p.head->chunks : (p.rows + kRows - 1) / kRows;
-    const int parts = p.head ? p.head->parts[p.which] : p.parts;
-    const int64_t items = static_cast<int64_t>(chunks) * p.nmat * p.nb * parts;
+    const int chunks = p.head ? uniform(p.head->chunks) : (p.rows + kRows - 1) / kRows;
+    const int parts = p.head ? uniform(p.head->parts[p.which]) : p.parts;
+    const uint32_t items = static_cast<uint32_t>(chunks) * p.nmat * p.nb * parts;  // below 2^31: see choose_parts
     const int64_t row_bytes = static_cast<int64_t>(p.kb) * 4 * kStripBytes;
     const int64_t cols = 128 * static_cast<int64_t>(p.nb);
     const int strips = 4 * p.kb;
 
-    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + w; item < items;
-         item += static_cast<int64_t>(gridDim.x) * kWaves) {
-        int rest = static_cast<int>(item / parts);
-        const int part = static_cast<int>(item - static_cast<int64_t>(rest) * parts);
-        const int cb = rest % p.nb;
+    for (uint32_t item = blockIdx.x * kWaves + w; item < items; item += gridDim.x * kWaves) {
+        uint32_t rest = item / parts;
+        const int part = static_cast<int>(item - rest * parts);
+        const int cb = static_cast<int>(rest % p.nb);
         rest /= p.nb;
-        const int mat = rest % p.nmat;
-        const int ci = rest / p.nmat;
-        Chunk c{0, ci * kRows, 0, 0};
+        const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+        const int ci = static_cast<int>(p.nmat == 2 ? rest >> 1 : rest);
+        int key = 0, first = ci * kRows, count;
         if (p.head) {
-            c = p.chunks[ci];
-            c.key = __builtin_amdgcn_readfirstlane(c.key);
-            c.first = __builtin_amdgcn_readfirstlane(c.first);
-            c.count = __builtin_amdgcn_readfirstlane(c.count);
+            key = uniform(p.chunks[ci].key);
+            first = uniform(p.chunks[ci].first);
+            count = uniform(p.chunks[ci].count);
         } else {
-            c.count = min(kRows, p.rows - c.first);
+            count = min(kRows, p.rows - first);
         }
+        int s = strips * part / parts;
+        const int end = strips * (part + 1) / parts;
         int row[G];
         const char* x[G];
 #pragma unroll
         for (int q = 0; q < G; ++q) {  // lanes past the last row repeat it; their sums are not stored
-            const int at = c.first + min(16 * q + n, c.count - 1);
+            const int at = first + min(16 * q + n, count - 1);
             row[q] = p.head ? p.order[at] : at;
-            x[q] = (mat ? p.x[1] : p.x[0]) + (row[q] / p.x_div) * row_bytes + 16 * g;
+            x[q] = (mat ? p.x[1] : p.x[0]) + (p.x_div == 1 ? row[q] : row[q] / p.x_div) * row_bytes + 16 * g + s * kStripBytes;
         }
         f32x4 acc[G][8];
 #pragma unroll
@@ -165,40 +184,30 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 #pragma unroll
             for (int t = 0; t < 8; ++t) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        const char* words = reinterpret_cast<const char*>((mat ? p.words[1] : p.words[0]) +
-                                                          c.key * (mat ? p.key_stride[1] : p.key_stride[0]));
-        const int64_t* records =
-            (mat ? p.records[1] : p.records[0]) + c.key * (mat ? p.record_stride[1] : p.record_stride[0]);
-        int s = static_cast<int>(static_cast<int64_t>(strips) * part / parts);
-        const int end = static_cast<int>(static_cast<int64_t>(strips) * (part + 1) / parts);
+        const char* words =
+            reinterpret_cast<const char*>((mat ? p.words[1] : p.words[0]) + key * (mat ? p.key_stride[1] : p.key_stride[0]));
+        const int64_t* records = (mat ? p.records[1] : p.records[0]) + key * (mat ? p.record_stride[1] : p.record_stride[0]);
         while (s < end) {  // runs of one rate
             const int r = p.axis ? cb : s >> 2;
-            const uint64_t rec = static_cast<uint64_t>(records[r]);
-            const int bits = __builtin_amdgcn_readfirstlane(static_cast<int>(rec & 7));
-            const int64_t first = static_cast<int64_t>(
-                (static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rec >> 32))) << 32 |
-                 __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rec))) >> 3);
+            const int64_t rec = uniform(records[r]);
+            const int bits = static_cast<int>(rec & 7);
             int stop = end;
             if (!p.axis) {  // records of one rate that follow one another are one strip of tiles
                 int r1 = r + 1;
-                while (4 * r1 < end && __builtin_amdgcn_readfirstlane(static_cast<int>(records[r1] & 7)) == bits) ++r1;
+                while (4 * r1 < end && (uniform(static_cast<int>(records[r1])) & 7) == bits) ++r1;
                 stop = min(end, 4 * r1);
             }
-            const int64_t tile = 32 * bits;
-            const int64_t tile_row = p.axis ? 8 * tile : 8 * p.nb * tile;
-            const char* tiles = words + 2 * first + (p.axis ? 2 * s * tile_row : 2 * (s - 4 * r) * tile_row + 8 * cb * tile);
-            const int slot = bits == p.lut_bits[0] ? 0 : (p.luts > 1 && bits == p.lut_bits[1]) ? 1 : -1;
-            if (slot >= 0) {
-                const uint8_t* lut = lut_s + 65536 * slot;
-                const char* xs[G];
+            const int tile = 32 * bits;
+            const int tile_row = p.axis ? 8 * tile : 8 * p.nb * tile;
+            const char* tiles = words + 2 * (rec >> 3) +
+                                (p.axis ? static_cast<int64_t>(2 * s) * tile_row
+                                        : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
+            if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
+                const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
+                multiply_strips<G>(tiles, tile_row, stop - s, bits, x, lut, lane, tables, acc);
+            } else {  // another pass has this rate
 #pragma unroll
-                for (int q = 0; q < G; ++q) xs[q] = x[q] + s * kStripBytes;
-                if (bits == 2)
-                    multiply_strips<2, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
-                else if (bits == 3)
-                    multiply_strips<3, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
-                else
-                    multiply_strips<4, G>(tiles, tile_row, stop - s, xs, lut, lane, acc);
+                for (int q = 0; q < G; ++q) x[q] += (stop - s) * kStripBytes;
             }
             s = stop;
         }
@@ -207,12 +216,13 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                      16 * (g >> 1) + 4 * (g & 1);
 #pragma unroll
         for (int q = 0; q < G; ++q) {
-            if (16 * q + n >= c.count) continue;
+            if (16 * q + n >= count) continue;
 #pragma unroll
             for (int t = 0; t < 8; ++t)
                 *reinterpret_cast<f32x4*>(out + row[q] * cols + 32 * (t >> 1) + 8 * (t & 1)) = acc[q][t];
         }
     }
+    tables.wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -230,36 +240,27 @@ struct RotateArgs {
     int rows, kb, nmat;
 };
 
-// One wave for 16 rows of 128 channels of one matrix.
+// One wave for 128 channels of one row and one matrix.
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs p) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
     const int kb = static_cast<int>(wave % p.kb);
     const int64_t rest = wave / p.kb;
-    const int mat = static_cast<int>(rest % p.nmat);
-    const int64_t r0 = rest / p.nmat * 16;
-    if (r0 >= p.rows) return;
-    const int row = static_cast<int>(min(r0 + n, static_cast<int64_t>(p.rows) - 1));
-    const int id = p.ids ? p.ids[row] : 0;
-    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + max(id, 0) * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
+    const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+    const int64_t row = p.nmat == 2 ? rest >> 1 : rest;
+    if (row >= p.rows) return;
+    const int id = p.ids ? max(p.ids[row], 0) : 0;
+    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + id * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
     const T* x = static_cast<const T*>(p.x) + (row / p.x_div) * p.ld + 128 * kb;
-    float v[32];
-    typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int a = 0; a < 8; ++a) {
-        const t4 xv = *reinterpret_cast<const t4*>(x + 16 * a + 4 * g);
-        const f16x4 sv = *reinterpret_cast<const f16x4*>(suh + 16 * a + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * a + i] = static_cast<float>(xv[i]) * static_cast<float>(sv[i]);
-    }
-    hadamard128(v, lane);
-    if (r0 + n >= p.rows) return;
-    char* block = (mat ? p.out[1] : p.out[0]) + (static_cast<int64_t>(row) * p.kb + kb) * 4 * kStripBytes;
-#pragma unroll
-    for (int a = 0; a < 8; ++a)
-        store_pieces(block, a, g, v[4 * a] * kHadamardScale, v[4 * a + 1] * kHadamardScale, v[4 * a + 2] * kHadamardScale,
-                     v[4 * a + 3] * kHadamardScale);
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 xv = reinterpret_cast<const t2*>(x)[lane];
+    const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];
+    float a = static_cast<float>(xv[0]) * static_cast<float>(sv[0]);
+    float b = static_cast<float>(xv[1]) * static_cast<float>(sv[1]);
+    hadamard128(a, b, lane);
+    store_pieces((mat ? p.out[1] : p.out[0]) + (row * p.kb + kb) * 4 * kStripBytes, lane, a * kHadamardScale,
+                 b * kHadamardScale);
 }
 
 // ---------------------------------------------------------------------------
@@ -283,56 +284,47 @@ __device__ __forceinline__ float activate(float g, float u, int act) {
     return act == 0 ? g * s * u : 4.0f * tanhf(0.25f * g) * s * (25.0f * tanhf(0.04f * u));
 }
 
-// One wave for 128 middle channels of one (token, expert) pair.  Lane n < 8 sums the gate's parts n, n + 8, ..., lane
-// n >= 8 the up's.
+// Sum over parts first, first + step, ... of the two channels 2 lane, 2 lane + 1; the loads of eight parts go out together.
+__device__ __forceinline__ f32x2 sum_parts(const float* src, int64_t stride, int first, int step, int parts) {
+    f32x2 sum = {0.f, 0.f};
+    int s = first;
+    for (; s + 7 * step < parts; s += 8 * step) {
+        f32x2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x2*>(src + (s + j * step) * stride);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += v[j];
+    }
+#pragma unroll 4
+    for (; s < parts; s += step) sum += *reinterpret_cast<const f32x2*>(src + s * stride);
+    return sum;
+}
+
+// One wave for 128 middle channels of one (token, expert) pair.
 __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
     const int ib = static_cast<int>(wave % p.ib);
-    const int pair = static_cast<int>(wave / p.ib);
+    const int64_t pair = wave / p.ib;
     if (pair >= p.pairs) return;
-    const int id = __builtin_amdgcn_readfirstlane(p.ids[pair]);
+    const int id = uniform(p.ids[pair]);
     if (id < 0) return;
-    const int64_t inter = 128 * static_cast<int64_t>(p.ib);
-    const int parts = p.passes * p.head->parts[0];
-    const int mat = n >> 3;
-    float v[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-    for (int s = n & 7; s < parts; s += 8) {
-        const float* src = p.part + ((static_cast<int64_t>(s) * 2 + mat) * p.pairs + pair) * inter + 128 * ib + 4 * g;
-#pragma unroll
-        for (int a = 0; a < 8; ++a) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * a + i] += x[i];
-        }
-    }
-#pragma unroll
-    for (int h = 1; h < 8; h <<= 1)
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += __shfl_xor(v[j], h);
-    hadamard128(v, lane);
-    const _Float16* svh = (mat ? p.svh[1] + id * p.svh_stride[1] : p.svh[0] + id * p.svh_stride[0]) + 128 * ib + 4 * g;
-    const _Float16* suh = p.suh + id * p.suh_stride + 128 * ib + 4 * g;
-#pragma unroll
-    for (int a = 0; a < 8; ++a) {
-        const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 16 * a);
-        const f16x4 su = *reinterpret_cast<const f16x4*>(suh + 16 * a);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float mine = v[4 * a + i] * kHadamardScale * static_cast<float>(sv[i]);
-            const float other = __shfl_xor(mine, 8);
-            v[4 * a + i] = activate(mat ? other : mine, mat ? mine : other, p.act) * static_cast<float>(su[i]);
-        }
-    }
-    hadamard128(v, lane);
-    if (n) return;
-    char* block = p.out + (static_cast<int64_t>(pair) * p.ib + ib) * 4 * kStripBytes;
-#pragma unroll
-    for (int a = 0; a < 8; ++a)
-        store_pieces(block, a, g, v[4 * a] * kHadamardScale, v[4 * a + 1] * kHadamardScale, v[4 * a + 2] * kHadamardScale,
-                     v[4 * a + 3] * kHadamardScale);
+    const int64_t inter = 128 * static_cast<int64_t>(p.ib), rows = static_cast<int64_t>(p.pairs) * inter;
+    const int parts = p.passes * uniform(p.head->parts[0]);
+    const float* src = p.part + pair * inter + 128 * ib + 2 * lane;
+    const f32x2 gs = sum_parts(src, 2 * rows, 0, 1, parts), us = sum_parts(src + rows, 2 * rows, 0, 1, parts);
+    float g0 = gs[0], g1 = gs[1], u0 = us[0], u1 = us[1];
+    hadamard128(g0, g1, lane);
+    hadamard128(u0, u1, lane);
+    const f16x2 sg = reinterpret_cast<const f16x2*>(p.svh[0] + id * p.svh_stride[0] + 128 * ib)[lane];
+    const f16x2 su = reinterpret_cast<const f16x2*>(p.svh[1] + id * p.svh_stride[1] + 128 * ib)[lane];
+    const f16x2 sd = reinterpret_cast<const f16x2*>(p.suh + id * p.suh_stride + 128 * ib)[lane];
+    float a = activate(g0 * kHadamardScale * static_cast<float>(sg[0]), u0 * kHadamardScale * static_cast<float>(su[0]), p.act) *
+              static_cast<float>(sd[0]);
+    float b = activate(g1 * kHadamardScale * static_cast<float>(sg[1]), u1 * kHadamardScale * static_cast<float>(su[1]), p.act) *
+              static_cast<float>(sd[1]);
+    hadamard128(a, b, lane);
+    store_pieces(p.out + (pair * p.ib + ib) * 4 * kStripBytes, lane, a * kHadamardScale, b * kHadamardScale);
 }
 
 // ---------------------------------------------------------------------------
@@ -351,80 +343,42 @@ struct CombineArgs {
     int tokens, k, hb, passes;
 };
 
-// One wave for 128 channels of one token.  With one svh for all experts the weighted part sums are rotated once; with one
-// for each, an expert at a time.  Lanes n split the parts of an expert.
+constexpr int kCombineWaves = 8;
+
+// One workgroup for 128 channels of one token, its waves share the token's experts.  With one svh for all experts the
+// weighted sum is rotated once, with one for each every expert's.
 template <typename T>
-__global__ __launch_bounds__(256) void combine_kernel(const CombineArgs p) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int hb = static_cast<int>(wave % p.hb);
-    const int64_t token = wave / p.hb;
-    if (token >= p.tokens) return;
-    const int64_t hidden = 128 * static_cast<int64_t>(p.hb);
-    const int64_t pairs = static_cast<int64_t>(p.tokens) * p.k;
-    const int parts = p.passes * p.head->parts[1];
-    float y[32], v[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = 0.f;
-    auto add_pair = [&](int64_t pair, float wt, float(&to)[32], int first, int step) {
-        for (int s = first; s < parts; s += step) {
-            const float* src = p.part + (s * pairs + pair) * hidden + 128 * hb + 4 * g;
-#pragma unroll
-            for (int a = 0; a < 8; ++a) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) to[4 * a + i] += wt * x[i];
-            }
-        }
+__global__ __launch_bounds__(64 * kCombineWaves) void combine_kernel(const CombineArgs p) {
+    __shared__ f32x2 sums[kCombineWaves][64];
+    const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6)), waves = blockDim.x >> 6;
+    const int hb = static_cast<int>(blockIdx.x % p.hb);
+    const int64_t token = blockIdx.x / p.hb;
+    const int64_t hidden = 128 * static_cast<int64_t>(p.hb), stride = static_cast<int64_t>(p.tokens) * p.k * hidden;
+    const int parts = p.passes * uniform(p.head->parts[1]);
+    const bool shared = p.svh_stride == 0;
+    auto rotated = [&](f32x2 v, const _Float16* svh) {
+        float a = v[0], b = v[1];
+        hadamard128(a, b, lane);
+        const f16x2 sv = reinterpret_cast<const f16x2*>(svh + 128 * hb)[lane];
+        return f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
     };
-    auto over_lanes = [&](float(&to)[32]) {
-#pragma unroll
-        for (int h = 1; h < 16; h <<= 1)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) to[j] += __shfl_xor(to[j], h);
-    };
-    auto scaled = [&](float(&to)[32], const _Float16* svh) {
-#pragma unroll
-        for (int a = 0; a < 8; ++a) {
-            const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 128 * hb + 4 * g + 16 * a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[4 * a + i] *= kHadamardScale * static_cast<float>(sv[i]);
-        }
-    };
-    if (p.svh_stride == 0) {
-        // (pair, part) couples over the 16 lanes
-        const int total = p.k * parts;
-        for (int c = n; c < total; c += 16) {
-            const int64_t pair = token * p.k + c / parts;
-            if (p.ids[pair] < 0) continue;
-            add_pair(pair, p.weights[pair], y, c % parts, parts);
-        }
-        over_lanes(y);
-        hadamard128(y, lane);
-        scaled(y, p.svh);
-    } else {
-        for (int j = 0; j < p.k; ++j) {
-            const int64_t pair = token * p.k + j;
-            const int id = __builtin_amdgcn_readfirstlane(p.ids[pair]);
-            if (id < 0) continue;
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = 0.f;
-            add_pair(pair, 1.0f, v, n, 16);
-            over_lanes(v);
-            hadamard128(v, lane);
-            scaled(v, p.svh + id * p.svh_stride);
-            const float wt = p.weights[pair];
-#pragma unroll
-            for (int q = 0; q < 32; ++q) y[q] += wt * v[q];
-        }
+    f32x2 y = {0.f, 0.f};
+    for (int j = w; j < p.k; j += waves) {
+        const int64_t pair = token * p.k + j;
+        const int id = uniform(p.ids[pair]);
+        if (id < 0) continue;
+        f32x2 v = sum_parts(p.part + pair * hidden + 128 * hb + 2 * lane, stride, 0, 1, parts);
+        if (!shared) v = rotated(v, p.svh + id * p.svh_stride);
+        y += v * p.weights[pair];
     }
-    if (n) return;
-    T* out = static_cast<T*>(p.out) + token * p.ld + 128 * hb + 4 * g;
-    typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int a = 0; a < 8; ++a)
-        *reinterpret_cast<t4*>(out + 16 * a) = t4{static_cast<T>(y[4 * a]), static_cast<T>(y[4 * a + 1]),
-                                                  static_cast<T>(y[4 * a + 2]), static_cast<T>(y[4 * a + 3])};
+    sums[w][lane] = y;
+    __syncthreads();
+    if (w) return;
+    for (int j = 1; j < waves; ++j) y += sums[j][lane];
+    if (shared) y = rotated(y, p.svh);
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    reinterpret_cast<t2*>(static_cast<T*>(p.out) + token * p.ld + 128 * hb)[lane] =
+        t2{static_cast<T>(y[0]), static_cast<T>(y[1])};
 }
 
 // ---------------------------------------------------------------------------
@@ -444,46 +398,56 @@ struct ShrinkArgs {
     int rows, k, rank, parts;
 };
 
-// x A_a^T of 16 rows of one adapter over a part of the K axis; a wave each.  Products of the inputs are exact, sums FP32.
-template <typename T>
+// x A_a^T of 16 rows of one adapter over a part of the K axis, 16 kTiles ranks at a time; a wave each.  Products of the
+// inputs are exact, sums FP32.
+template <typename T, int kTiles>
 __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int64_t nw = static_cast<int64_t>(gridDim.x) * 4;
-    const int64_t items = static_cast<int64_t>(p.head->chunks) * p.parts;
-    const int steps = p.k / 32, tiles = p.rank / 16;
+    const int64_t items = static_cast<int64_t>(uniform(p.head->chunks)) * p.parts * (p.rank / (16 * kTiles));
+    const int steps = p.k / 32, groups = p.rank / (16 * kTiles);
     typedef T t8 __attribute__((ext_vector_type(8)));
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
          item < items; item += nw) {
-        const int ci = static_cast<int>(item / p.parts), part = static_cast<int>(item % p.parts);
-        const Chunk c = p.chunks[ci];
-        const int key = __builtin_amdgcn_readfirstlane(c.key);
+        const int part = static_cast<int>(item % p.parts), rest = static_cast<int>(item / p.parts);
+        const int group = rest % groups;
+        const Chunk c = p.chunks[rest / groups];
+        const int key = uniform(c.key);
         if (key < 0) continue;
         const int row = p.order[c.first + min(n, c.count - 1)];
         const T* x = static_cast<const T*>(p.x) + row * p.ld + 8 * g;
-        const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + n) * p.k + 8 * g;
-        f32x4 acc[kMaxRank / 16];
+        const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + 16 * kTiles * group + n) * p.k + 8 * g;
+        f32x4 acc[kTiles];
 #pragma unroll
-        for (int t = 0; t < kMaxRank / 16; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.parts);
-        for (int s = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts); s < s1; ++s) {
-            const t8 xv = *reinterpret_cast<const t8*>(x + 32 * s);
+        auto steps_at = [&](int s, auto count) {  // the loads of all `count` steps go out together
+            constexpr int kSteps = decltype(count)::value;
+            t8 xv[kSteps], av[kSteps][kTiles];
 #pragma unroll
-            for (int t = 0; t < kMaxRank / 16; ++t) {
-                if (t >= tiles) break;
-                const t8 av = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * s);
-                if constexpr (__is_same(T, __bf16))
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, xv, acc[t], 0, 0, 0);
-                else
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, xv, acc[t], 0, 0, 0);
+            for (int j = 0; j < kSteps; ++j) {
+                xv[j] = *reinterpret_cast<const t8*>(x + 32 * (s + j));
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    av[j][t] = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * (s + j));
             }
-        }
-        if (n >= c.count) continue;
-        float* out = p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank + 4 * g;
 #pragma unroll
-        for (int t = 0; t < kMaxRank / 16; ++t) {
-            if (t >= tiles) break;
-            *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
-        }
+            for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    if constexpr (__is_same(T, __bf16))
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[j][t], xv[j], acc[t], 0, 0, 0);
+                    else
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][t], xv[j], acc[t], 0, 0, 0);
+                }
+        };
+        int s = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts);
+        for (; s + 4 <= s1; s += 4) steps_at(s, std::integral_constant<int, 4>{});
+        for (; s < s1; ++s) steps_at(s, std::integral_constant<int, 1>{});
+        if (n >= c.count) continue;
+        float* out = p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank + 16 * kTiles * group + 4 * g;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
     }
 }
 
@@ -504,91 +468,96 @@ struct FinishArgs {
     int rows, nb;
 };
 
-// Sum of the parts, back into the output's basis, plus the adapter's second product; a wave for 16 rows by 128 columns.
+// Sum of the parts, back into the output's basis, plus the adapter's second product: a workgroup of four waves for the (at
+// most 16) rows of a chunk by 128 columns.  Each wave has every fourth row and reads the adapter's slice once for them;
+// under four rows the waves share the parts of each instead.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nb = static_cast<int>(wave % p.nb);
-    const int ci = static_cast<int>(wave / p.nb);
-    if (ci >= (p.head ? p.head->chunks : (p.rows + 15) / 16)) return;
-    Chunk c{-1, 16 * ci, 0, 0};
-    if (p.head)
-        c = p.chunks[ci];
-    else
-        c.count = min(16, p.rows - c.first);
-    const int64_t cols = 128 * static_cast<int64_t>(p.nb);
-    // the lanes beyond the chunk's rows (in powers of two) share the parts
-    int width = 1;
-    while (width < c.count) width <<= 1;
-    const int mine = n & (width - 1), sub = n / width, subs = 16 / width;
-    const int at = c.first + min(mine, c.count - 1);
-    const int row = p.head ? p.order[at] : at;
-    float v[32];
+    __shared__ f32x2 sums[4][64];
+    const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int nb = static_cast<int>(blockIdx.x % p.nb), ci = static_cast<int>(blockIdx.x / p.nb);
+    if (ci >= (p.head ? uniform(p.head->chunks) : (p.rows + 15) / 16)) return;
+    int key = -1, first = 16 * ci, count;
+    if (p.head) {
+        key = uniform(p.chunks[ci].key);
+        first = uniform(p.chunks[ci].first);
+        count = uniform(p.chunks[ci].count);
+    } else {
+        count = min(16, p.rows - first);
+    }
+    const int64_t cols = 128 * static_cast<int64_t>(p.nb), stride = p.rows * cols;
+    const float* src = p.part + 128 * nb + 2 * lane;
+    int row[4];
+    f32x2 v[4];
+    int mine = 0;  // rows of this wave
+    if (count < 4) {
+        for (int r = 0; r < count; ++r) {
+            const int at = p.head ? uniform(p.order[first + r]) : first + r;
+            sums[w][lane] = sum_parts(src + at * cols, stride, w, 4, p.parts);
+            __syncthreads();
+            if (w == r) {
+                row[0] = at;
+                v[0] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+                mine = 1;
+            }
+            __syncthreads();
+        }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-    for (int s = sub; s < p.parts; s += subs) {
-        const float* src = p.part + (static_cast<int64_t>(s) * p.rows + row) * cols + 128 * nb + 4 * g;
-#pragma unroll
-        for (int a = 0; a < 8; ++a) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(src + 16 * a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * a + i] += x[i];
+        for (int i = 0; i < 4; ++i) {
+            const int r = w + 4 * i;
+            if (r >= count) break;
+            row[i] = p.head ? uniform(p.order[first + r]) : first + r;
+            v[i] = sum_parts(src + row[i] * cols, stride, 0, 1, p.parts);
+            mine = i + 1;
         }
     }
-    for (int h = width; h < 16; h <<= 1)
+    const f16x2 sv = reinterpret_cast<const f16x2*>(p.svh + 128 * nb)[lane];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += __shfl_xor(v[j], h);
-    hadamard128(v, lane);
-    const _Float16* svh = p.svh + 128 * nb + 4 * g;
-    f32x4 acc[8];
-#pragma unroll
-    for (int a = 0; a < 8; ++a) {
-        const f16x4 sv = *reinterpret_cast<const f16x4*>(svh + 16 * a);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[a][i] = v[4 * a + i] * kHadamardScale * static_cast<float>(sv[i]);
+    for (int i = 0; i < 4; ++i) {
+        if (i >= mine) break;
+        float a = v[i][0], b = v[i][1];
+        hadamard128(a, b, lane);
+        v[i] = f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
     }
-    const int key = __builtin_amdgcn_readfirstlane(c.key);
-    if (key >= 0) {
+    if (key >= 0 && mine) {
         typedef T t8 __attribute__((ext_vector_type(8)));
         const float scale = p.scale[key];
-        const T* b = static_cast<const T*>(p.b) + (static_cast<int64_t>(key) * cols + 128 * nb + n) * p.rank + 8 * g;
-        const float* low = p.low + static_cast<int64_t>(row) * p.rank + 8 * g;
-        for (int r = 0; r < p.rank; r += 32) {
-            const bool in = r + 8 * g < p.rank;  // the rank is a multiple of 16
-            float xv[8];
+        const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(key) * cols + 128 * nb + 2 * lane) * p.rank;
+        for (int r0 = 0; r0 < p.rank; r0 += 64) {
+            float low[4];  // lane l: rank r0 + l of each row
 #pragma unroll
-            for (int j = 0; j < 8; ++j) xv[j] = 0.f;
-            if (in) {
-                for (int s = 0; s < p.low_parts; ++s) {
-                    const float* src = low + static_cast<int64_t>(s) * p.rows * p.rank + r;
-                    const f32x4 x0 = *reinterpret_cast<const f32x4*>(src), x1 = *reinterpret_cast<const f32x4*>(src + 4);
+            for (int i = 0; i < 4; ++i) {
+                low[i] = 0.f;
+                if (i < mine && r0 + lane < p.rank)
+                    for (int s = 0; s < p.low_parts; ++s)
+                        low[i] += p.low[(static_cast<int64_t>(s) * p.rows + row[i]) * p.rank + r0 + lane];
+                low[i] *= scale;
+            }
+            for (int r = 0; r < 64 && r0 + r < p.rank; r += 8) {
+                const t8 x0 = *reinterpret_cast<const t8*>(b0 + r0 + r);
+                const t8 x1 = *reinterpret_cast<const t8*>(b0 + p.rank + r0 + r);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        xv[j] += x0[j];
-                        xv[4 + j] += x1[j];
+                for (int i = 0; i < 4; ++i) {
+                    if (i >= mine) break;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float f = __builtin_bit_cast(
+                            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, low[i]), r + j));
+                        v[i][0] = __builtin_fmaf(f, static_cast<float>(x0[j]), v[i][0]);
+                        v[i][1] = __builtin_fmaf(f, static_cast<float>(x1[j]), v[i][1]);
                     }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) xv[j] *= scale;
-            const t8 zero = {};
-#pragma unroll
-            for (int a = 0; a < 8; ++a) {
-                const t8 bv = in ? *reinterpret_cast<const t8*>(b + static_cast<int64_t>(16 * a) * p.rank + r) : zero;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(static_cast<float>(bv[j]), xv[j], acc[a], 0, 0, 0);
-            }
         }
     }
-    if (n >= c.count) return;
-    T* out = static_cast<T*>(p.out) + row * p.ld + 128 * nb + 4 * g;
-    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
-        *reinterpret_cast<t4*>(out + 16 * a) = t4{static_cast<T>(acc[a][0]), static_cast<T>(acc[a][1]),
-                                                  static_cast<T>(acc[a][2]), static_cast<T>(acc[a][3])};
+    for (int i = 0; i < 4; ++i) {
+        if (i >= mine) break;
+        reinterpret_cast<t2*>(static_cast<T*>(p.out) + row[i] * p.ld + 128 * nb)[lane] =
+            t2{static_cast<T>(v[i][0]), static_cast<T>(v[i][1])};
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -597,19 +566,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
 
 constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one product, unless one part alone takes more
 
-template <int G>
-struct Shape {
-    static constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
-};
-
-template <int G>
+template <int G, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
-    constexpr int kWaves = Shape<G>::kWaves;
-    const size_t lds = static_cast<size_t>(65536) * args.luts;
-    if (args.luts > 1)
-        QSRT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<G, kWaves>),
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, 131072));
-    hipLaunchKernelGGL((product_kernel<G, kWaves>), dim3(cus), dim3(64 * kWaves), lds, stream, args);
+    constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
+    hipLaunchKernelGGL((product_kernel<G, kWaves, kTables>), dim3(cus), dim3(64 * kWaves), 0, stream, args);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
@@ -628,9 +588,10 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
             args.lut_bits[j] = set[first + j];
             args.lut[j] = luts[set[first + j] - 2];
         }
-        const int rc = groups == 1   ? launch_product_g<1>(args, cus, stream)
-                       : groups == 2 ? launch_product_g<2>(args, cus, stream)
-                                     : launch_product_g<4>(args, cus, stream);
+        const bool two = args.luts > 1;
+        const int rc = groups == 1   ? (two ? launch_product_g<1, 2> : launch_product_g<1, 1>)(args, cus, stream)
+                       : groups == 2 ? (two ? launch_product_g<2, 2> : launch_product_g<2, 1>)(args, cus, stream)
+                                     : (two ? launch_product_g<4, 2> : launch_product_g<4, 1>)(args, cus, stream);
         if (rc != kOk) return rc;
     }
     return kOk;
@@ -795,7 +756,7 @@ extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_m
     ra.rows = static_cast<int>(shared ? tokens : pairs);
     ra.kb = static_cast<int>(hidden / 128);
     ra.nmat = 2;
-    const dim3 rgrid(blocks_of((ra.rows + 15) / 16 * static_cast<int64_t>(ra.kb) * 2));
+    const dim3 rgrid(blocks_of(static_cast<int64_t>(ra.rows) * ra.kb * 2));
     if (dtype == 0)
         hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
     else
@@ -861,11 +822,11 @@ extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_m
     ca.k = k;
     ca.hb = static_cast<int>(hidden / 128);
     ca.passes = s.passes[1];
-    const dim3 cgrid(blocks_of(tokens * ca.hb));
+    const dim3 cgrid(static_cast<unsigned>(tokens * ca.hb)), cblock(64 * std::min(k, kCombineWaves));
     if (dtype == 0)
-        hipLaunchKernelGGL(combine_kernel<__bf16>, cgrid, dim3(256), 0, stream, ca);
+        hipLaunchKernelGGL(combine_kernel<__bf16>, cgrid, cblock, 0, stream, ca);
     else
-        hipLaunchKernelGGL(combine_kernel<_Float16>, cgrid, dim3(256), 0, stream, ca);
+        hipLaunchKernelGGL(combine_kernel<_Float16>, cgrid, cblock, 0, stream, ca);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
@@ -960,7 +921,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     ra.rows = static_cast<int>(rows);
     ra.kb = static_cast<int>(k / 128);
     ra.nmat = 1;
-    const dim3 rgrid(blocks_of((rows + 15) / 16 * ra.kb));
+    const dim3 rgrid(blocks_of(rows * ra.kb));
     if (dtype == 0)
         hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
     else
@@ -991,12 +952,17 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         sa.k = static_cast<int>(k);
         sa.rank = static_cast<int>(rank);
         sa.parts = s.low_parts;
-        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1) * s.low_parts;
+        const int tiles = rank % 64 == 0 ? 4 : rank % 32 == 0 ? 2 : 1;  // of 16 ranks a wave
+        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1) * s.low_parts * (rank / (16 * tiles));
         const dim3 sgrid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most), 8 * cus)));
+#define QSRT_SHRINK(T)                                                                                  \
+    hipLaunchKernelGGL((tiles == 4 ? shrink_kernel<T, 4> : tiles == 2 ? shrink_kernel<T, 2> : shrink_kernel<T, 1>), \
+                       sgrid, dim3(256), 0, stream, sa)
         if (dtype == 0)
-            hipLaunchKernelGGL(shrink_kernel<__bf16>, sgrid, dim3(256), 0, stream, sa);
+            QSRT_SHRINK(__bf16);
         else
-            hipLaunchKernelGGL(shrink_kernel<_Float16>, sgrid, dim3(256), 0, stream, sa);
+            QSRT_SHRINK(_Float16);
+#undef QSRT_SHRINK
         QSRT_HIP_TRY(hipGetLastError());
     }
 
@@ -1027,7 +993,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     fa.rows = static_cast<int>(rows);
     fa.nb = static_cast<int>(n / 128);
     const int64_t most = adapters ? std::min(rows, (rows + 15) / 16 + adapters + 1) : (rows + 15) / 16;
-    const dim3 fgrid(blocks_of(most * fa.nb));
+    const dim3 fgrid(static_cast<unsigned>(most * fa.nb));
     if (dtype == 0)
         hipLaunchKernelGGL(finish_kernel<__bf16>, fgrid, dim3(256), 0, stream, fa);
     else

@@ -24,15 +24,28 @@ __global__ __launch_bounds__(64 * kRouterWaves) void router_logits_kernel(const 
     const T* wr = w + min(e0 + m, experts - 1) * w_ld + 8 * g;  // rows past the end repeat the last; not stored
     const T* xr = x + min(t0 + m, tokens - 1) * ld + 8 * g;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const t8 zero = {};
-    for (int h = 32 * wave; h < hidden; h += 32 * kRouterWaves) {
-        const bool in = h + 8 * g < hidden;  // hidden is a multiple of 8
-        const t8 a = in ? *reinterpret_cast<const t8*>(wr + h) : zero;
-        const t8 b = in ? *reinterpret_cast<const t8*>(xr + h) : zero;
-        if constexpr (sizeof(T) == 2 && __is_same(T, __bf16))
+    auto multiply = [&](t8 a, t8 b) {
+        if constexpr (__is_same(T, __bf16))
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
         else
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
+    };
+    constexpr int kStep = 32 * kRouterWaves, kBatch = 7;
+    int h = 32 * wave;
+    for (; h + (kBatch - 1) * kStep + 32 <= hidden; h += kBatch * kStep) {  // a batch of loads in flight
+        t8 a[kBatch], b[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            a[j] = *reinterpret_cast<const t8*>(wr + h + j * kStep);
+            b[j] = *reinterpret_cast<const t8*>(xr + h + j * kStep);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) multiply(a[j], b[j]);
+    }
+    const t8 zero = {};
+    for (; h < hidden; h += kStep) {
+        const bool in = h + 8 * g < hidden;  // hidden is a multiple of 8
+        multiply(in ? *reinterpret_cast<const t8*>(wr + h) : zero, in ? *reinterpret_cast<const t8*>(xr + h) : zero);
     }
     sums[wave][lane] = acc;
     __syncthreads();
@@ -46,7 +59,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void router_logits_kernel(const 
         if (e0 + 4 * g + i < experts) logits[static_cast<int64_t>(t) * experts + e0 + 4 * g + i] = acc[i];
 }
 
-constexpr int kMaxExperts = 1024, kPerLane = kMaxExperts / 64;
+constexpr int kMaxExperts = 1024;
 
 // Order of float keys as unsigned integers; NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t sortable(float key) {
@@ -56,93 +69,117 @@ __device__ __forceinline__ uint32_t sortable(float key) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// Over a wave, without LDS: rows of 16 lanes by data-parallel moves, then across rows.
+template <typename Op, typename V>
+__device__ __forceinline__ V over_wave(V v, Op op) {
+    auto with = [&](auto moved) { v = op(v, __builtin_bit_cast(V, moved)); };
+    with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+    with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+    with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));
+    with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = op(__builtin_bit_cast(V, uint32_t(a[0])), __builtin_bit_cast(V, uint32_t(a[1])));
+    const uint32_t t = __builtin_bit_cast(uint32_t, v);
+    const auto b = __builtin_amdgcn_permlane32_swap(t, t, false, false);
+    return op(__builtin_bit_cast(V, uint32_t(b[0])), __builtin_bit_cast(V, uint32_t(b[1])));
+}
 __device__ __forceinline__ float wave_max(float v) {
-    for (int h = 1; h < 64; h <<= 1) v = fmaxf(v, __shfl_xor(v, h));
-    return v;
+    return over_wave(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    return over_wave(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 __device__ __forceinline__ float wave_sum(float v) {
-    for (int h = 1; h < 64; h <<= 1) v += __shfl_xor(v, h);
-    return v;
+    return over_wave(v, [](float a, float b) { return a + b; });
 }
 
-// One wave a token: scores, k rounds of (largest key, lowest index), weights.
-__global__ __launch_bounds__(256) void choose_kernel(const float* __restrict__ logits, const float* __restrict__ bias,
-                                                     int tokens, int experts, int k, int scoring, int normalize,
-                                                     float scale, float* __restrict__ weights, int* __restrict__ ids) {
-    const int lane = threadIdx.x & 63;
-    const int token = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (token >= tokens) return;
-    float score[kPerLane];
-    uint64_t key[kPerLane];  // (sortable key, ~index); 0: none, or taken
+struct ChooseArgs {
+    const float *logits, *bias;
+    int tokens, experts, k, scoring, normalize;
+    float scale;
+    float* weights;
+    int* ids;
+};
+
+// One wave a token, expert 64 j + lane in slot j: scores, k rounds of (largest key, lowest index), weights.
+template <int kSlots>
+__device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane) {
+    float score[kSlots];
+    uint32_t key[kSlots];  // sortable; 0: none, or taken (the least of real keys, -inf, is above 0)
     float top = -__builtin_inff();
-    const float* row = logits + static_cast<int64_t>(token) * experts;
+    const float* row = p.logits + static_cast<int64_t>(token) * p.experts;
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
+    for (int j = 0; j < kSlots; ++j) {
         const int e = 64 * j + lane;
-        score[j] = e < experts ? row[e] : -__builtin_inff();
-        key[j] = 0;
-        if (e < experts) {
-            key[j] = static_cast<uint64_t>(sortable(score[j])) << 32 | static_cast<uint32_t>(~e);
-            top = fmaxf(top, score[j]);
-        }
+        const bool in = e < p.experts;
+        score[j] = in ? row[e] : -__builtin_inff();
+        key[j] = in ? sortable(score[j]) : 0u;
+        top = fmaxf(top, score[j]);
     }
-    if (scoring == 0) {  // softmax over all experts
+    if (p.scoring == 0) {  // softmax over all experts
         top = wave_max(top);
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j)
-            if (64 * j + lane < experts) {
-                score[j] = expf(score[j] - top);
-                sum += score[j];
-            }
+        for (int j = 0; j < kSlots; ++j) {
+            score[j] = 64 * j + lane < p.experts ? expf(score[j] - top) : 0.f;
+            sum += score[j];
+        }
         sum = wave_sum(sum);
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) score[j] /= sum;
+        for (int j = 0; j < kSlots; ++j) score[j] /= sum;
     } else {
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) score[j] = 1.0f / (1.0f + expf(-score[j]));
+        for (int j = 0; j < kSlots; ++j) score[j] = 1.0f / (1.0f + expf(-score[j]));
     }
-    if (bias) {
+    if (p.bias) {
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) {
+        for (int j = 0; j < kSlots; ++j) {
             const int e = 64 * j + lane;
-            if (e < experts)
-                key[j] = static_cast<uint64_t>(sortable(score[j] + bias[e])) << 32 | static_cast<uint32_t>(~e);
+            if (e < p.experts) key[j] = sortable(score[j] + p.bias[e]);
         }
     }
-    float chosen = 0.f;  // lane j < k: weight of the j-th
+    float chosen = 0.f, total = 0.f;  // lane r: weight and expert of the r-th
     int id = 0;
-    float total = 0.f;
-    for (int r = 0; r < k; ++r) {
-        uint64_t best = 0;
-        float s = 0.f;
+    for (int r = 0; r < p.k; ++r) {
+        uint32_t best = 0;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j)
-            if (key[j] > best) {
-                best = key[j];
+        for (int j = 0; j < kSlots; ++j) best = key[j] > best ? key[j] : best;
+        best = wave_max(best);
+        uint64_t at = 0;
+        float s = 0.f;
+        int e = 0;
+#pragma unroll
+        for (int j = kSlots - 1; j >= 0; --j) {  // the lowest slot that holds it, and there the lowest lane
+            const uint64_t has = __ballot(key[j] == best);
+            if (has) {
+                at = has;
+                e = 64 * j;
                 s = score[j];
             }
-        uint64_t all = best;
-        for (int h = 1; h < 64; h <<= 1) {
-            const uint64_t o = static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(all), h));
-            all = o > all ? o : all;
         }
-        const int e = static_cast<int>(~static_cast<uint32_t>(all));
-        s = __shfl(s, e & 63);  // the winner's lane holds it
+        const int winner = __builtin_ctzll(at);
+        s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), winner));
+        e += winner;
         if (lane == r) {
             chosen = s;
             id = e;
         }
         total += s;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j)
-            if (key[j] == all) key[j] = 0;
+        for (int j = 0; j < kSlots; ++j)
+            if (64 * j + lane == e) key[j] = 0;
     }
-    if (lane < k) {
-        if (normalize) chosen /= total;
-        weights[static_cast<int64_t>(token) * k + lane] = chosen * scale;
-        ids[static_cast<int64_t>(token) * k + lane] = id;
+    if (lane < p.k) {
+        if (p.normalize) chosen /= total;
+        p.weights[static_cast<int64_t>(token) * p.k + lane] = chosen * p.scale;
+        p.ids[static_cast<int64_t>(token) * p.k + lane] = id;
     }
+}
+
+template <int kSlots>
+__global__ __launch_bounds__(64) void choose_kernel(const ChooseArgs p) {
+    choose<kSlots>(p, blockIdx.x, threadIdx.x);
 }
 
 // Rows 0 .. n - 1 by key, in one workgroup: counts, offsets, chunks of at most chunk_rows, then the rows of each key.
@@ -264,8 +301,14 @@ extern "C" int qsrt_route(const void* x, int64_t x_ld, const void* weight, int64
                            static_cast<const _Float16*>(x), x_ld, static_cast<const _Float16*>(weight), weight_ld,
                            static_cast<int>(tokens), static_cast<int>(hidden), static_cast<int>(experts), logits);
     QSRT_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(choose_kernel, dim3(static_cast<unsigned>((tokens + 3) / 4)), dim3(256), 0, stream, logits, bias,
-                       static_cast<int>(tokens), static_cast<int>(experts), k, scoring, normalize, scale, weights, ids);
+    const ChooseArgs ca{logits, bias, static_cast<int>(tokens), static_cast<int>(experts), k, scoring, normalize, scale,
+                        weights, ids};
+    hipLaunchKernelGGL((experts <= 64    ? choose_kernel<1>
+                        : experts <= 128 ? choose_kernel<2>
+                        : experts <= 256 ? choose_kernel<4>
+                        : experts <= 512 ? choose_kernel<8>
+                                         : choose_kernel<16>),
+                       dim3(static_cast<unsigned>(tokens)), dim3(64), 0, stream, ca);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
