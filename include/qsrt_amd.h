@@ -458,7 +458,7 @@ typedef struct qsrt_packed_matrix {
  * [tokens, k].  hidden and both leading dimensions multiples of 8, rows
  * 16-byte aligned; experts <= 1024, k <= min(64, experts).
  */
-size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t experts);
+size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t hidden, int64_t experts);
 int qsrt_route(const void *x, int64_t x_ld, const void *weight, int64_t weight_ld, int dtype, int64_t tokens,
                int64_t hidden, int64_t experts, int k, const float *bias, int scoring, int normalize, float scale,
                float *weights, int32_t *ids, void *ws, size_t ws_bytes, void *stream);
@@ -480,6 +480,17 @@ int qsrt_packed_moe(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, 
                     const uint8_t *const *luts, int64_t experts, int activation, const void *x, int64_t x_ld, int dtype,
                     int64_t tokens, int k, const int32_t *ids, const float *weights, void *out, int64_t out_ld, void *ws,
                     size_t ws_bytes, void *stream);
+
+/*
+ * The whole layer: qsrt_route's choice (weights and ids are outputs, the
+ * router's weight [experts, hidden] in x's type), then qsrt_packed_moe, in
+ * fewer launches.  x rows 16-byte aligned; the same workspace.
+ */
+int qsrt_packed_moe_layer(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, const qsrt_packed_matrix *w2,
+                          const uint8_t *const *luts, int64_t experts, int activation, const void *router,
+                          int64_t router_ld, const float *bias, int scoring, int normalize, float scale, const void *x,
+                          int64_t x_ld, int dtype, int64_t tokens, int k, float *weights, int32_t *ids, void *out,
+                          int64_t out_ld, void *ws, size_t ws_bytes, void *stream);
 
 /*
  * A packed projection with low-rank adapters, each row its own or none:

@@ -111,7 +111,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_void_p, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     ),
-    "qsrt_route_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "qsrt_route_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "qsrt_route": (
         _c_int,
         [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p, _c_int, _c_int,
@@ -122,6 +122,12 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_int,
          _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
+    ),
+    "qsrt_packed_moe_layer": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_void_p, _c_int, _c_int,
+         ctypes.c_float, _c_void_p, _c_i64, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
+         _c_size, _c_void_p],
     ),
     "qsrt_adapter_linear_workspace_bytes": (_c_size, [_c_void_p, _c_i64, _c_i64, _c_i64]),
     "qsrt_adapter_linear": (

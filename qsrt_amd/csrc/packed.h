@@ -18,10 +18,22 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// Rotated rows in memory: a row of K channels is K / 32 strips of 128 bytes, one for 32 payload rows: the strip's 32 hi
-// pieces, then its 32 lo pieces, both in the order in which a lane of the product takes them: for lane group g = 0..3 the
-// eight channels 16 h + {2g, 2g + 1, 2g + 8, 2g + 9}, h = 0, 1 (the rows that a trellis window of a tile covers).
-constexpr int kStripBytes = 128;
+// Rotated rows in memory.  A row of K channels is K / 32 strips, one for 32 payload rows: 32 hi pieces and 32 lo pieces, each
+// as four times 16 bytes, what a lane of the product takes: for lane group g = 0..3 the eight channels 16 h + {2g, 2g + 1,
+// 2g + 8, 2g + 9}, h = 0, 1 (the rows that a trellis window of a tile covers).  A few rows lie one after another; more are
+// laid out by 16, [16 rows][strip][hi, lo][g][row][16 bytes], so that a wave's load is one stretch (rows apart by a
+// multiple of 4 KiB came from one L2 channel: a 2048 x 5120 x 1536 product took 125 us).
+struct RowLayout {
+    int row, strip, piece, group;  // bytes between neighbours
+    int64_t sixteen;               // bytes of 16 rows
+};
+constexpr int kStripBytes = 128;  // of one row
+__host__ __device__ inline RowLayout row_layout(int kb, bool grouped) {
+    const int64_t bytes = static_cast<int64_t>(kb) * 4 * kStripBytes;
+    return grouped ? RowLayout{16, 16 * kStripBytes, 1024, 256, 16 * bytes}
+                   : RowLayout{static_cast<int>(bytes), kStripBytes, 64, 16, 16 * bytes};
+}
+__host__ __device__ inline int64_t row_place(const RowLayout& l, int64_t row) { return (row >> 4) * l.sixteen + (row & 15) * l.row; }
 
 constexpr float kHadamardScale = 0.08838834764831845f;  // 128^-1/2
 
@@ -61,61 +73,107 @@ __device__ __forceinline__ void hadamard128(float& a, float& b, int lane) {
 #undef QSRT_STAGE
 }
 
-// Channels 2 lane, 2 lane + 1 of a rotated row's block of 128, split and stored in the product's order: channel rho of a
-// tile's 16 lies in lane group (rho % 8) / 2, at place (rho & 1) + 2 (rho / 8) of the tile's four.
-__device__ __forceinline__ void store_pieces(char* block, int lane, float a, float b) {
+// Channels 2 lane, 2 lane + 1 of a rotated row's kb-th block of 128, split and stored in the product's order: channel rho of
+// a tile's 16 lies in lane group (rho % 8) / 2, at place (rho & 1) + 2 (rho / 8) of the tile's four.
+__device__ __forceinline__ void store_pieces(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
     const __bf16 h0 = static_cast<__bf16>(a), h1 = static_cast<__bf16>(b);
     const bf16x2 lo = {static_cast<__bf16>(a - static_cast<float>(h0)), static_cast<__bf16>(b - static_cast<float>(h1))};
     const int tile = lane >> 3, pair = lane & 7;  // channels 2 pair, 2 pair + 1 of the tile
-    char* dst = block + (tile >> 1) * kStripBytes + (pair & 3) * 16 + (tile & 1) * 8 + (pair >> 2) * 4;
+    char* dst = row + (4 * kb + (tile >> 1)) * l.strip + (pair & 3) * l.group + (tile & 1) * 8 + (pair >> 2) * 4;
     *reinterpret_cast<bf16x2*>(dst) = bf16x2{h0, h1};
-    *reinterpret_cast<bf16x2*>(dst + 64) = lo;
+    *reinterpret_cast<bf16x2*>(dst + l.piece) = lo;
 }
 
-// Rows of one key (an expert, an adapter) in groups that one wave multiplies at once.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Rows into a payload's basis: (x * suh) H in pieces.
+struct RotateArgs {
+    const void* x;  // [rows / x_div][ld]
+    int64_t ld;
+    const _Float16* suh[2];
+    int64_t suh_stride[2];
+    const int* ids;  // null: one scale vector for all; else row r of the result is row r / x_div of x at scale ids[r]
+    int x_div;
+    char* out[2];
+    int64_t rows;
+    int kb, nmat;
+    RowLayout layout;
+};
+
+inline int64_t rotate_waves(const RotateArgs& p) { return (p.rows + 15) / 16 * 16 * p.kb * p.nmat; }
+
+// The `wave`-th 128 channels of a row and matrix; neighbouring waves have the same channels of neighbouring rows.
+template <typename T>
+__device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, int lane) {
+    const int64_t sixteen = wave >> 4, rest = sixteen / p.kb;
+    const int kb = static_cast<int>(sixteen - rest * p.kb);
+    const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+    const int64_t row = 16 * (p.nmat == 2 ? rest >> 1 : rest) + (wave & 15);
+    if (row >= p.rows) return;
+    const int id = p.ids ? max(p.ids[row], 0) : 0;
+    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + id * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
+    const T* x = static_cast<const T*>(p.x) + (p.x_div == 1 ? row : row / p.x_div) * p.ld + 128 * kb;
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 xv = reinterpret_cast<const t2*>(x)[lane];
+    const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];
+    float a = static_cast<float>(xv[0]) * static_cast<float>(sv[0]);
+    float b = static_cast<float>(xv[1]) * static_cast<float>(sv[1]);
+    hadamard128(a, b, lane);
+    store_pieces((mat ? p.out[1] : p.out[0]) + row_place(p.layout, row), p.layout, kb, lane, a * kHadamardScale,
+                 b * kHadamardScale);
+}
+
+// At most chunk_rows rows of one key (an expert, an adapter): order[first .. first + count), the first of them row0.
+// Chunks follow one another; the table's rest has count 0.
 struct Chunk {
-    int key, first, count, pad;  // rows order[first .. first + count)
+    int key, first, count, row0;
 };
-
-// Head of a grouping: what the host cannot know when it launches what reads it.
-struct GroupHead {
-    int chunks;
-    int parts[2];  // parts that the K axis of a layer's first and second product is cut into
-    int pad;
-};
-
-// Cuts the K axis (`strips`) of `units` products into parts so that `waves` waves come out even: the fewest strips in turn
-// on one wave, with two strips' time for what an item costs beside them.  A whole wave asks; every lane gets the answer.
-__device__ __forceinline__ int choose_parts(int64_t units, int strips, int max_parts, int waves, int lane) {
-    int64_t best = INT64_MAX;
-    for (int s = lane + 1; s <= min(max_parts, strips); s += 64) {
-        if (units * s >= int64_t(1) << 31) break;  // the product counts its items in 32 bits
-        const int64_t rounds = (units * s + waves - 1) / waves;
-        const int64_t cost = rounds * ((strips + s - 1) / s + 2) << 16 | s;  // ties: the fewest parts
-        best = cost < best ? cost : best;
-    }
-    for (int h = 1; h < 64; h <<= 1) {
-        const int64_t o = __shfl_xor(static_cast<long long>(best), h);
-        best = o < best ? o : best;
-    }
-    return best == INT64_MAX ? 1 : static_cast<int>(best & 0xFFFF);
-}
+typedef const __attribute__((address_space(4))) Chunk* ConstChunk;  // constant for the kernels that read them
 
 struct GroupArgs {
     const int* ids;
     int n, keys;
-    bool none;       // rows without a key form a group of their own (key -1)
-    int chunk_rows;
-    GroupHead* head;
+    bool none;  // rows without a key form a group of their own (key -1)
+    int chunk_rows, max_chunks;
     Chunk* chunks;
     int* order;
-    int* clean;      // ids with everything outside [0, keys) as -1
-    int units[2], strips[2], max_parts[2];  // per product: column blocks (times matrices) a chunk has, K axis, limit
-    int waves;
+    int* clean;  // ids with everything outside [0, keys) as -1
 };
 
 constexpr int kMaxKeys = 8191;  // their counters fit LDS
 
-int launch_group(const GroupArgs& args, hipStream_t stream);
+// Chunks that n rows can make at the most.
+inline int64_t most_chunks(int64_t n, int64_t keys, int64_t chunk_rows) {
+    const int64_t full = (n + chunk_rows - 1) / chunk_rows;
+    return n < full + keys ? n : full + keys;
+}
+
+// Groups, and rotates beside it what does not need the groups (rows 0: nothing).
+int launch_group(const GroupArgs& args, const RotateArgs& beside, int dtype, hipStream_t stream);
+
+// Router of `tokens` rows, with what else of a layer can run beside it: the rotation of the same rows (rows 0: none), and
+// the grouping of the chosen experts (null: none).
+struct RouterArgs {
+    const void* x;
+    int64_t x_ld;
+    const void* weight;
+    int64_t weight_ld;
+    int dtype;
+    int tokens, hidden, experts, k;
+    const float* bias;
+    int scoring, normalize;
+    float scale;
+    float* weights;
+    int* ids;
+    float* logits;
+};
+const char* router_fault(const RouterArgs& args);
+size_t router_logit_bytes(int64_t tokens, int64_t hidden, int64_t experts);
+int launch_router(const RouterArgs& args, const RotateArgs& beside, const GroupArgs* group, hipStream_t stream);
 
 }  // namespace qsrt

@@ -1,5 +1,6 @@
 // Products of a few rows with packed trellis matrices, and what stands around them in a mixture-of-experts layer.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "packed.h"
@@ -19,12 +20,11 @@ struct ProductArgs {
     const int64_t* records[2];    // per record: first word << 3 | bits
     int64_t record_stride[2];     // 0: one table for every key
     const char* x[2];             // rotated rows
+    RowLayout layout;
     int x_div;                    // row of order entry o: o / x_div
-    const GroupHead* head;        // null: chunks are runs of kRows rows of `rows`
-    const Chunk* chunks;
+    const Chunk* chunks;          // null: runs of kRows rows of `rows`
     const int* order;
-    int which;                    // head->parts[which]
-    int parts;                    // without a head
+    int max_chunks, parts;
     const uint8_t* lut[2];
     int lut_bits[2];
     int luts;
@@ -35,13 +35,6 @@ struct ProductArgs {
 };
 
 typedef const __attribute__((address_space(1))) bf16x8* gbf8;
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
-    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-}
 
 // The label tables come to LDS while a wave looks up its first item and asks for its first words; one barrier a wave.
 struct Tables {
@@ -61,8 +54,8 @@ struct Tables {
 // the same instructions with other shifts, where a body for each rate made the compiler keep a second set of sums.
 template <int G>
 __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_bytes, int strips, int K,
-                                                const char* (&x)[G], const uint8_t* lut, int lane, Tables& tables,
-                                                f32x4 (&acc)[G][8]) {
+                                                const char* (&x)[G], int x_strip, int x_piece, const uint8_t* lut,
+                                                int lane, Tables& tables, f32x4 (&acc)[G][8]) {
     const int m = lane & 15, g = lane >> 4;
     int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;
     if (b0 < 0) b0 += 256 * K;
@@ -89,8 +82,8 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
 #pragma unroll
         for (int q = 0; q < G; ++q) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) b[q][p] = *(gbf8)(x[q] + p * 64);
-            x[q] += kStripBytes;
+            for (int p = 0; p < 2; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
+            x[q] += x_strip;
         }
         uint32_t next[16];
         auto gather = [&](int t) {
@@ -111,6 +104,7 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
 #pragma unroll
             for (int j = 0; j < 16; ++j) label[j] = next[j];
             if (t < 3) gather(t + 1);
+            bf16x8 av[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 u32x4 a;
@@ -121,13 +115,16 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
                         uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
                                       __builtin_amdgcn_perm(label[j + 1], label[j], 0x0C0C0400u), 1.0f, false));
                 }
-                const bf16x8 av = __builtin_bit_cast(bf16x8, a);
-#pragma unroll
-                for (int q = 0; q < G; ++q) {
-                    acc[q][2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[q][0], acc[q][2 * t + u], 0, 0, 0);
-                    acc[q][2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[q][1], acc[q][2 * t + u], 0, 0, 0);
-                }
+                av[u] = __builtin_bit_cast(bf16x8, a);
             }
+#pragma unroll
+            for (int p = 0; p < 2; ++p)  // hi pieces of all sums, then lo: a sum's two products do not follow each other
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int q = 0; q < G; ++q)
+                        acc[q][2 * t + u] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[u], b[q][p], acc[q][2 * t + u], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);  // two pairs' labels in registers at most
         }
     } while (++s < strips);
@@ -146,27 +143,52 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 
     constexpr int kRows = 16 * G;
     const int n = lane & 15, g = lane >> 4;
-    const int chunks = p.head ? uniform(p.head->chunks) : (p.rows + kRows - 1) / kRows;
-    const int parts = p.head ? uniform(p.head->parts[p.which]) : p.parts;
-    const uint32_t items = static_cast<uint32_t>(chunks) * p.nmat * p.nb * parts;  // below 2^31: see choose_parts
-    const int64_t row_bytes = static_cast<int64_t>(p.kb) * 4 * kStripBytes;
+    const int parts = p.parts;
+    const uint32_t items = static_cast<uint32_t>(p.max_chunks) * p.nmat * p.nb * parts;  // below 2^31: see cut_parts
     const int64_t cols = 128 * static_cast<int64_t>(p.nb);
     const int strips = 4 * p.kb;
 
-    for (uint32_t item = blockIdx.x * kWaves + w; item < items; item += gridDim.x * kWaves) {
-        uint32_t rest = item / parts;
-        const int part = static_cast<int>(item - rest * parts);
-        const int cb = static_cast<int>(rest % p.nb);
-        rest /= p.nb;
-        const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
-        const int ci = static_cast<int>(p.nmat == 2 ? rest >> 1 : rest);
-        int key = 0, first = ci * kRows, count;
-        if (p.head) {
-            key = uniform(p.chunks[ci].key);
-            first = uniform(p.chunks[ci].first);
-            count = uniform(p.chunks[ci].count);
+    // Rounds of an item a wave.
+    const uint32_t grid = gridDim.x, per_round = grid * kWaves;
+    uint32_t turn = blockIdx.x + 37 * w;
+    for (uint32_t base = 0; base < items; base += per_round, turn += 101) {
+        uint32_t item;
+        int part, cb, mat, ci;
+        if constexpr (G == 1) {
+            // One group of rows: the items of a round are dealt out to the workgroups one by one.  The deal is turned from
+            // wave to wave and round to round: column blocks come in a period that divides the grid's, and a workgroup that
+            // only ever met the blocks of the highest rate would finish last (7168 x 2048 at K3 and K4 records: 1.84 ms
+            // where 1.54 will do).
+            item = base + w * grid + turn % grid;
+            if (item >= items) break;
+            uint32_t rest = item / parts;
+            part = static_cast<int>(item - rest * parts);
+            cb = static_cast<int>(rest % p.nb);
+            rest /= p.nb;
+            mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+            ci = static_cast<int>(p.nmat == 2 ? rest >> 1 : rest);
         } else {
-            count = min(kRows, p.rows - first);
+            // Many rows: a strip of them is more than the payload's, so neighbouring waves, and the workgroups of one
+            // chiplet (blockIdx.x % 8), take the column blocks of the same rows and find these in their caches.
+            const uint32_t eighth = grid >> 3;
+            const uint32_t b = (grid & 7) ? blockIdx.x : (blockIdx.x & 7) * eighth + (blockIdx.x >> 3);
+            item = base + (items - base >= per_round ? b * kWaves + w : w * grid + b);
+            if (item >= items) break;
+            uint32_t rest = item / p.nb;
+            cb = static_cast<int>(item - rest * p.nb);
+            mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+            if (p.nmat == 2) rest >>= 1;
+            ci = static_cast<int>(rest / parts);
+            part = static_cast<int>(rest - ci * parts);
+        }
+        int key = 0, first = ci * kRows, count = min(kRows, p.rows - first), row0 = first;
+        if (p.chunks) {
+            const ConstChunk c = (ConstChunk)p.chunks + ci;
+            key = c->key;
+            first = c->first;
+            count = c->count;
+            row0 = c->row0;
+            if (count == 0) break;  // the last chunk is behind
         }
         int s = strips * part / parts;
         const int end = strips * (part + 1) / parts;
@@ -175,8 +197,9 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 #pragma unroll
         for (int q = 0; q < G; ++q) {  // lanes past the last row repeat it; their sums are not stored
             const int at = first + min(16 * q + n, count - 1);
-            row[q] = p.head ? p.order[at] : at;
-            x[q] = (mat ? p.x[1] : p.x[0]) + (p.x_div == 1 ? row[q] : row[q] / p.x_div) * row_bytes + 16 * g + s * kStripBytes;
+            row[q] = !p.chunks ? at : count == 1 ? row0 : p.order[at];
+            x[q] = (mat ? p.x[1] : p.x[0]) + row_place(p.layout, p.x_div == 1 ? row[q] : row[q] / p.x_div) +
+                   g * p.layout.group + s * p.layout.strip;
         }
         f32x4 acc[G][8];
 #pragma unroll
@@ -186,15 +209,17 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 
         const char* words =
             reinterpret_cast<const char*>((mat ? p.words[1] : p.words[0]) + key * (mat ? p.key_stride[1] : p.key_stride[0]));
-        const int64_t* records = (mat ? p.records[1] : p.records[0]) + key * (mat ? p.record_stride[1] : p.record_stride[0]);
+        typedef const __attribute__((address_space(4))) int64_t* ConstRecord;
+        const ConstRecord records = (ConstRecord)(mat ? p.records[1] : p.records[0]) +
+                                    key * (mat ? p.record_stride[1] : p.record_stride[0]);
         while (s < end) {  // runs of one rate
             const int r = p.axis ? cb : s >> 2;
-            const int64_t rec = uniform(records[r]);
+            const int64_t rec = records[r];
             const int bits = static_cast<int>(rec & 7);
             int stop = end;
             if (!p.axis) {  // records of one rate that follow one another are one strip of tiles
                 int r1 = r + 1;
-                while (4 * r1 < end && (uniform(static_cast<int>(records[r1])) & 7) == bits) ++r1;
+                while (4 * r1 < end && static_cast<int>(records[r1] & 7) == bits) ++r1;
                 stop = min(end, 4 * r1);
             }
             const int tile = 32 * bits;
@@ -204,10 +229,10 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                                         : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
             if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
                 const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
-                multiply_strips<G>(tiles, tile_row, stop - s, bits, x, lut, lane, tables, acc);
+                multiply_strips<G>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
             } else {  // another pass has this rate
 #pragma unroll
-                for (int q = 0; q < G; ++q) x[q] += (stop - s) * kStripBytes;
+                for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
             }
             s = stop;
         }
@@ -229,38 +254,9 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 // Rows into the payload's basis
 // ---------------------------------------------------------------------------
 
-struct RotateArgs {
-    const void* x;  // [rows][ld]
-    int64_t ld;
-    const _Float16* suh[2];
-    int64_t suh_stride[2];
-    const int* ids;  // null: one scale vector for all; else row r of the result is row r / x_div of x at scale ids[r]
-    int x_div;
-    char* out[2];
-    int rows, kb, nmat;
-};
-
-// One wave for 128 channels of one row and one matrix.
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
-    const int kb = static_cast<int>(wave % p.kb);
-    const int64_t rest = wave / p.kb;
-    const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
-    const int64_t row = p.nmat == 2 ? rest >> 1 : rest;
-    if (row >= p.rows) return;
-    const int id = p.ids ? max(p.ids[row], 0) : 0;
-    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + id * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
-    const T* x = static_cast<const T*>(p.x) + (row / p.x_div) * p.ld + 128 * kb;
-    typedef T t2 __attribute__((ext_vector_type(2)));
-    const t2 xv = reinterpret_cast<const t2*>(x)[lane];
-    const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];
-    float a = static_cast<float>(xv[0]) * static_cast<float>(sv[0]);
-    float b = static_cast<float>(xv[1]) * static_cast<float>(sv[1]);
-    hadamard128(a, b, lane);
-    store_pieces((mat ? p.out[1] : p.out[0]) + (row * p.kb + kb) * 4 * kStripBytes, lane, a * kHadamardScale,
-                 b * kHadamardScale);
+    rotate_block<T>(p, static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6)), threadIdx.x & 63);
 }
 
 // ---------------------------------------------------------------------------
@@ -268,15 +264,16 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs p) {
 // ---------------------------------------------------------------------------
 
 struct MiddleArgs {
-    const float* part;  // [passes * parts][2][pairs][inter]
-    const GroupHead* head;
+    const float* part;  // [parts][2][pairs][inter]
+    int parts;
     const int* ids;
     const _Float16* svh[2];
     int64_t svh_stride[2];
     const _Float16* suh;  // of the second product
     int64_t suh_stride;
     char* out;
-    int pairs, ib, passes, act;
+    RowLayout layout;
+    int pairs, ib, act;
 };
 
 __device__ __forceinline__ float activate(float g, float u, int act) {
@@ -310,21 +307,39 @@ __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
     const int id = uniform(p.ids[pair]);
     if (id < 0) return;
     const int64_t inter = 128 * static_cast<int64_t>(p.ib), rows = static_cast<int64_t>(p.pairs) * inter;
-    const int parts = p.passes * uniform(p.head->parts[0]);
-    const float* src = p.part + pair * inter + 128 * ib + 2 * lane;
-    const f32x2 gs = sum_parts(src, 2 * rows, 0, 1, parts), us = sum_parts(src + rows, 2 * rows, 0, 1, parts);
-    float g0 = gs[0], g1 = gs[1], u0 = us[0], u1 = us[1];
-    hadamard128(g0, g1, lane);
-    hadamard128(u0, u1, lane);
     const f16x2 sg = reinterpret_cast<const f16x2*>(p.svh[0] + id * p.svh_stride[0] + 128 * ib)[lane];
     const f16x2 su = reinterpret_cast<const f16x2*>(p.svh[1] + id * p.svh_stride[1] + 128 * ib)[lane];
     const f16x2 sd = reinterpret_cast<const f16x2*>(p.suh + id * p.suh_stride + 128 * ib)[lane];
+    const float* src = p.part + pair * inter + 128 * ib + 2 * lane;
+    f32x2 gs = {0.f, 0.f}, us = {0.f, 0.f};
+    int s = 0;
+    for (; s + 8 <= p.parts; s += 8) {  // the loads of eight parts go out together
+        f32x2 v[8], t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = *reinterpret_cast<const f32x2*>(src + (s + j) * 2 * rows);
+            t[j] = *reinterpret_cast<const f32x2*>(src + ((s + j) * 2 + 1) * rows);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            gs += v[j];
+            us += t[j];
+        }
+    }
+#pragma unroll 4
+    for (; s < p.parts; ++s) {
+        gs += *reinterpret_cast<const f32x2*>(src + s * 2 * rows);
+        us += *reinterpret_cast<const f32x2*>(src + (s * 2 + 1) * rows);
+    }
+    float g0 = gs[0], g1 = gs[1], u0 = us[0], u1 = us[1];
+    hadamard128(g0, g1, lane);
+    hadamard128(u0, u1, lane);
     float a = activate(g0 * kHadamardScale * static_cast<float>(sg[0]), u0 * kHadamardScale * static_cast<float>(su[0]), p.act) *
               static_cast<float>(sd[0]);
     float b = activate(g1 * kHadamardScale * static_cast<float>(sg[1]), u1 * kHadamardScale * static_cast<float>(su[1]), p.act) *
               static_cast<float>(sd[1]);
     hadamard128(a, b, lane);
-    store_pieces(p.out + (pair * p.ib + ib) * 4 * kStripBytes, lane, a * kHadamardScale, b * kHadamardScale);
+    store_pieces(p.out + row_place(p.layout, pair), p.layout, ib, lane, a * kHadamardScale, b * kHadamardScale);
 }
 
 // ---------------------------------------------------------------------------
@@ -332,15 +347,15 @@ __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
 // ---------------------------------------------------------------------------
 
 struct CombineArgs {
-    const float* part;  // [passes * parts][pairs][hidden]
-    const GroupHead* head;
+    const float* part;  // [parts][pairs][hidden]
+    int parts;
     const int* ids;
     const float* weights;
     const _Float16* svh;
     int64_t svh_stride;
     void* out;
     int64_t ld;
-    int tokens, k, hb, passes;
+    int tokens, k, hb;
 };
 
 constexpr int kCombineWaves = 8;
@@ -354,7 +369,6 @@ __global__ __launch_bounds__(64 * kCombineWaves) void combine_kernel(const Combi
     const int hb = static_cast<int>(blockIdx.x % p.hb);
     const int64_t token = blockIdx.x / p.hb;
     const int64_t hidden = 128 * static_cast<int64_t>(p.hb), stride = static_cast<int64_t>(p.tokens) * p.k * hidden;
-    const int parts = p.passes * uniform(p.head->parts[1]);
     const bool shared = p.svh_stride == 0;
     auto rotated = [&](f32x2 v, const _Float16* svh) {
         float a = v[0], b = v[1];
@@ -367,7 +381,7 @@ __global__ __launch_bounds__(64 * kCombineWaves) void combine_kernel(const Combi
         const int64_t pair = token * p.k + j;
         const int id = uniform(p.ids[pair]);
         if (id < 0) continue;
-        f32x2 v = sum_parts(p.part + pair * hidden + 128 * hb + 2 * lane, stride, 0, 1, parts);
+        f32x2 v = sum_parts(p.part + pair * hidden + 128 * hb + 2 * lane, stride, 0, 1, p.parts);
         if (!shared) v = rotated(v, p.svh + id * p.svh_stride);
         y += v * p.weights[pair];
     }
@@ -391,11 +405,10 @@ struct ShrinkArgs {
     const void* x;
     int64_t ld;
     const void* a;  // [adapters][rank][k]
-    const GroupHead* head;
     const Chunk* chunks;
     const int* order;
     float* out;  // [parts][rows][rank]
-    int rows, k, rank, parts;
+    int max_chunks, rows, k, rank, parts;
 };
 
 // x A_a^T of 16 rows of one adapter over a part of the K axis, 16 kTiles ranks at a time; a wave each.  Products of the
@@ -404,17 +417,18 @@ template <typename T, int kTiles>
 __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int64_t nw = static_cast<int64_t>(gridDim.x) * 4;
-    const int64_t items = static_cast<int64_t>(uniform(p.head->chunks)) * p.parts * (p.rank / (16 * kTiles));
+    const int64_t items = static_cast<int64_t>(p.max_chunks) * p.parts * (p.rank / (16 * kTiles));
     const int steps = p.k / 32, groups = p.rank / (16 * kTiles);
     typedef T t8 __attribute__((ext_vector_type(8)));
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
          item < items; item += nw) {
         const int part = static_cast<int>(item % p.parts), rest = static_cast<int>(item / p.parts);
         const int group = rest % groups;
-        const Chunk c = p.chunks[rest / groups];
-        const int key = uniform(c.key);
+        const ConstChunk c = (ConstChunk)p.chunks + rest / groups;
+        const int key = c->key, count = c->count;
+        if (count == 0) break;  // the last chunk is behind
         if (key < 0) continue;
-        const int row = p.order[c.first + min(n, c.count - 1)];
+        const int row = p.order[c->first + min(n, count - 1)];
         const T* x = static_cast<const T*>(p.x) + row * p.ld + 8 * g;
         const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + 16 * kTiles * group + n) * p.k + 8 * g;
         f32x4 acc[kTiles];
@@ -444,7 +458,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
         int s = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts);
         for (; s + 4 <= s1; s += 4) steps_at(s, std::integral_constant<int, 4>{});
         for (; s < s1; ++s) steps_at(s, std::integral_constant<int, 1>{});
-        if (n >= c.count) continue;
+        if (n >= count) continue;
         float* out = p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank + 16 * kTiles * group + 4 * g;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
@@ -454,8 +468,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
 struct FinishArgs {
     const float* part;  // [parts][rows][cols]
     int parts;
-    const GroupHead* head;  // null: no adapters, chunks are runs of 16 rows
-    const Chunk* chunks;
+    const Chunk* chunks;  // null: no adapters, chunks are runs of 16 rows
     const int* order;
     const _Float16* svh;
     const float* low;  // [low_parts][rows][rank]
@@ -476,14 +489,13 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     __shared__ f32x2 sums[4][64];
     const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
     const int nb = static_cast<int>(blockIdx.x % p.nb), ci = static_cast<int>(blockIdx.x / p.nb);
-    if (ci >= (p.head ? uniform(p.head->chunks) : (p.rows + 15) / 16)) return;
-    int key = -1, first = 16 * ci, count;
-    if (p.head) {
-        key = uniform(p.chunks[ci].key);
-        first = uniform(p.chunks[ci].first);
-        count = uniform(p.chunks[ci].count);
-    } else {
-        count = min(16, p.rows - first);
+    int key = -1, first = 16 * ci, count = min(16, p.rows - first);
+    if (p.chunks) {
+        const ConstChunk c = (ConstChunk)p.chunks + ci;
+        key = c->key;
+        first = c->first;
+        count = c->count;
+        if (count == 0) return;
     }
     const int64_t cols = 128 * static_cast<int64_t>(p.nb), stride = p.rows * cols;
     const float* src = p.part + 128 * nb + 2 * lane;
@@ -492,7 +504,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     int mine = 0;  // rows of this wave
     if (count < 4) {
         for (int r = 0; r < count; ++r) {
-            const int at = p.head ? uniform(p.order[first + r]) : first + r;
+            const int at = p.chunks ? uniform(p.order[first + r]) : first + r;
             sums[w][lane] = sum_parts(src + at * cols, stride, w, 4, p.parts);
             __syncthreads();
             if (w == r) {
@@ -507,7 +519,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
         for (int i = 0; i < 4; ++i) {
             const int r = w + 4 * i;
             if (r >= count) break;
-            row[i] = p.head ? uniform(p.order[first + r]) : first + r;
+            row[i] = p.chunks ? uniform(p.order[first + r]) : first + r;
             v[i] = sum_parts(src + row[i] * cols, stride, 0, 1, p.parts);
             mine = i + 1;
         }
@@ -529,9 +541,19 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 low[i] = 0.f;
-                if (i < mine && r0 + lane < p.rank)
-                    for (int s = 0; s < p.low_parts; ++s)
-                        low[i] += p.low[(static_cast<int64_t>(s) * p.rows + row[i]) * p.rank + r0 + lane];
+                if (i < mine && r0 + lane < p.rank) {
+                    const float* src = p.low + static_cast<int64_t>(row[i]) * p.rank + r0 + lane;
+                    const int64_t step = static_cast<int64_t>(p.rows) * p.rank;
+                    int s = 0;
+                    for (; s + 8 <= p.low_parts; s += 8) {
+                        float t[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) t[j] = src[(s + j) * step];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) low[i] += t[j];
+                    }
+                    for (; s < p.low_parts; ++s) low[i] += src[s * step];
+                }
                 low[i] *= scale;
             }
             for (int r = 0; r < 64 && r0 + r < p.rank; r += 8) {
@@ -569,12 +591,31 @@ constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one produ
 template <int G, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
     constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
-    hipLaunchKernelGGL((product_kernel<G, kWaves, kTables>), dim3(cus), dim3(64 * kWaves), 0, stream, args);
+    const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nmat * args.nb * args.parts;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
+    hipLaunchKernelGGL((product_kernel<G, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
 
-int waves_of(int groups, int cus) { return cus * (groups == 1 ? 16 : 8); }
+// Parts that the K axis (`strips`) of `units` column blocks is cut into, chosen so that the compute units come out even: the
+// time of a strip on one is the table reads of its wave, shared by the unit's waves; with few waves their latencies show
+// (0.9 of a wave's time beside the reads of all: 16 waves decode 4.96e12 labels a second, 8 waves 4.73e12); and a part
+// costs its set-up, about a strip, and its sums' way to memory and back, 0.28 strips a row.  `most`: units there can be.
+int cut_parts(double units, int64_t most, int strips, int limit, int rows, int cus) {
+    int best = 1;
+    double least = 0.0;
+    for (int p = 1; p <= std::min(limit, strips); ++p) {
+        if (most * p >= int64_t(1) << 31) break;  // the product counts its items in 32 bits
+        const double turns = std::ceil(units * p / cus);
+        const double cost = (turns + 0.9) * ((strips + p - 1) / p + 1.0 + 0.28 * rows);
+        if (p == 1 || cost < least) {
+            least = cost;
+            best = p;
+        }
+    }
+    return best;
+}
 
 // All passes of a product: the tables of at most two rates fit LDS at once.
 int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
@@ -635,37 +676,48 @@ struct Carve {
 
 int part_limit(int64_t row_floats, int strips) {
     const int64_t fit = kMaxPartBytes / (row_floats * 4);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(fit, strips), 64)));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, strips)));
 }
 
+int64_t sixteens(int64_t rows) { return (rows + 15) / 16 * 16; }
+
 struct MoeSpace {
-    GroupHead* head;
     Chunk* chunks;
     int *order, *clean;
     char *x[2], *mid;
-    float* part;
-    int max_parts[2], passes[2], groups;
+    float *part, *logits;
+    int parts[2], passes[2], groups, max_chunks;
     size_t bytes;
 };
 
 MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inter, int64_t experts, int rates13, int rates2,
-                   bool shared) {
+                   bool shared, bool router, int cus) {
     MoeSpace s;
     const int64_t pairs = tokens * k;
     s.groups = pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;  // groups of 16 rows a wave multiplies at once
+    s.max_chunks = static_cast<int>(most_chunks(pairs, experts, 16 * s.groups));
+    // chunks to expect under an even router; the parts are cut for them, as the host does not wait for the real ones
+    const double touched = experts * (1.0 - std::pow(1.0 - 1.0 / experts, static_cast<double>(pairs)));
+    const double each = pairs / touched, chunks = std::max(1.0, touched * std::ceil(each / (16.0 * s.groups)));
+    const int rows = static_cast<int>(std::min<double>(16 * s.groups, std::ceil(each)));
     Carve c{static_cast<char*>(ws)};
-    s.head = c.take<GroupHead>(1);
-    s.chunks = c.take<Chunk>(pairs);
+    s.chunks = c.take<Chunk>(s.max_chunks);
     s.order = c.take<int>(pairs);
     s.clean = c.take<int>(pairs);
-    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>((shared ? tokens : pairs) * hidden * 4);
-    s.mid = c.take<char>(pairs * inter * 4);
+    s.logits = c.take<float>(router ? router_logit_bytes(tokens, hidden, experts) / sizeof(float) : 0);
+    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>(sixteens(shared ? tokens : pairs) * hidden * 4);
+    s.mid = c.take<char>(sixteens(pairs) * inter * 4);
     s.passes[0] = passes_of(rates13);
     s.passes[1] = passes_of(rates2);
-    s.max_parts[0] = part_limit(2 * pairs * inter * s.passes[0], static_cast<int>(hidden / 32));
-    s.max_parts[1] = part_limit(pairs * hidden * s.passes[1], static_cast<int>(inter / 32));
-    s.part = c.take<float>(std::max(s.max_parts[0] * s.passes[0] * 2 * pairs * inter,
-                                    s.max_parts[1] * s.passes[1] * pairs * hidden));
+    const int64_t row_floats[2] = {2 * pairs * inter * s.passes[0], pairs * hidden * s.passes[1]};
+    const int64_t units[2] = {2 * inter / 128, hidden / 128}, strips[2] = {hidden / 32, inter / 32};
+    int64_t floats = 0;
+    for (int i = 0; i < 2; ++i) {
+        s.parts[i] = cut_parts(chunks * units[i], s.max_chunks * units[i], static_cast<int>(strips[i]),
+                               part_limit(row_floats[i], static_cast<int>(strips[i])), rows, cus);
+        floats = std::max(floats, s.parts[i] * row_floats[i]);
+    }
+    s.part = c.take<float>(floats);
     s.bytes = c.used;
     return s;
 }
@@ -682,6 +734,16 @@ void set_matrix(ProductArgs& a, int i, const qsrt_packed_matrix* m) {
 
 unsigned blocks_of(int64_t waves) { return static_cast<unsigned>((waves + 3) / 4); }
 
+int launch_rotate(const RotateArgs& args, int dtype, hipStream_t stream) {
+    const dim3 grid(blocks_of(rotate_waves(args)));
+    if (dtype == 0)
+        hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, grid, dim3(256), 0, stream, args);
+    else
+        hipLaunchKernelGGL(rotate_rows_kernel<_Float16>, grid, dim3(256), 0, stream, args);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
 const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
                       const uint8_t* const* luts, int64_t experts, int64_t tokens, int k) {
     for (const qsrt_packed_matrix* m : {w1, w3, w2})
@@ -691,139 +753,150 @@ const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3
         return "w1, w3 [hidden, inter] and w2 [inter, hidden] do not match";
     if ((w1->suh_stride == 0) != (w3->suh_stride == 0)) return "w1 and w3 must both share their suh, or neither";
     if (experts < 1 || experts > kMaxKeys) return "experts must be 1 .. 8191";
-    if (k < 1 || tokens < 0 || tokens * k > (1 << 20)) return "tokens * k must be at most 2^20";
+    if (k < 1 || k > (1 << 20) || tokens < 0 || tokens > (1 << 20) || tokens * k > (1 << 20))
+        return "tokens * k must be at most 2^20";
+    if (tokens * k * std::max(2 * w1->cols, w1->rows) / 128 >= int64_t(1) << 31) return "too many tokens for these matrices";
     return nullptr;
 }
 
 }  // namespace
 
-extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
-                                                  const qsrt_packed_matrix* w2, int64_t experts, int64_t tokens, int k) {
-    if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0) return 0;
-    return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates,
-                     w1->suh_stride == 0).bytes;
-}
+namespace {
 
-extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
-                               const uint8_t* const* luts, int64_t experts, int activation, const void* x, int64_t x_ld,
-                               int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
-                               int64_t out_ld, void* ws, size_t ws_bytes, void* stream_) {
-    if (const char* e = moe_fault(w1, w3, w2, luts, experts, tokens, k)) return fail(kBadArgument, "qsrt_packed_moe: %s", e);
-    if (tokens == 0) return kOk;
-    const int64_t hidden = w1->rows, inter = w1->cols, pairs = tokens * k;
-    if (dtype != 0 && dtype != 1) return fail(kBadArgument, "qsrt_packed_moe: dtype must be 0 (bf16) or 1 (f16)");
-    if (activation != 0 && activation != 1) return fail(kBadArgument, "qsrt_packed_moe: unknown activation");
-    if (const char* e = rows_fault(x, x_ld, hidden, 8)) return fail(kBadArgument, "qsrt_packed_moe: x: %s", e);
-    if (const char* e = rows_fault(out, out_ld, hidden, 8)) return fail(kBadArgument, "qsrt_packed_moe: out: %s", e);
-    if (!ids || !weights) return fail(kBadArgument, "qsrt_packed_moe: null routing");
-    const bool shared = w1->suh_stride == 0;
-    const int rates13 = w1->rates | w3->rates;
-    const MoeSpace s = moe_space(ws, tokens, k, hidden, inter, experts, rates13, w2->rates, shared);
-    if (!ws || ws_bytes < s.bytes) return fail(kWorkspaceTooSmall, "qsrt_packed_moe: needs %zu workspace bytes", s.bytes);
+struct MoeCall {
+    const qsrt_packed_matrix *w1, *w3, *w2;
+    const uint8_t* const* luts;
+    int64_t experts;
+    int activation;
+    const void* x;
+    int64_t x_ld;
+    int dtype;
+    int64_t tokens;
+    int k;
+    const int32_t* ids;
+    const float* weights;
+    void* out;
+    int64_t out_ld;
+};
+
+// The experts of a layer; with a router (its logits' place is filled in here) also its choice.
+int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, size_t ws_bytes, hipStream_t stream) {
+    if (const char* e = moe_fault(c.w1, c.w3, c.w2, c.luts, c.experts, c.tokens, c.k))
+        return fail(kBadArgument, "%s: %s", name, e);
+    if (c.dtype != 0 && c.dtype != 1) return fail(kBadArgument, "%s: dtype must be 0 (bf16) or 1 (f16)", name);
+    if (c.activation != 0 && c.activation != 1) return fail(kBadArgument, "%s: unknown activation", name);
+    if (c.tokens == 0) return kOk;
+    const int64_t hidden = c.w1->rows, inter = c.w1->cols, pairs = c.tokens * c.k;
+    if (const char* e = rows_fault(c.x, c.x_ld, hidden, 8)) return fail(kBadArgument, "%s: x: %s", name, e);
+    if (const char* e = rows_fault(c.out, c.out_ld, hidden, 8)) return fail(kBadArgument, "%s: out: %s", name, e);
+    if (!c.ids || !c.weights) return fail(kBadArgument, "%s: null routing", name);
     int cus = 0;
     if (const int rc = current_cu_count(&cus)) return rc;
-    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const bool shared = c.w1->suh_stride == 0;
+    const int rates13 = c.w1->rates | c.w3->rates;
+    const MoeSpace s =
+        moe_space(ws, c.tokens, c.k, hidden, inter, c.experts, rates13, c.w2->rates, shared, router != nullptr, cus);
+    if (!ws || ws_bytes < s.bytes) return fail(kWorkspaceTooSmall, "%s: needs %zu workspace bytes", name, s.bytes);
 
     GroupArgs ga{};
-    ga.ids = ids;
+    ga.ids = c.ids;
     ga.n = static_cast<int>(pairs);
-    ga.keys = static_cast<int>(experts);
+    ga.keys = static_cast<int>(c.experts);
     ga.none = false;
     ga.chunk_rows = 16 * s.groups;
-    ga.head = s.head;
+    ga.max_chunks = s.max_chunks;
     ga.chunks = s.chunks;
     ga.order = s.order;
     ga.clean = s.clean;
-    ga.units[0] = 2 * static_cast<int>(inter / 128);
-    ga.units[1] = static_cast<int>(hidden / 128);
-    ga.strips[0] = static_cast<int>(hidden / 32);
-    ga.strips[1] = static_cast<int>(inter / 32);
-    for (int i = 0; i < 2; ++i) ga.max_parts[i] = s.max_parts[i];
-    ga.waves = waves_of(s.groups, cus);
-    if (const int rc = launch_group(ga, stream)) return rc;
-
     RotateArgs ra{};
-    ra.x = x;
-    ra.ld = x_ld;
-    ra.suh[0] = reinterpret_cast<const _Float16*>(w1->suh);
-    ra.suh[1] = reinterpret_cast<const _Float16*>(w3->suh);
-    ra.suh_stride[0] = w1->suh_stride;
-    ra.suh_stride[1] = w3->suh_stride;
+    ra.x = c.x;
+    ra.ld = c.x_ld;
+    ra.suh[0] = static_cast<const _Float16*>(c.w1->suh);
+    ra.suh[1] = static_cast<const _Float16*>(c.w3->suh);
+    ra.suh_stride[0] = c.w1->suh_stride;
+    ra.suh_stride[1] = c.w3->suh_stride;
     ra.ids = shared ? nullptr : s.clean;
-    ra.x_div = shared ? 1 : k;
+    ra.x_div = shared ? 1 : c.k;
     ra.out[0] = s.x[0];
     ra.out[1] = s.x[1];
-    ra.rows = static_cast<int>(shared ? tokens : pairs);
+    ra.rows = shared ? c.tokens : pairs;
     ra.kb = static_cast<int>(hidden / 128);
     ra.nmat = 2;
-    const dim3 rgrid(blocks_of(static_cast<int64_t>(ra.rows) * ra.kb * 2));
-    if (dtype == 0)
-        hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
-    else
-        hipLaunchKernelGGL(rotate_rows_kernel<_Float16>, rgrid, dim3(256), 0, stream, ra);
-    QSRT_HIP_TRY(hipGetLastError());
+    ra.layout = row_layout(ra.kb, s.groups > 1);
+    RotateArgs beside = ra;  // rows that all experts share are rotated beside the router or the grouping
+    if (!shared) beside.rows = 0;
+    if (router) {
+        router->logits = s.logits;
+        if (const char* e = router_fault(*router)) return fail(kBadArgument, "%s: %s", name, e);
+        if (const int rc = launch_router(*router, beside, &ga, stream)) return rc;
+    } else if (const int rc = launch_group(ga, beside, c.dtype, stream)) {
+        return rc;
+    }
+    if (!shared)
+        if (const int rc = launch_rotate(ra, c.dtype, stream)) return rc;
 
     ProductArgs pa{};
-    set_matrix(pa, 0, w1);
-    set_matrix(pa, 1, w3);
+    set_matrix(pa, 0, c.w1);
+    set_matrix(pa, 1, c.w3);
     pa.x[0] = s.x[0];
     pa.x[1] = s.x[1];
-    pa.x_div = shared ? k : 1;
-    pa.head = s.head;
+    pa.x_div = shared ? c.k : 1;
+    pa.layout = ra.layout;
     pa.chunks = s.chunks;
     pa.order = s.order;
-    pa.which = 0;
+    pa.max_chunks = s.max_chunks;
+    pa.parts = s.parts[0];
     pa.part = s.part;
     pa.nmat = 2;
     pa.rows = static_cast<int>(pairs);
-    if (const int rc = launch_product(pa, s.groups, rates13, luts, cus, stream)) return rc;
+    if (const int rc = launch_product(pa, s.groups, rates13, c.luts, cus, stream)) return rc;
 
     MiddleArgs ma{};
     ma.part = s.part;
-    ma.head = s.head;
+    ma.parts = s.parts[0] * s.passes[0];
     ma.ids = s.clean;
-    ma.svh[0] = reinterpret_cast<const _Float16*>(w1->svh);
-    ma.svh[1] = reinterpret_cast<const _Float16*>(w3->svh);
-    ma.svh_stride[0] = w1->svh_stride;
-    ma.svh_stride[1] = w3->svh_stride;
-    ma.suh = reinterpret_cast<const _Float16*>(w2->suh);
-    ma.suh_stride = w2->suh_stride;
+    ma.svh[0] = static_cast<const _Float16*>(c.w1->svh);
+    ma.svh[1] = static_cast<const _Float16*>(c.w3->svh);
+    ma.svh_stride[0] = c.w1->svh_stride;
+    ma.svh_stride[1] = c.w3->svh_stride;
+    ma.suh = static_cast<const _Float16*>(c.w2->suh);
+    ma.suh_stride = c.w2->suh_stride;
     ma.out = s.mid;
     ma.pairs = static_cast<int>(pairs);
     ma.ib = static_cast<int>(inter / 128);
-    ma.passes = s.passes[0];
-    ma.act = activation;
+    ma.layout = row_layout(ma.ib, s.groups > 1);
+    ma.act = c.activation;
     hipLaunchKernelGGL(middle_kernel, dim3(blocks_of(pairs * ma.ib)), dim3(256), 0, stream, ma);
     QSRT_HIP_TRY(hipGetLastError());
 
     ProductArgs pb{};
-    set_matrix(pb, 0, w2);
+    set_matrix(pb, 0, c.w2);
     pb.x[0] = s.mid;
     pb.x_div = 1;
-    pb.head = s.head;
+    pb.layout = ma.layout;
     pb.chunks = s.chunks;
     pb.order = s.order;
-    pb.which = 1;
+    pb.max_chunks = s.max_chunks;
+    pb.parts = s.parts[1];
     pb.part = s.part;
     pb.nmat = 1;
     pb.rows = static_cast<int>(pairs);
-    if (const int rc = launch_product(pb, s.groups, w2->rates, luts, cus, stream)) return rc;
+    if (const int rc = launch_product(pb, s.groups, c.w2->rates, c.luts, cus, stream)) return rc;
 
     CombineArgs ca{};
     ca.part = s.part;
-    ca.head = s.head;
+    ca.parts = s.parts[1] * s.passes[1];
     ca.ids = s.clean;
-    ca.weights = weights;
-    ca.svh = reinterpret_cast<const _Float16*>(w2->svh);
-    ca.svh_stride = w2->svh_stride;
-    ca.out = out;
-    ca.ld = out_ld;
-    ca.tokens = static_cast<int>(tokens);
-    ca.k = k;
+    ca.weights = c.weights;
+    ca.svh = static_cast<const _Float16*>(c.w2->svh);
+    ca.svh_stride = c.w2->svh_stride;
+    ca.out = c.out;
+    ca.ld = c.out_ld;
+    ca.tokens = static_cast<int>(c.tokens);
+    ca.k = c.k;
     ca.hb = static_cast<int>(hidden / 128);
-    ca.passes = s.passes[1];
-    const dim3 cgrid(static_cast<unsigned>(tokens * ca.hb)), cblock(64 * std::min(k, kCombineWaves));
-    if (dtype == 0)
+    const dim3 cgrid(static_cast<unsigned>(c.tokens * ca.hb)), cblock(64 * std::min(c.k, kCombineWaves));
+    if (c.dtype == 0)
         hipLaunchKernelGGL(combine_kernel<__bf16>, cgrid, cblock, 0, stream, ca);
     else
         hipLaunchKernelGGL(combine_kernel<_Float16>, cgrid, cblock, 0, stream, ca);
@@ -831,52 +904,69 @@ extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_m
     return kOk;
 }
 
+}  // namespace
+
+extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
+                                                  const qsrt_packed_matrix* w2, int64_t experts, int64_t tokens, int k) {
+    int cus = 0;
+    if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0 || current_cu_count(&cus))
+        return 0;
+    return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates, w1->suh_stride == 0,
+                     true, cus)
+        .bytes;
+}
+
+extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                               const uint8_t* const* luts, int64_t experts, int activation, const void* x, int64_t x_ld,
+                               int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
+                               int64_t out_ld, void* ws, size_t ws_bytes, void* stream) {
+    const MoeCall call{w1, w3, w2, luts, experts, activation, x, x_ld, dtype, tokens, k, ids, weights, out, out_ld};
+    return run_moe("qsrt_packed_moe", call, nullptr, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int qsrt_packed_moe_layer(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
+                                     const qsrt_packed_matrix* w2, const uint8_t* const* luts, int64_t experts,
+                                     int activation, const void* router, int64_t router_ld, const float* bias, int scoring,
+                                     int normalize, float scale, const void* x, int64_t x_ld, int dtype, int64_t tokens,
+                                     int k, float* weights, int32_t* ids, void* out, int64_t out_ld, void* ws,
+                                     size_t ws_bytes, void* stream) {
+    const MoeCall call{w1, w3, w2, luts, experts, activation, x, x_ld, dtype, tokens, k, ids, weights, out, out_ld};
+    if (tokens < 0 || tokens > (1 << 20) || !w1 || w1->rows > (1 << 22))
+        return fail(kBadArgument, "qsrt_packed_moe_layer: bad sizes");
+    RouterArgs r{x, x_ld, router, router_ld, dtype, static_cast<int>(tokens), static_cast<int>(w1->rows),
+                 static_cast<int>(experts), k, bias, scoring, normalize, scale, weights, ids, nullptr};
+    return run_moe("qsrt_packed_moe_layer", call, &r, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
 namespace {
 
 struct LinearSpace {
-    GroupHead* head;
     Chunk* chunks;
     int *order, *clean;
     char* x;
     float *low, *part;
-    int low_parts, parts, passes, groups;
+    int low_parts, parts, passes, groups, max_chunks;
     size_t bytes;
 };
 
 LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates, int64_t adapters, int64_t rank, int cus) {
-    LinearSpace s;
+    LinearSpace s{};
     Carve c{static_cast<char*>(ws)};
     s.groups = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     s.passes = passes_of(rates);
-    const int64_t chunks = (rows + 16 * s.groups - 1) / (16 * s.groups);
+    const int64_t group_rows = 16 * s.groups, chunks = (rows + group_rows - 1) / group_rows;
     const int strips = static_cast<int>(k / 32);
-    const int limit = part_limit(rows * n * s.passes, strips);
-    int64_t best = INT64_MAX;
-    s.parts = 1;
-    for (int p = 1; p <= limit; ++p) {  // as choose_parts
-        const int64_t rounds = (chunks * (n / 128) * p + waves_of(s.groups, cus) - 1) / waves_of(s.groups, cus);
-        const int64_t cost = rounds * ((strips + p - 1) / p + 2);
-        if (cost < best) {
-            best = cost;
-            s.parts = p;
-        }
-    }
-    s.low_parts = 1;
+    s.parts = cut_parts(static_cast<double>(chunks * (n / 128)), chunks * (n / 128), strips, part_limit(rows * n * s.passes, strips),
+                        static_cast<int>(std::min(rows, group_rows)), cus);
     if (adapters) {
-        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1);  // chunks of one adapter's rows
-        s.low_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / most, k / 256)));
-        s.head = c.take<GroupHead>(1);
-        s.chunks = c.take<Chunk>(rows);
+        s.max_chunks = static_cast<int>(most_chunks(rows, adapters + 1, 16));
+        s.low_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / s.max_chunks, k / 256)));
+        s.chunks = c.take<Chunk>(s.max_chunks);
         s.order = c.take<int>(rows);
         s.clean = c.take<int>(rows);
         s.low = c.take<float>(s.low_parts * rows * rank);
-    } else {
-        s.head = nullptr;
-        s.chunks = nullptr;
-        s.order = s.clean = nullptr;
-        s.low = nullptr;
     }
-    s.x = c.take<char>(rows * k * 4);
+    s.x = c.take<char>(sixteens(rows) * k * 4);
     s.part = c.take<float>(static_cast<int64_t>(s.parts) * s.passes * rows * n);
     s.bytes = c.used;
     return s;
@@ -904,6 +994,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a, b of a rank 16, 32 .. 128, scales and ids");
     if (rows == 0) return kOk;
     const int64_t k = w->rows, n = w->cols;
+    if (rows * (n / 128) >= int64_t(1) << 31) return fail(kBadArgument, "qsrt_adapter_linear: too many rows for this matrix");
     if (const char* e = rows_fault(x, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
     if (const char* e = rows_fault(out, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
     int cus = 0;
@@ -918,16 +1009,10 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     ra.suh[0] = reinterpret_cast<const _Float16*>(w->suh);
     ra.x_div = 1;
     ra.out[0] = s.x;
-    ra.rows = static_cast<int>(rows);
+    ra.rows = rows;
     ra.kb = static_cast<int>(k / 128);
     ra.nmat = 1;
-    const dim3 rgrid(blocks_of(rows * ra.kb));
-    if (dtype == 0)
-        hipLaunchKernelGGL(rotate_rows_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
-    else
-        hipLaunchKernelGGL(rotate_rows_kernel<_Float16>, rgrid, dim3(256), 0, stream, ra);
-    QSRT_HIP_TRY(hipGetLastError());
-
+    ra.layout = row_layout(ra.kb, rows > 4);
     if (adapters) {
         GroupArgs ga{};
         ga.ids = ids;
@@ -935,16 +1020,16 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         ga.keys = static_cast<int>(adapters);
         ga.none = true;
         ga.chunk_rows = 16;
-        ga.head = s.head;
+        ga.max_chunks = s.max_chunks;
         ga.chunks = s.chunks;
         ga.order = s.order;
         ga.clean = s.clean;
-        if (const int rc = launch_group(ga, stream)) return rc;
+        if (const int rc = launch_group(ga, ra, dtype, stream)) return rc;
         ShrinkArgs sa{};
         sa.x = x;
         sa.ld = x_ld;
         sa.a = a;
-        sa.head = s.head;
+        sa.max_chunks = s.max_chunks;
         sa.chunks = s.chunks;
         sa.order = s.order;
         sa.out = s.low;
@@ -953,7 +1038,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         sa.rank = static_cast<int>(rank);
         sa.parts = s.low_parts;
         const int tiles = rank % 64 == 0 ? 4 : rank % 32 == 0 ? 2 : 1;  // of 16 ranks a wave
-        const int64_t most = std::min(rows, (rows + 15) / 16 + adapters + 1) * s.low_parts * (rank / (16 * tiles));
+        const int64_t most = static_cast<int64_t>(s.max_chunks) * s.low_parts * (rank / (16 * tiles));
         const dim3 sgrid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most), 8 * cus)));
 #define QSRT_SHRINK(T)                                                                                  \
     hipLaunchKernelGGL((tiles == 4 ? shrink_kernel<T, 4> : tiles == 2 ? shrink_kernel<T, 2> : shrink_kernel<T, 1>), \
@@ -964,12 +1049,16 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
             QSRT_SHRINK(_Float16);
 #undef QSRT_SHRINK
         QSRT_HIP_TRY(hipGetLastError());
+    } else if (const int rc = launch_rotate(ra, dtype, stream)) {
+        return rc;
     }
 
     ProductArgs pa{};
     set_matrix(pa, 0, w);
     pa.x[0] = s.x;
     pa.x_div = 1;
+    pa.layout = ra.layout;
+    pa.max_chunks = static_cast<int>((rows + 16 * s.groups - 1) / (16 * s.groups));
     pa.parts = s.parts;
     pa.part = s.part;
     pa.nmat = 1;
@@ -979,7 +1068,6 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     FinishArgs fa{};
     fa.part = s.part;
     fa.parts = s.parts * s.passes;
-    fa.head = s.head;
     fa.chunks = s.chunks;
     fa.order = s.order;
     fa.svh = reinterpret_cast<const _Float16*>(w->svh);
@@ -992,7 +1080,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     fa.ld = out_ld;
     fa.rows = static_cast<int>(rows);
     fa.nb = static_cast<int>(n / 128);
-    const int64_t most = adapters ? std::min(rows, (rows + 15) / 16 + adapters + 1) : (rows + 15) / 16;
+    const int64_t most = adapters ? s.max_chunks : (rows + 15) / 16;
     const dim3 fgrid(static_cast<unsigned>(most * fa.nb));
     if (dtype == 0)
         hipLaunchKernelGGL(finish_kernel<__bf16>, fgrid, dim3(256), 0, stream, fa);

@@ -7,22 +7,33 @@
 namespace qsrt {
 namespace {
 
-// logits[t][e] = sum_h x[t][h] w[e][h].  One workgroup for 16 experts and 16 tokens; its 16 waves take every 16th step of
-// 32 channels, products exact and sums FP32 on the matrix cores, and add up in LDS in wave order.
-constexpr int kRouterWaves = 16;
+// logits[split][t][e] = sum over the split's channels of x[t][h] w[e][h].  One workgroup for 16 experts, 16 tokens and one
+// split; its four waves take every fourth step of 32 channels, products exact and sums FP32 on the matrix cores, and add up
+// in LDS in wave order.  The splits spread a token's router over the chip; workgroups behind them rotate the same rows.
+struct LogitsArgs {
+    const void *x, *w;
+    int64_t ld, w_ld;
+    int tokens, hidden, experts, splits, etiles, ttiles;
+    float* logits;
+    RotateArgs beside;
+};
 
 template <typename T>
-__global__ __launch_bounds__(64 * kRouterWaves) void router_logits_kernel(const T* __restrict__ x, int64_t ld,
-                                                                          const T* __restrict__ w, int64_t w_ld,
-                                                                          int tokens, int hidden, int experts,
-                                                                          float* __restrict__ logits) {
-    __shared__ f32x4 sums[kRouterWaves][64];
+__global__ __launch_bounds__(256) void router_logits_kernel(const LogitsArgs p) {
+    __shared__ f32x4 sums[4][64];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int e0 = 16 * blockIdx.x, t0 = 16 * blockIdx.y;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int routers = p.etiles * p.ttiles * p.splits;
+    if (static_cast<int>(blockIdx.x) >= routers) {
+        rotate_block<T>(p.beside, static_cast<int64_t>(blockIdx.x - routers) * 4 + wave, lane);
+        return;
+    }
+    const int e0 = 16 * (blockIdx.x % p.etiles), t0 = 16 * (blockIdx.x / p.etiles % p.ttiles);
+    const int split = blockIdx.x / (p.etiles * p.ttiles);
     typedef T t8 __attribute__((ext_vector_type(8)));
-    const T* wr = w + min(e0 + m, experts - 1) * w_ld + 8 * g;  // rows past the end repeat the last; not stored
-    const T* xr = x + min(t0 + m, tokens - 1) * ld + 8 * g;
+    // rows past the end repeat the last; not stored
+    const T* wr = static_cast<const T*>(p.w) + min(e0 + m, p.experts - 1) * p.w_ld + 8 * g;
+    const T* xr = static_cast<const T*>(p.x) + min(t0 + m, p.tokens - 1) * p.ld + 8 * g;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](t8 a, t8 b) {
         if constexpr (__is_same(T, __bf16))
@@ -30,9 +41,11 @@ __global__ __launch_bounds__(64 * kRouterWaves) void router_logits_kernel(const 
         else
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
     };
-    constexpr int kStep = 32 * kRouterWaves, kBatch = 7;
-    int h = 32 * wave;
-    for (; h + (kBatch - 1) * kStep + 32 <= hidden; h += kBatch * kStep) {  // a batch of loads in flight
+    constexpr int kStep = 32 * 4, kBatch = 7;
+    const int steps = (p.hidden + 31) / 32;
+    const int end = min(p.hidden, 32 * static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits));
+    int h = 32 * static_cast<int>(static_cast<int64_t>(steps) * split / p.splits) + 32 * wave;
+    for (; h + (kBatch - 1) * kStep + 32 <= end; h += kBatch * kStep) {  // a batch of loads in flight
         t8 a[kBatch], b[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -43,20 +56,26 @@ __global__ __launch_bounds__(64 * kRouterWaves) void router_logits_kernel(const 
         for (int j = 0; j < kBatch; ++j) multiply(a[j], b[j]);
     }
     const t8 zero = {};
-    for (; h < hidden; h += kStep) {
-        const bool in = h + 8 * g < hidden;  // hidden is a multiple of 8
+    for (; h < end; h += kStep) {
+        const bool in = h + 8 * g < end;  // hidden is a multiple of 8
         multiply(in ? *reinterpret_cast<const t8*>(wr + h) : zero, in ? *reinterpret_cast<const t8*>(xr + h) : zero);
     }
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave) return;
-#pragma unroll
-    for (int v = 1; v < kRouterWaves; ++v) acc += sums[v][lane];
+    acc = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
     const int t = t0 + m;
-    if (t >= tokens) return;
+    if (t >= p.tokens) return;
+    float* out = p.logits + (static_cast<int64_t>(split) * p.tokens + t) * p.experts + e0 + 4 * g;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (e0 + 4 * g + i < experts) logits[static_cast<int64_t>(t) * experts + e0 + 4 * g + i] = acc[i];
+        if (e0 + 4 * g + i < p.experts) out[i] = acc[i];
+}
+
+// Splits of the channels: workgroups for every compute unit, each wave with a batch of steps at the least.
+int router_splits(int64_t tokens, int64_t hidden, int64_t experts) {
+    const int64_t tiles = ((tokens + 15) / 16) * ((experts + 15) / 16);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, std::min<int64_t>(8, hidden / 512))));
 }
 
 constexpr int kMaxExperts = 1024;
@@ -96,24 +115,39 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 struct ChooseArgs {
     const float *logits, *bias;
-    int tokens, experts, k, scoring, normalize;
+    int tokens, experts, splits, k, scoring, normalize;
     float scale;
     float* weights;
     int* ids;
 };
 
 // One wave a token, expert 64 j + lane in slot j: scores, k rounds of (largest key, lowest index), weights.
+// `local`: a second place for the ids, in LDS (null: none).
 template <int kSlots>
-__device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane) {
+__device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane, int* local) {
     float score[kSlots];
     uint32_t key[kSlots];  // sortable; 0: none, or taken (the least of real keys, -inf, is above 0)
     float top = -__builtin_inff();
     const float* row = p.logits + static_cast<int64_t>(token) * p.experts;
+    const int64_t step = static_cast<int64_t>(p.tokens) * p.experts;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) score[j] = 0.f;
+    for (int q = 0; q < p.splits; q += 8) {  // the loads of eight splits go out together; slots past the last expert repeat it
+        float part[8][kSlots];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < kSlots; ++j)
+                part[i][j] = row[min(q + i, p.splits - 1) * step + min(64 * j + lane, p.experts - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < kSlots; ++j) score[j] += q + i < p.splits ? part[i][j] : 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-        const int e = 64 * j + lane;
-        const bool in = e < p.experts;
-        score[j] = in ? row[e] : -__builtin_inff();
+        const bool in = 64 * j + lane < p.experts;
+        if (!in) score[j] = -__builtin_inff();
         key[j] = in ? sortable(score[j]) : 0u;
         top = fmaxf(top, score[j]);
     }
@@ -174,12 +208,13 @@ __device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane)
         if (p.normalize) chosen /= total;
         p.weights[static_cast<int64_t>(token) * p.k + lane] = chosen * p.scale;
         p.ids[static_cast<int64_t>(token) * p.k + lane] = id;
+        if (local) local[token * p.k + lane] = id;
     }
 }
 
 template <int kSlots>
 __global__ __launch_bounds__(64) void choose_kernel(const ChooseArgs p) {
-    choose<kSlots>(p, blockIdx.x, threadIdx.x);
+    choose<kSlots>(p, blockIdx.x, threadIdx.x, nullptr);
 }
 
 // Rows 0 .. n - 1 by key, in one workgroup: counts, offsets, chunks of at most chunk_rows, then the rows of each key.
@@ -187,19 +222,49 @@ __global__ __launch_bounds__(64) void choose_kernel(const ChooseArgs p) {
 // A row whose key is outside [0, keys) is left out (clean = -1), or with `none` put under the key -1.
 constexpr int kGroupThreads = 1024;
 
-__global__ __launch_bounds__(kGroupThreads) void group_kernel(const GroupArgs p) {
-    extern __shared__ int lds[];
-    int* at = lds;  // [keys + 1]: counts, then next place
-    __shared__ int waves[2][kGroupThreads / 64];
+// Adds one to at[slot] for each active lane and returns the lane's place; lanes of the same slot share an addition for the
+// first few slots (long runs of one key), the rest add by themselves.
+__device__ __forceinline__ int take_place(int* at, int slot, bool active, int lane) {
+    int place = -1;
+    for (int round = 0; round < 4; ++round) {
+        const uint64_t left = __ballot(active);
+        if (!left) return place;
+        const int leader = __builtin_ctzll(left);
+        const int common = __builtin_amdgcn_readlane(slot, leader);
+        const bool same = active && slot == common;
+        const uint64_t group = __ballot(same);
+        int base = 0;
+        if (lane == leader) base = atomicAdd(&at[common], __popcll(group));
+        base = __builtin_amdgcn_readlane(base, leader);
+        if (same) {
+            place = base + __popcll(group & ((uint64_t(1) << lane) - 1));
+            active = false;
+        }
+    }
+    if (active) place = atomicAdd(&at[slot], 1);
+    return place;
+}
+
+struct GroupLds {
+    int waves[2][kGroupThreads / 64];
+    int ids[kGroupThreads], order[kGroupThreads];  // of up to kGroupThreads rows
+};
+
+// ids in l.ids already (`local`), or in memory.
+__device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds& l, bool local) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int slots = p.keys + 1;
+    const int slots = p.keys + 1, padded = (p.n + 63) & ~63;
+    const bool small = p.n <= kGroupThreads;
     for (int i = tid; i < slots; i += kGroupThreads) at[i] = 0;
     __syncthreads();
-    for (int i = tid; i < p.n; i += kGroupThreads) {
-        const int id = p.ids[i];
+    for (int i = tid; i < padded; i += kGroupThreads) {  // whole waves
+        const int id = i < p.n ? (local ? l.ids[i] : p.ids[i]) : -1;
         const bool ok = id >= 0 && id < p.keys;
-        p.clean[i] = ok ? id : -1;
-        if (ok || p.none) atomicAdd(&at[ok ? id : p.keys], 1);
+        if (i < p.n) {
+            p.clean[i] = ok ? id : -1;
+            if (small) l.ids[i] = id;
+        }
+        take_place(at, ok ? id : p.keys, i < p.n && (ok || p.none), lane);
     }
     __syncthreads();
     // each thread owns a run of keys
@@ -219,96 +284,149 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(const GroupArgs p)
         }
     }
     if (lane == 63) {
-        waves[0][wave] = rs;
-        waves[1][wave] = cs;
+        l.waves[0][wave] = rs;
+        l.waves[1][wave] = cs;
     }
     __syncthreads();
     int total = 0, r0 = rs - rows, c0 = cs - chunks;
     for (int q = 0; q < kGroupThreads / 64; ++q) {
         if (q < wave) {
-            r0 += waves[0][q];
-            c0 += waves[1][q];
+            r0 += l.waves[0][q];
+            c0 += l.waves[1][q];
         }
-        total += waves[1][q];
+        total += l.waves[1][q];
     }
-    for (int q = k0; q < k1; ++q) {
+    for (int q = k0, r = r0; q < k1; ++q) {  // counts become the next place
         const int count = at[q];
-        for (int c = 0; c < count; c += p.chunk_rows)
-            p.chunks[c0++] = Chunk{q == p.keys ? -1 : q, r0 + c, min(p.chunk_rows, count - c), 0};
-        at[q] = r0;
-        r0 += count;
+        at[q] = r;
+        r += count;
     }
     __syncthreads();
-    for (int i = tid; i < p.n; i += kGroupThreads) {
-        const int id = p.ids[i];
-        const bool ok = id >= 0 && id < p.keys;
-        if (ok || p.none) p.order[atomicAdd(&at[ok ? id : p.keys], 1)] = i;
-    }
-    if (wave < 2) {  // how to cut the K axis: wave 0 for the first product, wave 1 for the second
-        const int64_t units = static_cast<int64_t>(total) * p.units[wave];
-        const int parts = choose_parts(units, p.strips[wave], p.max_parts[wave], p.waves, lane);
-        if (lane == 0) {
-            p.head->parts[wave] = parts;
-            if (wave == 0) p.head->chunks = total;
+    for (int i = tid; i < padded; i += kGroupThreads) {
+        const int id = i < p.n ? (small ? l.ids[i] : p.ids[i]) : -1;
+        const bool ok = id >= 0 && id < p.keys, in = i < p.n && (ok || p.none);
+        const int place = take_place(at, ok ? id : p.keys, in, lane);
+        if (in) {
+            p.order[place] = i;
+            if (small) l.order[place] = i;
         }
     }
+    __syncthreads();
+    for (int q = k0; q < k1; ++q)  // and now the place behind the key's last row
+        for (const int end = at[q]; r0 < end; r0 = min(r0 + p.chunk_rows, end))
+            p.chunks[c0++] = Chunk{q == p.keys ? -1 : q, r0, min(p.chunk_rows, end - r0), small ? l.order[r0] : p.order[r0]};
+    for (int i = total + tid; i < p.max_chunks; i += kGroupThreads) p.chunks[i] = Chunk{-1, 0, 0, 0};
+}
+
+// One workgroup groups; those behind it rotate rows (the same that it groups, or others).
+template <typename T>
+__global__ __launch_bounds__(kGroupThreads) void group_kernel(const GroupArgs p, const RotateArgs beside) {
+    extern __shared__ int at[];  // [keys + 1]: counts, then places
+    __shared__ GroupLds l;
+    if (blockIdx.x == 0)
+        group_rows(p, at, l, false);
+    else
+        rotate_block<T>(beside, static_cast<int64_t>(blockIdx.x - 1) * (kGroupThreads / 64) +
+                                    uniform(static_cast<int>(threadIdx.x >> 6)), threadIdx.x & 63);
+}
+
+// Choice and grouping of at most 16 tokens in one workgroup: a wave chooses for each.
+template <int kSlots>
+__global__ __launch_bounds__(kGroupThreads) void choose_group_kernel(const ChooseArgs c, const GroupArgs p) {
+    extern __shared__ int at[];
+    __shared__ GroupLds l;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    if (wave < c.tokens) choose<kSlots>(c, wave, threadIdx.x & 63, l.ids);
+    __syncthreads();
+    group_rows(p, at, l, true);
 }
 
 }  // namespace
 
-int launch_group(const GroupArgs& args, hipStream_t stream) {
+int launch_group(const GroupArgs& args, const RotateArgs& beside, int dtype, hipStream_t stream) {
     const size_t lds = sizeof(int) * (static_cast<size_t>(args.keys) + 1);
-    hipLaunchKernelGGL(group_kernel, dim3(1), dim3(kGroupThreads), lds, stream, args);
+    const int64_t each = kGroupThreads / 64;
+    const dim3 grid(static_cast<unsigned>(1 + (rotate_waves(beside) + each - 1) / each));
+    if (dtype == 0)
+        hipLaunchKernelGGL(group_kernel<__bf16>, grid, dim3(kGroupThreads), lds, stream, args, beside);
+    else
+        hipLaunchKernelGGL(group_kernel<_Float16>, grid, dim3(kGroupThreads), lds, stream, args, beside);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
+}
+
+const char* router_fault(const RouterArgs& a) {
+    if (!a.x || !a.weight || !a.weights || !a.ids || a.tokens < 0 || a.hidden <= 0 || a.experts <= 0)
+        return "null pointer or bad size in the router";
+    if (a.dtype != 0 && a.dtype != 1) return "dtype must be 0 (bf16) or 1 (f16)";
+    if (a.experts > kMaxExperts) return "the router takes at most 1024 experts";
+    if (a.k < 1 || a.k > 64 || a.k > a.experts) return "k must be 1 .. min(64, experts)";
+    if (a.scoring != 0 && a.scoring != 1) return "scoring must be 0 (softmax) or 1 (sigmoid)";
+    if (a.hidden % 8 || a.x_ld % 8 || a.weight_ld % 8 || a.x_ld < a.hidden || a.weight_ld < a.hidden ||
+        reinterpret_cast<uintptr_t>(a.x) % 16 || reinterpret_cast<uintptr_t>(a.weight) % 16)
+        return "the router's rows must be 16-byte aligned and a multiple of 8 channels";
+    return nullptr;
+}
+
+size_t router_logit_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
+    return sizeof(float) * static_cast<size_t>(router_splits(tokens, hidden, experts)) * tokens * experts;
+}
+
+int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs* group, hipStream_t stream) {
+    LogitsArgs la{a.x, a.weight, a.x_ld, a.weight_ld, a.tokens, a.hidden, a.experts,
+                  router_splits(a.tokens, a.hidden, a.experts), (a.experts + 15) / 16, (a.tokens + 15) / 16, a.logits, beside};
+    const int64_t blocks = static_cast<int64_t>(la.etiles) * la.ttiles * la.splits + (rotate_waves(beside) + 3) / 4;
+    if (a.dtype == 0)
+        hipLaunchKernelGGL(router_logits_kernel<__bf16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, la);
+    else
+        hipLaunchKernelGGL(router_logits_kernel<_Float16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, la);
+    QSRT_HIP_TRY(hipGetLastError());
+    const ChooseArgs ca{a.logits, a.bias, a.tokens, a.experts, la.splits, a.k, a.scoring, a.normalize, a.scale, a.weights, a.ids};
+    const bool together = group && a.tokens <= kGroupThreads / 64;
+#define QSRT_CHOOSE(SLOTS)                                                                                             \
+    if (together)                                                                                                      \
+        hipLaunchKernelGGL(choose_group_kernel<SLOTS>, dim3(1), dim3(kGroupThreads), sizeof(int) * (group->keys + 1), \
+                           stream, ca, *group);                                                                        \
+    else                                                                                                               \
+        hipLaunchKernelGGL(choose_kernel<SLOTS>, dim3(static_cast<unsigned>(a.tokens)), dim3(64), 0, stream, ca)
+    if (a.experts <= 64) {
+        QSRT_CHOOSE(1);
+    } else if (a.experts <= 128) {
+        QSRT_CHOOSE(2);
+    } else if (a.experts <= 256) {
+        QSRT_CHOOSE(4);
+    } else if (a.experts <= 384) {
+        QSRT_CHOOSE(6);
+    } else if (a.experts <= 512) {
+        QSRT_CHOOSE(8);
+    } else {
+        QSRT_CHOOSE(16);
+    }
+#undef QSRT_CHOOSE
+    QSRT_HIP_TRY(hipGetLastError());
+    return group && !together ? launch_group(*group, RotateArgs{}, a.dtype, stream) : kOk;
 }
 
 }  // namespace qsrt
 
 using namespace qsrt;
 
-extern "C" size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t experts) {
-    if (tokens <= 0 || experts <= 0) return 0;
-    return static_cast<size_t>(tokens) * static_cast<size_t>(experts) * sizeof(float);
+extern "C" size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
+    if (tokens <= 0 || hidden <= 0 || experts <= 0) return 0;
+    return router_logit_bytes(tokens, hidden, experts);
 }
 
 extern "C" int qsrt_route(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, int dtype, int64_t tokens,
                           int64_t hidden, int64_t experts, int k, const float* bias, int scoring, int normalize,
-                          float scale, float* weights, int32_t* ids, void* ws, size_t ws_bytes, void* stream_) {
+                          float scale, float* weights, int32_t* ids, void* ws, size_t ws_bytes, void* stream) {
     if (tokens == 0) return kOk;
-    if (!x || !weight || !weights || !ids || tokens < 0 || hidden <= 0 || experts <= 0)
-        return fail(kBadArgument, "qsrt_route: null pointer or bad size");
-    if (dtype != 0 && dtype != 1) return fail(kBadArgument, "qsrt_route: dtype must be 0 (bf16) or 1 (f16)");
-    if (experts > kMaxExperts) return fail(kBadArgument, "qsrt_route: at most %d experts", kMaxExperts);
-    if (k < 1 || k > 64 || k > experts) return fail(kBadArgument, "qsrt_route: k must be 1 .. min(64, experts)");
-    if (scoring != 0 && scoring != 1) return fail(kBadArgument, "qsrt_route: scoring must be 0 (softmax) or 1 (sigmoid)");
-    if (tokens > (1 << 20) || hidden > (1 << 24)) return fail(kBadArgument, "qsrt_route: too many tokens or channels");
-    if (hidden % 8 || x_ld % 8 || weight_ld % 8 || x_ld < hidden || weight_ld < hidden ||
-        reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(weight) % 16)
-        return fail(kBadArgument, "qsrt_route: rows must be 16-byte aligned and a multiple of 8 channels");
-    if (!ws || ws_bytes < qsrt_route_workspace_bytes(tokens, experts))
-        return fail(kWorkspaceTooSmall, "qsrt_route: needs %zu workspace bytes",
-                    qsrt_route_workspace_bytes(tokens, experts));
-    hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const dim3 grid(static_cast<unsigned>((experts + 15) / 16), static_cast<unsigned>((tokens + 15) / 16));
-    float* logits = static_cast<float*>(ws);
-    if (dtype == 0)
-        hipLaunchKernelGGL(router_logits_kernel<__bf16>, grid, dim3(64 * kRouterWaves), 0, stream,
-                           static_cast<const __bf16*>(x), x_ld, static_cast<const __bf16*>(weight), weight_ld,
-                           static_cast<int>(tokens), static_cast<int>(hidden), static_cast<int>(experts), logits);
-    else
-        hipLaunchKernelGGL(router_logits_kernel<_Float16>, grid, dim3(64 * kRouterWaves), 0, stream,
-                           static_cast<const _Float16*>(x), x_ld, static_cast<const _Float16*>(weight), weight_ld,
-                           static_cast<int>(tokens), static_cast<int>(hidden), static_cast<int>(experts), logits);
-    QSRT_HIP_TRY(hipGetLastError());
-    const ChooseArgs ca{logits, bias, static_cast<int>(tokens), static_cast<int>(experts), k, scoring, normalize, scale,
-                        weights, ids};
-    hipLaunchKernelGGL((experts <= 64    ? choose_kernel<1>
-                        : experts <= 128 ? choose_kernel<2>
-                        : experts <= 256 ? choose_kernel<4>
-                        : experts <= 512 ? choose_kernel<8>
-                                         : choose_kernel<16>),
-                       dim3(static_cast<unsigned>(tokens)), dim3(64), 0, stream, ca);
-    QSRT_HIP_TRY(hipGetLastError());
-    return kOk;
+    if (tokens < 0 || tokens > (1 << 20) || hidden <= 0 || hidden > (1 << 24) || experts <= 0 || experts > kMaxExperts)
+        return fail(kBadArgument, "qsrt_route: bad sizes (at most 2^20 tokens, 2^24 channels, %d experts)", kMaxExperts);
+    const RouterArgs args{x, x_ld, weight, weight_ld, dtype, static_cast<int>(tokens), static_cast<int>(hidden),
+                          static_cast<int>(experts), k, bias, scoring, normalize, scale, weights, ids,
+                          static_cast<float*>(ws)};
+    if (const char* e = router_fault(args)) return fail(kBadArgument, "qsrt_route: %s", e);
+    const size_t need = router_logit_bytes(tokens, hidden, experts);
+    if (!ws || ws_bytes < need) return fail(kWorkspaceTooSmall, "qsrt_route: needs %zu workspace bytes", need);
+    return launch_router(args, RotateArgs{}, nullptr, static_cast<hipStream_t>(stream));
 }

@@ -1,7 +1,7 @@
 """A mixture-of-experts layer for a few tokens, straight from its packed payloads.
 
 ``route_tokens`` chooses each token's experts, ``PackedExperts`` multiplies by them and ``PackedMoELayer`` is both
-(``qsrt_route`` and ``qsrt_packed_moe`` in ``include/qsrt_amd.h``).  Nothing waits for the device: which experts are
+(``qsrt_route``, ``qsrt_packed_moe`` and ``qsrt_packed_moe_layer`` in ``include/qsrt_amd.h``).  Nothing waits for the device: which experts are
 chosen is known there alone.
 """
 
@@ -45,12 +45,12 @@ def _route(x, weight, k, bias, scoring, normalize, scale):
     ids = torch.empty((t, k), dtype=torch.int32, device=x.device)
     if t == 0:
         return weights, ids
-    ws = torch.empty((t, e), dtype=torch.float32, device=x.device)
+    lib = _native.lib()
+    ws = torch.empty(lib.qsrt_route_workspace_bytes(t, h, e), dtype=torch.uint8, device=x.device)
     _native.check(
-        _native.lib().qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
-                                 k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize),
-                                 float(scale), weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), 4 * ws.numel(),
-                                 _native.stream_handle(x.device)),
+        lib.qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
+                       k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize), float(scale),
+                       weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(x.device)),
         "qsrt_route",
     )
     return weights, ids
@@ -153,8 +153,29 @@ class PackedMoELayer:
         self.experts, self.k, self.scoring, self.normalize, self.scale = experts, k, scoring, normalize, scale
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None):
-        weights, ids = _route(x, self.router, self.k, self.bias, self.scoring, self.normalize, self.scale)
-        return self.experts(x, weights, ids, out=out), weights, ids
+        e = self.experts
+        if x.dtype != self.router.dtype:
+            raise ValueError("x must be of the router's type")
+        x = checked_rows(x, e.hidden, e.device)
+        out = checked_out(out, x, e.hidden)
+        t, k = x.shape[0], self.k
+        weights = torch.empty((t, k), dtype=torch.float32, device=e.device)
+        ids = torch.empty((t, k), dtype=torch.int32, device=e.device)
+        if t == 0:
+            return out, weights, ids
+        lib = _native.lib()
+        ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(e.w1.ref, e.w3.ref, e.w2.ref, e.experts, t, k),
+                         dtype=torch.uint8, device=e.device)
+        _native.check(
+            lib.qsrt_packed_moe_layer(
+                e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, self.router.data_ptr(),
+                self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
+                int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
+                weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                _native.stream_handle(e.device)),
+            "qsrt_packed_moe_layer",
+        )
+        return out, weights, ids
 
 
 __all__ = ["PackedExperts", "PackedMoELayer", "route_tokens"]
