@@ -13,6 +13,7 @@ namespace qsrt {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -108,27 +109,64 @@ struct RotateArgs {
 inline int64_t rotate_waves(const RotateArgs& p) { return (p.rows + 15) / 16 * 16 * p.kb * p.nmat; }
 
 // The `wave`-th 128 channels of a row and matrix; neighbouring waves have the same channels of neighbouring rows.
-template <typename T>
-__device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, int lane) {
+struct RotateAt {
+    int64_t row;
+    int kb, mat;
+};
+__device__ __forceinline__ RotateAt rotate_at(const RotateArgs& p, int64_t wave) {
     const int64_t sixteen = wave >> 4, rest = sixteen / p.kb;
-    const int kb = static_cast<int>(sixteen - rest * p.kb);
-    const int mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
-    const int64_t row = 16 * (p.nmat == 2 ? rest >> 1 : rest) + (wave & 15);
-    if (row >= p.rows) return;
-    const int id = p.ids ? max(p.ids[row], 0) : 0;
-    const _Float16* suh = (mat ? p.suh[1] : p.suh[0]) + id * (mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * kb;
-    const T* x = static_cast<const T*>(p.x) + (p.x_div == 1 ? row : row / p.x_div) * p.ld + 128 * kb;
+    return RotateAt{16 * (p.nmat == 2 ? rest >> 1 : rest) + (wave & 15), static_cast<int>(sixteen - rest * p.kb),
+                    p.nmat == 2 ? static_cast<int>(rest & 1) : 0};
+}
+
+template <typename T>
+__device__ __forceinline__ f32x2 rotated(const RotateArgs& p, const RotateAt& at, int lane) {
+    const int id = p.ids ? max(p.ids[at.row], 0) : 0;
+    const _Float16* suh =
+        (at.mat ? p.suh[1] : p.suh[0]) + id * (at.mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * at.kb;
+    const T* x = static_cast<const T*>(p.x) + (p.x_div == 1 ? at.row : at.row / p.x_div) * p.ld + 128 * at.kb;
     typedef T t2 __attribute__((ext_vector_type(2)));
     const t2 xv = reinterpret_cast<const t2*>(x)[lane];
     const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];
     float a = static_cast<float>(xv[0]) * static_cast<float>(sv[0]);
     float b = static_cast<float>(xv[1]) * static_cast<float>(sv[1]);
     hadamard128(a, b, lane);
-    store_pieces((mat ? p.out[1] : p.out[0]) + row_place(p.layout, row), p.layout, kb, lane, a * kHadamardScale,
-                 b * kHadamardScale);
+    return f32x2{a * kHadamardScale, b * kHadamardScale};
 }
 
-// At most chunk_rows rows of one key (an expert, an adapter): order[first .. first + count), the first of them row0.
+template <typename T>
+__device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, int lane) {
+    const RotateAt at = rotate_at(p, wave);
+    if (at.row >= p.rows) return;
+    const f32x2 v = rotated<T>(p, at, lane);
+    store_pieces((at.mat ? p.out[1] : p.out[0]) + row_place(p.layout, at.row), p.layout, at.kb, lane, v[0], v[1]);
+}
+
+// The same by a workgroup of 16 waves for rows laid out by 16, four blocks of channels at once: 16 rows by 512 channels, whose
+// 32 KiB leave in one stretch.
+constexpr int kRotateBlocks = 4;
+inline int64_t rotate_quads(const RotateArgs& p) { return (p.rows + 15) / 16 * p.nmat * ((p.kb + kRotateBlocks - 1) / kRotateBlocks); }
+template <typename T>
+__device__ __forceinline__ void rotate_quad(const RotateArgs& p, int64_t quad, u32x4 (&staged)[512 * kRotateBlocks]) {
+    const int lane = threadIdx.x & 63;
+    const int quads = (p.kb + kRotateBlocks - 1) / kRotateBlocks;
+    const int64_t rest = quad / quads, sixteen = p.nmat == 2 ? rest >> 1 : rest;
+    const int kb0 = kRotateBlocks * static_cast<int>(quad - rest * quads), mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
+    const int64_t row = 16 * sixteen + uniform(static_cast<int>(threadIdx.x >> 6));
+    f32x2 v[kRotateBlocks];
+#pragma unroll
+    for (int j = 0; j < kRotateBlocks; ++j)
+        v[j] = row < p.rows ? rotated<T>(p, RotateAt{row, min(kb0 + j, p.kb - 1), mat}, lane) : f32x2{0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kRotateBlocks; ++j)
+        store_pieces(reinterpret_cast<char*>(staged) + (row & 15) * p.layout.row, p.layout, j, lane, v[j][0], v[j][1]);
+    __syncthreads();
+    u32x4* out = reinterpret_cast<u32x4*>((mat ? p.out[1] : p.out[0]) + sixteen * p.layout.sixteen + 4 * kb0 * p.layout.strip);
+    const int end = 512 * min(kRotateBlocks, p.kb - kb0);
+    for (int i = threadIdx.x; i < end; i += 1024) out[i] = staged[i];
+}
+
+// At most chunk_rows rows of one key (an expert): order[first .. first + count), the first of them row0.
 // Chunks follow one another; the table's rest has count 0.
 struct Chunk {
     int key, first, count, row0;
@@ -138,7 +176,6 @@ typedef const __attribute__((address_space(4))) Chunk* ConstChunk;  // constant 
 struct GroupArgs {
     const int* ids;
     int n, keys;
-    bool none;  // rows without a key form a group of their own (key -1)
     int chunk_rows, max_chunks;
     Chunk* chunks;
     int* order;

@@ -251,6 +251,169 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 }
 
 // ---------------------------------------------------------------------------
+// The product of many rows: a workgroup decodes a strip once for 128 G of them
+// ---------------------------------------------------------------------------
+
+constexpr int kRowWaves = 8;
+
+// Eight waves of 16 G rows each over the same columns.  Wave w decodes one window a lane of every strip (tile column pair
+// w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips' worth of them, then multiplies all of the
+// strip's by its own rows; one barrier a strip.  The table reads, which bound the product of a few rows, fall to an eighth a
+// row; the matrix cores (two pieces a row) are left as the bound.
+template <int G>
+__device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
+                                              const uint8_t* lut, u32x2 (&frags)[2][8][128], int lane, int w, bool& ready,
+                                              f32x4 (&acc)[G][8]) {
+    const int m = lane & 15, g = lane >> 4, t = w >> 1, h = w & 1;
+    int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;  // as in multiply_strips
+    if (b0 < 0) b0 += 256 * K;
+    const int d0 = b0 >> 5, d1 = d0 + 1 == 8 * K ? 0 : d0 + 1;
+    const uint32_t sh = b0 & 31, rsh = 32u - sh;
+    const uint32_t o0 = 4 * d0 + (m >> 3) * 32 * K + t * 64 * K, o1 = 4 * d1 + (m >> 3) * 32 * K + t * 64 * K;
+    const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(tiles), 0, (2 * strips - 1) * tile_row_bytes + 256 * K, 0x00027000);
+    uint32_t lo[2], hi[2];
+    bf16x8 b[G][2], next[G][2];
+    auto fetch_words = [&](int s, int slot) {
+        const int at = (2 * min(s, strips - 1) + h) * tile_row_bytes;
+        lo[slot] = __builtin_amdgcn_raw_buffer_load_b32(src, o0, at, 0);
+        hi[slot] = __builtin_amdgcn_raw_buffer_load_b32(src, o1, at, 0);
+    };
+    auto fetch_rows = [&](int s) {
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                next[q][p] = *(gbf8)(x[q] + static_cast<int64_t>(min(s, strips - 1)) * (16 * kStripBytes) + 1024 * p);
+    };
+    auto decode = [&](int slot, int buffer) {
+        const uint32_t w0 = __builtin_amdgcn_alignbit(lo[slot], hi[slot], rsh);
+        const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[slot] << sh, 32 - 4 * K);
+        uint32_t label[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) label[j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            u32x2 half;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                half[q] = __builtin_bit_cast(
+                    uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                  __builtin_amdgcn_perm(label[4 * u + 2 * q + 1], label[4 * u + 2 * q], 0x0C0C0400u), 1.0f, false));
+            frags[buffer][2 * t + u][2 * lane + h] = half;
+        }
+    };
+    fetch_words(0, 0);
+    fetch_words(1, 1);
+    fetch_rows(0);
+    if (!ready) {
+        __builtin_amdgcn_s_waitcnt(0);  // the direct loads to LDS are not ordered by the barrier alone
+        ready = true;
+    }
+    __syncthreads();  // the tables are there, and no wave reads the operands of an earlier run
+    decode(0, 0);
+    fetch_words(2, 0);
+    __syncthreads();
+    for (int s = 0; s < strips; s += 2) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // strip s + e of buffer e
+            if (s + e < strips) {
+#pragma unroll
+                for (int q = 0; q < G; ++q) {
+                    b[q][0] = next[q][0];
+                    b[q][1] = next[q][1];
+                }
+                fetch_rows(s + e + 1);
+                decode(e ^ 1, e ^ 1);  // past the last strip: the last again, which nobody reads
+                fetch_words(s + e + 3, e ^ 1);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const bf16x8 a = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&frags[e][c][2 * lane]));
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int q = 0; q < G; ++q)
+                            acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[q][p], acc[q][c], 0, 0, 0);
+                }
+                __syncthreads();
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < G; ++q) x[q] += static_cast<int64_t>(strips) * (16 * kStripBytes);
+}
+
+template <int G, int kTables>
+__global__ __launch_bounds__(64 * kRowWaves) void product_rows_kernel(const ProductArgs p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lut_s[65536 * kTables];
+    __shared__ __attribute__((aligned(16))) u32x2 frags[2][8][128];
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int w = uniform(static_cast<int>(threadIdx.x >> 6));
+    for (int i = w; i < kTables * 64; i += kRowWaves)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)((i < 64 ? p.lut[0] : p.lut[1]) + 1024 * (i & 63) + 16 * lane),
+            (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
+    bool ready = false;
+    const uint32_t items = static_cast<uint32_t>(p.max_chunks) * p.nb * p.parts, grid = gridDim.x;
+    const int64_t cols = 128 * static_cast<int64_t>(p.nb);
+    const int strips = 4 * p.kb, sixteens = (p.rows + 15) / 16;
+    // the workgroups of one chiplet (blockIdx.x % 8) take the column blocks of the same rows and find these in their cache
+    const uint32_t turn = (grid & 7) ? blockIdx.x : (blockIdx.x & 7) * (grid >> 3) + (blockIdx.x >> 3);
+    for (uint32_t item = turn; item < items; item += grid) {
+        uint32_t rest = item / p.nb;
+        const int cb = static_cast<int>(item - rest * p.nb);
+        const int ci = static_cast<int>(rest / p.parts), part = static_cast<int>(rest - ci * p.parts);
+        const int first = (ci * kRowWaves + w) * G;  // in groups of 16 rows
+        int s = strips * part / p.parts;
+        const int end = strips * (part + 1) / p.parts;
+        const char* x[G];
+        f32x4 acc[G][8];
+#pragma unroll
+        for (int q = 0; q < G; ++q) {  // groups past the last repeat it; their sums are not stored
+            x[q] = p.x[0] + min(first + q, sixteens - 1) * p.layout.sixteen + s * p.layout.strip + 16 * lane;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const char* words = reinterpret_cast<const char*>(p.words[0]);
+        typedef const __attribute__((address_space(4))) int64_t* ConstRecord;
+        const ConstRecord records = (ConstRecord)p.records[0];
+        while (s < end) {  // runs of one rate, as in product_kernel
+            const int r = p.axis ? cb : s >> 2;
+            const int64_t rec = records[r];
+            const int bits = static_cast<int>(rec & 7);
+            int stop = end;
+            if (!p.axis) {
+                int r1 = r + 1;
+                while (4 * r1 < end && static_cast<int>(records[r1] & 7) == bits) ++r1;
+                stop = min(end, 4 * r1);
+            }
+            const int tile = 32 * bits, tile_row = p.axis ? 8 * tile : 8 * p.nb * tile;
+            const char* tiles = words + 2 * (rec >> 3) +
+                                (p.axis ? static_cast<int64_t>(2 * s) * tile_row
+                                        : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
+            if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
+                const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
+                multiply_rows<G>(tiles, tile_row, stop - s, bits, x, lut, frags, lane, w, ready, acc);
+            } else {  // another pass has this rate
+#pragma unroll
+                for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
+            }
+            s = stop;
+        }
+        float* out = p.part + static_cast<int64_t>(p.pass * p.parts + part) * p.rows * cols + 128 * cb + 16 * (g >> 1) + 4 * (g & 1);
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            const int64_t row = 16 * static_cast<int64_t>(first + q) + n;
+            if (row >= p.rows) continue;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                *reinterpret_cast<f32x4*>(out + row * cols + 32 * (t >> 1) + 8 * (t & 1)) = acc[q][t];
+        }
+    }
+    if (!ready) __builtin_amdgcn_s_waitcnt(0);  // no wave ends with loads to LDS on their way
+}
+
+// ---------------------------------------------------------------------------
 // Rows into the payload's basis
 // ---------------------------------------------------------------------------
 
@@ -405,48 +568,66 @@ struct ShrinkArgs {
     const void* x;
     int64_t ld;
     const void* a;  // [adapters][rank][k]
-    const Chunk* chunks;
-    const int* order;
-    float* out;  // [parts][rows][rank]
-    int max_chunks, rows, k, rank, parts;
+    const int* ids;
+    float* out;     // [parts][rows][rank]
+    int rows, k, adapters, rank, parts;
+    int shares;     // workgroups that share the adapters of 16 rows
 };
+constexpr int kShrinkWaves = 16, kShrinkSteps = 8;  // a workgroup's part of the K axis: 4096 channels at the most
 
-// x A_a^T of 16 rows of one adapter over a part of the K axis, 16 kTiles ranks at a time; a wave each.  Products of the
-// inputs are exact, sums FP32.
+inline int64_t shrink_blocks(const ShrinkArgs& p, int tiles) {
+    return p.adapters ? static_cast<int64_t>((p.rows + 15) / 16) * p.parts * p.shares * (p.rank / (16 * tiles)) : 0;
+}
+
+// x A_a^T of 16 rows over a part of the K axis, 16 kTiles ranks at a time, for each adapter a that these rows name and that
+// is this workgroup's.  The rows are read once; a wave has up to eight steps of 32 channels, all their loads in flight, and
+// the waves add up in LDS in wave order.  Products of the inputs are exact, sums FP32.
 template <typename T, int kTiles>
-__global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
+__device__ __forceinline__ void shrink(const ShrinkArgs& p, int block, f32x4 (&sums)[kShrinkWaves][kTiles][64]) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t nw = static_cast<int64_t>(gridDim.x) * 4;
-    const int64_t items = static_cast<int64_t>(p.max_chunks) * p.parts * (p.rank / (16 * kTiles));
-    const int steps = p.k / 32, groups = p.rank / (16 * kTiles);
+    const int w = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int share = block % p.shares;
+    block /= p.shares;
+    const int part = block % p.parts;
+    block /= p.parts;
+    const int groups = p.rank / (16 * kTiles), group = block % groups;
+    const int row = 16 * (block / groups) + n;
+    const int id = row < p.rows ? p.ids[row] : -1;
+    uint32_t left = static_cast<uint32_t>(__ballot(lane < 16 && id >= 0 && id < p.adapters));
+    if (!left) return;
+    const int steps = p.k / 32, end = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.parts);
+    const int s0 = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts) + w;
     typedef T t8 __attribute__((ext_vector_type(8)));
-    for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-         item < items; item += nw) {
-        const int part = static_cast<int>(item % p.parts), rest = static_cast<int>(item / p.parts);
-        const int group = rest % groups;
-        const ConstChunk c = (ConstChunk)p.chunks + rest / groups;
-        const int key = c->key, count = c->count;
-        if (count == 0) break;  // the last chunk is behind
-        if (key < 0) continue;
-        const int row = p.order[c->first + min(n, count - 1)];
-        const T* x = static_cast<const T*>(p.x) + row * p.ld + 8 * g;
+    const t8 zero = {};
+    const T* x = static_cast<const T*>(p.x) + min(row, p.rows - 1) * p.ld + 8 * g;
+    t8 xv[kShrinkSteps];
+#pragma unroll
+    for (int j = 0; j < kShrinkSteps; ++j) {
+        const int s = s0 + kShrinkWaves * j;
+        xv[j] = s < end ? *reinterpret_cast<const t8*>(x + 32 * s) : zero;
+    }
+    for (int index = 0; left; ++index) {
+        const int key = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+        const uint32_t same = static_cast<uint32_t>(__ballot(lane < 16 && id == key));
+        left &= ~same;
+        if (index % p.shares != share) continue;
         const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + 16 * kTiles * group + n) * p.k + 8 * g;
         f32x4 acc[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.parts);
-        auto steps_at = [&](int s, auto count) {  // the loads of all `count` steps go out together
-            constexpr int kSteps = decltype(count)::value;
-            t8 xv[kSteps], av[kSteps][kTiles];
+        t8 av[kShrinkSteps][kTiles];
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                xv[j] = *reinterpret_cast<const t8*>(x + 32 * (s + j));
+        for (int j = 0; j < kShrinkSteps; ++j) {
+            const int s = s0 + kShrinkWaves * j;
+            if (s < end) {
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
-                    av[j][t] = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * (s + j));
+                    av[j][t] = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * s);
             }
+        }
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j)
+        for (int j = 0; j < kShrinkSteps; ++j) {
+            if (s0 + kShrinkWaves * j < end) {
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     if constexpr (__is_same(T, __bf16))
@@ -454,26 +635,48 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs p) {
                     else
                         acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][t], xv[j], acc[t], 0, 0, 0);
                 }
-        };
-        int s = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts);
-        for (; s + 4 <= s1; s += 4) steps_at(s, std::integral_constant<int, 4>{});
-        for (; s < s1; ++s) steps_at(s, std::integral_constant<int, 1>{});
-        if (n >= count) continue;
-        float* out = p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank + 16 * kTiles * group + 4 * g;
+            }
+        }
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
+        for (int t = 0; t < kTiles; ++t) sums[w][t][lane] = acc[t];
+        __syncthreads();
+        if (w < kTiles) {
+            f32x4 sum = sums[0][w][lane];
+#pragma unroll
+            for (int v = 1; v < kShrinkWaves; ++v) sum += sums[v][w][lane];
+            if (same >> n & 1)
+                *reinterpret_cast<f32x4*>(p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank +
+                                          16 * (kTiles * group + w) + 4 * g) = sum;
+        }
+        __syncthreads();
     }
+}
+
+// What an adapter projection needs before its product: the rows' rotation, and beside it the adapters' first products.
+template <typename T, int kTiles>
+__global__ __launch_bounds__(64 * kShrinkWaves) void prepare_rows_kernel(const RotateArgs r, const ShrinkArgs p, int shrinks) {
+    __shared__ __attribute__((aligned(16))) union {
+        f32x4 sums[kShrinkWaves][kTiles][64];
+        u32x4 staged[512 * kRotateBlocks];
+    } l;
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < shrinks)
+        shrink<T, kTiles>(p, block, l.sums);
+    else if (r.layout.row == 16)
+        rotate_quad<T>(r, block - shrinks, l.staged);
+    else
+        rotate_block<T>(r, static_cast<int64_t>(block - shrinks) * 16 + uniform(static_cast<int>(threadIdx.x >> 6)),
+                        threadIdx.x & 63);
 }
 
 struct FinishArgs {
     const float* part;  // [parts][rows][cols]
     int parts;
-    const Chunk* chunks;  // null: no adapters, chunks are runs of 16 rows
-    const int* order;
     const _Float16* svh;
-    const float* low;  // [low_parts][rows][rank]
-    int low_parts;
-    const void* b;  // [adapters][cols][rank]
+    const int* ids;     // null: no adapters
+    const float* low;   // [low_parts][rows][rank]
+    int low_parts, adapters;
+    const void* b;      // [adapters][cols][rank]
     const float* scale;
     int rank;
     void* out;
@@ -481,48 +684,56 @@ struct FinishArgs {
     int rows, nb;
 };
 
-// Sum of the parts, back into the output's basis, plus the adapter's second product: a workgroup of four waves for the (at
-// most 16) rows of a chunk by 128 columns.  Each wave has every fourth row and reads the adapter's slice once for them;
-// under four rows the waves share the parts of each instead.
+// Sum of the parts, back into the output's basis, plus the adapter's second product: a workgroup of four waves for 16 rows by
+// 128 columns.  Each wave has every fourth row and reads an adapter's slice once for those of them that name it; under four
+// rows the waves share the parts of each instead.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     __shared__ f32x2 sums[4][64];
     const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
-    const int nb = static_cast<int>(blockIdx.x % p.nb), ci = static_cast<int>(blockIdx.x / p.nb);
-    int key = -1, first = 16 * ci, count = min(16, p.rows - first);
-    if (p.chunks) {
-        const ConstChunk c = (ConstChunk)p.chunks + ci;
-        key = c->key;
-        first = c->first;
-        count = c->count;
-        if (count == 0) return;
-    }
+    const int nb = static_cast<int>(blockIdx.x % p.nb), first = 16 * static_cast<int>(blockIdx.x / p.nb);
+    const int count = min(16, p.rows - first);
     const int64_t cols = 128 * static_cast<int64_t>(p.nb), stride = p.rows * cols;
     const float* src = p.part + 128 * nb + 2 * lane;
-    int row[4];
+    int row[4], key[4];
     f32x2 v[4];
-    int mine = 0;  // rows of this wave
+    int mine;  // rows of this wave
     if (count < 4) {
+        mine = w < count;
         for (int r = 0; r < count; ++r) {
-            const int at = p.chunks ? uniform(p.order[first + r]) : first + r;
-            sums[w][lane] = sum_parts(src + at * cols, stride, w, 4, p.parts);
+            sums[w][lane] = sum_parts(src + (first + r) * cols, stride, w, 4, p.parts);
             __syncthreads();
-            if (w == r) {
-                row[0] = at;
-                v[0] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
-                mine = 1;
-            }
+            if (w == r) v[0] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
             __syncthreads();
         }
-    } else {
+        if (!mine) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = w + 4 * i;
-            if (r >= count) break;
-            row[i] = p.chunks ? uniform(p.order[first + r]) : first + r;
-            v[i] = sum_parts(src + row[i] * cols, stride, 0, 1, p.parts);
-            mine = i + 1;
+        for (int i = 0; i < 4; ++i) row[i] = first + w;
+    } else {
+        mine = (count - w + 3) >> 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // rows past the last repeat the wave's first; not stored
+            row[i] = first + (i < mine ? w + 4 * i : w);
+            v[i] = f32x2{0.f, 0.f};
         }
+        for (int s = 0; s < p.parts; s += 4) {  // sixteen loads in flight
+            f32x2 t[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    t[j][i] = *reinterpret_cast<const f32x2*>(src + min(s + j, p.parts - 1) * stride + row[i] * cols);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (s + j < p.parts) v[i] += t[j][i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        key[i] = p.ids && i < mine ? uniform(p.ids[row[i]]) : -1;
+        if (key[i] >= p.adapters) key[i] = -1;
     }
     const f16x2 sv = reinterpret_cast<const f16x2*>(p.svh + 128 * nb)[lane];
 #pragma unroll
@@ -532,46 +743,40 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
         hadamard128(a, b, lane);
         v[i] = f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
     }
-    if (key >= 0 && mine) {
-        typedef T t8 __attribute__((ext_vector_type(8)));
-        const float scale = p.scale[key];
-        const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(key) * cols + 128 * nb + 2 * lane) * p.rank;
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    for (int turn = 0; turn < mine; ++turn) {
+        const int k = turn == 0 ? key[0] : turn == 1 ? key[1] : turn == 2 ? key[2] : key[3];
+        if (k < 0) continue;  // no adapter, or done with an earlier row
+        const float scale = p.scale[k];
+        const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(k) * cols + 128 * nb + 2 * lane) * p.rank;
         for (int r0 = 0; r0 < p.rank; r0 += 64) {
-            float low[4];  // lane l: rank r0 + l of each row
+            float low[4] = {0.f, 0.f, 0.f, 0.f};  // lane l: rank r0 + l of each row
+            const int r = min(r0 + lane, p.rank - 1);
+            for (int s = 0; s < p.low_parts; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                low[i] = 0.f;
-                if (i < mine && r0 + lane < p.rank) {
-                    const float* src = p.low + static_cast<int64_t>(row[i]) * p.rank + r0 + lane;
-                    const int64_t step = static_cast<int64_t>(p.rows) * p.rank;
-                    int s = 0;
-                    for (; s + 8 <= p.low_parts; s += 8) {
-                        float t[8];
+                for (int i = 0; i < 4; ++i)
+                    low[i] += p.low[(static_cast<int64_t>(s) * p.rows + row[key[i] == k ? i : turn]) * p.rank + r];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) t[j] = src[(s + j) * step];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) low[i] += t[j];
-                    }
-                    for (; s < p.low_parts; ++s) low[i] += src[s * step];
-                }
-                low[i] *= scale;
-            }
-            for (int r = 0; r < 64 && r0 + r < p.rank; r += 8) {
-                const t8 x0 = *reinterpret_cast<const t8*>(b0 + r0 + r);
-                const t8 x1 = *reinterpret_cast<const t8*>(b0 + p.rank + r0 + r);
+            for (int i = 0; i < 4; ++i) low[i] *= scale;
+            for (int q = 0; q < 64 && r0 + q < p.rank; q += 8) {
+                const t8 x0 = *reinterpret_cast<const t8*>(b0 + r0 + q);
+                const t8 x1 = *reinterpret_cast<const t8*>(b0 + p.rank + r0 + q);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (i >= mine) break;
+                    if (key[i] != k) continue;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float f = __builtin_bit_cast(
-                            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, low[i]), r + j));
+                            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, low[i]), q + j));
                         v[i][0] = __builtin_fmaf(f, static_cast<float>(x0[j]), v[i][0]);
                         v[i][1] = __builtin_fmaf(f, static_cast<float>(x1[j]), v[i][1]);
                     }
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (key[i] == k) key[i] = -1;
     }
     typedef T t2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -617,6 +822,18 @@ int cut_parts(double units, int64_t most, int strips, int limit, int rows, int c
     return best;
 }
 
+template <int G, int kTables>
+int launch_rows_g(const ProductArgs& args, int cus, hipStream_t stream) {
+    const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nb * args.parts;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
+    hipLaunchKernelGGL((product_rows_kernel<G, kTables>), grid, dim3(64 * kRowWaves), 0, stream, args);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
+// Groups of 16 rows that each of a workgroup's eight waves has in product_rows_kernel; 0: the rows are too few for it.
+int row_groups(int64_t rows) { return rows <= 128 ? 0 : rows <= 256 ? 2 : 4; }
+
 // All passes of a product: the tables of at most two rates fit LDS at once.
 int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
     int set[3], n = 0;
@@ -630,6 +847,12 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
             args.lut[j] = luts[set[first + j] - 2];
         }
         const bool two = args.luts > 1;
+        if (!args.chunks && row_groups(args.rows)) {
+            const int rc = row_groups(args.rows) == 2 ? (two ? launch_rows_g<2, 2> : launch_rows_g<2, 1>)(args, cus, stream)
+                                                      : (two ? launch_rows_g<4, 2> : launch_rows_g<4, 1>)(args, cus, stream);
+            if (rc != kOk) return rc;
+            continue;
+        }
         const int rc = groups == 1   ? (two ? launch_product_g<1, 2> : launch_product_g<1, 1>)(args, cus, stream)
                        : groups == 2 ? (two ? launch_product_g<2, 2> : launch_product_g<2, 1>)(args, cus, stream)
                                      : (two ? launch_product_g<4, 2> : launch_product_g<4, 1>)(args, cus, stream);
@@ -639,6 +862,22 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
 }
 
 int passes_of(int rates) { return __builtin_popcount(rates & 0x1C) > 2 ? 2 : 1; }
+
+// The same for product_rows_kernel, a workgroup an item: a strip takes its eight waves about 1.1 us, a part's sums (256 KB a
+// workgroup) as long as 16 strips, there and back, and its set-up 3.
+int cut_row_parts(int64_t units, int strips, int limit, int cus) {
+    int best = 1;
+    double least = 0.0;
+    for (int p = 1; p <= std::min(limit, strips); ++p) {
+        if (units * p >= int64_t(1) << 31) break;
+        const double cost = std::ceil(static_cast<double>(units * p) / cus) * ((strips + p - 1) / p + 19.0);
+        if (p == 1 || cost < least) {
+            least = cost;
+            best = p;
+        }
+    }
+    return best;
+}
 
 const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts) {
     if (!m || !m->words || !m->records || !m->suh || !m->svh) return "null pointer in a matrix";
@@ -802,7 +1041,6 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ga.ids = c.ids;
     ga.n = static_cast<int>(pairs);
     ga.keys = static_cast<int>(c.experts);
-    ga.none = false;
     ga.chunk_rows = 16 * s.groups;
     ga.max_chunks = s.max_chunks;
     ga.chunks = s.chunks;
@@ -941,11 +1179,9 @@ extern "C" int qsrt_packed_moe_layer(const qsrt_packed_matrix* w1, const qsrt_pa
 namespace {
 
 struct LinearSpace {
-    Chunk* chunks;
-    int *order, *clean;
     char* x;
     float *low, *part;
-    int low_parts, parts, passes, groups, max_chunks;
+    int low_parts, parts, passes, groups, product_chunks;
     size_t bytes;
 };
 
@@ -954,16 +1190,16 @@ LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates
     Carve c{static_cast<char*>(ws)};
     s.groups = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     s.passes = passes_of(rates);
-    const int64_t group_rows = 16 * s.groups, chunks = (rows + group_rows - 1) / group_rows;
-    const int strips = static_cast<int>(k / 32);
-    s.parts = cut_parts(static_cast<double>(chunks * (n / 128)), chunks * (n / 128), strips, part_limit(rows * n * s.passes, strips),
-                        static_cast<int>(std::min(rows, group_rows)), cus);
+    const int64_t group_rows = 16 * (row_groups(rows) ? kRowWaves * row_groups(rows) : s.groups);
+    const int64_t chunks = (rows + group_rows - 1) / group_rows;
+    s.product_chunks = static_cast<int>(chunks);
+    const int strips = static_cast<int>(k / 32), limit = part_limit(rows * n * s.passes, strips);
+    s.parts = row_groups(rows) ? cut_row_parts(chunks * (n / 128), strips, limit, cus)
+                               : cut_parts(static_cast<double>(chunks * (n / 128)), chunks * (n / 128), strips, limit,
+                                           static_cast<int>(std::min(rows, group_rows)), cus);
     if (adapters) {
-        s.max_chunks = static_cast<int>(most_chunks(rows, adapters + 1, 16));
-        s.low_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / s.max_chunks, k / 256)));
-        s.chunks = c.take<Chunk>(s.max_chunks);
-        s.order = c.take<int>(rows);
-        s.clean = c.take<int>(rows);
+        constexpr int64_t kPart = 32 * kShrinkWaves * kShrinkSteps;
+        s.low_parts = static_cast<int>((k + kPart - 1) / kPart);
         s.low = c.take<float>(s.low_parts * rows * rank);
     }
     s.x = c.take<char>(sixteens(rows) * k * 4);
@@ -1013,52 +1249,42 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     ra.kb = static_cast<int>(k / 128);
     ra.nmat = 1;
     ra.layout = row_layout(ra.kb, rows > 4);
-    if (adapters) {
-        GroupArgs ga{};
-        ga.ids = ids;
-        ga.n = static_cast<int>(rows);
-        ga.keys = static_cast<int>(adapters);
-        ga.none = true;
-        ga.chunk_rows = 16;
-        ga.max_chunks = s.max_chunks;
-        ga.chunks = s.chunks;
-        ga.order = s.order;
-        ga.clean = s.clean;
-        if (const int rc = launch_group(ga, ra, dtype, stream)) return rc;
-        ShrinkArgs sa{};
-        sa.x = x;
-        sa.ld = x_ld;
-        sa.a = a;
-        sa.max_chunks = s.max_chunks;
-        sa.chunks = s.chunks;
-        sa.order = s.order;
-        sa.out = s.low;
-        sa.rows = static_cast<int>(rows);
-        sa.k = static_cast<int>(k);
-        sa.rank = static_cast<int>(rank);
-        sa.parts = s.low_parts;
-        const int tiles = rank % 64 == 0 ? 4 : rank % 32 == 0 ? 2 : 1;  // of 16 ranks a wave
-        const int64_t most = static_cast<int64_t>(s.max_chunks) * s.low_parts * (rank / (16 * tiles));
-        const dim3 sgrid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most), 8 * cus)));
-#define QSRT_SHRINK(T)                                                                                  \
-    hipLaunchKernelGGL((tiles == 4 ? shrink_kernel<T, 4> : tiles == 2 ? shrink_kernel<T, 2> : shrink_kernel<T, 1>), \
-                       sgrid, dim3(256), 0, stream, sa)
-        if (dtype == 0)
-            QSRT_SHRINK(__bf16);
-        else
-            QSRT_SHRINK(_Float16);
-#undef QSRT_SHRINK
-        QSRT_HIP_TRY(hipGetLastError());
-    } else if (const int rc = launch_rotate(ra, dtype, stream)) {
-        return rc;
-    }
+    ShrinkArgs sa{};
+    sa.x = x;
+    sa.ld = x_ld;
+    sa.a = a;
+    sa.ids = ids;
+    sa.out = s.low;
+    sa.rows = static_cast<int>(rows);
+    sa.k = static_cast<int>(k);
+    sa.adapters = static_cast<int>(adapters);
+    sa.rank = static_cast<int>(rank);
+    sa.parts = s.low_parts;
+    const int tiles = adapters && rank % 32 == 0 ? 2 : 1;  // of 16 ranks a workgroup
+    // the adapters of 16 rows are shared out while that leaves no more workgroups than two a compute unit
+    if (adapters)
+        sa.shares = static_cast<int>(std::max<int64_t>(
+            1, std::min<int64_t>(std::min<int64_t>(16, rows), 2 * cus / std::max<int64_t>(1, sixteens(rows) / 16 * s.low_parts * (rank / (16 * tiles))))));
+    const int64_t shrinks = shrink_blocks(sa, tiles);
+    const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + 15) / 16;
+    if (shrinks + rotates >= int64_t(1) << 31) return fail(kBadArgument, "qsrt_adapter_linear: too many rows");
+    const dim3 pgrid(static_cast<unsigned>(shrinks + rotates)), pblock(64 * kShrinkWaves);
+#define QSRT_PREPARE(T)                                                                                              \
+    hipLaunchKernelGGL((tiles == 2 ? prepare_rows_kernel<T, 2> : prepare_rows_kernel<T, 1>), pgrid, pblock, 0, stream, ra, \
+                       sa, static_cast<int>(shrinks))
+    if (dtype == 0)
+        QSRT_PREPARE(__bf16);
+    else
+        QSRT_PREPARE(_Float16);
+#undef QSRT_PREPARE
+    QSRT_HIP_TRY(hipGetLastError());
 
     ProductArgs pa{};
     set_matrix(pa, 0, w);
     pa.x[0] = s.x;
     pa.x_div = 1;
     pa.layout = ra.layout;
-    pa.max_chunks = static_cast<int>((rows + 16 * s.groups - 1) / (16 * s.groups));
+    pa.max_chunks = s.product_chunks;
     pa.parts = s.parts;
     pa.part = s.part;
     pa.nmat = 1;
@@ -1068,11 +1294,11 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     FinishArgs fa{};
     fa.part = s.part;
     fa.parts = s.parts * s.passes;
-    fa.chunks = s.chunks;
-    fa.order = s.order;
-    fa.svh = reinterpret_cast<const _Float16*>(w->svh);
+    fa.svh = static_cast<const _Float16*>(w->svh);
+    fa.ids = adapters ? ids : nullptr;
     fa.low = s.low;
     fa.low_parts = s.low_parts;
+    fa.adapters = static_cast<int>(adapters);
     fa.b = b;
     fa.scale = scale;
     fa.rank = static_cast<int>(rank);
@@ -1080,8 +1306,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     fa.ld = out_ld;
     fa.rows = static_cast<int>(rows);
     fa.nb = static_cast<int>(n / 128);
-    const int64_t most = adapters ? s.max_chunks : (rows + 15) / 16;
-    const dim3 fgrid(static_cast<unsigned>(most * fa.nb));
+    const dim3 fgrid(static_cast<unsigned>((rows + 15) / 16 * fa.nb));
     if (dtype == 0)
         hipLaunchKernelGGL(finish_kernel<__bf16>, fgrid, dim3(256), 0, stream, fa);
     else

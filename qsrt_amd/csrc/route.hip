@@ -1,4 +1,4 @@
-// The router of a mixture-of-experts layer, and the grouping of rows by expert or adapter.
+// The router of a mixture-of-experts layer, and the grouping of rows by expert.
 #include <algorithm>
 
 #include "packed.h"
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64) void choose_kernel(const ChooseArgs p) {
 
 // Rows 0 .. n - 1 by key, in one workgroup: counts, offsets, chunks of at most chunk_rows, then the rows of each key.
 // Rows of a key are placed by an LDS counter, in no fixed order: no result depends on a row's neighbours in its chunk.
-// A row whose key is outside [0, keys) is left out (clean = -1), or with `none` put under the key -1.
+// A row whose key is outside [0, keys) is left out (clean = -1).
 constexpr int kGroupThreads = 1024;
 
 // Adds one to at[slot] for each active lane and returns the lane's place; lanes of the same slot share an addition for the
@@ -253,7 +253,7 @@ struct GroupLds {
 // ids in l.ids already (`local`), or in memory.
 __device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds& l, bool local) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int slots = p.keys + 1, padded = (p.n + 63) & ~63;
+    const int slots = p.keys, padded = (p.n + 63) & ~63;
     const bool small = p.n <= kGroupThreads;
     for (int i = tid; i < slots; i += kGroupThreads) at[i] = 0;
     __syncthreads();
@@ -264,7 +264,7 @@ __device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds
             p.clean[i] = ok ? id : -1;
             if (small) l.ids[i] = id;
         }
-        take_place(at, ok ? id : p.keys, i < p.n && (ok || p.none), lane);
+        take_place(at, id, ok, lane);
     }
     __syncthreads();
     // each thread owns a run of keys
@@ -304,9 +304,9 @@ __device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds
     __syncthreads();
     for (int i = tid; i < padded; i += kGroupThreads) {
         const int id = i < p.n ? (small ? l.ids[i] : p.ids[i]) : -1;
-        const bool ok = id >= 0 && id < p.keys, in = i < p.n && (ok || p.none);
-        const int place = take_place(at, ok ? id : p.keys, in, lane);
-        if (in) {
+        const bool ok = id >= 0 && id < p.keys;
+        const int place = take_place(at, id, ok, lane);
+        if (ok) {
             p.order[place] = i;
             if (small) l.order[place] = i;
         }
@@ -314,14 +314,14 @@ __device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds
     __syncthreads();
     for (int q = k0; q < k1; ++q)  // and now the place behind the key's last row
         for (const int end = at[q]; r0 < end; r0 = min(r0 + p.chunk_rows, end))
-            p.chunks[c0++] = Chunk{q == p.keys ? -1 : q, r0, min(p.chunk_rows, end - r0), small ? l.order[r0] : p.order[r0]};
+            p.chunks[c0++] = Chunk{q, r0, min(p.chunk_rows, end - r0), small ? l.order[r0] : p.order[r0]};
     for (int i = total + tid; i < p.max_chunks; i += kGroupThreads) p.chunks[i] = Chunk{-1, 0, 0, 0};
 }
 
-// One workgroup groups; those behind it rotate rows (the same that it groups, or others).
+// One workgroup groups; those behind it rotate rows.
 template <typename T>
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(const GroupArgs p, const RotateArgs beside) {
-    extern __shared__ int at[];  // [keys + 1]: counts, then places
+    extern __shared__ int at[];  // [keys]: counts, then places
     __shared__ GroupLds l;
     if (blockIdx.x == 0)
         group_rows(p, at, l, false);
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kGroupThreads) void choose_group_kernel(const Choos
 }  // namespace
 
 int launch_group(const GroupArgs& args, const RotateArgs& beside, int dtype, hipStream_t stream) {
-    const size_t lds = sizeof(int) * (static_cast<size_t>(args.keys) + 1);
+    const size_t lds = sizeof(int) * static_cast<size_t>(args.keys);
     const int64_t each = kGroupThreads / 64;
     const dim3 grid(static_cast<unsigned>(1 + (rotate_waves(beside) + each - 1) / each));
     if (dtype == 0)
@@ -385,7 +385,7 @@ int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs
     const bool together = group && a.tokens <= kGroupThreads / 64;
 #define QSRT_CHOOSE(SLOTS)                                                                                             \
     if (together)                                                                                                      \
-        hipLaunchKernelGGL(choose_group_kernel<SLOTS>, dim3(1), dim3(kGroupThreads), sizeof(int) * (group->keys + 1), \
+        hipLaunchKernelGGL(choose_group_kernel<SLOTS>, dim3(1), dim3(kGroupThreads), sizeof(int) * group->keys,      \
                            stream, ca, *group);                                                                        \
     else                                                                                                               \
         hipLaunchKernelGGL(choose_kernel<SLOTS>, dim3(static_cast<unsigned>(a.tokens)), dim3(64), 0, stream, ca)

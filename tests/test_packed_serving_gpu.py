@@ -293,6 +293,9 @@ def test_layer_in_a_graph():
     (31, 256, 256, (3, 4), "n", 40, 8, torch.bfloat16),
     (65, 128, 128, (4,), "k", 3, 33, torch.bfloat16),
     (200, 640, 128, (2,) * 5, "k", 1, 64, torch.float16),
+    (129, 384, 256, (2, 4, 3), "k", 9, 16, torch.bfloat16),            # three rates, many rows
+    (700, 512, 256, (3, 4), "n", 4, 40, torch.float16),
+    (1030, 256, 128, (4, 4), "k", 2, 5, torch.bfloat16),
 ])
 def test_adapters(t, k, n, bits, axis, adapters, rank, dtype):
     rng = np.random.default_rng(t + k + rank)
