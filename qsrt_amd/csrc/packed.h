@@ -142,28 +142,31 @@ __device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, 
     store_pieces((at.mat ? p.out[1] : p.out[0]) + row_place(p.layout, at.row), p.layout, at.kb, lane, v[0], v[1]);
 }
 
-// The same by a workgroup of 16 waves for rows laid out by 16, four blocks of channels at once: 16 rows by 512 channels, whose
-// 32 KiB leave in one stretch.
+// The same by a workgroup of four waves for rows laid out by 16, four blocks of channels at once: 16 rows by 512 channels,
+// whose 32 KiB leave in one stretch.
 constexpr int kRotateBlocks = 4;
 inline int64_t rotate_quads(const RotateArgs& p) { return (p.rows + 15) / 16 * p.nmat * ((p.kb + kRotateBlocks - 1) / kRotateBlocks); }
 template <typename T>
 __device__ __forceinline__ void rotate_quad(const RotateArgs& p, int64_t quad, u32x4 (&staged)[512 * kRotateBlocks]) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
     const int quads = (p.kb + kRotateBlocks - 1) / kRotateBlocks;
     const int64_t rest = quad / quads, sixteen = p.nmat == 2 ? rest >> 1 : rest;
     const int kb0 = kRotateBlocks * static_cast<int>(quad - rest * quads), mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
-    const int64_t row = 16 * sixteen + uniform(static_cast<int>(threadIdx.x >> 6));
-    f32x2 v[kRotateBlocks];
 #pragma unroll
-    for (int j = 0; j < kRotateBlocks; ++j)
-        v[j] = row < p.rows ? rotated<T>(p, RotateAt{row, min(kb0 + j, p.kb - 1), mat}, lane) : f32x2{0.f, 0.f};
+    for (int r = 0; r < 4; ++r) {
+        const int64_t row = 16 * sixteen + 4 * w + r;
+        f32x2 v[kRotateBlocks];
 #pragma unroll
-    for (int j = 0; j < kRotateBlocks; ++j)
-        store_pieces(reinterpret_cast<char*>(staged) + (row & 15) * p.layout.row, p.layout, j, lane, v[j][0], v[j][1]);
+        for (int j = 0; j < kRotateBlocks; ++j)  // past the last row and channel another's; not read by anyone who counts
+            v[j] = rotated<T>(p, RotateAt{min(row, p.rows - 1), min(kb0 + j, p.kb - 1), mat}, lane);
+#pragma unroll
+        for (int j = 0; j < kRotateBlocks; ++j)
+            store_pieces(reinterpret_cast<char*>(staged) + (row & 15) * p.layout.row, p.layout, j, lane, v[j][0], v[j][1]);
+    }
     __syncthreads();
     u32x4* out = reinterpret_cast<u32x4*>((mat ? p.out[1] : p.out[0]) + sixteen * p.layout.sixteen + 4 * kb0 * p.layout.strip);
     const int end = 512 * min(kRotateBlocks, p.kb - kb0);
-    for (int i = threadIdx.x; i < end; i += 1024) out[i] = staged[i];
+    for (int i = threadIdx.x; i < end; i += 256) out[i] = staged[i];
 }
 
 // At most chunk_rows rows of one key (an expert): order[first .. first + count), the first of them row0.

@@ -52,7 +52,9 @@ struct Tables {
 // window of 16 + 7 K bits of the tile's stream, two dwords.  Lane 16 g + m reads it in tile column 2 t + m / 8 of each pair
 // t, for i8 = 4 (m % 8) + g; MFMA 2 t + u has its columns m % 8 + 8 u as rows.  K is a value and not a template argument:
 // the same instructions with other shifts, where a body for each rate made the compiler keep a second set of sums.
-template <int G>
+// kPieces 2: 16 G rows, hi and lo pieces multiplied one after the other.  kPieces 1 (G 1): up to 8 rows, the hi piece of row n
+// in lanes n and the lo piece in lanes n + 8 of one product.
+template <int G, int kPieces>
 __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_bytes, int strips, int K,
                                                 const char* (&x)[G], int x_strip, int x_piece, const uint8_t* lut,
                                                 int lane, Tables& tables, f32x4 (&acc)[G][8]) {
@@ -78,11 +80,11 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
     tables.wait();
     int s = 0;
     do {
-        bf16x8 b[G][2];
+        bf16x8 b[G][kPieces];
 #pragma unroll
         for (int q = 0; q < G; ++q) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
+            for (int p = 0; p < kPieces; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
             x[q] += x_strip;
         }
         uint32_t next[16];
@@ -118,7 +120,7 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
                 av[u] = __builtin_bit_cast(bf16x8, a);
             }
 #pragma unroll
-            for (int p = 0; p < 2; ++p)  // hi pieces of all sums, then lo: a sum's two products do not follow each other
+            for (int p = 0; p < kPieces; ++p)  // hi pieces of all sums, then lo: a sum's two products do not follow each other
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -130,8 +132,9 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
     } while (++s < strips);
 }
 
-template <int G, int kWaves, int kTables>
+template <int G, int kPieces, int kWaves, int kTables>
 __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs p) {
+    static_assert(kPieces == 2 || G == 1, "half a group of rows is the least there is");
     __shared__ __attribute__((aligned(16))) uint8_t lut_s[65536 * kTables];
     const int lane = threadIdx.x & 63;
     const int w = uniform(static_cast<int>(threadIdx.x >> 6));
@@ -141,8 +144,8 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
             (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
     Tables tables;
 
-    constexpr int kRows = 16 * G;
-    const int n = lane & 15, g = lane >> 4;
+    constexpr int kRows = kPieces == 1 ? 8 : 16 * G;
+    const int g = lane >> 4, n = kPieces == 1 ? lane & 7 : lane & 15, piece = kPieces == 1 ? (lane >> 3) & 1 : 0;
     const int parts = p.parts;
     const uint32_t items = static_cast<uint32_t>(p.max_chunks) * p.nmat * p.nb * parts;  // below 2^31: see cut_parts
     const int64_t cols = 128 * static_cast<int64_t>(p.nb);
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
             const int at = first + min(16 * q + n, count - 1);
             row[q] = !p.chunks ? at : count == 1 ? row0 : p.order[at];
             x[q] = (mat ? p.x[1] : p.x[0]) + row_place(p.layout, p.x_div == 1 ? row[q] : row[q] / p.x_div) +
-                   g * p.layout.group + s * p.layout.strip;
+                   g * p.layout.group + s * p.layout.strip + piece * p.layout.piece;
         }
         f32x4 acc[G][8];
 #pragma unroll
@@ -229,19 +232,25 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                                         : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
             if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
                 const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
-                multiply_strips<G>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
+                multiply_strips<G, kPieces>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
             } else {  // another pass has this rate
 #pragma unroll
                 for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
             }
             s = stop;
         }
+        if constexpr (kPieces == 1) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[0][t][i] += dpp<0x128>(acc[0][t][i]);  // row rotated by 8: the other piece's
+        }
         // MFMA rows 4 g .. 4 g + 3: columns 16 (2 t + g / 2) + 8 u + 4 (g % 2) + 0..3 of row n
         float* out = p.part + (static_cast<int64_t>(p.pass * parts + part) * p.nmat + mat) * p.rows * cols + 128 * cb +
                      16 * (g >> 1) + 4 * (g & 1);
 #pragma unroll
         for (int q = 0; q < G; ++q) {
-            if (16 * q + n >= count) continue;
+            if (16 * q + n >= count || piece) continue;
 #pragma unroll
             for (int t = 0; t < 8; ++t)
                 *reinterpret_cast<f32x4*>(out + row[q] * cols + 32 * (t >> 1) + 8 * (t & 1)) = acc[q][t];
@@ -260,6 +269,13 @@ constexpr int kRowWaves = 8;
 // w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips' worth of them, then multiplies all of the
 // strip's by its own rows; one barrier a strip.  The table reads, which bound the product of a few rows, fall to an eighth a
 // row; the matrix cores (two pieces a row) are left as the bound.
+// A barrier that orders LDS alone: loads from memory stay on their way across it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int G>
 __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
                                               const uint8_t* lut, u32x2 (&frags)[2][8][128], int lane, int w, bool& ready,
@@ -286,12 +302,14 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
             for (int p = 0; p < 2; ++p)
                 next[q][p] = *(gbf8)(x[q] + static_cast<int64_t>(min(s, strips - 1)) * (16 * kStripBytes) + 1024 * p);
     };
-    auto decode = [&](int slot, int buffer) {
+    uint32_t label[8];
+    auto look_up = [&](int slot) {
         const uint32_t w0 = __builtin_amdgcn_alignbit(lo[slot], hi[slot], rsh);
         const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[slot] << sh, 32 - 4 * K);
-        uint32_t label[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) label[j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+    };
+    auto write_operands = [&](int buffer) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             u32x2 half;
@@ -311,9 +329,10 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
         ready = true;
     }
     __syncthreads();  // the tables are there, and no wave reads the operands of an earlier run
-    decode(0, 0);
+    look_up(0);
+    write_operands(0);
     fetch_words(2, 0);
-    __syncthreads();
+    lds_barrier();
     for (int s = 0; s < strips; s += 2) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // strip s + e of buffer e
@@ -324,8 +343,9 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
                     b[q][1] = next[q][1];
                 }
                 fetch_rows(s + e + 1);
-                decode(e ^ 1, e ^ 1);  // past the last strip: the last again, which nobody reads
+                look_up(e ^ 1);  // the next strip's labels are on their way while this one is multiplied
                 fetch_words(s + e + 3, e ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const bf16x8 a = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&frags[e][c][2 * lane]));
@@ -335,7 +355,9 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
                         for (int q = 0; q < G; ++q)
                             acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[q][p], acc[q][c], 0, 0, 0);
                 }
-                __syncthreads();
+                __builtin_amdgcn_sched_barrier(0);
+                write_operands(e ^ 1);  // past the last strip: the last again, which nobody reads
+                lds_barrier();
             }
         }
     }
@@ -573,7 +595,7 @@ struct ShrinkArgs {
     int rows, k, adapters, rank, parts;
     int shares;     // workgroups that share the adapters of 16 rows
 };
-constexpr int kShrinkWaves = 16, kShrinkSteps = 8;  // a workgroup's part of the K axis: 4096 channels at the most
+constexpr int kShrinkWaves = 4, kShrinkSteps = 8;  // a workgroup's part of the K axis: 1024 channels at the most
 
 inline int64_t shrink_blocks(const ShrinkArgs& p, int tiles) {
     return p.adapters ? static_cast<int64_t>((p.rows + 15) / 16) * p.parts * p.shares * (p.rank / (16 * tiles)) : 0;
@@ -665,7 +687,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void prepare_rows_kernel(const R
     else if (r.layout.row == 16)
         rotate_quad<T>(r, block - shrinks, l.staged);
     else
-        rotate_block<T>(r, static_cast<int64_t>(block - shrinks) * 16 + uniform(static_cast<int>(threadIdx.x >> 6)),
+        rotate_block<T>(r, static_cast<int64_t>(block - shrinks) * kShrinkWaves + uniform(static_cast<int>(threadIdx.x >> 6)),
                         threadIdx.x & 63);
 }
 
@@ -695,11 +717,29 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     const int count = min(16, p.rows - first);
     const int64_t cols = 128 * static_cast<int64_t>(p.nb), stride = p.rows * cols;
     const float* src = p.part + 128 * nb + 2 * lane;
+    const bool share = count < 4;
+    const int mine = share ? w < count : (count - w + 3) >> 2;  // rows of this wave
     int row[4], key[4];
     f32x2 v[4];
-    int mine;  // rows of this wave
-    if (count < 4) {
-        mine = w < count;
+    float low[2][4] = {};  // lane l: ranks l and 64 + l of each row's first product
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // rows past the last repeat another; not stored
+        row[i] = first + (share ? min(w, count - 1) : i < mine ? w + 4 * i : w);
+        v[i] = f32x2{0.f, 0.f};
+        key[i] = p.ids && i < mine ? uniform(p.ids[row[i]]) : -1;
+        if (key[i] >= p.adapters) key[i] = -1;
+    }
+    if (p.ids) {
+#pragma unroll 4
+        for (int s = 0; s < p.low_parts; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* at = p.low + (static_cast<int64_t>(s) * p.rows + row[i]) * p.rank;
+                low[0][i] += at[min(lane, p.rank - 1)];
+                if (p.rank > 64) low[1][i] += at[min(64 + lane, p.rank - 1)];
+            }
+    }
+    if (share) {
         for (int r = 0; r < count; ++r) {
             sums[w][lane] = sum_parts(src + (first + r) * cols, stride, w, 4, p.parts);
             __syncthreads();
@@ -707,15 +747,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
             __syncthreads();
         }
         if (!mine) return;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) row[i] = first + w;
     } else {
-        mine = (count - w + 3) >> 2;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // rows past the last repeat the wave's first; not stored
-            row[i] = first + (i < mine ? w + 4 * i : w);
-            v[i] = f32x2{0.f, 0.f};
-        }
         for (int s = 0; s < p.parts; s += 4) {  // sixteen loads in flight
             f32x2 t[4][4];
 #pragma unroll
@@ -729,11 +761,6 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
                 for (int i = 0; i < 4; ++i)
                     if (s + j < p.parts) v[i] += t[j][i];
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        key[i] = p.ids && i < mine ? uniform(p.ids[row[i]]) : -1;
-        if (key[i] >= p.adapters) key[i] = -1;
     }
     const f16x2 sv = reinterpret_cast<const f16x2*>(p.svh + 128 * nb)[lane];
 #pragma unroll
@@ -749,28 +776,29 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
         if (k < 0) continue;  // no adapter, or done with an earlier row
         const float scale = p.scale[k];
         const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(k) * cols + 128 * nb + 2 * lane) * p.rank;
-        for (int r0 = 0; r0 < p.rank; r0 += 64) {
-            float low[4] = {0.f, 0.f, 0.f, 0.f};  // lane l: rank r0 + l of each row
-            const int r = min(r0 + lane, p.rank - 1);
-            for (int s = 0; s < p.low_parts; ++s)
+        t8 next[4];  // sixteen ranks of both columns, asked for one turn ahead
+        auto fetch = [&](int r) {
+            r = min(r, p.rank - 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    low[i] += p.low[(static_cast<int64_t>(s) * p.rows + row[key[i] == k ? i : turn]) * p.rank + r];
+            for (int j = 0; j < 4; ++j)
+                next[j] = *reinterpret_cast<const t8*>(b0 + (j >> 1) * p.rank + r + 8 * (j & 1));
+        };
+        fetch(0);
+        for (int r = 0; r < p.rank; r += 16) {
+            t8 x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) low[i] *= scale;
-            for (int q = 0; q < 64 && r0 + q < p.rank; q += 8) {
-                const t8 x0 = *reinterpret_cast<const t8*>(b0 + r0 + q);
-                const t8 x1 = *reinterpret_cast<const t8*>(b0 + p.rank + r0 + q);
+            for (int j = 0; j < 4; ++j) x[j] = next[j];
+            fetch(r + 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (key[i] != k) continue;
+            for (int i = 0; i < 4; ++i) {
+                if (key[i] != k) continue;
+                const float mine_low = (r < 64 ? low[0][i] : low[1][i]) * scale;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float f = __builtin_bit_cast(
-                            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, low[i]), q + j));
-                        v[i][0] = __builtin_fmaf(f, static_cast<float>(x0[j]), v[i][0]);
-                        v[i][1] = __builtin_fmaf(f, static_cast<float>(x1[j]), v[i][1]);
-                    }
+                for (int j = 0; j < 16; ++j) {
+                    const float f = __builtin_bit_cast(
+                        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine_low), (r & 63) + j));
+                    v[i][0] = __builtin_fmaf(f, static_cast<float>(x[j >> 3][j & 7]), v[i][0]);
+                    v[i][1] = __builtin_fmaf(f, static_cast<float>(x[2 + (j >> 3)][j & 7]), v[i][1]);
                 }
             }
         }
@@ -793,12 +821,12 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
 
 constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one product, unless one part alone takes more
 
-template <int G, int kTables>
+template <int G, int kPieces, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
     constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
     const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nmat * args.nb * args.parts;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
-    hipLaunchKernelGGL((product_kernel<G, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
+    hipLaunchKernelGGL((product_kernel<G, kPieces, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
@@ -834,6 +862,9 @@ int launch_rows_g(const ProductArgs& args, int cus, hipStream_t stream) {
 // Groups of 16 rows that each of a workgroup's eight waves has in product_rows_kernel; 0: the rows are too few for it.
 int row_groups(int64_t rows) { return rows <= 128 ? 0 : rows <= 256 ? 2 : 4; }
 
+// Rows that a wave multiplies at once: `groups` times 16, or 8 with groups 0.
+int chunk_rows_of(int groups) { return groups ? 16 * groups : 8; }
+
 // All passes of a product: the tables of at most two rates fit LDS at once.
 int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
     int set[3], n = 0;
@@ -853,9 +884,10 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
             if (rc != kOk) return rc;
             continue;
         }
-        const int rc = groups == 1   ? (two ? launch_product_g<1, 2> : launch_product_g<1, 1>)(args, cus, stream)
-                       : groups == 2 ? (two ? launch_product_g<2, 2> : launch_product_g<2, 1>)(args, cus, stream)
-                                     : (two ? launch_product_g<4, 2> : launch_product_g<4, 1>)(args, cus, stream);
+        const int rc = groups == 0   ? (two ? launch_product_g<1, 1, 2> : launch_product_g<1, 1, 1>)(args, cus, stream)
+                       : groups == 1 ? (two ? launch_product_g<1, 2, 2> : launch_product_g<1, 2, 1>)(args, cus, stream)
+                       : groups == 2 ? (two ? launch_product_g<2, 2, 2> : launch_product_g<2, 2, 1>)(args, cus, stream)
+                                     : (two ? launch_product_g<4, 2, 2> : launch_product_g<4, 2, 1>)(args, cus, stream);
         if (rc != kOk) return rc;
     }
     return kOk;
@@ -933,12 +965,14 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
                    bool shared, bool router, int cus) {
     MoeSpace s;
     const int64_t pairs = tokens * k;
-    s.groups = pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;  // groups of 16 rows a wave multiplies at once
-    s.max_chunks = static_cast<int>(most_chunks(pairs, experts, 16 * s.groups));
+    // an expert's rows are one chunk more often than not: 2% of experts get over 8 of 4 a head
+    s.groups = pairs <= 4 * experts ? 0 : pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;
+    const int chunk_rows = chunk_rows_of(s.groups);
+    s.max_chunks = static_cast<int>(most_chunks(pairs, experts, chunk_rows));
     // chunks to expect under an even router; the parts are cut for them, as the host does not wait for the real ones
     const double touched = experts * (1.0 - std::pow(1.0 - 1.0 / experts, static_cast<double>(pairs)));
-    const double each = pairs / touched, chunks = std::max(1.0, touched * std::ceil(each / (16.0 * s.groups)));
-    const int rows = static_cast<int>(std::min<double>(16 * s.groups, std::ceil(each)));
+    const double each = pairs / touched, chunks = std::max(1.0, touched * std::ceil(each / chunk_rows));
+    const int rows = static_cast<int>(std::min<double>(chunk_rows, std::ceil(each)));
     Carve c{static_cast<char*>(ws)};
     s.chunks = c.take<Chunk>(s.max_chunks);
     s.order = c.take<int>(pairs);
@@ -1041,7 +1075,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ga.ids = c.ids;
     ga.n = static_cast<int>(pairs);
     ga.keys = static_cast<int>(c.experts);
-    ga.chunk_rows = 16 * s.groups;
+    ga.chunk_rows = chunk_rows_of(s.groups);
     ga.max_chunks = s.max_chunks;
     ga.chunks = s.chunks;
     ga.order = s.order;
@@ -1188,9 +1222,9 @@ struct LinearSpace {
 LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates, int64_t adapters, int64_t rank, int cus) {
     LinearSpace s{};
     Carve c{static_cast<char*>(ws)};
-    s.groups = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    s.groups = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     s.passes = passes_of(rates);
-    const int64_t group_rows = 16 * (row_groups(rows) ? kRowWaves * row_groups(rows) : s.groups);
+    const int64_t group_rows = row_groups(rows) ? 16 * kRowWaves * row_groups(rows) : chunk_rows_of(s.groups);
     const int64_t chunks = (rows + group_rows - 1) / group_rows;
     s.product_chunks = static_cast<int>(chunks);
     const int strips = static_cast<int>(k / 32), limit = part_limit(rows * n * s.passes, strips);
@@ -1261,12 +1295,12 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     sa.rank = static_cast<int>(rank);
     sa.parts = s.low_parts;
     const int tiles = adapters && rank % 32 == 0 ? 2 : 1;  // of 16 ranks a workgroup
-    // the adapters of 16 rows are shared out while that leaves no more workgroups than two a compute unit
+    // the adapters of 16 rows are shared out while that leaves no more workgroups than four a compute unit
     if (adapters)
         sa.shares = static_cast<int>(std::max<int64_t>(
-            1, std::min<int64_t>(std::min<int64_t>(16, rows), 2 * cus / std::max<int64_t>(1, sixteens(rows) / 16 * s.low_parts * (rank / (16 * tiles))))));
+            1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / std::max<int64_t>(1, sixteens(rows) / 16 * s.low_parts * (rank / (16 * tiles))))));
     const int64_t shrinks = shrink_blocks(sa, tiles);
-    const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + 15) / 16;
+    const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + kShrinkWaves - 1) / kShrinkWaves;
     if (shrinks + rotates >= int64_t(1) << 31) return fail(kBadArgument, "qsrt_adapter_linear: too many rows");
     const dim3 pgrid(static_cast<unsigned>(shrinks + rotates)), pblock(64 * kShrinkWaves);
 #define QSRT_PREPARE(T)                                                                                              \
