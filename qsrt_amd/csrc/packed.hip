@@ -54,7 +54,10 @@ struct Tables {
 // the same instructions with other shifts, where a body for each rate made the compiler keep a second set of sums.
 // kPieces 2: 16 G rows, hi and lo pieces multiplied one after the other.  kPieces 1 (G 1): up to 8 rows, the hi piece of row n
 // in lanes n and the lo piece in lanes n + 8 of one product.
-template <int G, int kPieces>
+// kPairs (K 2 alone): `lut` holds a row of 8 bytes for each 14 bits that two successive states share, the label of the first
+// state for each value x of its other bits at byte 2 x, of the second for each y at byte 2 y + 1.  A lookup costs the banks
+// the same at 8 bytes as at one (7.3 clocks for 64 random lanes), so this halves what bounds the product.
+template <int G, int kPieces, bool kPairs>
 __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_bytes, int strips, int K,
                                                 const char* (&x)[G], int x_strip, int x_piece, const uint8_t* lut,
                                                 int lane, Tables& tables, f32x4 (&acc)[G][8]) {
@@ -87,35 +90,70 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
             for (int p = 0; p < kPieces; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
             x[q] += x_strip;
         }
-        uint32_t next[16];
+        uint32_t next[16], window[2];
+        uint32_t rest = 0x0C000C01u;  // the selector's fixed part, in a vector register: one instruction takes one scalar
+        asm volatile("" : "+v"(rest));
+        u32x2 next_row[8];
         auto gather = [&](int t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // bits 0..31 of the window, and 4 K .. 4 K + 31: four labels in each
                 const uint32_t w0 = __builtin_amdgcn_alignbit(lo[2 * t + h], hi[2 * t + h], rsh);
-                const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[2 * t + h] << sh, 32 - 4 * K);
+                if constexpr (kPairs) {
+                    window[h] = w0;  // 30 bits: x, 14 shared bits, y of each pair, two bits further on for the next but one
 #pragma unroll
-                for (int j = 0; j < 8; ++j) next[8 * h + j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+                    for (int j = 0; j < 4; ++j)
+                        next_row[4 * h + j] = *reinterpret_cast<const u32x2*>(lut + ((w0 >> (13 - 4 * j)) & 0x1FFF8u));
+                } else {
+                    // bits 0..31 of the window, and 4 K .. 4 K + 31: four labels in each
+                    const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[2 * t + h] << sh, 32 - 4 * K);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        next[8 * h + j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+                }
             }
             fetch(min(s + 1, strips - 1), t);  // the last strip asks for itself again: no branch, so that waits stay exact
         };
         gather(0);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            uint32_t label[16];
+            uint32_t label[16], seen[2];
+            u32x2 row[8];
+            if constexpr (kPairs) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) label[j] = next[j];
+                for (int j = 0; j < 8; ++j) row[j] = next_row[j];
+                seen[0] = window[0];
+                seen[1] = window[1];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) label[j] = next[j];
+            }
             if (t < 3) gather(t + 1);
             bf16x8 av[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 u32x4 a;
+                if constexpr (kPairs) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int j = 8 * (q >> 1) + 4 * u + 2 * (q & 1);
-                    a[q] = __builtin_bit_cast(
-                        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-                                      __builtin_amdgcn_perm(label[j + 1], label[j], 0x0C0C0400u), 1.0f, false));
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t two[2];  // a pair's second label in byte 0, its first in byte 2
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int j = 2 * u + q;
+                            two[q] = __builtin_amdgcn_perm(row[4 * h + j][1], row[4 * h + j][0],
+                                                           ((seen[h] >> (13 - 4 * j)) & 0x00060006u) | rest);
+                        }
+                        const uint32_t four = __builtin_amdgcn_perm(two[1], two[0], 0x04060002u);
+                        a[2 * h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, false));
+                        a[2 * h + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, true));
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int j = 8 * (q >> 1) + 4 * u + 2 * (q & 1);
+                        a[q] = __builtin_bit_cast(
+                            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                          __builtin_amdgcn_perm(label[j + 1], label[j], 0x0C0C0400u), 1.0f, false));
+                    }
                 }
                 av[u] = __builtin_bit_cast(bf16x8, a);
             }
@@ -132,16 +170,45 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
     } while (++s < strips);
 }
 
+// Rows of label pairs from the K2 table: four rows a thread and turn, their first states' labels from the table's quarters.
+template <int kThreads>
+__device__ __forceinline__ void build_pairs(const uint8_t* table, uint8_t* rows) {
+#pragma unroll
+    for (int i = 0; i < 4096 / kThreads; ++i) {
+        const int c = 4 * (threadIdx.x + i * kThreads);
+        uint32_t quarter[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) quarter[x] = *reinterpret_cast<const uint32_t*>(table + 16384 * x + c);
+        const u32x4 second = *reinterpret_cast<const u32x4*>(table + 4 * c);
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            u32x4 two;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {  // row r + d / 2: {first x, second x, first x + 1, second x + 1}, x = 2 (d % 2)
+                const int at = r + (d >> 1), x = 2 * (d & 1);
+                const uint32_t first = __builtin_amdgcn_perm(quarter[x + 1], quarter[x], 0x0C040C00u + 0x00010001u * at);
+                const uint32_t other = __builtin_amdgcn_perm(0u, second[at], x ? 0x030C020Cu : 0x010C000Cu);
+                two[d] = first | other;
+            }
+            *reinterpret_cast<u32x4*>(rows + 8 * (c + r)) = two;
+        }
+    }
+}
+
+// kTables: label tables in LDS; 0: the pairs of the K2 table.
 template <int G, int kPieces, int kWaves, int kTables>
 __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs p) {
     static_assert(kPieces == 2 || G == 1, "half a group of rows is the least there is");
-    __shared__ __attribute__((aligned(16))) uint8_t lut_s[65536 * kTables];
+    __shared__ __attribute__((aligned(16))) uint8_t lut_s[kTables ? 65536 * kTables : 131072];
     const int lane = threadIdx.x & 63;
     const int w = uniform(static_cast<int>(threadIdx.x >> 6));
-    for (int i = w; i < kTables * 64; i += kWaves)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)((i < 64 ? p.lut[0] : p.lut[1]) + 1024 * (i & 63) + 16 * lane),
-            (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
+    if constexpr (kTables == 0)
+        build_pairs<64 * kWaves>(p.lut[0], lut_s);
+    else
+        for (int i = w; i < kTables * 64; i += kWaves)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)((i < 64 ? p.lut[0] : p.lut[1]) + 1024 * (i & 63) + 16 * lane),
+                (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
     Tables tables;
 
     constexpr int kRows = kPieces == 1 ? 8 : 16 * G;
@@ -232,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                                         : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
             if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
                 const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
-                multiply_strips<G, kPieces>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
+                multiply_strips<G, kPieces, kTables == 0>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
             } else {  // another pass has this rate
 #pragma unroll
                 for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
@@ -884,10 +951,14 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
             if (rc != kOk) return rc;
             continue;
         }
-        const int rc = groups == 0   ? (two ? launch_product_g<1, 1, 2> : launch_product_g<1, 1, 1>)(args, cus, stream)
-                       : groups == 1 ? (two ? launch_product_g<1, 2, 2> : launch_product_g<1, 2, 1>)(args, cus, stream)
-                       : groups == 2 ? (two ? launch_product_g<2, 2, 2> : launch_product_g<2, 2, 1>)(args, cus, stream)
-                                     : (two ? launch_product_g<4, 2, 2> : launch_product_g<4, 2, 1>)(args, cus, stream);
+        const bool pairs = args.luts == 1 && args.lut_bits[0] == 2;
+#define QSRT_PRODUCT(G, PIECES) \
+    (pairs ? launch_product_g<G, PIECES, 0> : two ? launch_product_g<G, PIECES, 2> : launch_product_g<G, PIECES, 1>)(args, cus, stream)
+        const int rc = groups == 0   ? QSRT_PRODUCT(1, 1)
+                       : groups == 1 ? QSRT_PRODUCT(1, 2)
+                       : groups == 2 ? QSRT_PRODUCT(2, 2)
+                                     : QSRT_PRODUCT(4, 2);
+#undef QSRT_PRODUCT
         if (rc != kOk) return rc;
     }
     return kOk;
