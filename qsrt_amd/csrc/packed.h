@@ -100,6 +100,7 @@ struct RotateArgs {
     int64_t suh_stride[2];
     const int* ids;  // null: one scale vector for all; else row r of the result is row r / x_div of x at scale ids[r]
     int x_div;
+    int every;       // not 0: that many rows of x at every scale, row r of the result is row r % every at scale r / every
     char* out[2];
     int64_t rows;
     int kb, nmat;
@@ -121,10 +122,11 @@ __device__ __forceinline__ RotateAt rotate_at(const RotateArgs& p, int64_t wave)
 
 template <typename T>
 __device__ __forceinline__ f32x2 rotated(const RotateArgs& p, const RotateAt& at, int lane) {
-    const int id = p.ids ? max(p.ids[at.row], 0) : 0;
+    const int64_t id = p.every ? at.row / p.every : p.ids ? max(p.ids[at.row], 0) : 0;
+    const int64_t from = p.every ? at.row - id * p.every : p.x_div == 1 ? at.row : at.row / p.x_div;
     const _Float16* suh =
         (at.mat ? p.suh[1] : p.suh[0]) + id * (at.mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * at.kb;
-    const T* x = static_cast<const T*>(p.x) + (p.x_div == 1 ? at.row : at.row / p.x_div) * p.ld + 128 * at.kb;
+    const T* x = static_cast<const T*>(p.x) + from * p.ld + 128 * at.kb;
     typedef T t2 __attribute__((ext_vector_type(2)));
     const t2 xv = reinterpret_cast<const t2*>(x)[lane];
     const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];

@@ -1,7 +1,6 @@
 // Products of a few rows with packed trellis matrices, and what stands around them in a mixture-of-experts layer.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "packed.h"
 #include "qsrt_amd.h"
@@ -21,7 +20,7 @@ struct ProductArgs {
     int64_t record_stride[2];     // 0: one table for every key
     const char* x[2];             // rotated rows
     RowLayout layout;
-    int x_div;                    // row of order entry o: o / x_div
+    int x_div, x_every;           // row of order entry o with key e: e x_every + o / x_div
     const Chunk* chunks;          // null: runs of kRows rows of `rows`
     const int* order;
     int max_chunks, parts;
@@ -174,8 +173,9 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
 template <int kThreads>
 __device__ __forceinline__ void build_pairs(const uint8_t* table, uint8_t* rows) {
 #pragma unroll
-    for (int i = 0; i < 4096 / kThreads; ++i) {
+    for (int i = 0; i < (4096 + kThreads - 1) / kThreads; ++i) {
         const int c = 4 * (threadIdx.x + i * kThreads);
+        if (c >= 16384) break;
         uint32_t quarter[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) quarter[x] = *reinterpret_cast<const uint32_t*>(table + 16384 * x + c);
@@ -268,8 +268,9 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
         for (int q = 0; q < G; ++q) {  // lanes past the last row repeat it; their sums are not stored
             const int at = first + min(16 * q + n, count - 1);
             row[q] = !p.chunks ? at : count == 1 ? row0 : p.order[at];
-            x[q] = (mat ? p.x[1] : p.x[0]) + row_place(p.layout, p.x_div == 1 ? row[q] : row[q] / p.x_div) +
-                   g * p.layout.group + s * p.layout.strip + piece * p.layout.piece;
+            const int64_t from = static_cast<int64_t>(key) * p.x_every + (p.x_div == 1 ? row[q] : row[q] / p.x_div);
+            x[q] = (mat ? p.x[1] : p.x[0]) + row_place(p.layout, from) + g * p.layout.group + s * p.layout.strip +
+                   piece * p.layout.piece;
         }
         f32x4 acc[G][8];
 #pragma unroll
@@ -299,7 +300,8 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                                         : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
             if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
                 const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
-                multiply_strips<G, kPieces, kTables == 0>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece, lut, lane, tables, acc);
+                multiply_strips<G, kPieces, kTables == 0>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece,
+                                                          lut, lane, tables, acc);
             } else {  // another pass has this rate
 #pragma unroll
                 for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
@@ -332,10 +334,6 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 
 constexpr int kRowWaves = 8;
 
-// Eight waves of 16 G rows each over the same columns.  Wave w decodes one window a lane of every strip (tile column pair
-// w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips' worth of them, then multiplies all of the
-// strip's by its own rows; one barrier a strip.  The table reads, which bound the product of a few rows, fall to an eighth a
-// row; the matrix cores (two pieces a row) are left as the bound.
 // A barrier that orders LDS alone: loads from memory stay on their way across it.
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -343,6 +341,10 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Eight waves of 16 G rows each over the same columns.  Wave w decodes one window a lane of every strip (tile column pair
+// w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips' worth of them, then multiplies all of the
+// strip's by its own rows; one barrier a strip.  The table reads, which bound the product of a few rows, fall to an eighth a
+// row; the matrix cores (two pieces a row) are left as the bound.
 template <int G>
 __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
                                               const uint8_t* lut, u32x2 (&frags)[2][8][128], int lane, int w, bool& ready,
@@ -489,7 +491,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void product_rows_kernel(const Prod
             }
             s = stop;
         }
-        float* out = p.part + static_cast<int64_t>(p.pass * p.parts + part) * p.rows * cols + 128 * cb + 16 * (g >> 1) + 4 * (g & 1);
+        float* out = p.part + static_cast<int64_t>(p.pass * p.parts + part) * p.rows * cols + 128 * cb + 16 * (g >> 1) +
+                     4 * (g & 1);
 #pragma unroll
         for (int q = 0; q < G; ++q) {
             const int64_t row = 16 * static_cast<int64_t>(first + q) + n;
@@ -890,7 +893,7 @@ constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one produ
 
 template <int G, int kPieces, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
-    constexpr int kWaves = G == 1 ? 16 : 8;  // 128 and 256 registers a lane
+    constexpr int kWaves = G == 1 ? 16 : G == 2 ? 12 : 8;  // 128, 168 and 256 registers a lane
     const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nmat * args.nb * args.parts;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
     hipLaunchKernelGGL((product_kernel<G, kPieces, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
@@ -926,14 +929,11 @@ int launch_rows_g(const ProductArgs& args, int cus, hipStream_t stream) {
     return kOk;
 }
 
-// Groups of 16 rows that each of a workgroup's eight waves has in product_rows_kernel; 0: the rows are too few for it.
-int row_groups(int64_t rows) { return rows <= 128 ? 0 : rows <= 256 ? 2 : 4; }
-
 // Rows that a wave multiplies at once: `groups` times 16, or 8 with groups 0.
 int chunk_rows_of(int groups) { return groups ? 16 * groups : 8; }
 
-// All passes of a product: the tables of at most two rates fit LDS at once.
-int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
+// All passes of a product: the tables of at most two rates fit LDS at once.  `row_groups`: as in cut_rows (0: product_kernel).
+int launch_product(ProductArgs args, int groups, int row_groups, int rates, const uint8_t* const* luts, int cus, hipStream_t stream) {
     int set[3], n = 0;
     for (int b = 2; b <= 4; ++b)
         if (rates >> b & 1) set[n++] = b;
@@ -945,9 +945,9 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
             args.lut[j] = luts[set[first + j] - 2];
         }
         const bool two = args.luts > 1;
-        if (!args.chunks && row_groups(args.rows)) {
-            const int rc = row_groups(args.rows) == 2 ? (two ? launch_rows_g<2, 2> : launch_rows_g<2, 1>)(args, cus, stream)
-                                                      : (two ? launch_rows_g<4, 2> : launch_rows_g<4, 1>)(args, cus, stream);
+        if (row_groups) {
+            const int rc = row_groups == 2 ? (two ? launch_rows_g<2, 2> : launch_rows_g<2, 1>)(args, cus, stream)
+                                           : (two ? launch_rows_g<4, 2> : launch_rows_g<4, 1>)(args, cus, stream);
             if (rc != kOk) return rc;
             continue;
         }
@@ -966,17 +966,27 @@ int launch_product(ProductArgs args, int groups, int rates, const uint8_t* const
 
 int passes_of(int rates) { return __builtin_popcount(rates & 0x1C) > 2 ? 2 : 1; }
 
-// The same for product_rows_kernel, a workgroup an item: a strip takes its eight waves about 1.1 us, a part's sums (256 KB a
-// workgroup) as long as 16 strips, there and back, and its set-up 3.
-int cut_row_parts(int64_t units, int strips, int limit, int cus) {
-    int best = 1;
+// The same for product_rows_kernel, with the groups of 16 rows that each of a workgroup's eight waves takes.  A workgroup is an
+// item; with 4 groups a strip takes it about 1.1 us, a part's sums (256 KB) as long as 16 strips, there and back, and its
+// set-up 3.  With 2 all of it takes 0.6 of that: half the rows, at the same reads of the payload and the tables.  So few
+// rows or items go with 2 (7168 x 7168, 256 rows: 92 us, with 4 124; 5120 x 2048, 512 rows: 60 and 66), many with 4
+// (7168 x 7168, 4096 rows: 897 us, with 2 1022).
+struct RowCut {
+    int groups, parts;
+};
+RowCut cut_rows(int64_t rows, int64_t nb, int strips, int limit, int cus) {
+    RowCut best{4, 1};
     double least = 0.0;
-    for (int p = 1; p <= std::min(limit, strips); ++p) {
-        if (units * p >= int64_t(1) << 31) break;
-        const double cost = std::ceil(static_cast<double>(units * p) / cus) * ((strips + p - 1) / p + 19.0);
-        if (p == 1 || cost < least) {
-            least = cost;
-            best = p;
+    for (const int groups : {4, 2}) {
+        const int64_t each = 16 * kRowWaves * groups, units = (rows + each - 1) / each * nb;
+        for (int p = 1; p <= std::min(limit, strips); ++p) {
+            if (units * p >= int64_t(1) << 31) break;
+            const double turns = std::ceil(static_cast<double>(units * p) / cus);
+            const double cost = turns * ((strips + p - 1) / p + 19.0) * (groups == 4 ? 1.0 : 0.6);
+            if (least == 0.0 || cost < least) {
+                least = cost;
+                best = RowCut{groups, p};
+            }
         }
     }
     return best;
@@ -985,7 +995,8 @@ int cut_row_parts(int64_t units, int strips, int limit, int cus) {
 const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts) {
     if (!m || !m->words || !m->records || !m->suh || !m->svh) return "null pointer in a matrix";
     if (m->rows <= 0 || m->cols <= 0 || m->rows % 128 || m->cols % 128) return "rows and cols must be multiples of 128";
-    if (m->rows > (1 << 22) || m->cols > (1 << 22)) return "matrix too large";
+    if (m->rows > (1 << 22) || m->cols > (1 << 22) || m->rows * m->cols >= int64_t(1) << 32)
+        return "matrix too large (2^32 weights)";  // the kernels' offsets in a payload have 31 bits, K4 takes half a byte
     if (m->rate_axis != 0 && m->rate_axis != 1) return "rate_axis must be 0 (rows) or 1 (columns)";
     if ((m->rates & 0x1C) == 0 || (m->rates & ~0x1C)) return "rates must name K2, K3 or K4";
     if (m->key_stride < 0 || m->record_stride < 0 || m->suh_stride < 0 || m->svh_stride < 0) return "negative stride";
@@ -998,6 +1009,9 @@ const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts
             return "a rate's label table is missing or not 16-byte aligned";
     return nullptr;
 }
+
+// A launch has fewer than 2^32 threads; none here takes more than one for two channels, of rows rounded up to 16.
+bool launch_fits(int64_t rows, int64_t a, int64_t b) { return (rows + 15) / 16 * 16 * std::max(a, b) < int64_t(1) << 32; }
 
 const char* rows_fault(const void* p, int64_t ld, int64_t cols, int align) {
     if (!p) return "null rows";
@@ -1029,6 +1043,7 @@ struct MoeSpace {
     char *x[2], *mid;
     float *part, *logits;
     int parts[2], passes[2], groups, max_chunks;
+    bool every;  // rows are rotated at every expert's scales, before the choice is known
     size_t bytes;
 };
 
@@ -1036,7 +1051,10 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
                    bool shared, bool router, int cus) {
     MoeSpace s;
     const int64_t pairs = tokens * k;
-    // an expert's rows are one chunk more often than not: 2% of experts get over 8 of 4 a head
+    // An expert's rows are one chunk more often than not: 2% of experts get over 8 of 4 a head.  Larger chunks cost more a
+    // strip, more chunks decode again (16 experts, 4096 x 1536 at K3, us a layer with chunks of 8, 16, 32, 64: 4 rows a head
+    // 91, 91, 94, 105; 8 rows 126, 95, 100, 112; 16 rows 182, 148, 107, 121; 24 rows 252, 164, 132, 155; 32 rows 319, 200,
+    // 177, 162).
     s.groups = pairs <= 4 * experts ? 0 : pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;
     const int chunk_rows = chunk_rows_of(s.groups);
     s.max_chunks = static_cast<int>(most_chunks(pairs, experts, chunk_rows));
@@ -1049,7 +1067,11 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
     s.order = c.take<int>(pairs);
     s.clean = c.take<int>(pairs);
     s.logits = c.take<float>(router ? router_logit_bytes(tokens, hidden, experts) / sizeof(float) : 0);
-    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>(sixteens(shared ? tokens : pairs) * hidden * 4);
+    // Scales of their own: a row at a scale is a wave's few microseconds, and while all of them fit the chip at once beside
+    // the router they save a launch behind the choice (8 experts, 256 channels: 33 -> 29 us a layer).
+    s.every = !shared && router && tokens * experts * (hidden / 128) <= 1024;
+    for (int m = 0; m < 2; ++m)
+        s.x[m] = c.take<char>(sixteens(shared ? tokens : s.every ? tokens * experts : pairs) * hidden * 4);
     s.mid = c.take<char>(sixteens(pairs) * inter * 4);
     s.passes[0] = passes_of(rates13);
     s.passes[1] = passes_of(rates2);
@@ -1099,13 +1121,9 @@ const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3
     if (experts < 1 || experts > kMaxKeys) return "experts must be 1 .. 8191";
     if (k < 1 || k > (1 << 20) || tokens < 0 || tokens > (1 << 20) || tokens * k > (1 << 20))
         return "tokens * k must be at most 2^20";
-    if (tokens * k * std::max(2 * w1->cols, w1->rows) / 128 >= int64_t(1) << 31) return "too many tokens for these matrices";
+    if (!launch_fits(tokens * k, w1->cols, w1->rows)) return "too many tokens for these matrices";
     return nullptr;
 }
-
-}  // namespace
-
-namespace {
 
 struct MoeCall {
     const qsrt_packed_matrix *w1, *w3, *w2;
@@ -1158,16 +1176,17 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ra.suh[1] = static_cast<const _Float16*>(c.w3->suh);
     ra.suh_stride[0] = c.w1->suh_stride;
     ra.suh_stride[1] = c.w3->suh_stride;
-    ra.ids = shared ? nullptr : s.clean;
+    ra.ids = shared || s.every ? nullptr : s.clean;
     ra.x_div = shared ? 1 : c.k;
+    ra.every = s.every ? static_cast<int>(c.tokens) : 0;
     ra.out[0] = s.x[0];
     ra.out[1] = s.x[1];
-    ra.rows = shared ? c.tokens : pairs;
+    ra.rows = shared ? c.tokens : s.every ? c.tokens * c.experts : pairs;
     ra.kb = static_cast<int>(hidden / 128);
     ra.nmat = 2;
     ra.layout = row_layout(ra.kb, s.groups > 1);
     RotateArgs beside = ra;  // rows that all experts share are rotated beside the router or the grouping
-    if (!shared) beside.rows = 0;
+    if (!shared && !s.every) beside.rows = 0;
     if (router) {
         router->logits = s.logits;
         if (const char* e = router_fault(*router)) return fail(kBadArgument, "%s: %s", name, e);
@@ -1175,7 +1194,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     } else if (const int rc = launch_group(ga, beside, c.dtype, stream)) {
         return rc;
     }
-    if (!shared)
+    if (!shared && !s.every)
         if (const int rc = launch_rotate(ra, c.dtype, stream)) return rc;
 
     ProductArgs pa{};
@@ -1183,7 +1202,8 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     set_matrix(pa, 1, c.w3);
     pa.x[0] = s.x[0];
     pa.x[1] = s.x[1];
-    pa.x_div = shared ? c.k : 1;
+    pa.x_div = shared || s.every ? c.k : 1;
+    pa.x_every = ra.every;
     pa.layout = ra.layout;
     pa.chunks = s.chunks;
     pa.order = s.order;
@@ -1192,7 +1212,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     pa.part = s.part;
     pa.nmat = 2;
     pa.rows = static_cast<int>(pairs);
-    if (const int rc = launch_product(pa, s.groups, rates13, c.luts, cus, stream)) return rc;
+    if (const int rc = launch_product(pa, s.groups, 0, rates13, c.luts, cus, stream)) return rc;
 
     MiddleArgs ma{};
     ma.part = s.part;
@@ -1224,7 +1244,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     pb.part = s.part;
     pb.nmat = 1;
     pb.rows = static_cast<int>(pairs);
-    if (const int rc = launch_product(pb, s.groups, c.w2->rates, c.luts, cus, stream)) return rc;
+    if (const int rc = launch_product(pb, s.groups, 0, c.w2->rates, c.luts, cus, stream)) return rc;
 
     CombineArgs ca{};
     ca.part = s.part;
@@ -1254,9 +1274,12 @@ extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, 
     int cus = 0;
     if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0 || current_cu_count(&cus))
         return 0;
-    return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates, w1->suh_stride == 0,
-                     true, cus)
-        .bytes;
+    size_t most = 0;  // of both calls
+    for (const bool router : {false, true})
+        most = std::max(most, moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates,
+                                        w1->suh_stride == 0, router, cus)
+                                  .bytes);
+    return most;
 }
 
 extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
@@ -1286,22 +1309,36 @@ namespace {
 struct LinearSpace {
     char* x;
     float *low, *part;
-    int low_parts, parts, passes, groups, product_chunks;
+    int low_parts, parts, passes, groups, row_groups, product_chunks;
+    bool grouped;  // layout of the rotated rows
     size_t bytes;
 };
 
 LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates, int64_t adapters, int64_t rank, int cus) {
     LinearSpace s{};
     Carve c{static_cast<char*>(ws)};
-    s.groups = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    // Chunks of 8, 16, 32 and 64 rows, each up to two of them: more rows a wave share a decode, fewer leave more waves to
+    // share the matrix (7168 x 7168 at K3: 12 rows 36 us in one chunk of 16, 45 in two of 8; 64 rows 51 in two of 32, 54 in
+    // one of 64; 96 rows 60 in two of 64, 64 in three of 32).  Beyond 128 a workgroup shares each decode (192 rows: 85 us,
+    // 111 without; 128 rows: 82, without 64).
+    s.groups = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 64 ? 2 : 4;
+    // Rows by 16 are rotated by a quarter of the waves, which costs 2 to 3 us until the reads of the product outweigh it
+    // (7168 x 7168: 24 rows 42.7 us as rows, 45 by 16; 48 rows the same; 64 rows 58 and 56).
+    s.grouped = rows > 48;
     s.passes = passes_of(rates);
-    const int64_t group_rows = row_groups(rows) ? 16 * kRowWaves * row_groups(rows) : chunk_rows_of(s.groups);
+    const int64_t nb = n / 128;
+    const int strips = static_cast<int>(k / 32), limit = part_limit(rows * n * s.passes, strips);
+    if (rows > 128) {
+        const RowCut cut = cut_rows(rows, nb, strips, limit, cus);
+        s.row_groups = cut.groups;
+        s.parts = cut.parts;
+    }
+    const int64_t group_rows = s.row_groups ? 16 * kRowWaves * s.row_groups : chunk_rows_of(s.groups);
     const int64_t chunks = (rows + group_rows - 1) / group_rows;
     s.product_chunks = static_cast<int>(chunks);
-    const int strips = static_cast<int>(k / 32), limit = part_limit(rows * n * s.passes, strips);
-    s.parts = row_groups(rows) ? cut_row_parts(chunks * (n / 128), strips, limit, cus)
-                               : cut_parts(static_cast<double>(chunks * (n / 128)), chunks * (n / 128), strips, limit,
-                                           static_cast<int>(std::min(rows, group_rows)), cus);
+    if (!s.row_groups)
+        s.parts = cut_parts(static_cast<double>(chunks * nb), chunks * nb, strips, limit,
+                            static_cast<int>(std::min(rows, group_rows)), cus);
     if (adapters) {
         constexpr int64_t kPart = 32 * kShrinkWaves * kShrinkSteps;
         s.low_parts = static_cast<int>((k + kPart - 1) / kPart);
@@ -1335,7 +1372,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a, b of a rank 16, 32 .. 128, scales and ids");
     if (rows == 0) return kOk;
     const int64_t k = w->rows, n = w->cols;
-    if (rows * (n / 128) >= int64_t(1) << 31) return fail(kBadArgument, "qsrt_adapter_linear: too many rows for this matrix");
+    if (!launch_fits(rows, k, n)) return fail(kBadArgument, "qsrt_adapter_linear: too many rows for this matrix");
     if (const char* e = rows_fault(x, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
     if (const char* e = rows_fault(out, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
     int cus = 0;
@@ -1353,7 +1390,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     ra.rows = rows;
     ra.kb = static_cast<int>(k / 128);
     ra.nmat = 1;
-    ra.layout = row_layout(ra.kb, rows > 4);
+    ra.layout = row_layout(ra.kb, s.grouped);
     ShrinkArgs sa{};
     sa.x = x;
     sa.ld = x_ld;
@@ -1372,7 +1409,6 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
             1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / std::max<int64_t>(1, sixteens(rows) / 16 * s.low_parts * (rank / (16 * tiles))))));
     const int64_t shrinks = shrink_blocks(sa, tiles);
     const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + kShrinkWaves - 1) / kShrinkWaves;
-    if (shrinks + rotates >= int64_t(1) << 31) return fail(kBadArgument, "qsrt_adapter_linear: too many rows");
     const dim3 pgrid(static_cast<unsigned>(shrinks + rotates)), pblock(64 * kShrinkWaves);
 #define QSRT_PREPARE(T)                                                                                              \
     hipLaunchKernelGGL((tiles == 2 ? prepare_rows_kernel<T, 2> : prepare_rows_kernel<T, 1>), pgrid, pblock, 0, stream, ra, \
@@ -1394,7 +1430,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     pa.part = s.part;
     pa.nmat = 1;
     pa.rows = static_cast<int>(rows);
-    if (const int rc = launch_product(pa, s.groups, w->rates, luts, cus, stream)) return rc;
+    if (const int rc = launch_product(pa, s.groups, s.row_groups, w->rates, luts, cus, stream)) return rc;
 
     FinishArgs fa{};
     fa.part = s.part;

@@ -132,15 +132,19 @@ __device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane,
     const int64_t step = static_cast<int64_t>(p.tokens) * p.experts;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) score[j] = 0.f;
-    for (int q = 0; q < p.splits; q += 8) {  // the loads of eight splits go out together; slots past the last expert repeat it
-        float part[8][kSlots];
+    // The loads of a few splits go out together (one after the other the choice of 256 experts took 17 us, with eight 8);
+    // fewer where the slots are many, so that all stay in registers.  Slots past the last expert repeat it.
+    constexpr int kTogether = kSlots <= 4 ? 8 : 32 / kSlots;
+#pragma unroll 1
+    for (int q = 0; q < p.splits; q += kTogether) {
+        float part[kTogether][kSlots];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kTogether; ++i)
 #pragma unroll
             for (int j = 0; j < kSlots; ++j)
                 part[i][j] = row[min(q + i, p.splits - 1) * step + min(64 * j + lane, p.experts - 1)];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kTogether; ++i)
 #pragma unroll
             for (int j = 0; j < kSlots; ++j) score[j] += q + i < p.splits ? part[i][j] : 0.f;
     }
@@ -176,25 +180,24 @@ __device__ __forceinline__ void choose(const ChooseArgs& p, int token, int lane,
     float chosen = 0.f, total = 0.f;  // lane r: weight and expert of the r-th
     int id = 0;
     for (int r = 0; r < p.k; ++r) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int j = 0; j < kSlots; ++j) best = key[j] > best ? key[j] : best;
-        best = wave_max(best);
-        uint64_t at = 0;
-        float s = 0.f;
+        uint32_t mine = 0;  // this lane's largest key, in its lowest slot
         int e = 0;
+        float s = 0.f;
 #pragma unroll
-        for (int j = kSlots - 1; j >= 0; --j) {  // the lowest slot that holds it, and there the lowest lane
-            const uint64_t has = __ballot(key[j] == best);
-            if (has) {
-                at = has;
-                e = 64 * j;
-                s = score[j];
-            }
+        for (int j = 0; j < kSlots; ++j) {
+            const bool larger = key[j] > mine;
+            mine = larger ? key[j] : mine;
+            e = larger ? 64 * j + lane : e;
+            s = larger ? score[j] : s;
         }
-        const int winner = __builtin_ctzll(at);
+        const uint64_t at = __ballot(mine == wave_max(mine));
+        int winner = __builtin_ctzll(at);
+        if (at & (at - 1)) {  // a tie between lanes: the lowest index
+            const uint32_t lowest = ~wave_max(at >> lane & 1 ? ~static_cast<uint32_t>(e) : 0u);
+            winner = static_cast<int>(lowest & 63);
+        }
+        e = __builtin_amdgcn_readlane(e, winner);
         s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), winner));
-        e += winner;
         if (lane == r) {
             chosen = s;
             id = e;
@@ -250,10 +253,37 @@ struct GroupLds {
     int ids[kGroupThreads], order[kGroupThreads];  // of up to kGroupThreads rows
 };
 
+// Up to 64 rows by one wave, a row a lane, keys in the order of their first rows; no LDS counters, no barriers.
+__device__ __forceinline__ void group_few(const GroupArgs& p, int id, int lane) {
+    const bool ok = lane < p.n && id >= 0 && id < p.keys;
+    if (lane < p.n) p.clean[lane] = ok ? id : -1;
+    uint64_t left = __ballot(ok);
+    int rows = 0, chunks = 0;
+    while (left) {
+        const int key = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const uint64_t same = __ballot(ok && id == key);
+        const int count = __popcll(same);
+        if (ok && id == key) {
+            const int place = __popcll(same & ((uint64_t(1) << lane) - 1));
+            p.order[rows + place] = lane;
+            if (place % p.chunk_rows == 0)
+                p.chunks[chunks + place / p.chunk_rows] = Chunk{key, rows + place, min(p.chunk_rows, count - place), lane};
+        }
+        left &= ~same;
+        rows += count;
+        chunks += (count + p.chunk_rows - 1) / p.chunk_rows;
+    }
+    for (int i = chunks + lane; i < p.max_chunks; i += 64) p.chunks[i] = Chunk{-1, 0, 0, 0};
+}
+
 // ids in l.ids already (`local`), or in memory.
 __device__ __forceinline__ void group_rows(const GroupArgs& p, int* at, GroupLds& l, bool local) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int slots = p.keys, padded = (p.n + 63) & ~63;
+    if (p.n <= 64) {
+        if (wave == 0) group_few(p, lane < p.n ? (local ? l.ids[lane] : p.ids[lane]) : -1, lane);
+        return;
+    }
     const bool small = p.n <= kGroupThreads;
     for (int i = tid; i < slots; i += kGroupThreads) at[i] = 0;
     __syncthreads();
@@ -382,7 +412,8 @@ int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs
         hipLaunchKernelGGL(router_logits_kernel<_Float16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, la);
     QSRT_HIP_TRY(hipGetLastError());
     const ChooseArgs ca{a.logits, a.bias, a.tokens, a.experts, la.splits, a.k, a.scoring, a.normalize, a.scale, a.weights, a.ids};
-    const bool together = group && a.tokens <= kGroupThreads / 64;
+    // 16 slots a lane do not fit the registers that a wave of a full workgroup has
+    const bool together = group && a.tokens <= kGroupThreads / 64 && a.experts <= 512;
 #define QSRT_CHOOSE(SLOTS)                                                                                             \
     if (together)                                                                                                      \
         hipLaunchKernelGGL(choose_group_kernel<SLOTS>, dim3(1), dim3(kGroupThreads), sizeof(int) * group->keys,      \
@@ -400,7 +431,7 @@ int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs
     } else if (a.experts <= 512) {
         QSRT_CHOOSE(8);
     } else {
-        QSRT_CHOOSE(16);
+        hipLaunchKernelGGL(choose_kernel<16>, dim3(static_cast<unsigned>(a.tokens)), dim3(64), 0, stream, ca);
     }
 #undef QSRT_CHOOSE
     QSRT_HIP_TRY(hipGetLastError());
