@@ -74,7 +74,7 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
         for (int h = 0; h < 2; ++h) {
             const int at = (2 * s + h) * tile_row_bytes + t * 64 * K;
             lo[2 * t + h] = __builtin_amdgcn_raw_buffer_load_b32(src, o0, at, 0);
-            hi[2 * t + h] = __builtin_amdgcn_raw_buffer_load_b32(src, o1, at, 0);
+            if constexpr (!kPairs) hi[2 * t + h] = __builtin_amdgcn_raw_buffer_load_b32(src, o1, at, 0);
         }
     };
 #pragma unroll
@@ -96,6 +96,9 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
         auto gather = [&](int t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                // At K2 the windows of odd i8 lie in one dword, which is the second one of i8 - 1, 16 lanes below.
+                if constexpr (kPairs)
+                    hi[2 * t + h] = __builtin_amdgcn_permlane16_swap(lo[2 * t + h], lo[2 * t + h], false, false)[1];
                 const uint32_t w0 = __builtin_amdgcn_alignbit(lo[2 * t + h], hi[2 * t + h], rsh);
                 if constexpr (kPairs) {
                     window[h] = w0;  // 30 bits: x, 14 shared bits, y of each pair, two bits further on for the next but one
