@@ -12,6 +12,7 @@ device pointers / streams are shared.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from functools import lru_cache
 from pathlib import Path
@@ -218,6 +219,15 @@ def stream_handle(device: torch.device) -> int:
 
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_here = contextlib.nullcontext()
+
+
+def current(device: torch.device):
+    """A context in which ``device`` is the current one, as kernel launches need it; free where it is already."""
+
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor) -> int:

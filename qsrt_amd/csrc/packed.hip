@@ -779,12 +779,69 @@ struct FinishArgs {
     int rows, nb;
 };
 
+// Two bf16 values whose sum is v to 17 bits.
+__device__ __forceinline__ void split(float v, __bf16& hi, __bf16& lo) {
+    hi = static_cast<__bf16>(v);
+    lo = static_cast<__bf16>(v - static_cast<float>(hi));
+}
+
+constexpr int kFinishLd = kMaxRank + 4;  // floats; rows start in different banks
+
+// low B^T of one adapter for 16 rows and the wave's 32 columns, on the matrix cores: low [16][rank] in two bf16 pieces, B as it
+// is (bf16) or in two pieces (f16, whose 11 bits they hold); the product of both lo pieces, 2^-17 of the rest, is left out.
+template <typename T>
+__device__ __forceinline__ void expand(const float (&low)[16][kFinishLd], const T* b, int rank, int lane, f32x4 (&acc)[2]) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const int n = lane & 15, g = lane >> 4;
+    const t8 zero = {};
+    t8 bv[kMaxRank / 32][2];
+#pragma unroll
+    for (int q = 0; q < kMaxRank / 32; ++q)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            bv[q][t] = 32 * q + 8 * g < rank
+                           ? *reinterpret_cast<const t8*>(b + static_cast<int64_t>(16 * t + n) * rank + 32 * q + 8 * g)
+                           : zero;
+#pragma unroll
+    for (int q = 0; q < kMaxRank / 32; ++q) {
+        if (32 * q >= rank) break;
+        const bool in = 32 * q + 8 * g < rank;
+        bf16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            __bf16 h, l;
+            split(in ? low[n][32 * q + 8 * g + j] : 0.f, h, l);
+            hi[j] = h;
+            lo[j] = l;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (__is_same(T, __bf16)) {
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bv[q][t], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bv[q][t], acc[t], 0, 0, 0);
+            } else {
+                bf16x8 bh, bl;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    __bf16 h, l;
+                    split(static_cast<float>(bv[q][t][j]), h, l);
+                    bh[j] = h;
+                    bl[j] = l;
+                }
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bh, acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bh, acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bl, acc[t], 0, 0, 0);
+            }
+        }
+    }
+}
+
 // Sum of the parts, back into the output's basis, plus the adapter's second product: a workgroup of four waves for 16 rows by
-// 128 columns.  Each wave has every fourth row and reads an adapter's slice once for those of them that name it; under four
-// rows the waves share the parts of each instead.
+// 128 columns.  Each wave has every fourth row; under four rows the waves share the parts of each instead.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     __shared__ f32x2 sums[4][64];
+    __shared__ __attribute__((aligned(16))) float low[16][kFinishLd], more[16][kFinishLd];
     const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
     const int nb = static_cast<int>(blockIdx.x % p.nb), first = 16 * static_cast<int>(blockIdx.x / p.nb);
     const int count = min(16, p.rows - first);
@@ -792,25 +849,28 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     const float* src = p.part + 128 * nb + 2 * lane;
     const bool share = count < 4;
     const int mine = share ? w < count : (count - w + 3) >> 2;  // rows of this wave
-    int row[4], key[4];
+    int row[4];
     f32x2 v[4];
-    float low[2][4] = {};  // lane l: ranks l and 64 + l of each row's first product
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // rows past the last repeat another; not stored
-        row[i] = first + (share ? min(w, count - 1) : i < mine ? w + 4 * i : w);
+        row[i] = share ? min(w, count - 1) : i < mine ? w + 4 * i : w;
         v[i] = f32x2{0.f, 0.f};
-        key[i] = p.ids && i < mine ? uniform(p.ids[row[i]]) : -1;
-        if (key[i] >= p.adapters) key[i] = -1;
     }
-    if (p.ids) {
+    int id = p.ids && lane < count ? p.ids[first + lane] : -1;  // lane r: row r's
+    if (id >= p.adapters) id = -1;
+    if (p.ids) {  // the first products of all rows, scaled
+        const int quads = p.rank >> 2;
+        for (int i = threadIdx.x; i < count * quads; i += 256) {
+            const int r = i / quads, c = 4 * (i - r * quads);
+            const int key = p.ids[first + r];
+            const float* at = p.low + static_cast<int64_t>(first + r) * p.rank + c;
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int s = 0; s < p.low_parts; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* at = p.low + (static_cast<int64_t>(s) * p.rows + row[i]) * p.rank;
-                low[0][i] += at[min(lane, p.rank - 1)];
-                if (p.rank > 64) low[1][i] += at[min(64 + lane, p.rank - 1)];
-            }
+            for (int s = 0; s < p.low_parts; ++s)
+                sum += *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(s) * p.rows * p.rank);
+            const bool has = key >= 0 && key < p.adapters;  // else nothing was written there
+            *reinterpret_cast<f32x4*>(&low[r][c]) = has ? sum * p.scale[key] : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
     }
     if (share) {
         for (int r = 0; r < count; ++r) {
@@ -819,7 +879,6 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
             if (w == r) v[0] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
             __syncthreads();
         }
-        if (!mine) return;
     } else {
         for (int s = 0; s < p.parts; s += 4) {  // sixteen loads in flight
             f32x2 t[4][4];
@@ -827,13 +886,14 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    t[j][i] = *reinterpret_cast<const f32x2*>(src + min(s + j, p.parts - 1) * stride + row[i] * cols);
+                    t[j][i] = *reinterpret_cast<const f32x2*>(src + min(s + j, p.parts - 1) * stride + (first + row[i]) * cols);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (s + j < p.parts) v[i] += t[j][i];
         }
+        __syncthreads();
     }
     const f16x2 sv = reinterpret_cast<const f16x2*>(p.svh + 128 * nb)[lane];
 #pragma unroll
@@ -843,47 +903,79 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
         hadamard128(a, b, lane);
         v[i] = f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
     }
+    const uint64_t with = __ballot(id >= 0);
+    const int key0 = __builtin_amdgcn_readlane(id, with ? __builtin_ctzll(with) : 0);
+    const uint64_t same0 = with & __ballot(id == key0), others = with & ~same0;
+    const int key1 = __builtin_amdgcn_readlane(id, others ? __builtin_ctzll(others) : 0);
+    const uint64_t same1 = others & __ballot(id == key1);
     typedef T t8 __attribute__((ext_vector_type(8)));
-    for (int turn = 0; turn < mine; ++turn) {
-        const int k = turn == 0 ? key[0] : turn == 1 ? key[1] : turn == 2 ? key[2] : key[3];
-        if (k < 0) continue;  // no adapter, or done with an earlier row
-        const float scale = p.scale[k];
-        const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(k) * cols + 128 * nb + 2 * lane) * p.rank;
-        t8 next[4];  // sixteen ranks of both columns, asked for one turn ahead
-        auto fetch = [&](int r) {
-            r = min(r, p.rank - 16);
+    if (with && !(others & ~same1)) {
+        // Rows of one or two adapters, as in prompts: every wave reads 32 columns of them once for all rows.
+        f32x4 sum[2] = {};
+        for (int turn = 0; turn < (others ? 2 : 1); ++turn) {
+            const uint32_t same = static_cast<uint32_t>(turn ? same1 : same0);
+            f32x4 acc[2] = {};
+            expand<T>(low, static_cast<const T*>(p.b) + (static_cast<int64_t>(turn ? key1 : key0) * cols + 128 * nb + 32 * w) * p.rank,
+                      p.rank, lane, acc);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                next[j] = *reinterpret_cast<const t8*>(b0 + (j >> 1) * p.rank + r + 8 * (j & 1));
-        };
-        fetch(0);
-        for (int r = 0; r < p.rank; r += 16) {
-            t8 x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = next[j];
-            fetch(r + 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (key[i] != k) continue;
-                const float mine_low = (r < 64 ? low[0][i] : low[1][i]) * scale;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float f = __builtin_bit_cast(
-                        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine_low), (r & 63) + j));
-                    v[i][0] = __builtin_fmaf(f, static_cast<float>(x[j >> 3][j & 7]), v[i][0]);
-                    v[i][1] = __builtin_fmaf(f, static_cast<float>(x[2 + (j >> 3)][j & 7]), v[i][1]);
+            for (int i = 0; i < 4; ++i)  // an adapter's infinities stay in its rows
+                if (same >> (4 * (lane >> 4) + i) & 1) {
+                    sum[0][i] = acc[0][i];
+                    sum[1][i] = acc[1][i];
                 }
-            }
         }
 #pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) more[4 * (lane >> 4) + i][32 * w + 16 * t + (lane & 15)] = sum[t][i];
+        __syncthreads();
+#pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (key[i] == k) key[i] = -1;
+            if (with >> row[i] & 1) v[i] += *reinterpret_cast<const f32x2*>(&more[row[i]][2 * lane]);
+    } else if (with) {
+        // Rows of many adapters, as in a decode batch: a wave reads 128 columns of an adapter once for those of its rows that
+        // name it, four at the most, where the matrix cores would go through all of the sixteen rows' adapters.
+        int key[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key[i] = i < mine ? __builtin_amdgcn_readlane(id, row[i]) : -1;
+        for (int turn = 0; turn < mine; ++turn) {
+            const int k = turn == 0 ? key[0] : turn == 1 ? key[1] : turn == 2 ? key[2] : key[3];
+            if (k < 0) continue;  // no adapter, or done with an earlier row
+            const T* b0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(k) * cols + 128 * nb + 2 * lane) * p.rank;
+            t8 next[4];  // sixteen ranks of both columns, asked for one turn ahead
+            auto fetch = [&](int r) {
+                r = min(r, p.rank - 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    next[j] = *reinterpret_cast<const t8*>(b0 + (j >> 1) * p.rank + r + 8 * (j & 1));
+            };
+            fetch(0);
+            for (int r = 0; r < p.rank; r += 16) {
+                t8 x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = next[j];
+                fetch(r + 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (key[i] != k) continue;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float f = low[row[i]][r + j];
+                        v[i][0] = __builtin_fmaf(f, static_cast<float>(x[j >> 3][j & 7]), v[i][0]);
+                        v[i][1] = __builtin_fmaf(f, static_cast<float>(x[2 + (j >> 3)][j & 7]), v[i][1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (key[i] == k) key[i] = -1;
+        }
     }
     typedef T t2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= mine) break;
-        reinterpret_cast<t2*>(static_cast<T*>(p.out) + row[i] * p.ld + 128 * nb)[lane] =
+        reinterpret_cast<t2*>(static_cast<T*>(p.out) + (first + row[i]) * p.ld + 128 * nb)[lane] =
             t2{static_cast<T>(v[i][0]), static_cast<T>(v[i][1])};
     }
 }

@@ -181,16 +181,17 @@ def _run(x, linear, bank, ids, out):
         return out
     lib = _native.lib()
     adapters, rank = (bank.adapters, bank.a.shape[1]) if bank is not None else (0, 0)
-    ws = torch.empty(lib.qsrt_adapter_linear_workspace_bytes(m.ref, rows, adapters, rank), dtype=torch.uint8,
-                     device=m.device)
-    _native.check(
-        lib.qsrt_adapter_linear(
-            m.ref, linear.luts.ref, None if bank is None else bank.a.data_ptr(),
-            None if bank is None else bank.b.data_ptr(), None if bank is None else bank.scale.data_ptr(), adapters, rank,
-            x.data_ptr(), x.stride(0), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
-            out.stride(0), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
-        "qsrt_adapter_linear",
-    )
+    with _native.current(m.device):
+        ws = torch.empty(lib.qsrt_adapter_linear_workspace_bytes(m.ref, rows, adapters, rank), dtype=torch.uint8,
+                         device=m.device)
+        _native.check(
+            lib.qsrt_adapter_linear(
+                m.ref, linear.luts.ref, None if bank is None else bank.a.data_ptr(),
+                None if bank is None else bank.b.data_ptr(), None if bank is None else bank.scale.data_ptr(), adapters, rank,
+                x.data_ptr(), x.stride(0), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
+                out.stride(0), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
+            "qsrt_adapter_linear",
+        )
     return out
 
 

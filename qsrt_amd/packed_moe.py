@@ -46,13 +46,14 @@ def _route(x, weight, k, bias, scoring, normalize, scale):
     if t == 0:
         return weights, ids
     lib = _native.lib()
-    ws = torch.empty(lib.qsrt_route_workspace_bytes(t, h, e), dtype=torch.uint8, device=x.device)
-    _native.check(
-        lib.qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
-                       k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize), float(scale),
-                       weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(x.device)),
-        "qsrt_route",
-    )
+    with _native.current(x.device):
+        ws = torch.empty(lib.qsrt_route_workspace_bytes(t, h, e), dtype=torch.uint8, device=x.device)
+        _native.check(
+            lib.qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
+                           k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize), float(scale),
+                           weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(x.device)),
+            "qsrt_route",
+        )
     return weights, ids
 
 
@@ -130,15 +131,16 @@ class PackedExperts:
             return out
         ids, weights = ids.contiguous(), weights.contiguous()
         lib = _native.lib()
-        ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(self.w1.ref, self.w3.ref, self.w2.ref, self.experts, t, k),
-                         dtype=torch.uint8, device=self.device)
-        _native.check(
-            lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
-                                x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
-                                out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
-                                _native.stream_handle(self.device)),
-            "qsrt_packed_moe",
-        )
+        with _native.current(self.device):
+            ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(self.w1.ref, self.w3.ref, self.w2.ref, self.experts, t, k),
+                             dtype=torch.uint8, device=self.device)
+            _native.check(
+                lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
+                                    x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
+                                    out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                                    _native.stream_handle(self.device)),
+                "qsrt_packed_moe",
+            )
         return out
 
 
@@ -164,17 +166,18 @@ class PackedMoELayer:
         if t == 0:
             return out, weights, ids
         lib = _native.lib()
-        ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(e.w1.ref, e.w3.ref, e.w2.ref, e.experts, t, k),
-                         dtype=torch.uint8, device=e.device)
-        _native.check(
-            lib.qsrt_packed_moe_layer(
-                e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, self.router.data_ptr(),
-                self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
-                int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
-                weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
-                _native.stream_handle(e.device)),
-            "qsrt_packed_moe_layer",
-        )
+        with _native.current(e.device):
+            ws = torch.empty(lib.qsrt_packed_moe_workspace_bytes(e.w1.ref, e.w3.ref, e.w2.ref, e.experts, t, k),
+                             dtype=torch.uint8, device=e.device)
+            _native.check(
+                lib.qsrt_packed_moe_layer(
+                    e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, self.router.data_ptr(),
+                    self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
+                    int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
+                    weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                    _native.stream_handle(e.device)),
+                "qsrt_packed_moe_layer",
+            )
         return out, weights, ids
 
 
