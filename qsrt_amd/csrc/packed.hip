@@ -670,15 +670,12 @@ struct ShrinkArgs {
 };
 constexpr int kShrinkWaves = 4, kShrinkSteps = 8;  // a workgroup's part of the K axis: 1024 channels at the most
 
-inline int64_t shrink_blocks(const ShrinkArgs& p, int tiles) {
-    return p.adapters ? static_cast<int64_t>((p.rows + 15) / 16) * p.parts * p.shares * (p.rank / (16 * tiles)) : 0;
-}
 
-// x A_a^T of 16 rows over a part of the K axis, 16 kTiles ranks at a time, for each adapter a that these rows name and that
-// is this workgroup's.  The rows are read once; a wave has up to eight steps of 32 channels, all their loads in flight, and
-// the waves add up in LDS in wave order.  Products of the inputs are exact, sums FP32.
-template <typename T, int kTiles>
-__device__ __forceinline__ void shrink(const ShrinkArgs& p, int block, f32x4 (&sums)[kShrinkWaves][kTiles][64]) {
+// x A_a^T of 16 kSets rows over a part of the K axis, 16 kTiles ranks at a time, for each adapter a that these rows name and
+// that is this workgroup's.  The rows are read once; a wave has up to eight steps of 32 channels, all their loads in flight
+// (two sets of rows: four and four), and the waves add up in LDS in wave order.  Products of the inputs are exact, sums FP32.
+template <typename T, int kTiles, int kSets>
+__device__ __forceinline__ void shrink(const ShrinkArgs& p, int block, f32x4 (&sums)[kShrinkWaves][kTiles][kSets][64]) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int w = uniform(static_cast<int>(threadIdx.x >> 6));
     const int share = block % p.shares;
@@ -686,77 +683,87 @@ __device__ __forceinline__ void shrink(const ShrinkArgs& p, int block, f32x4 (&s
     const int part = block % p.parts;
     block /= p.parts;
     const int groups = p.rank / (16 * kTiles), group = block % groups;
-    const int row = 16 * (block / groups) + n;
-    const int id = row < p.rows ? p.ids[row] : -1;
-    uint32_t left = static_cast<uint32_t>(__ballot(lane < 16 && id >= 0 && id < p.adapters));
+    const int row0 = 16 * kSets * (block / groups);
+    const int id = lane < 16 * kSets && row0 + lane < p.rows ? p.ids[row0 + lane] : -1;  // lane r: row r's
+    uint64_t left = __ballot(id >= 0 && id < p.adapters);
     if (!left) return;
     const int steps = p.k / 32, end = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / p.parts);
     const int s0 = static_cast<int>(static_cast<int64_t>(steps) * part / p.parts) + w;
     typedef T t8 __attribute__((ext_vector_type(8)));
     const t8 zero = {};
-    const T* x = static_cast<const T*>(p.x) + min(row, p.rows - 1) * p.ld + 8 * g;
-    t8 xv[kShrinkSteps];
+    t8 xv[kSets][kShrinkSteps];
 #pragma unroll
-    for (int j = 0; j < kShrinkSteps; ++j) {
-        const int s = s0 + kShrinkWaves * j;
-        xv[j] = s < end ? *reinterpret_cast<const t8*>(x + 32 * s) : zero;
-    }
-    for (int index = 0; left; ++index) {
-        const int key = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-        const uint32_t same = static_cast<uint32_t>(__ballot(lane < 16 && id == key));
-        left &= ~same;
-        if (index % p.shares != share) continue;
-        const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + 16 * kTiles * group + n) * p.k + 8 * g;
-        f32x4 acc[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        t8 av[kShrinkSteps][kTiles];
+    for (int q = 0; q < kSets; ++q) {
+        const T* x = static_cast<const T*>(p.x) + min(row0 + 16 * q + n, p.rows - 1) * p.ld + 8 * g;
 #pragma unroll
         for (int j = 0; j < kShrinkSteps; ++j) {
             const int s = s0 + kShrinkWaves * j;
-            if (s < end) {
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t)
-                    av[j][t] = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * s);
-            }
+            xv[q][j] = s < end ? *reinterpret_cast<const t8*>(x + 32 * s) : zero;
         }
+    }
+    for (int index = 0; left; ++index) {
+        const int key = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const uint64_t same = __ballot(id == key);
+        left &= ~same;
+        if (index % p.shares != share) continue;
+        const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(key) * p.rank + 16 * kTiles * group + n) * p.k + 8 * g;
+        f32x4 acc[kTiles][kSets] = {};
+        constexpr int kAhead = kShrinkSteps / kSets;
 #pragma unroll
-        for (int j = 0; j < kShrinkSteps; ++j) {
-            if (s0 + kShrinkWaves * j < end) {
+        for (int j0 = 0; j0 < kShrinkSteps; j0 += kAhead) {
+            t8 av[kAhead][kTiles];
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    if constexpr (__is_same(T, __bf16))
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[j][t], xv[j], acc[t], 0, 0, 0);
-                    else
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][t], xv[j], acc[t], 0, 0, 0);
+            for (int j = 0; j < kAhead; ++j) {
+                const int s = s0 + kShrinkWaves * (j0 + j);
+                if (s < end) {
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+                        av[j][t] = *reinterpret_cast<const t8*>(a + static_cast<int64_t>(16 * t) * p.k + 32 * s);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (s0 + kShrinkWaves * (j0 + j) < end) {
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                        for (int q = 0; q < kSets; ++q) {
+                            if constexpr (__is_same(T, __bf16))
+                                acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[j][t], xv[q][j0 + j], acc[t][q], 0, 0, 0);
+                            else
+                                acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][t], xv[q][j0 + j], acc[t][q], 0, 0, 0);
+                        }
                 }
             }
         }
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) sums[w][t][lane] = acc[t];
-        __syncthreads();
-        if (w < kTiles) {
-            f32x4 sum = sums[0][w][lane];
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int v = 1; v < kShrinkWaves; ++v) sum += sums[v][w][lane];
-            if (same >> n & 1)
-                *reinterpret_cast<f32x4*>(p.out + (static_cast<int64_t>(part) * p.rows + row) * p.rank +
-                                          16 * (kTiles * group + w) + 4 * g) = sum;
+            for (int q = 0; q < kSets; ++q) sums[w][t][q][lane] = acc[t][q];
+        __syncthreads();
+        for (int i = w; i < kTiles * kSets; i += kShrinkWaves) {
+            const int t = i / kSets, q = i % kSets;
+            f32x4 sum = sums[0][t][q][lane];
+#pragma unroll
+            for (int v = 1; v < kShrinkWaves; ++v) sum += sums[v][t][q][lane];
+            if (same >> (16 * q + n) & 1)
+                *reinterpret_cast<f32x4*>(p.out + (static_cast<int64_t>(part) * p.rows + row0 + 16 * q + n) * p.rank +
+                                          16 * (kTiles * group + t) + 4 * g) = sum;
         }
         __syncthreads();
     }
 }
 
 // What an adapter projection needs before its product: the rows' rotation, and beside it the adapters' first products.
-template <typename T, int kTiles>
+template <typename T, int kTiles, int kSets>
 __global__ __launch_bounds__(64 * kShrinkWaves) void prepare_rows_kernel(const RotateArgs r, const ShrinkArgs p, int shrinks) {
     __shared__ __attribute__((aligned(16))) union {
-        f32x4 sums[kShrinkWaves][kTiles][64];
+        f32x4 sums[kShrinkWaves][kTiles][kSets][64];
         u32x4 staged[512 * kRotateBlocks];
     } l;
     const int block = static_cast<int>(blockIdx.x);
     if (block < shrinks)
-        shrink<T, kTiles>(p, block, l.sums);
+        shrink<T, kTiles, kSets>(p, block, l.sums);
     else if (r.layout.row == 16)
         rotate_quad<T>(r, block - shrinks, l.staged);
     else
@@ -1498,16 +1505,24 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     sa.rank = static_cast<int>(rank);
     sa.parts = s.low_parts;
     const int tiles = adapters && rank % 32 == 0 ? 2 : 1;  // of 16 ranks a workgroup
-    // the adapters of 16 rows are shared out while that leaves no more workgroups than four a compute unit
-    if (adapters)
-        sa.shares = static_cast<int>(std::max<int64_t>(
-            1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / std::max<int64_t>(1, sixteens(rows) / 16 * s.low_parts * (rank / (16 * tiles))))));
-    const int64_t shrinks = shrink_blocks(sa, tiles);
+    int sets = 1;                                          // of 16 rows
+    int64_t shrinks = 0;
+    if (adapters) {
+        const auto blocks = [&](int q) { return (rows + 16 * q - 1) / (16 * q) * s.low_parts * (rank / (16 * tiles)); };
+        // Beyond four workgroups a unit 32 rows share the reads of A (2048 rows, K 5120, rank 64: 32 us for this kernel, 37
+        // with 16; 512 rows: 57 us for all with 32, 54 with 16); below, the adapters of a workgroup's rows are shared out.
+        if (tiles == 2 && blocks(1) > 4 * cus) sets = 2;
+        shrinks = blocks(sets);
+        sa.shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / shrinks)));
+        shrinks *= sa.shares;
+    }
     const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + kShrinkWaves - 1) / kShrinkWaves;
     const dim3 pgrid(static_cast<unsigned>(shrinks + rotates)), pblock(64 * kShrinkWaves);
 #define QSRT_PREPARE(T)                                                                                              \
-    hipLaunchKernelGGL((tiles == 2 ? prepare_rows_kernel<T, 2> : prepare_rows_kernel<T, 1>), pgrid, pblock, 0, stream, ra, \
-                       sa, static_cast<int>(shrinks))
+    hipLaunchKernelGGL((sets == 2    ? prepare_rows_kernel<T, 2, 2>                                                   \
+                        : tiles == 2 ? prepare_rows_kernel<T, 2, 1>                                                   \
+                                     : prepare_rows_kernel<T, 1, 1>),                                                 \
+                       pgrid, pblock, 0, stream, ra, sa, static_cast<int>(shrinks))
     if (dtype == 0)
         QSRT_PREPARE(__bf16);
     else

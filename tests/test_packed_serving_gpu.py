@@ -407,3 +407,65 @@ def test_refusals():
                 lambda: PackedMoELayer(torch.zeros((4, 128), dtype=x.dtype).cuda(), layer.packed, 5)):
         with pytest.raises(ValueError):
             bad()
+
+
+# ---------------------------------------------------------------------------
+# runs, sharing and files
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t,k,n,adapters,rank,run,dtype", [
+    (2, 256, 128, 2, 16, 1, torch.bfloat16),       # under four rows
+    (15, 256, 128, 2, 48, 8, torch.float16),       # two adapters in a block of 16 rows
+    (50, 128, 256, 3, 40, 16, torch.bfloat16),     # one and none
+    (64, 384, 128, 9, 128, 5, torch.float16),      # four: some blocks take the other way
+    (2100, 2048, 128, 5, 128, 300, torch.bfloat16),  # first products of 32 rows at once
+])
+def test_adapters_in_runs(t, k, n, adapters, rank, run, dtype):
+    rng = np.random.default_rng(t + rank)
+    bits = (3,) * (k // 128)
+    p = payload(rng, k, n, bits, "k")
+    linear = PackedLinear(*(torch.from_numpy(v).cuda() for v in p), bits, LUTS)
+    x = rows(rng, t, k, dtype)
+    a = (rows(rng, adapters * rank, k, dtype) / k**0.5).view(adapters, rank, k)
+    b = (rows(rng, adapters * n, rank, dtype) / rank**0.5).view(adapters, n, rank)
+    scale = torch.from_numpy(rng.uniform(0.5, 2, adapters)).float()
+    ids = ((torch.arange(t) // run) % (adapters + 1)).int() - 1
+    want = x.double() @ dense(*p, bits, "k")
+    for i in range(adapters):
+        want[ids == i] += float(scale[i]) * ((x[ids == i].double() @ a[i].double().T) @ b[i].double().T)
+    bank = LowRankAdapters(a.cuda(), b.cuda(), scale.cuda())
+    close(adapter_linear(x.cuda(), linear, bank, ids.cuda()), want, dtype)
+    if adapters > 1:  # an adapter's infinities stay in its rows
+        bank.b[0, 3, 1] = float("inf")
+        got = adapter_linear(x.cuda(), linear, bank, ids.cuda()).cpu()
+        keep = ids != 0
+        close(got[keep], want[keep], dtype)
+        assert not bool(torch.isfinite(got[~keep][:, 3]).any())
+
+
+def test_router_of_many_experts_in_a_layer():
+    """More experts than one workgroup chooses from: choice and grouping are launches of their own."""
+
+    experts = Experts(41, 128, 128, 600, (3,))
+    rng = np.random.default_rng(42)
+    x, router = rows(rng, 3, 128, torch.bfloat16), rows(rng, 600, 128, torch.bfloat16) / 8
+    y, weights, ids = PackedMoELayer(router.cuda(), experts.packed, 5)(x.cuda())
+    want_w, want = choose64(x, router, 5, None, "softmax", True, 1.0)
+    assert torch.equal(ids.cpu().long(), want)
+    close(y, experts(x, want_w, want), torch.bfloat16)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_layer_rotates_beside_its_router(shared):
+    experts = Experts(43, 256, 128, 7, (3, ), shared)
+    rng = np.random.default_rng(44)
+    router = rows(rng, 7, 256, torch.float16) / 16
+    layer = PackedMoELayer(router.cuda(), experts.packed, 3, scoring="sigmoid")
+    for t in (1, 2, 70, 90):  # with scales of their own: rotated before the choice is known, 90 after it
+        x = rows(rng, t, 256, torch.float16)
+        y, weights, ids = layer(x.cuda())
+        want_w, want = choose64(x, router, 3, None, "sigmoid", True, 1.0)
+        keep = (ids.cpu().long() == want).all(-1)  # scores nearer than FP32 sums tell apart are no fault of the experts
+        assert int(keep.sum()) >= t - 1
+        close(y.cpu()[keep], experts(x, want_w, want)[keep], torch.float16)
