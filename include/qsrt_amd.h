@@ -473,13 +473,21 @@ int qsrt_route(const void *x, int64_t x_ld, const void *weight, int64_t weight_l
  * [0, experts) contributes nothing.  x and out bf16 (dtype 0) or f16 (1),
  * rows 8-byte aligned; sums are FP32 and rounded once.  Needs
  * qsrt_packed_moe_workspace_bytes bytes of workspace.
+ *
+ * pre_signs (f32 [2 inter]) and post_signs (f32 [inter]) are null for plain
+ * weights.  With both, the payloads hold coupled weights: x and out turned by
+ * the normalised Hadamard on blocks of 512 of the hidden axis, gate and up
+ * channels interleaved and turned by pre_signs and H on blocks of 128 (w1 has
+ * the first half of that axis, w3 the second), the middle by post_signs and H
+ * on blocks of 128.  hidden must then be a multiple of 512.
  */
 size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3,
                                        const qsrt_packed_matrix *w2, int64_t experts, int64_t tokens, int k);
 int qsrt_packed_moe(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, const qsrt_packed_matrix *w2,
-                    const uint8_t *const *luts, int64_t experts, int activation, const void *x, int64_t x_ld, int dtype,
-                    int64_t tokens, int k, const int32_t *ids, const float *weights, void *out, int64_t out_ld, void *ws,
-                    size_t ws_bytes, void *stream);
+                    const uint8_t *const *luts, int64_t experts, int activation, const float *pre_signs,
+                    const float *post_signs, const void *x, int64_t x_ld, int dtype, int64_t tokens, int k,
+                    const int32_t *ids, const float *weights, void *out, int64_t out_ld, void *ws, size_t ws_bytes,
+                    void *stream);
 
 /*
  * The whole layer: qsrt_route's choice (weights and ids are outputs, the
@@ -487,10 +495,11 @@ int qsrt_packed_moe(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, 
  * fewer launches.  x rows 16-byte aligned; the same workspace.
  */
 int qsrt_packed_moe_layer(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, const qsrt_packed_matrix *w2,
-                          const uint8_t *const *luts, int64_t experts, int activation, const void *router,
-                          int64_t router_ld, const float *bias, int scoring, int normalize, float scale, const void *x,
-                          int64_t x_ld, int dtype, int64_t tokens, int k, float *weights, int32_t *ids, void *out,
-                          int64_t out_ld, void *ws, size_t ws_bytes, void *stream);
+                          const uint8_t *const *luts, int64_t experts, int activation, const float *pre_signs,
+                          const float *post_signs, const void *router, int64_t router_ld, const float *bias,
+                          int scoring, int normalize, float scale, const void *x, int64_t x_ld, int dtype,
+                          int64_t tokens, int k, float *weights, int32_t *ids, void *out, int64_t out_ld, void *ws,
+                          size_t ws_bytes, void *stream);
 
 /*
  * A packed projection with low-rank adapters, each row its own or none:

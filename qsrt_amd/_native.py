@@ -121,12 +121,14 @@ SIGNATURES: dict[str, tuple] = {
     "qsrt_packed_moe_workspace_bytes": (_c_size, [_c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_int]),
     "qsrt_packed_moe": (
         _c_int,
-        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_i64,
+         _c_int,
          _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
     ),
     "qsrt_packed_moe_layer": (
         _c_int,
-        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_void_p, _c_int, _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
+         _c_int, _c_int,
          ctypes.c_float, _c_void_p, _c_i64, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
          _c_size, _c_void_p],
     ),

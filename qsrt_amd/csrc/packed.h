@@ -85,6 +85,19 @@ __device__ __forceinline__ void store_pieces(char* row, const RowLayout& l, int 
     *reinterpret_cast<bf16x2*>(dst + l.piece) = lo;
 }
 
+// The same for channels `lane` and 64 + lane.
+__device__ __forceinline__ void store_halves(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float v = h ? b : a;
+        const int tile = 4 * h + (lane >> 4), pair = (lane & 15) >> 1;
+        char* dst = row + (4 * kb + (tile >> 1)) * l.strip + (pair & 3) * l.group + (tile & 1) * 8 + (pair >> 2) * 4 + (lane & 1) * 2;
+        const __bf16 hi = static_cast<__bf16>(v);
+        *reinterpret_cast<__bf16*>(dst) = hi;
+        *reinterpret_cast<__bf16*>(dst + l.piece) = static_cast<__bf16>(v - static_cast<float>(hi));
+    }
+}
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
@@ -92,7 +105,8 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
     return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// Rows into a payload's basis: (x * suh) H in pieces.
+// Rows into a payload's basis: (x * suh) H in pieces.  `residual`: x is turned by the normalised Hadamard on blocks of 512
+// first, as coupled weights take it.
 struct RotateArgs {
     const void* x;  // [rows / x_div][ld]
     int64_t ld;
@@ -105,7 +119,11 @@ struct RotateArgs {
     int64_t rows;
     int kb, nmat;
     RowLayout layout;
+    bool residual;
 };
+
+// Entry (i, j) of the 4 x 4 Sylvester matrix, which turns blocks of 128 into blocks of 512.
+__device__ __forceinline__ float sign4(int i, int j) { return __builtin_popcount(i & j) & 1 ? -1.f : 1.f; }
 
 inline int64_t rotate_waves(const RotateArgs& p) { return (p.rows + 15) / 16 * 16 * p.kb * p.nmat; }
 
@@ -128,10 +146,27 @@ __device__ __forceinline__ f32x2 rotated(const RotateArgs& p, const RotateAt& at
         (at.mat ? p.suh[1] : p.suh[0]) + id * (at.mat ? p.suh_stride[1] : p.suh_stride[0]) + 128 * at.kb;
     const T* x = static_cast<const T*>(p.x) + from * p.ld + 128 * at.kb;
     typedef T t2 __attribute__((ext_vector_type(2)));
-    const t2 xv = reinterpret_cast<const t2*>(x)[lane];
     const f16x2 sv = reinterpret_cast<const f16x2*>(suh)[lane];
-    float a = static_cast<float>(xv[0]) * static_cast<float>(sv[0]);
-    float b = static_cast<float>(xv[1]) * static_cast<float>(sv[1]);
+    float a, b;
+    if (p.residual) {
+        const int block = at.kb & 3;
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const t2 xv = reinterpret_cast<const t2*>(x + 128 * (i - block))[lane];
+            a += sign4(i, block) * static_cast<float>(xv[0]);
+            b += sign4(i, block) * static_cast<float>(xv[1]);
+        }
+        hadamard128(a, b, lane);
+        a *= 0.5f * kHadamardScale;
+        b *= 0.5f * kHadamardScale;
+    } else {
+        const t2 xv = reinterpret_cast<const t2*>(x)[lane];
+        a = static_cast<float>(xv[0]);
+        b = static_cast<float>(xv[1]);
+    }
+    a *= static_cast<float>(sv[0]);
+    b *= static_cast<float>(sv[1]);
     hadamard128(a, b, lane);
     return f32x2{a * kHadamardScale, b * kHadamardScale};
 }

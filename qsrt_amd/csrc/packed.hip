@@ -532,6 +532,7 @@ struct MiddleArgs {
     char* out;
     RowLayout layout;
     int pairs, ib, act;
+    const float *pre_signs, *post_signs;  // [2 inter], [inter] of coupled weights; else null
 };
 
 __device__ __forceinline__ float activate(float g, float u, int act) {
@@ -555,6 +556,30 @@ __device__ __forceinline__ f32x2 sum_parts(const float* src, int64_t stride, int
     return sum;
 }
 
+// Both sums of 128 channels over all parts; the loads of eight parts go out together.  `step`: floats from part to part.
+__device__ __forceinline__ void sum_two(const float* s0, const float* s1, int64_t step, int parts, f32x2& a, f32x2& b) {
+    a = b = f32x2{0.f, 0.f};
+    int s = 0;
+    for (; s + 8 <= parts; s += 8) {
+        f32x2 v[8], t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = *reinterpret_cast<const f32x2*>(s0 + (s + j) * step);
+            t[j] = *reinterpret_cast<const f32x2*>(s1 + (s + j) * step);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            a += v[j];
+            b += t[j];
+        }
+    }
+#pragma unroll 4
+    for (; s < parts; ++s) {
+        a += *reinterpret_cast<const f32x2*>(s0 + s * step);
+        b += *reinterpret_cast<const f32x2*>(s1 + s * step);
+    }
+}
+
 // One wave for 128 middle channels of one (token, expert) pair.
 __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
     const int lane = threadIdx.x & 63;
@@ -569,26 +594,8 @@ __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
     const f16x2 su = reinterpret_cast<const f16x2*>(p.svh[1] + id * p.svh_stride[1] + 128 * ib)[lane];
     const f16x2 sd = reinterpret_cast<const f16x2*>(p.suh + id * p.suh_stride + 128 * ib)[lane];
     const float* src = p.part + pair * inter + 128 * ib + 2 * lane;
-    f32x2 gs = {0.f, 0.f}, us = {0.f, 0.f};
-    int s = 0;
-    for (; s + 8 <= p.parts; s += 8) {  // the loads of eight parts go out together
-        f32x2 v[8], t[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = *reinterpret_cast<const f32x2*>(src + (s + j) * 2 * rows);
-            t[j] = *reinterpret_cast<const f32x2*>(src + ((s + j) * 2 + 1) * rows);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            gs += v[j];
-            us += t[j];
-        }
-    }
-#pragma unroll 4
-    for (; s < p.parts; ++s) {
-        gs += *reinterpret_cast<const f32x2*>(src + s * 2 * rows);
-        us += *reinterpret_cast<const f32x2*>(src + (s * 2 + 1) * rows);
-    }
+    f32x2 gs, us;
+    sum_two(src, src + rows, 2 * rows, p.parts, gs, us);
     float g0 = gs[0], g1 = gs[1], u0 = us[0], u1 = us[1];
     hadamard128(g0, g1, lane);
     hadamard128(u0, u1, lane);
@@ -598,6 +605,52 @@ __global__ __launch_bounds__(256) void middle_kernel(const MiddleArgs p) {
               static_cast<float>(sd[1]);
     hadamard128(a, b, lane);
     store_pieces(p.out + row_place(p.layout, pair), p.layout, ib, lane, a * kHadamardScale, b * kHadamardScale);
+}
+
+// The same for coupled weights.  Their gate and up channels are interleaved, the interleaved axis turned by the signed
+// Hadamard on blocks of 128 (which turns back to signs * H z), and its first half is the first product's, its second half the
+// second's.  So block z of the turned axis holds channels 64 z .. 64 z + 63 of both, and after turning it back lane l has gate
+// and up of channel 64 z + l: no exchange between lanes.  A wave takes two such blocks, whose channels lie as l and 64 + l of
+// its 128: the butterflies are the same in that order.  The second product's turn is H (signs * middle).
+__global__ __launch_bounds__(256) void middle_coupled_kernel(const MiddleArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
+    const int ib = static_cast<int>(wave % p.ib);
+    const int64_t pair = wave / p.ib;
+    if (pair >= p.pairs) return;
+    const int id = uniform(p.ids[pair]);
+    if (id < 0) return;
+    const int64_t inter = 128 * static_cast<int64_t>(p.ib), rows = static_cast<int64_t>(p.pairs) * inter;
+    const float* src[2];
+    f32x2 sums[2];
+    float middle[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int z = 2 * ib + h, mat = z >= p.ib;
+        src[h] = p.part + mat * rows + pair * inter + 128 * (z - mat * p.ib) + 2 * lane;
+    }
+    sum_two(src[0], src[1], 2 * rows, p.parts, sums[0], sums[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int z = 2 * ib + h, mat = z >= p.ib;
+        const _Float16* svh = (mat ? p.svh[1] + id * p.svh_stride[1] : p.svh[0] + id * p.svh_stride[0]) + 128 * (z - mat * p.ib);
+        const f16x2 sv = reinterpret_cast<const f16x2*>(svh)[lane];
+        const f32x2 sign = reinterpret_cast<const f32x2*>(p.pre_signs + 128 * z)[lane];
+        float g = sums[h][0], u = sums[h][1];
+        hadamard128(g, u, lane);
+        g *= kHadamardScale * static_cast<float>(sv[0]);
+        u *= kHadamardScale * static_cast<float>(sv[1]);
+        hadamard128(g, u, lane);
+        middle[h] = activate(g * kHadamardScale * sign[0], u * kHadamardScale * sign[1], p.act) *
+                    p.post_signs[128 * ib + 64 * h + lane];
+    }
+    float a = middle[0], b = middle[1];
+    hadamard128(a, b, lane);
+    const _Float16* suh = p.suh + id * p.suh_stride + 128 * ib + lane;
+    a *= kHadamardScale * static_cast<float>(suh[0]);
+    b *= kHadamardScale * static_cast<float>(suh[64]);
+    hadamard128(a, b, lane);
+    store_halves(p.out + row_place(p.layout, pair), p.layout, ib, lane, a * kHadamardScale, b * kHadamardScale);
 }
 
 // ---------------------------------------------------------------------------
@@ -616,7 +669,15 @@ struct CombineArgs {
     int tokens, k, hb;
 };
 
-constexpr int kCombineWaves = 8;
+constexpr int kCombineWaves = 8, kCoupledShares = 4;
+
+// (v H) * svh of 128 channels.
+__device__ __forceinline__ f32x2 scaled_turn(f32x2 v, const _Float16* svh, int lane) {
+    float a = v[0], b = v[1];
+    hadamard128(a, b, lane);
+    const f16x2 sv = reinterpret_cast<const f16x2*>(svh)[lane];
+    return f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
+}
 
 // One workgroup for 128 channels of one token, its waves share the token's experts.  With one svh for all experts the
 // weighted sum is rotated once, with one for each every expert's.
@@ -628,29 +689,59 @@ __global__ __launch_bounds__(64 * kCombineWaves) void combine_kernel(const Combi
     const int64_t token = blockIdx.x / p.hb;
     const int64_t hidden = 128 * static_cast<int64_t>(p.hb), stride = static_cast<int64_t>(p.tokens) * p.k * hidden;
     const bool shared = p.svh_stride == 0;
-    auto rotated = [&](f32x2 v, const _Float16* svh) {
-        float a = v[0], b = v[1];
-        hadamard128(a, b, lane);
-        const f16x2 sv = reinterpret_cast<const f16x2*>(svh + 128 * hb)[lane];
-        return f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
-    };
     f32x2 y = {0.f, 0.f};
     for (int j = w; j < p.k; j += waves) {
         const int64_t pair = token * p.k + j;
         const int id = uniform(p.ids[pair]);
         if (id < 0) continue;
         f32x2 v = sum_parts(p.part + pair * hidden + 128 * hb + 2 * lane, stride, 0, 1, p.parts);
-        if (!shared) v = rotated(v, p.svh + id * p.svh_stride);
+        if (!shared) v = scaled_turn(v, p.svh + id * p.svh_stride + 128 * hb, lane);
         y += v * p.weights[pair];
     }
     sums[w][lane] = y;
     __syncthreads();
     if (w) return;
     for (int j = 1; j < waves; ++j) y += sums[j][lane];
-    if (shared) y = rotated(y, p.svh);
+    if (shared) y = scaled_turn(y, p.svh + 128 * hb, lane);
     typedef T t2 __attribute__((ext_vector_type(2)));
     reinterpret_cast<t2*>(static_cast<T*>(p.out) + token * p.ld + 128 * hb)[lane] =
         t2{static_cast<T>(y[0]), static_cast<T>(y[1])};
+}
+
+// The same for coupled weights, whose results are turned by the Hadamard on blocks of 512: a workgroup takes four blocks of
+// 128 channels, wave w the w % 4-th of them for a share of the token's experts, and then one block of the result.
+template <typename T>
+__global__ __launch_bounds__(256 * kCoupledShares) void combine_coupled_kernel(const CombineArgs p) {
+    __shared__ f32x2 sums[4 * kCoupledShares][64], turned[4][64];
+    const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6)), shares = blockDim.x >> 8;
+    const int block = w & 3, hb = 4 * static_cast<int>(blockIdx.x % (p.hb >> 2)) + block;
+    const int64_t token = blockIdx.x / (p.hb >> 2);
+    const int64_t hidden = 128 * static_cast<int64_t>(p.hb), stride = static_cast<int64_t>(p.tokens) * p.k * hidden;
+    const bool shared = p.svh_stride == 0;
+    f32x2 y = {0.f, 0.f};
+    for (int j = w >> 2; j < p.k; j += shares) {
+        const int64_t pair = token * p.k + j;
+        const int id = uniform(p.ids[pair]);
+        if (id < 0) continue;
+        f32x2 v = sum_parts(p.part + pair * hidden + 128 * hb + 2 * lane, stride, 0, 1, p.parts);
+        if (!shared) v = scaled_turn(v, p.svh + id * p.svh_stride + 128 * hb, lane);
+        y += v * p.weights[pair];
+    }
+    sums[w][lane] = y;
+    __syncthreads();
+    if (w < 4) {
+        for (int j = 1; j < shares; ++j) y += sums[4 * j + w][lane];
+        turned[w][lane] = shared ? scaled_turn(y, p.svh + 128 * hb, lane) : y;
+    }
+    __syncthreads();
+    if (w >= 4) return;
+    y = f32x2{0.f, 0.f};
+    for (int i = 0; i < 4; ++i) y += turned[i][lane] * sign4(i, w);
+    float a = y[0], b = y[1];
+    hadamard128(a, b, lane);
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    reinterpret_cast<t2*>(static_cast<T*>(p.out) + token * p.ld + 128 * hb)[lane] =
+        t2{static_cast<T>(a * 0.5f * kHadamardScale), static_cast<T>(b * 0.5f * kHadamardScale)};
 }
 
 // ---------------------------------------------------------------------------
@@ -1232,6 +1323,7 @@ struct MoeCall {
     const uint8_t* const* luts;
     int64_t experts;
     int activation;
+    const float *pre_signs, *post_signs;
     const void* x;
     int64_t x_ld;
     int dtype;
@@ -1249,6 +1341,10 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
         return fail(kBadArgument, "%s: %s", name, e);
     if (c.dtype != 0 && c.dtype != 1) return fail(kBadArgument, "%s: dtype must be 0 (bf16) or 1 (f16)", name);
     if (c.activation != 0 && c.activation != 1) return fail(kBadArgument, "%s: unknown activation", name);
+    const bool coupled = c.pre_signs != nullptr;
+    if (coupled != (c.post_signs != nullptr) || reinterpret_cast<uintptr_t>(c.pre_signs) % 8)
+        return fail(kBadArgument, "%s: coupled weights need both sign vectors, 8-byte aligned", name);
+    if (coupled && c.w1->rows % 512) return fail(kBadArgument, "%s: coupled weights need a multiple of 512 hidden channels", name);
     if (c.tokens == 0) return kOk;
     const int64_t hidden = c.w1->rows, inter = c.w1->cols, pairs = c.tokens * c.k;
     if (const char* e = rows_fault(c.x, c.x_ld, hidden, 8)) return fail(kBadArgument, "%s: x: %s", name, e);
@@ -1287,6 +1383,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ra.kb = static_cast<int>(hidden / 128);
     ra.nmat = 2;
     ra.layout = row_layout(ra.kb, s.groups > 1);
+    ra.residual = coupled;
     RotateArgs beside = ra;  // rows that all experts share are rotated beside the router or the grouping
     if (!shared && !s.every) beside.rows = 0;
     if (router) {
@@ -1331,7 +1428,9 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ma.ib = static_cast<int>(inter / 128);
     ma.layout = row_layout(ma.ib, s.groups > 1);
     ma.act = c.activation;
-    hipLaunchKernelGGL(middle_kernel, dim3(blocks_of(pairs * ma.ib)), dim3(256), 0, stream, ma);
+    ma.pre_signs = c.pre_signs;
+    ma.post_signs = c.post_signs;
+    hipLaunchKernelGGL((coupled ? middle_coupled_kernel : middle_kernel), dim3(blocks_of(pairs * ma.ib)), dim3(256), 0, stream, ma);
     QSRT_HIP_TRY(hipGetLastError());
 
     ProductArgs pb{};
@@ -1360,11 +1459,12 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ca.tokens = static_cast<int>(c.tokens);
     ca.k = c.k;
     ca.hb = static_cast<int>(hidden / 128);
-    const dim3 cgrid(static_cast<unsigned>(c.tokens * ca.hb)), cblock(64 * std::min(c.k, kCombineWaves));
+    const dim3 cgrid(static_cast<unsigned>(c.tokens * (coupled ? ca.hb / 4 : ca.hb)));
+    const dim3 cblock(coupled ? 256 * std::min(c.k, kCoupledShares) : 64 * std::min(c.k, kCombineWaves));
     if (c.dtype == 0)
-        hipLaunchKernelGGL(combine_kernel<__bf16>, cgrid, cblock, 0, stream, ca);
+        hipLaunchKernelGGL((coupled ? combine_coupled_kernel<__bf16> : combine_kernel<__bf16>), cgrid, cblock, 0, stream, ca);
     else
-        hipLaunchKernelGGL(combine_kernel<_Float16>, cgrid, cblock, 0, stream, ca);
+        hipLaunchKernelGGL((coupled ? combine_coupled_kernel<_Float16> : combine_kernel<_Float16>), cgrid, cblock, 0, stream, ca);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
@@ -1385,20 +1485,22 @@ extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, 
 }
 
 extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
-                               const uint8_t* const* luts, int64_t experts, int activation, const void* x, int64_t x_ld,
-                               int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
+                               const uint8_t* const* luts, int64_t experts, int activation, const float* pre_signs,
+                               const float* post_signs, const void* x, int64_t x_ld, int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
                                int64_t out_ld, void* ws, size_t ws_bytes, void* stream) {
-    const MoeCall call{w1, w3, w2, luts, experts, activation, x, x_ld, dtype, tokens, k, ids, weights, out, out_ld};
+    const MoeCall call{w1, w3, w2, luts, experts, activation, pre_signs, post_signs, x, x_ld, dtype,
+                       tokens, k, ids, weights, out, out_ld};
     return run_moe("qsrt_packed_moe", call, nullptr, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int qsrt_packed_moe_layer(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
                                      const qsrt_packed_matrix* w2, const uint8_t* const* luts, int64_t experts,
-                                     int activation, const void* router, int64_t router_ld, const float* bias, int scoring,
+                                     int activation, const float* pre_signs, const float* post_signs, const void* router, int64_t router_ld, const float* bias, int scoring,
                                      int normalize, float scale, const void* x, int64_t x_ld, int dtype, int64_t tokens,
                                      int k, float* weights, int32_t* ids, void* out, int64_t out_ld, void* ws,
                                      size_t ws_bytes, void* stream) {
-    const MoeCall call{w1, w3, w2, luts, experts, activation, x, x_ld, dtype, tokens, k, ids, weights, out, out_ld};
+    const MoeCall call{w1, w3, w2, luts, experts, activation, pre_signs, post_signs, x, x_ld, dtype,
+                       tokens, k, ids, weights, out, out_ld};
     if (tokens < 0 || tokens > (1 << 20) || !w1 || w1->rows > (1 << 22))
         return fail(kBadArgument, "qsrt_packed_moe_layer: bad sizes");
     RouterArgs r{x, x_ld, router, router_ld, dtype, static_cast<int>(tokens), static_cast<int>(w1->rows),

@@ -1,8 +1,9 @@
 """A mixture-of-experts layer for a few tokens, straight from its packed payloads.
 
 ``route_tokens`` chooses each token's experts, ``PackedExperts`` multiplies by them and ``PackedMoELayer`` is both
-(``qsrt_route``, ``qsrt_packed_moe`` and ``qsrt_packed_moe_layer`` in ``include/qsrt_amd.h``).  Nothing waits for the device: which experts are
-chosen is known there alone.
+(``qsrt_route``, ``qsrt_packed_moe`` and ``qsrt_packed_moe_layer`` in ``include/qsrt_amd.h``).  Nothing waits for the
+device: which experts are chosen is known there alone.  Workspaces come from torch's allocator on the current stream, so a
+call can be captured in a graph; the first call of a shape need not come before.
 """
 
 from __future__ import annotations
@@ -11,6 +12,7 @@ import torch
 
 from . import _native
 from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows
+from .qsrt_coupled import CoupledHadamardSpec, rotation_signs
 
 SCORING = {"softmax": 0, "sigmoid": 1}
 ACTIVATIONS = {"swiglu": 0, "situ": 1}
@@ -74,9 +76,12 @@ class PackedExperts:
     """The experts of one layer: ``w1`` and ``w3 [hidden, inter]`` (gate and up) and ``w2 [inter, hidden]`` (down), each a
     dict of the stacked payloads of all experts: ``trellis`` int16 ``[experts, words]``, ``suh``/``svh`` float16 (one
     vector for the layer or ``[experts, ...]``), ``record_bits`` (one rate, one schedule, or one for each expert) and
-    ``rate_axis`` (default: columns for w1 and w3, rows for w2, as stored)."""
+    ``rate_axis`` (default: columns for w1 and w3, rows for w2, as stored).  ``coupled``: the payloads hold coupled
+    coordinates (``qsrt_coupled.encode_coupled_weights``) of that spec, of its default block sizes; ``x`` and the result
+    are in the source's coordinates all the same."""
 
-    def __init__(self, w1: dict, w3: dict, w2: dict, luts_by_bits: dict, *, activation: str = "swiglu"):
+    def __init__(self, w1: dict, w3: dict, w2: dict, luts_by_bits: dict, *, activation: str = "swiglu",
+                 coupled: CoupledHadamardSpec | None = None):
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
         self.experts = int(w1["trellis"].shape[0])
@@ -92,10 +97,18 @@ class PackedExperts:
             raise ValueError("w1 and w3 must both share their suh, or neither")
         self.luts = LabelTables(luts_by_bits, self.w1.rates | self.w3.rates | self.w2.rates, self.device)
         self.activation = ACTIVATIONS[activation]
+        self.signs, self.sign_pointers = (), (None, None)
+        if coupled is not None:
+            if (coupled.residual_block_size, coupled.preactivation_block_size, coupled.postactivation_block_size) != \
+                    (512, 128, 128) or self.hidden % 512:
+                raise ValueError("coupled experts need blocks of 512, 128 and 128 and a multiple of 512 hidden channels")
+            self.signs = tuple(rotation_signs(n, draw=coupled.intermediate_draw, axis=axis, device=self.device)
+                               for n, axis in ((2 * self.inter, 1), (self.inter, 2)))
+            self.sign_pointers = tuple(s.data_ptr() for s in self.signs)
 
     @classmethod
     def from_experts(cls, experts: list, record_bits, luts_by_bits: dict, *, activation: str = "swiglu",
-                     device="cuda:0") -> "PackedExperts":
+                     coupled: CoupledHadamardSpec | None = None, device="cuda:0") -> "PackedExperts":
         """From a list of ``{"w1", "w3", "w2"}`` dicts as a layer file's reader returns them (``read_expert``)."""
 
         def stack(name):
@@ -112,7 +125,7 @@ class PackedExperts:
         if w1["suh"].dim() != w3["suh"].dim():  # both shared or neither
             for w in (w1, w3):
                 w["suh"] = w["suh"].expand(len(experts), -1).contiguous()
-        return cls(w1, w3, w2, luts_by_bits, activation=activation)
+        return cls(w1, w3, w2, luts_by_bits, activation=activation, coupled=coupled)
 
     def __call__(self, x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, *,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -136,7 +149,7 @@ class PackedExperts:
                              dtype=torch.uint8, device=self.device)
             _native.check(
                 lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
-                                    x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
+                                    *self.sign_pointers, x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
                                     out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
                                     _native.stream_handle(self.device)),
                 "qsrt_packed_moe",
@@ -171,7 +184,8 @@ class PackedMoELayer:
                              dtype=torch.uint8, device=e.device)
             _native.check(
                 lib.qsrt_packed_moe_layer(
-                    e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, self.router.data_ptr(),
+                    e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, *e.sign_pointers,
+                    self.router.data_ptr(),
                     self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
                     int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
                     weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),

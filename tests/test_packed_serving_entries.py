@@ -87,7 +87,7 @@ def test_too_many_rows_for_one_launch():
 
 
 def moe(w1, w3, w2, **changes):
-    a = {"luts": ctypes.addressof(LUTS), "experts": 4, "activation": 0, "x": P, "x_ld": 256, "dtype": 0, "tokens": 2, "k": 2,
+    a = {"luts": ctypes.addressof(LUTS), "experts": 4, "activation": 0, "pre": None, "post": None, "x": P, "x_ld": 256, "dtype": 0, "tokens": 2, "k": 2,
          "ids": P, "weights": P, "out": P, "out_ld": 256, "ws": P, "ws_bytes": 0, "stream": None}
     a.update(changes)
     return _native.lib().qsrt_packed_moe(*(ctypes.byref(w) for w in (w1, w3, w2)), *a.values())
@@ -97,7 +97,8 @@ def moe(w1, w3, w2, **changes):
     ({"experts": 0}, "experts"), ({"experts": 8192}, "experts"), ({"tokens": -1}, "tokens"), ({"k": 0}, "tokens"),
     ({"tokens": 1 << 20}, "tokens"), ({"dtype": 5}, "dtype"), ({"activation": 2}, "activation"), ({"x": None}, "null"),
     ({"x": P + 4}, "aligned"), ({"x_ld": 128}, "aligned"), ({"out": P + 4}, "aligned"), ({"ids": None}, "routing"),
-    ({"weights": None}, "routing"),
+    ({"weights": None}, "routing"), ({"pre": P}, "sign"), ({"post": P}, "sign"), ({"pre": P + 4, "post": P}, "sign"),
+    ({"pre": P, "post": P}, "512"),
 ])
 def test_experts_refuse(changes, words):
     up, down = matrix(), matrix(rows=128, cols=256)
@@ -116,7 +117,7 @@ def test_experts_refuse_matrices_that_do_not_match():
 
 def test_layer_refuses_what_its_router_cannot_read():
     up, down = matrix(), matrix(rows=128, cols=256)
-    tail = [ctypes.addressof(LUTS), 4, 0]
+    tail = [ctypes.addressof(LUTS), 4, 0, None, None]
     call = _native.lib().qsrt_packed_moe_layer
     refused(call(*(ctypes.byref(w) for w in (up, up, down)), *tail, P, 256, None, 0, 1, 1.0, P, 256, 0, -1, 2, P, P, P, 256, P,
                  0, None), "sizes")

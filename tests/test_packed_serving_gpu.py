@@ -16,6 +16,7 @@ import torch
 from oracle import fmt
 from qsrt_amd.packed_linear import LowRankAdapters, PackedLinear, adapter_linear, packed_linear
 from qsrt_amd.packed_moe import PackedExperts, PackedMoELayer, route_tokens
+from qsrt_amd.qsrt_coupled import CoupledHadamardSpec, decode_coupled_weights, rotation_signs
 from qsrt_amd.sqg_e4m3 import sqg_xor_cheb_t12_bytes
 
 pytestmark = pytest.mark.gpu
@@ -469,3 +470,59 @@ def test_layer_rotates_beside_its_router(shared):
         keep = (ids.cpu().long() == want).all(-1)  # scores nearer than FP32 sums tell apart are no fault of the experts
         assert int(keep.sum()) >= t - 1
         close(y.cpu()[keep], experts(x, want_w, want)[keep], torch.float16)
+
+
+def block_hadamard64(v, size):
+    h = torch.tensor([[1.0]], dtype=torch.float64)
+    while h.shape[0] < size:
+        h = torch.cat((torch.cat((h, h), 1), torch.cat((h, -h), 1)))
+    return (v.reshape(*v.shape[:-1], -1, size) @ h / size**0.5).reshape(v.shape)
+
+
+@pytest.mark.parametrize("hidden,inter,experts,bits,shared,act,t,k,draw,dtype", [
+    (512, 128, 3, (3,), True, "swiglu", 1, 1, 0, torch.bfloat16),      # one block of channels, half from each product
+    (1024, 384, 4, (2, 4, 3), False, "situ", 5, 2, 3, torch.float16),  # three blocks: one from both products
+    (512, 256, 5, (3, 4), True, "swiglu", 90, 5, 7, torch.bfloat16),   # rows laid out by 16
+    (512, 256, 5, (2, 2), False, "swiglu", 3, 9, 1, torch.bfloat16),   # more experts than shares
+])
+def test_coupled_experts(hidden, inter, experts, bits, shared, act, t, k, draw, dtype):
+    spec = CoupledHadamardSpec(intermediate_draw=draw)
+    layer = Experts(hidden + t, hidden, inter, experts, bits, shared, act)
+    mats = [[m[e].clone() for m in layer.mats] for e in range(experts)]
+    signs = [rotation_signs(n, draw=draw, axis=a, device="cpu").double() for n, a in ((2 * inter, 1), (inter, 2))]
+    stacked = [{"trellis": m.words.view(experts, -1), "suh": m.suh, "svh": m.svh, "record_bits": bits}
+               for m in (layer.packed.w1, layer.packed.w3, layer.packed.w2)]
+    packed = PackedExperts(*stacked, LUTS, activation=act, coupled=spec)
+    rng = np.random.default_rng(t)
+    x = rows(rng, t, hidden, dtype)
+    ids = torch.from_numpy(rng.integers(-1, experts, (t, k))).int()
+    weights = torch.from_numpy(rng.uniform(0.1, 1, (t, k))).float()
+    want, turned = torch.zeros((t, hidden), dtype=torch.float64), block_hadamard64(x.double(), 512)
+    for i in range(t):
+        for j, e in enumerate(ids[i].tolist()):
+            if e < 0:
+                continue
+            z = torch.cat((turned[i] @ mats[e][0], turned[i] @ mats[e][1]))
+            both = block_hadamard64(z, 128) * signs[0]
+            g, u = both[0::2], both[1::2]
+            mid = (g * torch.sigmoid(g) * u if act == "swiglu" else
+                   4 * torch.tanh(g / 4) * torch.sigmoid(g) * 25 * torch.tanh(u / 25))
+            want[i] += float(weights[i, j]) * (block_hadamard64(mid * signs[1], 128) @ mats[e][2])
+    want = block_hadamard64(want, 512)
+    close(packed(x.cuda(), weights.cuda(), ids.cuda()), want, dtype)
+    # the source's weights, from the framework's own inverse (FP32), mean the same
+    w1, w3, w2 = decode_coupled_weights(tuple(m.T.float().contiguous() for m in mats[0]), spec)
+    got = packed(x.cuda(), torch.ones((t, 1)).cuda(), torch.zeros((t, 1), dtype=torch.int32).cuda())
+    g, u = x.double() @ w1.double().T, x.double() @ w3.double().T
+    mid = g * torch.sigmoid(g) * u if act == "swiglu" else \
+        4 * torch.tanh(g / 4) * torch.sigmoid(g) * 25 * torch.tanh(u / 25)
+    close(got, mid @ w2.double().T, dtype)
+
+
+def test_coupled_refusals():
+    layer = Experts(61, 384, 128, 2, (3,))
+    stacked = [{"trellis": m.words.view(2, -1), "suh": m.suh, "svh": m.svh, "record_bits": (3,)}
+               for m in (layer.packed.w1, layer.packed.w3, layer.packed.w2)]
+    for spec in (CoupledHadamardSpec(), CoupledHadamardSpec(residual_block_size=128)):
+        with pytest.raises(ValueError):
+            PackedExperts(*stacked, LUTS, coupled=spec)
