@@ -317,7 +317,8 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[0][t][i] += dpp<0x128>(acc[0][t][i]);  // row rotated by 8: the other piece's
         }
-        // MFMA rows 4 g .. 4 g + 3: columns 16 (2 t + g / 2) + 8 u + 4 (g % 2) + 0..3 of row n
+        // MFMA rows 4 g .. 4 g + 3: columns 16 (2 t + g / 2) + 8 u + 4 (g % 2) + 0..3 of row n.  (Exchanging halves of the wave
+        // so that a store covers 64 bytes of a row and not 32 made no difference.)
         float* out = p.part + (static_cast<int64_t>(p.pass * parts + part) * p.nmat + mat) * p.rows * cols + 128 * cb +
                      16 * (g >> 1) + 4 * (g & 1);
 #pragma unroll
@@ -345,12 +346,15 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // Eight waves of 16 G rows each over the same columns.  Wave w decodes one window a lane of every strip (tile column pair
-// w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips' worth of them, then multiplies all of the
-// strip's by its own rows; one barrier a strip.  The table reads, which bound the product of a few rows, fall to an eighth a
-// row; the matrix cores (two pieces a row) are left as the bound.
+// w / 2, tile row w % 2) into the MFMA operands of the strip in LDS, two strips ahead, and multiplies all of a strip's by its
+// own rows; one barrier a strip, across which the first operands of the next are on their way.  The table reads, which bound
+// the product of a few rows, fall to an eighth a row and are spread over the strip's products (all at its start, with two
+// buffers of operands: 1.39 us a strip of 4 groups and 0.86 of 2, so 1.19 and 0.72).  The matrix cores take 0.95 and 0.48 of
+// that at two pieces a row and the 2.2 GHz that they leave; before and after it a workgroup waits 8 us for tables and first
+// rows and 6 to 12 for its sums' stores (2048 x 5120 x 1536: 69 us, 930 TFLOP/s of pieces).
 template <int G>
 __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
-                                              const uint8_t* lut, u32x2 (&frags)[2][8][128], int lane, int w, bool& ready,
+                                              const uint8_t* lut, u32x2 (&frags)[3][8][128], int lane, int w, bool& ready,
                                               f32x4 (&acc)[G][8]) {
     const int m = lane & 15, g = lane >> 4, t = w >> 1, h = w & 1;
     int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;  // as in multiply_strips
@@ -374,13 +378,12 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
             for (int p = 0; p < 2; ++p)
                 next[q][p] = *(gbf8)(x[q] + static_cast<int64_t>(min(s, strips - 1)) * (16 * kStripBytes) + 1024 * p);
     };
-    uint32_t label[8];
-    auto look_up = [&](int slot) {
-        const uint32_t w0 = __builtin_amdgcn_alignbit(lo[slot], hi[slot], rsh);
-        const uint32_t w1 = __builtin_amdgcn_alignbit(w0, hi[slot] << sh, 32 - 4 * K);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) label[j] = lut[__builtin_amdgcn_ubfe(j < 4 ? w0 : w1, 16 - (j & 3) * K, 16)];
+    uint32_t label[8], window[2];
+    auto open_window = [&](int slot) {
+        window[0] = __builtin_amdgcn_alignbit(lo[slot], hi[slot], rsh);
+        window[1] = __builtin_amdgcn_alignbit(window[0], hi[slot] << sh, 32 - 4 * K);
     };
+    auto look_up = [&](int j) { label[j] = lut[__builtin_amdgcn_ubfe(window[j >> 2], 16 - (j & 3) * K, 16)]; };
     auto write_operands = [&](int buffer) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -401,13 +404,21 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
         ready = true;
     }
     __syncthreads();  // the tables are there, and no wave reads the operands of an earlier run
-    look_up(0);
-    write_operands(0);
-    fetch_words(2, 0);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        open_window(e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) look_up(j);
+        write_operands(e);
+        fetch_words(2 + e, e);
+    }
     lds_barrier();
+    int now = 0, then = 1, after = 2;  // buffers of this strip and the next two
+    auto operand = [&](int buffer, int c) { return *reinterpret_cast<const u32x4*>(&frags[buffer][c][2 * lane]); };
+    u32x4 ahead[2] = {operand(0, 0), operand(0, 1)};
     for (int s = 0; s < strips; s += 2) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // strip s + e of buffer e
+        for (int e = 0; e < 2; ++e) {  // words of strips s + e + 2 in slot e
             if (s + e < strips) {
 #pragma unroll
                 for (int q = 0; q < G; ++q) {
@@ -415,21 +426,29 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
                     b[q][1] = next[q][1];
                 }
                 fetch_rows(s + e + 1);
-                look_up(e ^ 1);  // the next strip's labels are on their way while this one is multiplied
-                fetch_words(s + e + 3, e ^ 1);
-                __builtin_amdgcn_sched_barrier(0);
+                open_window(e);
+                fetch_words(s + e + 4, e);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const bf16x8 a = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&frags[e][c][2 * lane]));
+                    // the labels of the strip after the next come in between, so that no operand waits behind all of them
+                    if (c < 2) look_up(2 * c);
+                    if (c < 2) look_up(2 * c + 1);
+                    if (c >= 2 && c < 6) look_up(c + 2);
+                    const bf16x8 a = __builtin_bit_cast(bf16x8, ahead[c & 1]);
+                    ahead[c & 1] = c < 6 ? operand(now, c + 2) : operand(then, c - 6);
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
 #pragma unroll
                         for (int q = 0; q < G; ++q)
                             acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[q][p], acc[q][c], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                write_operands(e ^ 1);  // past the last strip: the last again, which nobody reads
+                write_operands(after);  // past the last strip: the last again, which nobody uses
                 lds_barrier();
+                const int free = now;
+                now = then;
+                then = after;
+                after = free;
             }
         }
     }
@@ -440,7 +459,7 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
 template <int G, int kTables>
 __global__ __launch_bounds__(64 * kRowWaves) void product_rows_kernel(const ProductArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t lut_s[65536 * kTables];
-    __shared__ __attribute__((aligned(16))) u32x2 frags[2][8][128];
+    __shared__ __attribute__((aligned(16))) u32x2 frags[3][8][128];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int w = uniform(static_cast<int>(threadIdx.x >> 6));
     for (int i = w; i < kTables * 64; i += kRowWaves)
@@ -1160,8 +1179,8 @@ int launch_product(ProductArgs args, int groups, int row_groups, int rates, cons
 int passes_of(int rates) { return __builtin_popcount(rates & 0x1C) > 2 ? 2 : 1; }
 
 // The same for product_rows_kernel, with the groups of 16 rows that each of a workgroup's eight waves takes.  A workgroup is an
-// item; with 4 groups a strip takes it about 1.1 us, a part's sums (256 KB) as long as 16 strips, there and back, and its
-// set-up 3.  With 2 all of it takes 0.6 of that: half the rows, at the same reads of the payload and the tables.  So few
+// item; with 4 groups a strip takes it about 1.2 us, a part's sums (256 KB) as long as 16 strips, there and back, and its
+// set-up 3 or more.  With 2 all of it takes 0.6 of that: half the rows, at the same reads of the payload and the tables.  So few
 // rows or items go with 2 (7168 x 7168, 256 rows: 92 us, with 4 124; 5120 x 2048, 512 rows: 60 and 66), many with 4
 // (7168 x 7168, 4096 rows: 897 us, with 2 1022).
 struct RowCut {
