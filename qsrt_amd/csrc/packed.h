@@ -179,9 +179,9 @@ __device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, 
     store_pieces((at.mat ? p.out[1] : p.out[0]) + row_place(p.layout, at.row), p.layout, at.kb, lane, v[0], v[1]);
 }
 
-// The same by a workgroup of four waves for rows laid out by 16, four blocks of channels at once: 16 rows by 512 channels,
-// whose 32 KiB leave in one stretch.
-constexpr int kRotateBlocks = 4;
+// The same by a workgroup of four waves for rows laid out by 16, two blocks of channels at once: 16 rows by 256 channels,
+// whose 16 KiB leave in one stretch (2048 x 5120: 20.1 us; four blocks 23.8, one 20.9).
+constexpr int kRotateBlocks = 2;
 inline int64_t rotate_quads(const RotateArgs& p) { return (p.rows + 15) / 16 * p.nmat * ((p.kb + kRotateBlocks - 1) / kRotateBlocks); }
 template <typename T>
 __device__ __forceinline__ void rotate_quad(const RotateArgs& p, int64_t quad, u32x4 (&staged)[512 * kRotateBlocks]) {
