@@ -14,6 +14,9 @@ import pytest
 import torch
 
 from oracle import fmt
+from qsrt_amd import qsrt as Q
+from qsrt_amd.decode import decode_packed
+from qsrt_amd.exl3_reference import reconstruct_trellis_states
 from qsrt_amd.packed_linear import LowRankAdapters, PackedLinear, adapter_linear, packed_linear
 from qsrt_amd.packed_moe import PackedExperts, PackedMoELayer, route_tokens
 from qsrt_amd.qsrt_coupled import CoupledHadamardSpec, decode_coupled_weights, rotation_signs
@@ -526,3 +529,25 @@ def test_coupled_refusals():
     for spec in (CoupledHadamardSpec(), CoupledHadamardSpec(residual_block_size=128)):
         with pytest.raises(ValueError):
             PackedExperts(*stacked, LUTS, coupled=spec)
+
+
+@pytest.mark.parametrize("rate_axis", ["k", "n"])
+def test_projection_of_a_packed_trellis(rate_axis):
+    """A mixed-rate ``PackedQSRTTrellis``, against the framework's own decode of it (FP32)."""
+
+    geometry = Q.Geometry(512, 256)
+    mode = Q.resolve_mode("R1", geometry)
+    rates = Q.record_bits(mode)
+    shape = (32, 16) if rate_axis == "k" else (16, 32)
+    states, gen = torch.empty((*shape, 256), dtype=torch.int16), torch.Generator().manual_seed(71)
+    for r, bits in enumerate(rates):
+        at = (slice(8 * r, 8 * r + 8), slice(None)) if rate_axis == "k" else (slice(None), slice(8 * r, 8 * r + 8))
+        states[at] = reconstruct_trellis_states(torch.randint(0, 1 << bits, (*states[at].shape[:2], 256), generator=gen), bits)
+    packed = Q.pack_qsrt_trellis(states.cuda(), mode, rate_axis=rate_axis)
+    k, n = 16 * shape[0], 16 * shape[1]
+    suh = (torch.rand(k, generator=gen) + 0.5).half().cuda()
+    svh = (torch.rand(n, generator=gen) - 0.5).half().cuda()
+    luts = {b: LUTS[b] for b in set(rates)}
+    x = rows(np.random.default_rng(72), 5, k, torch.bfloat16)
+    want = x.double() @ decode_packed(packed, suh, svh, luts, out_dtype=torch.float32).cpu().double()
+    close(packed_linear(x.cuda(), PackedLinear.from_packed(packed, suh, svh, luts)), want, torch.bfloat16)
