@@ -430,7 +430,7 @@ int qsrt_ldlq_commit(float *Q, int16_t *encoded, const float *recon, const uint1
  * without a gap.  Key e reads words + e key_stride, records + e
  * record_stride and its scales likewise (FP16, as stored; stride 0: one for
  * all keys).  words 4-byte aligned, scales 8-byte aligned, strides in
- * elements, rows and cols multiples of 128.
+ * elements, rows and cols multiples of 128, rows * cols below 2^32.
  */
 typedef struct qsrt_packed_matrix {
     const int16_t *words;

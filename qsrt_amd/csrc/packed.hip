@@ -1116,6 +1116,12 @@ int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
     return kOk;
 }
 
+// The next number of parts after p that makes them shorter: between the two only the turns grow.
+int next_cut(int strips, int p) {
+    const int length = (strips + p - 1) / p;
+    return length == 1 ? strips + 1 : (strips + length - 2) / (length - 1);
+}
+
 // Parts that the K axis (`strips`) of `units` column blocks is cut into, chosen so that the compute units come out even: the
 // time of a strip on one is the table reads of its wave, shared by the unit's waves; with few waves their latencies show
 // (0.9 of a wave's time beside the reads of all: 16 waves decode 4.96e12 labels a second, 8 waves 4.73e12); and a part
@@ -1123,7 +1129,7 @@ int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
 int cut_parts(double units, int64_t most, int strips, int limit, int rows, int cus) {
     int best = 1;
     double least = 0.0;
-    for (int p = 1; p <= std::min(limit, strips); ++p) {
+    for (int p = 1; p <= std::min(limit, strips); p = next_cut(strips, p)) {
         if (most * p >= int64_t(1) << 31) break;  // the product counts its items in 32 bits
         const double turns = std::ceil(units * p / cus);
         const double cost = (turns + 0.9) * ((strips + p - 1) / p + 1.0 + 0.28 * rows);
@@ -1194,7 +1200,7 @@ RowCut cut_rows(int64_t rows, int64_t nb, int strips, int limit, int cus) {
     double least = 0.0;
     for (const int groups : {4, 2}) {
         const int64_t each = 16 * kRowWaves * groups, units = (rows + each - 1) / each * nb;
-        for (int p = 1; p <= std::min(limit, strips); ++p) {
+        for (int p = 1; p <= std::min(limit, strips); p = next_cut(strips, p)) {
             if (units * p >= int64_t(1) << 31) break;
             const double turns = std::ceil(static_cast<double>(units * p) / cus);
             const double cost = turns * ((strips + p - 1) / p + 19.0) * (groups == 4 ? 1.0 : 0.6);
@@ -1263,7 +1269,7 @@ struct MoeSpace {
 };
 
 MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inter, int64_t experts, int rates13, int rates2,
-                   bool shared, bool router, int cus) {
+                   bool shared, bool router, bool either, int cus) {
     MoeSpace s;
     const int64_t pairs = tokens * k;
     // An expert's rows are one chunk more often than not: 2% of experts get over 8 of 4 a head.  Larger chunks cost more a
@@ -1285,8 +1291,9 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
     // Scales of their own: a row at a scale is a wave's few microseconds, and while all of them fit the chip at once beside
     // the router they save a launch behind the choice (8 experts, 256 channels: 33 -> 29 us a layer).
     s.every = !shared && router && tokens * experts * (hidden / 128) <= 1024;
-    for (int m = 0; m < 2; ++m)
-        s.x[m] = c.take<char>(sixteens(shared ? tokens : s.every ? tokens * experts : pairs) * hidden * 4);
+    int64_t rotated = shared ? tokens : s.every ? tokens * experts : pairs;
+    if (either && s.every) rotated = std::max(rotated, pairs);  // room for a call without a router too
+    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>(sixteens(rotated) * hidden * 4);
     s.mid = c.take<char>(sixteens(pairs) * inter * 4);
     s.passes[0] = passes_of(rates13);
     s.passes[1] = passes_of(rates2);
@@ -1377,7 +1384,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     const bool shared = c.w1->suh_stride == 0;
     const int rates13 = c.w1->rates | c.w3->rates;
     const MoeSpace s =
-        moe_space(ws, c.tokens, c.k, hidden, inter, c.experts, rates13, c.w2->rates, shared, router != nullptr, cus);
+        moe_space(ws, c.tokens, c.k, hidden, inter, c.experts, rates13, c.w2->rates, shared, router != nullptr, false, cus);
     if (!ws || ws_bytes < s.bytes) return fail(kWorkspaceTooSmall, "%s: needs %zu workspace bytes", name, s.bytes);
 
     GroupArgs ga{};
@@ -1498,12 +1505,9 @@ extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, 
     int cus = 0;
     if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0 || current_cu_count(&cus))
         return 0;
-    size_t most = 0;  // of both calls
-    for (const bool router : {false, true})
-        most = std::max(most, moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates,
-                                        w1->suh_stride == 0, router, cus)
-                                  .bytes);
-    return most;
+    return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates, w1->suh_stride == 0,
+                     true, true, cus)
+        .bytes;
 }
 
 extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
