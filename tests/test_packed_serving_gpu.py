@@ -551,3 +551,14 @@ def test_projection_of_a_packed_trellis(rate_axis):
     x = rows(np.random.default_rng(72), 5, k, torch.bfloat16)
     want = x.double() @ decode_packed(packed, suh, svh, luts, out_dtype=torch.float32).cpu().double()
     close(packed_linear(x.cuda(), PackedLinear.from_packed(packed, suh, svh, luts)), want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("experts,t", [(96, 16), (96, 17), (200, 8), (200, 9)])
+def test_layer_chooses_and_groups_at_once_or_apart(experts, t):
+    layer = Experts(81, 128, 128, experts, (3,))
+    rng = np.random.default_rng(82)
+    x, router = rows(rng, t, 128, torch.bfloat16), rows(rng, experts, 128, torch.bfloat16) / 8
+    y, weights, ids = PackedMoELayer(router.cuda(), layer.packed, 5)(x.cuda())
+    alone = route_tokens(x.cuda(), router.cuda(), 5)
+    assert torch.equal(weights, alone[0]) and torch.equal(ids, alone[1])
+    close(y, layer(x, weights.cpu(), ids.cpu()), torch.bfloat16)
