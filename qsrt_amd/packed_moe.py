@@ -3,7 +3,7 @@
 ``route_tokens`` chooses each token's experts, ``PackedExperts`` multiplies by them and ``PackedMoELayer`` is both
 (``qsrt_route``, ``qsrt_packed_moe`` and ``qsrt_packed_moe_layer`` in ``include/qsrt_amd.h``).  Nothing waits for the
 device: which experts are chosen is known there alone.  Workspaces come from torch's allocator on the current stream, so a
-call can be captured in a graph; the first call of a shape need not come before.
+call can be captured in a graph (after one outside it, which loads the kernels).
 """
 
 from __future__ import annotations
