@@ -3,8 +3,13 @@
 // A packed matrix stands for W = diag(suh) H_L X H_R diag(svh), with E4M3 labels X and H the normalised Hadamard on
 // blocks of 128.  H and the scales move to the activations:
 //   x W = ((xr X) H_R) * svh,   xr = (x * suh) H
-// so a product reads the payload's bits and nothing wider: the rows xr go in as two bf16 pieces (hi + lo, 16 bits of
-// significand), the labels are exact in bf16, sums are FP32.
+// so a product reads the payload's bits and nothing wider: the labels are exact in bf16 and f16, the rows xr go in as pieces
+// that hold the 24 bits of an FP32 value between them, sums are FP32.
+//   kBf16Pieces  hi + mid + lo, 8 bits and a sign each: any FP32 value, exactly
+//   kF16Pieces   hi + lo, 11 bits and a sign each, of a row scaled by a power of two so that its largest value is near the
+//                top of the type: 23 bits of values down to 2^-13 of the row's bound, 2^-40 of that bound below.  Two products
+//                where bf16 takes three, for calls of many rows, which the matrix cores bound; the scale needs a look at the
+//                whole row first.
 #pragma once
 
 #include "common.h"
@@ -18,21 +23,24 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// Rotated rows in memory.  A row of K channels is K / 32 strips, one for 32 payload rows: 32 hi pieces and 32 lo pieces, each
-// as four times 16 bytes, what a lane of the product takes: for lane group g = 0..3 the eight channels 16 h + {2g, 2g + 1,
-// 2g + 8, 2g + 9}, h = 0, 1 (the rows that a trellis window of a tile covers).  A few rows lie one after another; more are
-// laid out by 16, [16 rows][strip][hi, lo][g][row][16 bytes], so that a wave's load is one stretch (rows apart by a
-// multiple of 4 KiB came from one L2 channel: a 2048 x 5120 x 1536 product took 125 us).
+constexpr int kBf16Pieces = 3, kF16Pieces = 2;
+
+// Rotated rows in memory.  A row of K channels is K / 32 strips, one for 32 payload rows: 32 values of each piece, as four
+// times 16 bytes, what a lane of the product takes: for lane group g = 0..3 the eight channels 16 h + {2g, 2g + 1, 2g + 8,
+// 2g + 9}, h = 0, 1 (the rows that a trellis window of a tile covers).  A few rows lie one after another; more are laid out
+// by 16, [16 rows][strip][piece][g][row][16 bytes], so that a wave's load is one stretch (rows apart by a multiple of 4 KiB
+// came from one L2 channel: a 2048 x 5120 x 1536 product took 125 us).
 struct RowLayout {
     int row, strip, piece, group;  // bytes between neighbours
     int64_t sixteen;               // bytes of 16 rows
 };
-constexpr int kStripBytes = 128;  // of one row
-__host__ __device__ inline RowLayout row_layout(int kb, bool grouped) {
-    const int64_t bytes = static_cast<int64_t>(kb) * 4 * kStripBytes;
-    return grouped ? RowLayout{16, 16 * kStripBytes, 1024, 256, 16 * bytes}
-                   : RowLayout{static_cast<int>(bytes), kStripBytes, 64, 16, 16 * bytes};
+__host__ __device__ constexpr int strip_bytes(int pieces) { return 64 * pieces; }  // of one row
+__host__ __device__ inline RowLayout row_layout(int kb, bool grouped, int pieces) {
+    const int strip = strip_bytes(pieces);
+    const int64_t bytes = static_cast<int64_t>(kb) * 4 * strip;
+    return grouped ? RowLayout{16, 16 * strip, 1024, 256, 16 * bytes} : RowLayout{static_cast<int>(bytes), strip, 64, 16, 16 * bytes};
 }
 __host__ __device__ inline int64_t row_place(const RowLayout& l, int64_t row) { return (row >> 4) * l.sixteen + (row & 15) * l.row; }
 
@@ -74,27 +82,49 @@ __device__ __forceinline__ void hadamard128(float& a, float& b, int lane) {
 #undef QSRT_STAGE
 }
 
+// The pieces of a value: each the nearest of what is left, which is exact in FP32.
+__device__ __forceinline__ void split(float v, __bf16 (&piece)[kBf16Pieces]) {
+#pragma unroll
+    for (int i = 0; i < kBf16Pieces; ++i) {
+        piece[i] = static_cast<__bf16>(v);
+        v -= static_cast<float>(piece[i]);
+    }
+}
+__device__ __forceinline__ void split(float v, _Float16 (&piece)[kF16Pieces]) {
+#pragma unroll
+    for (int i = 0; i < kF16Pieces; ++i) {
+        piece[i] = static_cast<_Float16>(v);
+        v -= static_cast<float>(piece[i]);
+    }
+}
+
 // Channels 2 lane, 2 lane + 1 of a rotated row's kb-th block of 128, split and stored in the product's order: channel rho of
 // a tile's 16 lies in lane group (rho % 8) / 2, at place (rho & 1) + 2 (rho / 8) of the tile's four.
-__device__ __forceinline__ void store_pieces(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
-    const __bf16 h0 = static_cast<__bf16>(a), h1 = static_cast<__bf16>(b);
-    const bf16x2 lo = {static_cast<__bf16>(a - static_cast<float>(h0)), static_cast<__bf16>(b - static_cast<float>(h1))};
+template <typename P, int kPieces>
+__device__ __forceinline__ void store_pairs(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
+    typedef P p2 __attribute__((ext_vector_type(2)));
+    P pa[kPieces], pb[kPieces];
+    split(a, pa);
+    split(b, pb);
     const int tile = lane >> 3, pair = lane & 7;  // channels 2 pair, 2 pair + 1 of the tile
     char* dst = row + (4 * kb + (tile >> 1)) * l.strip + (pair & 3) * l.group + (tile & 1) * 8 + (pair >> 2) * 4;
-    *reinterpret_cast<bf16x2*>(dst) = bf16x2{h0, h1};
-    *reinterpret_cast<bf16x2*>(dst + l.piece) = lo;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<p2*>(dst + i * l.piece) = p2{pa[i], pb[i]};
+}
+__device__ __forceinline__ void store_pieces(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
+    store_pairs<__bf16, kBf16Pieces>(row, l, kb, lane, a, b);
 }
 
 // The same for channels `lane` and 64 + lane.
 __device__ __forceinline__ void store_halves(char* row, const RowLayout& l, int kb, int lane, float a, float b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const float v = h ? b : a;
+        __bf16 piece[kBf16Pieces];
+        split(h ? b : a, piece);
         const int tile = 4 * h + (lane >> 4), pair = (lane & 15) >> 1;
         char* dst = row + (4 * kb + (tile >> 1)) * l.strip + (pair & 3) * l.group + (tile & 1) * 8 + (pair >> 2) * 4 + (lane & 1) * 2;
-        const __bf16 hi = static_cast<__bf16>(v);
-        *reinterpret_cast<__bf16*>(dst) = hi;
-        *reinterpret_cast<__bf16*>(dst + l.piece) = static_cast<__bf16>(v - static_cast<float>(hi));
+#pragma unroll
+        for (int i = 0; i < kBf16Pieces; ++i) *reinterpret_cast<__bf16*>(dst + i * l.piece) = piece[i];
     }
 }
 
@@ -120,6 +150,7 @@ struct RotateArgs {
     int kb, nmat;
     RowLayout layout;
     bool residual;
+    const int* exponents;  // of kF16Pieces: row r is scaled by 2^exponents[r]
 };
 
 // Entry (i, j) of the 4 x 4 Sylvester matrix, which turns blocks of 128 into blocks of 512.
@@ -180,29 +211,36 @@ __device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, 
 }
 
 // The same by a workgroup of four waves for rows laid out by 16, two blocks of channels at once: 16 rows by 256 channels,
-// whose 16 KiB leave in one stretch (2048 x 5120: 20.1 us; four blocks 23.8, one 20.9).
+// which leave in one stretch (2048 x 5120 in two pieces: 20.1 us; four blocks 23.8, one 20.9).
 constexpr int kRotateBlocks = 2;
 inline int64_t rotate_quads(const RotateArgs& p) { return (p.rows + 15) / 16 * p.nmat * ((p.kb + kRotateBlocks - 1) / kRotateBlocks); }
-template <typename T>
-__device__ __forceinline__ void rotate_quad(const RotateArgs& p, int64_t quad, u32x4 (&staged)[512 * kRotateBlocks]) {
+template <typename T, int kPieces>
+__device__ __forceinline__ void rotate_quad(const RotateArgs& p, int64_t quad, u32x4 (&staged)[256 * kPieces * kRotateBlocks]) {
     const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
     const int quads = (p.kb + kRotateBlocks - 1) / kRotateBlocks;
     const int64_t rest = quad / quads, sixteen = p.nmat == 2 ? rest >> 1 : rest;
     const int kb0 = kRotateBlocks * static_cast<int>(quad - rest * quads), mat = p.nmat == 2 ? static_cast<int>(rest & 1) : 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int64_t row = 16 * sixteen + 4 * w + r;
+        const int64_t row = 16 * sixteen + 4 * w + r, from = min(row, p.rows - 1);
         f32x2 v[kRotateBlocks];
 #pragma unroll
         for (int j = 0; j < kRotateBlocks; ++j)  // past the last row and channel another's; not read by anyone who counts
-            v[j] = rotated<T>(p, RotateAt{min(row, p.rows - 1), min(kb0 + j, p.kb - 1), mat}, lane);
+            v[j] = rotated<T>(p, RotateAt{from, min(kb0 + j, p.kb - 1), mat}, lane);
+        char* to = reinterpret_cast<char*>(staged) + (row & 15) * p.layout.row;
 #pragma unroll
-        for (int j = 0; j < kRotateBlocks; ++j)
-            store_pieces(reinterpret_cast<char*>(staged) + (row & 15) * p.layout.row, p.layout, j, lane, v[j][0], v[j][1]);
+        for (int j = 0; j < kRotateBlocks; ++j) {
+            if constexpr (kPieces == kF16Pieces) {
+                const int e = p.exponents[from];
+                store_pairs<_Float16, kF16Pieces>(to, p.layout, j, lane, ldexpf(v[j][0], e), ldexpf(v[j][1], e));
+            } else {
+                store_pieces(to, p.layout, j, lane, v[j][0], v[j][1]);
+            }
+        }
     }
     __syncthreads();
     u32x4* out = reinterpret_cast<u32x4*>((mat ? p.out[1] : p.out[0]) + sixteen * p.layout.sixteen + 4 * kb0 * p.layout.strip);
-    const int end = 512 * min(kRotateBlocks, p.kb - kb0);
+    const int end = 256 * kPieces * min(kRotateBlocks, p.kb - kb0);
     for (int i = threadIdx.x; i < end; i += 256) out[i] = staged[i];
 }
 

@@ -34,6 +34,7 @@ struct ProductArgs {
 };
 
 typedef const __attribute__((address_space(1))) bf16x8* gbf8;
+typedef const __attribute__((address_space(1))) f16x8* gf8;
 
 // The label tables come to LDS while a wave looks up its first item and asks for its first words; one barrier a wave.
 struct Tables {
@@ -51,12 +52,13 @@ struct Tables {
 // window of 16 + 7 K bits of the tile's stream, two dwords.  Lane 16 g + m reads it in tile column 2 t + m / 8 of each pair
 // t, for i8 = 4 (m % 8) + g; MFMA 2 t + u has its columns m % 8 + 8 u as rows.  K is a value and not a template argument:
 // the same instructions with other shifts, where a body for each rate made the compiler keep a second set of sums.
-// kPieces 2: 16 G rows, hi and lo pieces multiplied one after the other.  kPieces 1 (G 1): up to 8 rows, the hi piece of row n
-// in lanes n and the lo piece in lanes n + 8 of one product.
+// kHalf false: 16 G rows, hi, mid and lo pieces multiplied one after the other.  kHalf (G 1): up to 8 rows, the hi piece of row
+// n in lanes n and the mid piece in lanes n + 8 of one product, the lo piece in lanes n of a second; `x` is then the lane's own
+// piece, x_piece the way from it to the lo piece.
 // kPairs (K 2 alone): `lut` holds a row of 8 bytes for each 14 bits that two successive states share, the label of the first
 // state for each value x of its other bits at byte 2 x, of the second for each y at byte 2 y + 1.  A lookup costs the banks
 // the same at 8 bytes as at one (7.3 clocks for 64 random lanes), so this halves what bounds the product.
-template <int G, int kPieces, bool kPairs>
+template <int G, bool kHalf, bool kPairs>
 __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_bytes, int strips, int K,
                                                 const char* (&x)[G], int x_strip, int x_piece, const uint8_t* lut,
                                                 int lane, Tables& tables, f32x4 (&acc)[G][8]) {
@@ -68,6 +70,7 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
     const uint32_t o0 = 4 * d0 + (m >> 3) * 32 * K, o1 = 4 * d1 + (m >> 3) * 32 * K;
     const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(tiles), 0, (2 * strips - 1) * tile_row_bytes + 256 * K, 0x00027000);
+    constexpr int kProducts = kHalf ? 2 : kBf16Pieces;
     uint32_t lo[8], hi[8];
     auto fetch = [&](int s, int t) {  // the pair's windows of both tile rows
 #pragma unroll
@@ -82,12 +85,15 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
     tables.wait();
     int s = 0;
     do {
-        bf16x8 b[G][kPieces];
+        bf16x8 b[G][kProducts];
 #pragma unroll
         for (int q = 0; q < G; ++q) {
 #pragma unroll
-            for (int p = 0; p < kPieces; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
+            for (int p = 0; p < kProducts; ++p) b[q][p] = *(gbf8)(x[q] + p * x_piece);
             x[q] += x_strip;
+        }
+        if constexpr (kHalf) {
+            if (m >= 8) b[0][1] = bf16x8{};
         }
         uint32_t next[16], window[2];
         uint32_t rest = 0x0C000C01u;  // the selector's fixed part, in a vector register: one instruction takes one scalar
@@ -160,7 +166,7 @@ __device__ __forceinline__ void multiply_strips(const char* tiles, int tile_row_
                 av[u] = __builtin_bit_cast(bf16x8, a);
             }
 #pragma unroll
-            for (int p = 0; p < kPieces; ++p)  // hi pieces of all sums, then lo: a sum's two products do not follow each other
+            for (int p = 0; p < kProducts; ++p)  // hi pieces of all sums, then the next: a sum's products do not follow each other
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -199,9 +205,9 @@ __device__ __forceinline__ void build_pairs(const uint8_t* table, uint8_t* rows)
 }
 
 // kTables: label tables in LDS; 0: the pairs of the K2 table.
-template <int G, int kPieces, int kWaves, int kTables>
+template <int G, bool kHalf, int kWaves, int kTables>
 __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs p) {
-    static_assert(kPieces == 2 || G == 1, "half a group of rows is the least there is");
+    static_assert(!kHalf || G == 1, "half a group of rows is the least there is");
     __shared__ __attribute__((aligned(16))) uint8_t lut_s[kTables ? 65536 * kTables : 131072];
     const int lane = threadIdx.x & 63;
     const int w = uniform(static_cast<int>(threadIdx.x >> 6));
@@ -214,8 +220,9 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                 (__attribute__((address_space(3))) void*)(lut_s + 1024 * i), 16, 0, 0);
     Tables tables;
 
-    constexpr int kRows = kPieces == 1 ? 8 : 16 * G;
-    const int g = lane >> 4, n = kPieces == 1 ? lane & 7 : lane & 15, piece = kPieces == 1 ? (lane >> 3) & 1 : 0;
+    constexpr int kRows = kHalf ? 8 : 16 * G;
+    const int g = lane >> 4, n = kHalf ? lane & 7 : lane & 15, piece = kHalf ? (lane >> 3) & 1 : 0;
+    const int x_piece = kHalf ? (2 - piece) * p.layout.piece : p.layout.piece;
     const int parts = p.parts;
     const uint32_t items = static_cast<uint32_t>(p.max_chunks) * p.nmat * p.nb * parts;  // below 2^31: see cut_parts
     const int64_t cols = 128 * static_cast<int64_t>(p.nb);
@@ -303,15 +310,15 @@ __global__ __launch_bounds__(64 * kWaves) void product_kernel(const ProductArgs 
                                         : static_cast<int64_t>(2 * (s - 4 * r)) * tile_row + 8 * cb * tile);
             if (bits == p.lut_bits[0] || (kTables > 1 && bits == p.lut_bits[1])) {
                 const uint8_t* lut = kTables > 1 && bits == p.lut_bits[1] ? lut_s + 65536 : lut_s;
-                multiply_strips<G, kPieces, kTables == 0>(tiles, tile_row, stop - s, bits, x, p.layout.strip, p.layout.piece,
-                                                          lut, lane, tables, acc);
+                multiply_strips<G, kHalf, kTables == 0>(tiles, tile_row, stop - s, bits, x, p.layout.strip, x_piece, lut, lane,
+                                                        tables, acc);
             } else {  // another pass has this rate
 #pragma unroll
                 for (int q = 0; q < G; ++q) x[q] += (stop - s) * p.layout.strip;
             }
             s = stop;
         }
-        if constexpr (kPieces == 1) {
+        if constexpr (kHalf) {
 #pragma unroll
             for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -356,6 +363,7 @@ template <int G>
 __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
                                               const uint8_t* lut, u32x2 (&frags)[3][8][128], int lane, int w, bool& ready,
                                               f32x4 (&acc)[G][8]) {
+    constexpr int kStrip = 16 * strip_bytes(kF16Pieces);
     const int m = lane & 15, g = lane >> 4, t = w >> 1, h = w & 1;
     int b0 = (8 * (4 * (m & 7) + g) + 1) * K - 16;  // as in multiply_strips
     if (b0 < 0) b0 += 256 * K;
@@ -365,7 +373,7 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
     const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(tiles), 0, (2 * strips - 1) * tile_row_bytes + 256 * K, 0x00027000);
     uint32_t lo[2], hi[2];
-    bf16x8 b[G][2], next[G][2];
+    f16x8 b[G][kF16Pieces], next[G][kF16Pieces];
     auto fetch_words = [&](int s, int slot) {
         const int at = (2 * min(s, strips - 1) + h) * tile_row_bytes;
         lo[slot] = __builtin_amdgcn_raw_buffer_load_b32(src, o0, at, 0);
@@ -376,7 +384,7 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
         for (int q = 0; q < G; ++q)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
-                next[q][p] = *(gbf8)(x[q] + static_cast<int64_t>(min(s, strips - 1)) * (16 * kStripBytes) + 1024 * p);
+                next[q][p] = *(gf8)(x[q] + static_cast<int64_t>(min(s, strips - 1)) * kStrip + 1024 * p);
     };
     uint32_t label[8], window[2];
     auto open_window = [&](int slot) {
@@ -391,7 +399,7 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
 #pragma unroll
             for (int q = 0; q < 2; ++q)
                 half[q] = __builtin_bit_cast(
-                    uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                    uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(
                                   __builtin_amdgcn_perm(label[4 * u + 2 * q + 1], label[4 * u + 2 * q], 0x0C0C0400u), 1.0f, false));
             frags[buffer][2 * t + u][2 * lane + h] = half;
         }
@@ -434,13 +442,13 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
                     if (c < 2) look_up(2 * c);
                     if (c < 2) look_up(2 * c + 1);
                     if (c >= 2 && c < 6) look_up(c + 2);
-                    const bf16x8 a = __builtin_bit_cast(bf16x8, ahead[c & 1]);
+                    const f16x8 a = __builtin_bit_cast(f16x8, ahead[c & 1]);
                     ahead[c & 1] = c < 6 ? operand(now, c + 2) : operand(then, c - 6);
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
 #pragma unroll
                         for (int q = 0; q < G; ++q)
-                            acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[q][p], acc[q][c], 0, 0, 0);
+                            acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b[q][p], acc[q][c], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 write_operands(after);  // past the last strip: the last again, which nobody uses
@@ -453,7 +461,7 @@ __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_by
         }
     }
 #pragma unroll
-    for (int q = 0; q < G; ++q) x[q] += static_cast<int64_t>(strips) * (16 * kStripBytes);
+    for (int q = 0; q < G; ++q) x[q] += static_cast<int64_t>(strips) * kStrip;
 }
 
 template <int G, int kTables>
@@ -864,21 +872,70 @@ __device__ __forceinline__ void shrink(const ShrinkArgs& p, int block, f32x4 (&s
     }
 }
 
-// What an adapter projection needs before its product: the rows' rotation, and beside it the adapters' first products.
+// Scale exponents of rows that go in as f16 pieces: the largest |x suh| of a row comes to 2^11 .. 2^12, and what it can rotate
+// to, 128^1/2 of it, under the type's 65504.  A row without a value, or with an infinity, is not scaled.
+struct ExponentArgs {
+    const void* x;
+    int64_t ld;
+    const _Float16* suh;
+    int k;
+    int* out;  // null: none are asked for
+};
+
+template <typename T>
+__device__ __forceinline__ void row_exponent(const ExponentArgs& p, int64_t row, float (&most)[kShrinkWaves]) {
+    const int lane = threadIdx.x & 63, w = uniform(static_cast<int>(threadIdx.x >> 6));
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    const T* x = static_cast<const T*>(p.x) + row * p.ld;
+    float m = 0.f;
+#pragma unroll 2
+    for (int c = 8 * threadIdx.x; c < p.k; c += 8 * 64 * kShrinkWaves) {
+        const t8 xv = *reinterpret_cast<const t8*>(x + c);
+        const f16x4 s0 = *reinterpret_cast<const f16x4*>(p.suh + c), s1 = *reinterpret_cast<const f16x4*>(p.suh + c + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m = fmaxf(m, fabsf(static_cast<float>(xv[j]) * static_cast<float>(s0[j])));
+            m = fmaxf(m, fabsf(static_cast<float>(xv[4 + j]) * static_cast<float>(s1[j])));
+        }
+    }
+#pragma unroll
+    for (int h = 1; h < 64; h <<= 1) m = fmaxf(m, __shfl_xor(m, h));
+    if (lane == 0) most[w] = m;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int v = 1; v < kShrinkWaves; ++v) m = fmaxf(m, most[v]);
+    const int exponent = static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23);
+    p.out[row] = m == 0.f || exponent == 255 ? 0 : 11 + 127 - exponent;
+}
+
+// What an adapter projection needs before its product: the rows' rotation, and beside it the adapters' first products.  Rows
+// that go in as f16 pieces are only looked at here, for their scales.
 template <typename T, int kTiles, int kSets>
-__global__ __launch_bounds__(64 * kShrinkWaves) void prepare_rows_kernel(const RotateArgs r, const ShrinkArgs p, int shrinks) {
+__global__ __launch_bounds__(64 * kShrinkWaves) void prepare_rows_kernel(const RotateArgs r, const ExponentArgs e,
+                                                                         const ShrinkArgs p, int shrinks) {
     __shared__ __attribute__((aligned(16))) union {
         f32x4 sums[kShrinkWaves][kTiles][kSets][64];
-        u32x4 staged[512 * kRotateBlocks];
+        u32x4 staged[256 * kBf16Pieces * kRotateBlocks];
+        float most[kShrinkWaves];
     } l;
     const int block = static_cast<int>(blockIdx.x);
     if (block < shrinks)
         shrink<T, kTiles, kSets>(p, block, l.sums);
+    else if (e.out)
+        row_exponent<T>(e, block - shrinks, l.most);
     else if (r.layout.row == 16)
-        rotate_quad<T>(r, block - shrinks, l.staged);
+        rotate_quad<T, kBf16Pieces>(r, block - shrinks, l.staged);
     else
         rotate_block<T>(r, static_cast<int64_t>(block - shrinks) * kShrinkWaves + uniform(static_cast<int>(threadIdx.x >> 6)),
                         threadIdx.x & 63);
+}
+
+// And their rotation, once the scales are known.
+template <typename T>
+__global__ __launch_bounds__(256) void rotate_scaled_kernel(const RotateArgs r) {
+    __shared__ __attribute__((aligned(16))) u32x4 staged[256 * kF16Pieces * kRotateBlocks];
+    rotate_quad<T, kF16Pieces>(r, blockIdx.x, staged);
 }
 
 struct FinishArgs {
@@ -894,18 +951,13 @@ struct FinishArgs {
     void* out;
     int64_t ld;
     int rows, nb;
+    const int* exponents;  // null: none; else row r's sums are 2^exponents[r] too large
 };
-
-// Two bf16 values whose sum is v to 17 bits.
-__device__ __forceinline__ void split(float v, __bf16& hi, __bf16& lo) {
-    hi = static_cast<__bf16>(v);
-    lo = static_cast<__bf16>(v - static_cast<float>(hi));
-}
 
 constexpr int kFinishLd = kMaxRank + 4;  // floats; rows start in different banks
 
-// low B^T of one adapter for 16 rows and the wave's 32 columns, on the matrix cores: low [16][rank] in two bf16 pieces, B as it
-// is (bf16) or in two pieces (f16, whose 11 bits they hold); the product of both lo pieces, 2^-17 of the rest, is left out.
+// low B^T of one adapter for 16 rows and the wave's 32 columns, on the matrix cores: low [16][rank] in three bf16 pieces, B as
+// it is (bf16) or in two (f16, whose 11 bits they hold): products of the FP32 values, sums FP32.
 template <typename T>
 __device__ __forceinline__ void expand(const float (&low)[16][kFinishLd], const T* b, int rank, int lane, f32x4 (&acc)[2]) {
     typedef T t8 __attribute__((ext_vector_type(8)));
@@ -923,31 +975,34 @@ __device__ __forceinline__ void expand(const float (&low)[16][kFinishLd], const 
     for (int q = 0; q < kMaxRank / 32; ++q) {
         if (32 * q >= rank) break;
         const bool in = 32 * q + 8 * g < rank;
-        bf16x8 hi, lo;
+        bf16x8 a[kBf16Pieces];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            __bf16 h, l;
-            split(in ? low[n][32 * q + 8 * g + j] : 0.f, h, l);
-            hi[j] = h;
-            lo[j] = l;
+            __bf16 piece[kBf16Pieces];
+            split(in ? low[n][32 * q + 8 * g + j] : 0.f, piece);
+#pragma unroll
+            for (int i = 0; i < kBf16Pieces; ++i) a[i][j] = piece[i];
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             if constexpr (__is_same(T, __bf16)) {
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bv[q][t], acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bv[q][t], acc[t], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < kBf16Pieces; ++i)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bv[q][t], acc[t], 0, 0, 0);
             } else {
                 bf16x8 bh, bl;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    __bf16 h, l;
-                    split(static_cast<float>(bv[q][t][j]), h, l);
+                    const float v = static_cast<float>(bv[q][t][j]);
+                    const __bf16 h = static_cast<__bf16>(v);
                     bh[j] = h;
-                    bl[j] = l;
+                    bl[j] = static_cast<__bf16>(v - static_cast<float>(h));
                 }
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bh, acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, bh, acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, bl, acc[t], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < kBf16Pieces; ++i) {
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bh, acc[t], 0, 0, 0);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bl, acc[t], 0, 0, 0);
+                }
             }
         }
     }
@@ -1017,6 +1072,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     for (int i = 0; i < 4; ++i) {
         if (i >= mine) break;
         float a = v[i][0], b = v[i][1];
+        if (p.exponents) {
+            const int e = -p.exponents[first + row[i]];
+            a = ldexpf(a, e);
+            b = ldexpf(b, e);
+        }
         hadamard128(a, b, lane);
         v[i] = f32x2{a * kHadamardScale * static_cast<float>(sv[0]), b * kHadamardScale * static_cast<float>(sv[1])};
     }
@@ -1106,12 +1166,12 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
 
 constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one product, unless one part alone takes more
 
-template <int G, int kPieces, int kTables>
+template <int G, bool kHalf, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
     constexpr int kWaves = G == 1 ? 16 : G == 2 ? 12 : 8;  // 128, 168 and 256 registers a lane
     const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nmat * args.nb * args.parts;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
-    hipLaunchKernelGGL((product_kernel<G, kPieces, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
+    hipLaunchKernelGGL((product_kernel<G, kHalf, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
@@ -1173,12 +1233,12 @@ int launch_product(ProductArgs args, int groups, int row_groups, int rates, cons
             continue;
         }
         const bool pairs = args.luts == 1 && args.lut_bits[0] == 2;
-#define QSRT_PRODUCT(G, PIECES) \
-    (pairs ? launch_product_g<G, PIECES, 0> : two ? launch_product_g<G, PIECES, 2> : launch_product_g<G, PIECES, 1>)(args, cus, stream)
-        const int rc = groups == 0   ? QSRT_PRODUCT(1, 1)
-                       : groups == 1 ? QSRT_PRODUCT(1, 2)
-                       : groups == 2 ? QSRT_PRODUCT(2, 2)
-                                     : QSRT_PRODUCT(4, 2);
+#define QSRT_PRODUCT(G, HALF) \
+    (pairs ? launch_product_g<G, HALF, 0> : two ? launch_product_g<G, HALF, 2> : launch_product_g<G, HALF, 1>)(args, cus, stream)
+        const int rc = groups == 0   ? QSRT_PRODUCT(1, true)
+                       : groups == 1 ? QSRT_PRODUCT(1, false)
+                       : groups == 2 ? QSRT_PRODUCT(2, false)
+                                     : QSRT_PRODUCT(4, false);
 #undef QSRT_PRODUCT
         if (rc != kOk) return rc;
     }
@@ -1256,7 +1316,7 @@ int part_limit(int64_t row_floats, int strips) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, strips)));
 }
 
-int64_t sixteens(int64_t rows) { return (rows + 15) / 16 * 16; }
+int64_t rotated_bytes(int64_t rows, int64_t channels, int pieces) { return (rows + 15) / 16 * 16 * (channels / 32) * strip_bytes(pieces); }
 
 struct MoeSpace {
     Chunk* chunks;
@@ -1293,8 +1353,8 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
     s.every = !shared && router && tokens * experts * (hidden / 128) <= 1024;
     int64_t rotated = shared ? tokens : s.every ? tokens * experts : pairs;
     if (either && s.every) rotated = std::max(rotated, pairs);  // room for a call without a router too
-    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>(sixteens(rotated) * hidden * 4);
-    s.mid = c.take<char>(sixteens(pairs) * inter * 4);
+    for (int m = 0; m < 2; ++m) s.x[m] = c.take<char>(rotated_bytes(rotated, hidden, kBf16Pieces));
+    s.mid = c.take<char>(rotated_bytes(pairs, inter, kBf16Pieces));
     s.passes[0] = passes_of(rates13);
     s.passes[1] = passes_of(rates2);
     const int64_t row_floats[2] = {2 * pairs * inter * s.passes[0], pairs * hidden * s.passes[1]};
@@ -1411,7 +1471,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ra.rows = shared ? c.tokens : s.every ? c.tokens * c.experts : pairs;
     ra.kb = static_cast<int>(hidden / 128);
     ra.nmat = 2;
-    ra.layout = row_layout(ra.kb, s.groups > 1);
+    ra.layout = row_layout(ra.kb, s.groups > 1, kBf16Pieces);
     ra.residual = coupled;
     RotateArgs beside = ra;  // rows that all experts share are rotated beside the router or the grouping
     if (!shared && !s.every) beside.rows = 0;
@@ -1455,7 +1515,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     ma.out = s.mid;
     ma.pairs = static_cast<int>(pairs);
     ma.ib = static_cast<int>(inter / 128);
-    ma.layout = row_layout(ma.ib, s.groups > 1);
+    ma.layout = row_layout(ma.ib, s.groups > 1, kBf16Pieces);
     ma.act = c.activation;
     ma.pre_signs = c.pre_signs;
     ma.post_signs = c.post_signs;
@@ -1539,7 +1599,8 @@ namespace {
 struct LinearSpace {
     char* x;
     float *low, *part;
-    int low_parts, parts, passes, groups, row_groups, product_chunks;
+    int* exponents;  // of rows in f16 pieces
+    int low_parts, parts, passes, groups, row_groups, product_chunks, pieces;
     bool grouped;  // layout of the rotated rows
     size_t bytes;
 };
@@ -1574,7 +1635,9 @@ LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates
         s.low_parts = static_cast<int>((k + kPart - 1) / kPart);
         s.low = c.take<float>(s.low_parts * rows * rank);
     }
-    s.x = c.take<char>(sixteens(rows) * k * 4);
+    s.pieces = s.row_groups ? kF16Pieces : kBf16Pieces;
+    if (s.pieces == kF16Pieces) s.exponents = c.take<int>(rows);
+    s.x = c.take<char>(rotated_bytes(rows, k, s.pieces));
     s.part = c.take<float>(static_cast<int64_t>(s.parts) * s.passes * rows * n);
     s.bytes = c.used;
     return s;
@@ -1620,7 +1683,10 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     ra.rows = rows;
     ra.kb = static_cast<int>(k / 128);
     ra.nmat = 1;
-    ra.layout = row_layout(ra.kb, s.grouped);
+    ra.layout = row_layout(ra.kb, s.grouped, s.pieces);
+    ra.exponents = s.exponents;
+    const bool scaled = s.pieces == kF16Pieces;
+    const ExponentArgs ea{x, x_ld, ra.suh[0], static_cast<int>(k), scaled ? s.exponents : nullptr};
     ShrinkArgs sa{};
     sa.x = x;
     sa.ld = x_ld;
@@ -1644,19 +1710,29 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         sa.shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / shrinks)));
         shrinks *= sa.shares;
     }
-    const int64_t rotates = ra.layout.row == 16 ? rotate_quads(ra) : (rotate_waves(ra) + kShrinkWaves - 1) / kShrinkWaves;
+    const int64_t rotates = scaled                 ? rows
+                            : ra.layout.row == 16 ? rotate_quads(ra)
+                                                  : (rotate_waves(ra) + kShrinkWaves - 1) / kShrinkWaves;
     const dim3 pgrid(static_cast<unsigned>(shrinks + rotates)), pblock(64 * kShrinkWaves);
 #define QSRT_PREPARE(T)                                                                                              \
     hipLaunchKernelGGL((sets == 2    ? prepare_rows_kernel<T, 2, 2>                                                   \
                         : tiles == 2 ? prepare_rows_kernel<T, 2, 1>                                                   \
                                      : prepare_rows_kernel<T, 1, 1>),                                                 \
-                       pgrid, pblock, 0, stream, ra, sa, static_cast<int>(shrinks))
+                       pgrid, pblock, 0, stream, ra, ea, sa, static_cast<int>(shrinks))
     if (dtype == 0)
         QSRT_PREPARE(__bf16);
     else
         QSRT_PREPARE(_Float16);
 #undef QSRT_PREPARE
     QSRT_HIP_TRY(hipGetLastError());
+    if (scaled) {
+        const dim3 rgrid(static_cast<unsigned>(rotate_quads(ra)));
+        if (dtype == 0)
+            hipLaunchKernelGGL(rotate_scaled_kernel<__bf16>, rgrid, dim3(256), 0, stream, ra);
+        else
+            hipLaunchKernelGGL(rotate_scaled_kernel<_Float16>, rgrid, dim3(256), 0, stream, ra);
+        QSRT_HIP_TRY(hipGetLastError());
+    }
 
     ProductArgs pa{};
     set_matrix(pa, 0, w);
@@ -1685,6 +1761,7 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     fa.ld = out_ld;
     fa.rows = static_cast<int>(rows);
     fa.nb = static_cast<int>(n / 128);
+    fa.exponents = scaled ? s.exponents : nullptr;
     const dim3 fgrid(static_cast<unsigned>((rows + 15) / 16 * fa.nb));
     if (dtype == 0)
         hipLaunchKernelGGL(finish_kernel<__bf16>, fgrid, dim3(256), 0, stream, fa);
