@@ -110,18 +110,23 @@ def checked_rows(x: torch.Tensor, cols: int, device) -> torch.Tensor:
         raise ValueError("x must be bfloat16 or float16")
     if x.device != device:
         raise ValueError("x must be on the payload's device")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < cols or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
+    ld = leading(x)
+    if x.stride(1) != 1 or ld % 8 or ld < cols or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
+
+
+def leading(rows: torch.Tensor) -> int:
+    """Elements from row to row.  The stride of a lone row says nothing: a view keeps whatever its base had."""
+
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
 def checked_out(out: torch.Tensor | None, x: torch.Tensor, cols: int) -> torch.Tensor:
     if out is None:
         return torch.empty((x.shape[0], cols), dtype=x.dtype, device=x.device)
     if (out.shape != (x.shape[0], cols) or out.dtype != x.dtype or out.device != x.device or out.stride(1) != 1
-            or out.stride(0) % 4 or out.stride(0) < cols or out.data_ptr() % 8):
+            or leading(out) % 4 or leading(out) < cols or out.data_ptr() % 8):
         raise ValueError("out must be a row-major [rows, N] tensor of x's type, its rows 8-byte aligned")
     return out
 
@@ -188,8 +193,8 @@ def _run(x, linear, bank, ids, out):
             lib.qsrt_adapter_linear(
                 m.ref, linear.luts.ref, None if bank is None else bank.a.data_ptr(),
                 None if bank is None else bank.b.data_ptr(), None if bank is None else bank.scale.data_ptr(), adapters, rank,
-                x.data_ptr(), x.stride(0), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
-                out.stride(0), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
+                x.data_ptr(), leading(x), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
+                leading(out), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
             "qsrt_adapter_linear",
         )
     return out

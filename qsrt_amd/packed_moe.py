@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows
+from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows, leading
 from .qsrt_coupled import CoupledHadamardSpec, rotation_signs
 
 SCORING = {"softmax": 0, "sigmoid": 1}
@@ -32,8 +32,8 @@ def _checked_router(weight: torch.Tensor, k: int, bias, scoring: str) -> tuple:
         raise ValueError(f"scoring must be one of {tuple(SCORING)}")
     if bias is not None and (bias.shape != (e,) or bias.dtype != torch.float32 or bias.device != weight.device):
         raise ValueError("bias must be float32 [experts] on the router's device")
-    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < h or weight.data_ptr() % 16:
-        weight = weight.contiguous().clone()
+    if weight.stride(1) != 1 or leading(weight) % 8 or leading(weight) < h or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
     return weight, None if bias is None else bias.contiguous()
 
 
@@ -51,7 +51,7 @@ def _route(x, weight, k, bias, scoring, normalize, scale):
     with _native.current(x.device):
         ws = torch.empty(lib.qsrt_route_workspace_bytes(t, h, e), dtype=torch.uint8, device=x.device)
         _native.check(
-            lib.qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
+            lib.qsrt_route(x.data_ptr(), leading(x), weight.data_ptr(), leading(weight), TYPES[x.dtype], t, h, e,
                            k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize), float(scale),
                            weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(x.device)),
             "qsrt_route",
@@ -149,8 +149,8 @@ class PackedExperts:
                              dtype=torch.uint8, device=self.device)
             _native.check(
                 lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
-                                    *self.sign_pointers, x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(), weights.data_ptr(),
-                                    out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                                    *self.sign_pointers, x.data_ptr(), leading(x), TYPES[x.dtype], t, k, ids.data_ptr(),
+                                    weights.data_ptr(), out.data_ptr(), leading(out), ws.data_ptr(), ws.numel(),
                                     _native.stream_handle(self.device)),
                 "qsrt_packed_moe",
             )
@@ -186,9 +186,9 @@ class PackedMoELayer:
                 lib.qsrt_packed_moe_layer(
                     e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, *e.sign_pointers,
                     self.router.data_ptr(),
-                    self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
-                    int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
-                    weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                    leading(self.router), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
+                    int(self.normalize), float(self.scale), x.data_ptr(), leading(x), TYPES[x.dtype], t, k,
+                    weights.data_ptr(), ids.data_ptr(), out.data_ptr(), leading(out), ws.data_ptr(), ws.numel(),
                     _native.stream_handle(e.device)),
                 "qsrt_packed_moe_layer",
             )
