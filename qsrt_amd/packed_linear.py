@@ -41,6 +41,13 @@ def _records(record_bits, lead: tuple, rate_axis: str, k: int, n: int, words: in
     return tables, rates
 
 
+def _aligned(t: torch.Tensor, size: int) -> torch.Tensor:
+    """``t`` in one piece at a multiple of ``size`` bytes, copied where it is not."""
+
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % size else t
+
+
 class PackedMatrix:
     """One payload, or those of several keys (a layer's experts), ready for products.
 
@@ -77,10 +84,10 @@ class PackedMatrix:
         elif trellis.dim() != len(lead) + 1:
             raise ValueError("record-major words must be [words] or [keys, words]")
         nested = len(record_bits) > 0 and not isinstance(record_bits[0], int)
-        trellis = trellis.reshape(*lead, -1).contiguous()
+        trellis = _aligned(trellis.reshape(*lead, -1), 4)
         tables, rates = _records(record_bits if nested else [record_bits], lead, rate_axis, k, n, trellis.shape[-1])
         self.device, self.keys, self.k, self.n, self.rates = trellis.device, keys, k, n, rates
-        self.words, self.suh, self.svh = trellis, suh.contiguous(), svh.contiguous()
+        self.words, self.suh, self.svh = trellis, _aligned(suh, 8), _aligned(svh, 8)
         self.records = torch.tensor(tables, dtype=torch.int64).to(self.device)
         self.struct = _native.PackedMatrixStruct(
             self.words.data_ptr(), trellis.shape[-1] if lead else 0, self.records.data_ptr(),
@@ -168,12 +175,8 @@ class LowRankAdapters:
         if scale.shape != (self.adapters,) or scale.dtype != torch.float32 or scale.device != a.device:
             raise ValueError("scale must be float32 [adapters] on the adapters' device")
         pad = -self.rank % 16
-        self.a = torch.nn.functional.pad(a, (0, 0, 0, pad)).contiguous() if pad else a.contiguous()
-        self.b = torch.nn.functional.pad(b, (0, pad)).contiguous() if pad else b.contiguous()
-        if self.a.data_ptr() % 16:
-            self.a = self.a.clone()
-        if self.b.data_ptr() % 16:
-            self.b = self.b.clone()
+        self.a = _aligned(torch.nn.functional.pad(a, (0, 0, 0, pad)) if pad else a, 16)
+        self.b = _aligned(torch.nn.functional.pad(b, (0, pad)) if pad else b, 16)
         self.scale = scale.contiguous()
 
 

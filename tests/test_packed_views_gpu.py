@@ -56,3 +56,20 @@ def test_a_lone_expert_of_any_stride():
     for view in lone_rows(router):
         got = route_tokens(x, view, 1, scoring="sigmoid", normalize=False)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_payloads_at_any_address():
+    """Words and scales cut from larger buffers, at addresses that the kernels' loads do not take."""
+
+    rng = np.random.default_rng(94)
+    words, suh, svh = (torch.from_numpy(v).cuda() for v in payload(rng, 256, 128, (3, 4), "k"))
+
+    def moved(v):
+        wide = torch.zeros(v.numel() + 1, dtype=v.dtype, device="cuda")
+        wide[1:] = v
+        return wide[1:]
+
+    x = rows(rng, 3, 256, torch.bfloat16).cuda()
+    want = packed_linear(x, PackedLinear(words, suh, svh, (3, 4), LUTS))
+    for cut in ((moved(words), suh, svh), (words, moved(suh), svh), (words, suh, moved(svh))):
+        assert torch.equal(packed_linear(x, PackedLinear(*cut, (3, 4), LUTS)), want)
