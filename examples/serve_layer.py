@@ -26,7 +26,7 @@ from qsrt_amd.ldlq import make_shared_h
 from qsrt_amd.packed_linear import LowRankAdapters, PackedLinear, adapter_linear
 from qsrt_amd.packed_moe import PackedExperts, PackedMoELayer
 from qsrt_amd.qsrt import Geometry
-from qsrt_amd.qsrt_coupled import CoupledHadamardSpec, decode_coupled_weights
+from qsrt_amd.qsrt_coupled import CoupledHadamardSpec, decode_coupled_weights, situ
 from qsrt_amd.qsrt_rate_atoms import QSRTRateLayerLayout, QSRTRateLayerReader, RateSchedule, materialize_rate_layer
 from qsrt_amd.sqg_e4m3 import sqg_xor_cheb_t12_bytes
 
@@ -58,14 +58,15 @@ def write_synthetic_layer(path: Path, *, hidden: int, inter: int, experts: int, 
     materialize_rate_layer(path, QSRTRateLayerLayout(24, schedule, tuple(range(experts))), payloads())
 
 
-def load_layer(path: Path, coupled, device) -> tuple:
+def load_layer(path: Path, coupled, activation: str, device) -> tuple:
     """The file's experts: ``(PackedExperts, their payloads for the check, the schedule)``."""
 
     luts = {b: sqg_xor_cheb_t12_bytes(b) for b in (2, 3, 4)}
     with QSRTRateLayerReader(path) as reader:
         schedule = reader.layout.schedule
         payloads = [reader.read_expert(e) for e in reader.layout.experts]
-    packed = PackedExperts.from_experts(payloads, schedule.record_bits, luts, coupled=coupled, device=device)
+    packed = PackedExperts.from_experts(payloads, schedule.record_bits, luts, activation=activation, coupled=coupled,
+                                        device=device)
     return packed, payloads, schedule
 
 
@@ -108,6 +109,7 @@ def main(argv=None) -> dict:
     args = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     args.add_argument("--file", type=Path, help="a rate-record layer file (default: a synthetic one)")
     args.add_argument("--coupled", action="store_true", help="its weights are in coupled coordinates (default profile)")
+    args.add_argument("--activation", choices=("swiglu", "situ"), default="swiglu", help="what the layer was calibrated with")
     args.add_argument("--hidden", type=int, default=1024)
     args.add_argument("--inter", type=int, default=512)
     args.add_argument("--experts", type=int, default=16)
@@ -123,7 +125,7 @@ def main(argv=None) -> dict:
         if path is None:
             path = Path(directory) / "qsrt-layer-00024.safetensors"
             write_synthetic_layer(path, hidden=args.hidden, inter=args.inter, experts=args.experts, generator=gen)
-        packed, payloads, schedule = load_layer(path, coupled, device)
+        packed, payloads, schedule = load_layer(path, coupled, args.activation, device)
     hidden, experts = packed.hidden, packed.experts
     linear, dense = encode_projection(hidden, device, gen)
 
@@ -150,7 +152,8 @@ def main(argv=None) -> dict:
     for i in range(args.tokens):
         for w, e in zip(weights[i].tolist(), chosen[i].tolist()):
             g, u = h[i].float() @ matrices[e]["w1"], h[i].float() @ matrices[e]["w3"]
-            want[i] += w * ((torch.nn.functional.silu(g) * u) @ matrices[e]["w2"])
+            middle = situ(g, u) if args.activation == "situ" else torch.nn.functional.silu(g) * u
+            want[i] += w * (middle @ matrices[e]["w2"])
     errors["layer"] = float((y.float() - want).norm() / want.norm())
     del matrices
 

@@ -76,12 +76,18 @@ class PackedExperts:
     """The experts of one layer: ``w1`` and ``w3 [hidden, inter]`` (gate and up) and ``w2 [inter, hidden]`` (down), each a
     dict of the stacked payloads of all experts: ``trellis`` int16 ``[experts, words]``, ``suh``/``svh`` float16 (one
     vector for the layer or ``[experts, ...]``), ``record_bits`` (one rate, one schedule, or one for each expert) and
-    ``rate_axis`` (default: columns for w1 and w3, rows for w2, as stored).  ``coupled``: the payloads hold coupled
-    coordinates (``qsrt_coupled.encode_coupled_weights``) of that spec, of its default block sizes; ``x`` and the result
-    are in the source's coordinates all the same."""
+    ``rate_axis`` (default: columns for w1 and w3, rows for w2, as stored).  ``activation``: the model's, ``"swiglu"`` or
+    ``"situ"``.  ``coupled``: the payloads hold coupled coordinates (``qsrt_coupled.encode_coupled_weights``) of that spec,
+    of its default block sizes; ``x`` and the result are in the source's coordinates all the same.  The activation has to
+    be named then: execution and calibration in coupled coordinates take ``situ`` unless told otherwise, plain payloads here
+    ``swiglu``."""
 
-    def __init__(self, w1: dict, w3: dict, w2: dict, luts_by_bits: dict, *, activation: str = "swiglu",
+    def __init__(self, w1: dict, w3: dict, w2: dict, luts_by_bits: dict, *, activation: str | None = None,
                  coupled: CoupledHadamardSpec | None = None):
+        if activation is None:
+            if coupled is not None:
+                raise ValueError(f"coupled experts need their activation named: one of {tuple(ACTIVATIONS)}")
+            activation = "swiglu"
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
         self.experts = int(w1["trellis"].shape[0])
@@ -107,9 +113,10 @@ class PackedExperts:
             self.sign_pointers = tuple(s.data_ptr() for s in self.signs)
 
     @classmethod
-    def from_experts(cls, experts: list, record_bits, luts_by_bits: dict, *, activation: str = "swiglu",
+    def from_experts(cls, experts: list, record_bits, luts_by_bits: dict, *, activation: str,
                      coupled: CoupledHadamardSpec | None = None, device="cuda:0") -> "PackedExperts":
-        """From a list of ``{"w1", "w3", "w2"}`` dicts as a layer file's reader returns them (``read_expert``)."""
+        """From a list of ``{"w1", "w3", "w2"}`` dicts as a layer file's reader returns them (``read_expert``).  The file does
+        not say which ``activation`` its layer was calibrated with, so the caller does."""
 
         def stack(name):
             def scale(part):
