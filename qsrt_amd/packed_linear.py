@@ -41,6 +41,13 @@ def _records(record_bits, lead: tuple, rate_axis: str, k: int, n: int, words: in
     return tables, rates
 
 
+def refuse_gradients(*tensors) -> None:
+    """Packed products have no backward pass: better no result than one that a gradient silently stops at."""
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("packed products have no backward pass: call them under torch.no_grad() or detach their inputs")
+
+
 def _aligned(t: torch.Tensor, size: int) -> torch.Tensor:
     """``t`` in one piece at a multiple of ``size`` bytes, copied where it is not."""
 
@@ -204,17 +211,19 @@ def _run(x, linear, bank, ids, out):
 
 
 def packed_linear(x: torch.Tensor, linear: PackedLinear, *, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x [T, K] @ W -> [T, N]`` in ``x``'s type (bf16 or f16), FP32 sums."""
+    """``x [T, K] @ W -> [T, N]`` in ``x``'s type (bf16 or f16), FP32 sums.  No backward pass."""
 
+    refuse_gradients(x, linear.matrix.suh, linear.matrix.svh)
     return _run(x, linear, None, None, out)
 
 
 def adapter_linear(x: torch.Tensor, linear: PackedLinear, adapters: LowRankAdapters, ids: torch.Tensor, *,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """``x W + scale[a] (x A_a^T) B_a^T`` with ``a = ids[t]`` for row ``t``; an id outside ``[0, adapters)`` (-1) means
-    none.  ``ids`` int32 ``[T]``, any order; one launch sequence serves all adapters."""
+    none.  ``ids`` int32 ``[T]``, any order; one launch sequence serves all adapters.  No backward pass."""
 
     m = linear.matrix
+    refuse_gradients(x, adapters.a, adapters.b, adapters.scale, m.suh, m.svh)
     if adapters.a.shape[2] != m.k or adapters.b.shape[1] != m.n:
         raise ValueError("the adapters do not match the projection")
     if adapters.a.dtype != x.dtype or adapters.a.device != m.device:

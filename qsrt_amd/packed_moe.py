@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows, leading
+from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows, leading, refuse_gradients
 from .qsrt_coupled import CoupledHadamardSpec, rotation_signs
 
 SCORING = {"softmax": 0, "sigmoid": 1}
@@ -66,8 +66,9 @@ def route_tokens(x: torch.Tensor, weight: torch.Tensor, k: int, *, bias: torch.T
     Scores are the softmax or the sigmoid of ``x weight^T`` (``weight [experts, hidden]``, of ``x``'s type).  The largest
     ``score + bias`` (without a bias: the largest logits) are chosen, ties to the lowest index, NaN last, and returned in
     falling order; their weights are the scores without the bias, divided by their sum where ``normalize``, times
-    ``scale``."""
+    ``scale``.  No backward pass."""
 
+    refuse_gradients(x, weight, bias)
     weight, bias = _checked_router(weight, k, bias, scoring)
     return _route(x, weight, k, bias, scoring, normalize, scale)
 
@@ -101,6 +102,7 @@ class PackedExperts:
             raise ValueError("w1, w3 [hidden, inter] and w2 [inter, hidden] do not match")
         if (self.w1.suh.dim() == 1) != (self.w3.suh.dim() == 1):
             raise ValueError("w1 and w3 must both share their suh, or neither")
+        self.scales = tuple(s for m in (self.w1, self.w3, self.w2) for s in (m.suh, m.svh))
         self.luts = LabelTables(luts_by_bits, self.w1.rates | self.w3.rates | self.w2.rates, self.device)
         self.activation = ACTIVATIONS[activation]
         self.signs, self.sign_pointers = (), (None, None)
@@ -138,8 +140,9 @@ class PackedExperts:
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """``out[t] = sum_j weights[t, j] act(x_t W1_e, x_t W3_e) W2_e`` with ``e = ids[t, j]``; an id outside
         ``[0, experts)`` (-1) contributes nothing.  ``x [T, hidden]`` bf16 or f16, ``weights`` float32 and ``ids`` int32
-        ``[T, k]``."""
+        ``[T, k]``.  No backward pass."""
 
+        refuse_gradients(x, weights, *self.scales)
         x = checked_rows(x, self.hidden, self.device)
         out = checked_out(out, x, self.hidden)
         if (ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape[1] < 1 or weights.shape != ids.shape
@@ -165,7 +168,8 @@ class PackedExperts:
 
 
 class PackedMoELayer:
-    """Router and packed experts of one layer; calling it on ``x [T, hidden]`` returns ``(y, weights, ids)``."""
+    """Router and packed experts of one layer; calling it on ``x [T, hidden]`` returns ``(y, weights, ids)``.  No backward
+    pass."""
 
     def __init__(self, router: torch.Tensor, experts: PackedExperts, k: int, *, bias: torch.Tensor | None = None,
                  scoring: str = "softmax", normalize: bool = True, scale: float = 1.0):
@@ -176,6 +180,7 @@ class PackedMoELayer:
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None):
         e = self.experts
+        refuse_gradients(x, self.router, self.bias, *e.scales)
         if x.dtype != self.router.dtype:
             raise ValueError("x must be of the router's type")
         x = checked_rows(x, e.hidden, e.device)
