@@ -1273,13 +1273,19 @@ RowCut cut_rows(int64_t rows, int64_t nb, int strips, int limit, int cus) {
     return best;
 }
 
-const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts) {
-    if (!m || !m->words || !m->records || !m->suh || !m->svh) return "null pointer in a matrix";
+// What a workspace's size depends on; its functions take any numbers, and answer 0 where the call would refuse them.
+const char* size_fault(const qsrt_packed_matrix* m) {
     if (m->rows <= 0 || m->cols <= 0 || m->rows % 128 || m->cols % 128) return "rows and cols must be multiples of 128";
     if (m->rows > (1 << 22) || m->cols > (1 << 22) || m->rows * m->cols >= int64_t(1) << 32)
         return "matrix too large (2^32 weights)";  // the kernels' offsets in a payload have 31 bits, K4 takes half a byte
     if (m->rate_axis != 0 && m->rate_axis != 1) return "rate_axis must be 0 (rows) or 1 (columns)";
     if ((m->rates & 0x1C) == 0 || (m->rates & ~0x1C)) return "rates must name K2, K3 or K4";
+    return nullptr;
+}
+
+const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts) {
+    if (!m || !m->words || !m->records || !m->suh || !m->svh) return "null pointer in a matrix";
+    if (const char* e = size_fault(m)) return e;
     if (m->key_stride < 0 || m->record_stride < 0 || m->suh_stride < 0 || m->svh_stride < 0) return "negative stride";
     if (reinterpret_cast<uintptr_t>(m->words) % 4 || m->key_stride % 2) return "words must be 4-byte aligned";
     if (reinterpret_cast<uintptr_t>(m->suh) % 8 || reinterpret_cast<uintptr_t>(m->svh) % 8 || m->suh_stride % 4 ||
@@ -1392,10 +1398,10 @@ int launch_rotate(const RotateArgs& args, int dtype, hipStream_t stream) {
     return kOk;
 }
 
-const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
-                      const uint8_t* const* luts, int64_t experts, int64_t tokens, int k) {
+const char* moe_size_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                           int64_t experts, int64_t tokens, int k) {
     for (const qsrt_packed_matrix* m : {w1, w3, w2})
-        if (const char* e = matrix_fault(m, luts)) return e;
+        if (const char* e = size_fault(m)) return e;
     if (w1->rows != w3->rows || w1->cols != w3->cols || w2->rows != w1->cols || w2->cols != w1->rows ||
         w1->rate_axis != w3->rate_axis)
         return "w1, w3 [hidden, inter] and w2 [inter, hidden] do not match";
@@ -1405,6 +1411,13 @@ const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3
         return "tokens * k must be at most 2^20";
     if (!launch_fits(tokens * k, w1->cols, w1->rows)) return "too many tokens for these matrices";
     return nullptr;
+}
+
+const char* moe_fault(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                      const uint8_t* const* luts, int64_t experts, int64_t tokens, int k) {
+    for (const qsrt_packed_matrix* m : {w1, w3, w2})
+        if (const char* e = matrix_fault(m, luts)) return e;
+    return moe_size_fault(w1, w3, w2, experts, tokens, k);
 }
 
 struct MoeCall {
@@ -1563,8 +1576,7 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
 extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3,
                                                   const qsrt_packed_matrix* w2, int64_t experts, int64_t tokens, int k) {
     int cus = 0;
-    if (!w1 || !w3 || !w2 || experts < 1 || tokens <= 0 || k < 1 || w1->rows <= 0 || w1->cols <= 0 || current_cu_count(&cus))
-        return 0;
+    if (!w1 || !w3 || !w2 || tokens == 0 || moe_size_fault(w1, w3, w2, experts, tokens, k) || current_cu_count(&cus)) return 0;
     return moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates, w1->suh_stride == 0,
                      true, true, cus)
         .bytes;
@@ -1643,12 +1655,21 @@ LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates
     return s;
 }
 
+const char* linear_size_fault(const qsrt_packed_matrix* w, int64_t rows, int64_t adapters, int64_t rank) {
+    if (const char* e = size_fault(w)) return e;
+    if (rows < 0 || rows > (1 << 20)) return "at most 2^20 rows";
+    if (adapters < 0 || adapters > kMaxKeys) return "at most 8191 adapters";
+    if (adapters && (rank < 16 || rank > kMaxRank || rank % 16)) return "adapters need a rank 16, 32 .. 128";
+    if (!launch_fits(rows, w->rows, w->cols)) return "too many rows for this matrix";
+    return nullptr;
+}
+
 }  // namespace
 
 extern "C" size_t qsrt_adapter_linear_workspace_bytes(const qsrt_packed_matrix* w, int64_t rows, int64_t adapters,
                                                       int64_t rank) {
     int cus = 0;
-    if (!w || rows <= 0 || w->rows <= 0 || w->cols <= 0 || current_cu_count(&cus)) return 0;
+    if (!w || rows == 0 || linear_size_fault(w, rows, adapters, rank) || current_cu_count(&cus)) return 0;
     return linear_space(nullptr, rows, w->rows, w->cols, w->rates, adapters, rank, cus).bytes;
 }
 
@@ -1657,15 +1678,12 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
                                    int dtype, int64_t rows, const int32_t* ids, void* out, int64_t out_ld, void* ws,
                                    size_t ws_bytes, void* stream_) {
     if (const char* e = matrix_fault(w, luts)) return fail(kBadArgument, "qsrt_adapter_linear: %s", e);
-    if (rows < 0 || rows > (1 << 20)) return fail(kBadArgument, "qsrt_adapter_linear: at most 2^20 rows");
+    if (const char* e = linear_size_fault(w, rows, adapters, rank)) return fail(kBadArgument, "qsrt_adapter_linear: %s", e);
     if (dtype != 0 && dtype != 1) return fail(kBadArgument, "qsrt_adapter_linear: dtype must be 0 (bf16) or 1 (f16)");
-    if (adapters < 0 || adapters > kMaxKeys) return fail(kBadArgument, "qsrt_adapter_linear: at most %d adapters", kMaxKeys);
-    if (adapters && (!a || !b || !scale || !ids || rank < 16 || rank > kMaxRank || rank % 16 ||
-                     reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(b) % 16))
-        return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a, b of a rank 16, 32 .. 128, scales and ids");
+    if (adapters && (!a || !b || !scale || !ids || reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(b) % 16))
+        return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a and b, scales and ids");
     if (rows == 0) return kOk;
     const int64_t k = w->rows, n = w->cols;
-    if (!launch_fits(rows, k, n)) return fail(kBadArgument, "qsrt_adapter_linear: too many rows for this matrix");
     if (const char* e = rows_fault(x, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
     if (const char* e = rows_fault(out, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
     int cus = 0;

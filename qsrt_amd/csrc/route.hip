@@ -386,6 +386,12 @@ int launch_group(const GroupArgs& args, const RotateArgs& beside, int dtype, hip
     return kOk;
 }
 
+namespace {
+bool route_sizes(int64_t tokens, int64_t hidden, int64_t experts) {
+    return tokens >= 0 && tokens <= 1 << 20 && hidden > 0 && hidden <= 1 << 24 && experts > 0 && experts <= kMaxExperts;
+}
+}  // namespace
+
 const char* router_fault(const RouterArgs& a) {
     if (!a.x || !a.weight || !a.weights || !a.ids || a.tokens < 0 || a.hidden <= 0 || a.experts <= 0)
         return "null pointer or bad size in the router";
@@ -446,7 +452,7 @@ int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs
 using namespace qsrt;
 
 extern "C" size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
-    if (tokens <= 0 || hidden <= 0 || experts <= 0) return 0;
+    if (tokens == 0 || !route_sizes(tokens, hidden, experts)) return 0;
     return router_logit_bytes(tokens, hidden, experts);
 }
 
@@ -454,7 +460,7 @@ extern "C" int qsrt_route(const void* x, int64_t x_ld, const void* weight, int64
                           int64_t hidden, int64_t experts, int k, const float* bias, int scoring, int normalize,
                           float scale, float* weights, int32_t* ids, void* ws, size_t ws_bytes, void* stream) {
     if (tokens == 0) return kOk;
-    if (tokens < 0 || tokens > (1 << 20) || hidden <= 0 || hidden > (1 << 24) || experts <= 0 || experts > kMaxExperts)
+    if (!route_sizes(tokens, hidden, experts))
         return fail(kBadArgument, "qsrt_route: bad sizes (at most 2^20 tokens, 2^24 channels, %d experts)", kMaxExperts);
     const RouterArgs args{x, x_ld, weight, weight_ld, dtype, static_cast<int>(tokens), static_cast<int>(hidden),
                           static_cast<int>(experts), k, bias, scoring, normalize, scale, weights, ids,
