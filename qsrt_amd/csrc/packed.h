@@ -289,6 +289,7 @@ struct RouterArgs {
 };
 const char* router_fault(const RouterArgs& args);
 size_t router_logit_bytes(int64_t tokens, int64_t hidden, int64_t experts);
+int64_t router_blocks(int64_t tokens, int64_t hidden, int64_t experts, const RotateArgs& beside);  // of 256 threads
 int launch_router(const RouterArgs& args, const RotateArgs& beside, const GroupArgs* group, hipStream_t stream);
 
 }  // namespace qsrt

@@ -1297,7 +1297,9 @@ const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts
     return nullptr;
 }
 
-// A launch has fewer than 2^32 threads; none here takes more than one for two channels, of rows rounded up to 16.
+// A launch has fewer than 2^32 threads.  None here takes more than one for two channels, of rows rounded up to 16, but for an
+// adapter projection's, which have 2^28 more at the most (256 a row), and the layer's router, which shares its launch with a
+// rotation and is looked at by itself.
 bool launch_fits(int64_t rows, int64_t a, int64_t b) { return (rows + 15) / 16 * 16 * std::max(a, b) < int64_t(1) << 32; }
 
 const char* rows_fault(const void* p, int64_t ld, int64_t cols, int align) {
@@ -1452,6 +1454,15 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     if (const char* e = rows_fault(c.x, c.x_ld, hidden, 8)) return fail(kBadArgument, "%s: x: %s", name, e);
     if (const char* e = rows_fault(c.out, c.out_ld, hidden, 8)) return fail(kBadArgument, "%s: out: %s", name, e);
     if (!c.ids || !c.weights) return fail(kBadArgument, "%s: null routing", name);
+    if (router) {
+        if (const char* e = router_fault(*router)) return fail(kBadArgument, "%s: %s", name, e);
+        RotateArgs rows{};  // those that all experts share are rotated beside it
+        rows.rows = c.w1->suh_stride == 0 ? c.tokens : 0;
+        rows.kb = static_cast<int>(hidden / 128);
+        rows.nmat = 2;
+        if (router_blocks(c.tokens, hidden, c.experts, rows) * 256 >= int64_t(1) << 32)
+            return fail(kBadArgument, "%s: too many tokens for these matrices", name);
+    }
     int cus = 0;
     if (const int rc = current_cu_count(&cus)) return rc;
     const bool shared = c.w1->suh_stride == 0;
@@ -1490,7 +1501,6 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     if (!shared && !s.every) beside.rows = 0;
     if (router) {
         router->logits = s.logits;
-        if (const char* e = router_fault(*router)) return fail(kBadArgument, "%s: %s", name, e);
         if (const int rc = launch_router(*router, beside, &ga, stream)) return rc;
     } else if (const int rc = launch_group(ga, beside, c.dtype, stream)) {
         return rc;

@@ -409,10 +409,14 @@ size_t router_logit_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
     return sizeof(float) * static_cast<size_t>(router_splits(tokens, hidden, experts)) * tokens * experts;
 }
 
+int64_t router_blocks(int64_t tokens, int64_t hidden, int64_t experts, const RotateArgs& beside) {
+    return (experts + 15) / 16 * ((tokens + 15) / 16) * router_splits(tokens, hidden, experts) + (rotate_waves(beside) + 3) / 4;
+}
+
 int launch_router(const RouterArgs& a, const RotateArgs& beside, const GroupArgs* group, hipStream_t stream) {
     LogitsArgs la{a.x, a.weight, a.x_ld, a.weight_ld, a.tokens, a.hidden, a.experts,
                   router_splits(a.tokens, a.hidden, a.experts), (a.experts + 15) / 16, (a.tokens + 15) / 16, a.logits, beside};
-    const int64_t blocks = static_cast<int64_t>(la.etiles) * la.ttiles * la.splits + (rotate_waves(beside) + 3) / 4;
+    const int64_t blocks = router_blocks(a.tokens, a.hidden, a.experts, beside);
     if (a.dtype == 0)
         hipLaunchKernelGGL(router_logits_kernel<__bf16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, la);
     else

@@ -40,6 +40,24 @@ def struct(**changes):
     return ctypes.byref(_native.PackedMatrixStruct(**fields))
 
 
+@needs_library
+@pytest.mark.parametrize("experts,words", [(1024, "too many tokens"), (8, None)])
+def test_a_layer_counts_the_threads_of_router_and_rotation_together(experts, words):
+    """2^20 tokens of 3968 channels: the rotation alone has 0.97 of the threads a launch can have."""
+
+    at = 1 << 12  # an aligned address; nothing reads it
+    tables = (ctypes.c_void_p * 3)(at, at, at)
+    up = struct(words=at, records=at, suh=at, svh=at, rows=3968, cols=128)
+    down = struct(words=at, records=at, suh=at, svh=at, rows=128, cols=3968)
+    rc = _native.lib().qsrt_packed_moe_layer(up, up, down, ctypes.addressof(tables), experts, 0, None, None, at, 3968, None, 0, 1,
+                                             1.0, at, 3968, 0, 1 << 20, 1, at, at, at, 3968, None, 0, None)
+    message = _native.lib().qsrt_last_error().decode()
+    if words:
+        assert rc == -1 and words in message, (rc, message)
+    else:  # goes on to its workspace, or without a GPU to the device
+        assert rc in (-2, -3), (rc, message)
+
+
 @pytest.mark.gpu
 def test_product_workspaces_of_any_sizes():
     up, down, lib = struct(), struct(rows=128, cols=256), _native.lib()
