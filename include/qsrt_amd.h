@@ -507,9 +507,10 @@ int qsrt_packed_moe_layer(const qsrt_packed_matrix *w1, const qsrt_packed_matrix
  *   out[t] = x_t W + scale[a] (x_t A_a^T) B_a^T,  a = ids[t]
  * A [adapters, rank, rows of W] and B [adapters, cols of W, rank] in x's
  * type, rank a multiple of 16 up to 128 (zero-padded), 16-byte aligned; an
- * id outside [0, adapters) has no adapter.  adapters = 0 leaves them out (a,
- * b, scale and ids may be NULL).  x rows 16-byte aligned, out rows 8-byte
- * aligned.  Needs qsrt_adapter_linear_workspace_bytes bytes of workspace.
+ * id outside [0, adapters) has no adapter; adapters <= 8191.  adapters = 0
+ * leaves them out (a, b, scale and ids may be NULL).  x rows 16-byte aligned,
+ * out rows 8-byte aligned.  Needs qsrt_adapter_linear_workspace_bytes bytes of
+ * workspace.
  */
 size_t qsrt_adapter_linear_workspace_bytes(const qsrt_packed_matrix *w, int64_t rows, int64_t adapters, int64_t rank);
 int qsrt_adapter_linear(const qsrt_packed_matrix *w, const uint8_t *const *luts, const void *a, const void *b,

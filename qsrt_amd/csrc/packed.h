@@ -129,11 +129,6 @@ __device__ __forceinline__ void store_halves(char* row, const RowLayout& l, int 
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
-    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-}
 
 // Rows into a payload's basis: (x * suh) H in pieces.  `residual`: x is turned by the normalised Hadamard on blocks of 512
 // first, as coupled weights take it.

@@ -776,6 +776,7 @@ __global__ __launch_bounds__(256 * kCoupledShares) void combine_coupled_kernel(c
 // ---------------------------------------------------------------------------
 
 constexpr int kMaxRank = 128;
+constexpr int kMaxAdapters = 8191;  // what callers are promised; no kernel depends on how many there are
 
 struct ShrinkArgs {
     const void* x;
@@ -1668,7 +1669,7 @@ LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates
 const char* linear_size_fault(const qsrt_packed_matrix* w, int64_t rows, int64_t adapters, int64_t rank) {
     if (const char* e = size_fault(w)) return e;
     if (rows < 0 || rows > (1 << 20)) return "at most 2^20 rows";
-    if (adapters < 0 || adapters > kMaxKeys) return "at most 8191 adapters";
+    if (adapters < 0 || adapters > kMaxAdapters) return "at most 8191 adapters";
     if (adapters && (rank < 16 || rank > kMaxRank || rank % 16)) return "adapters need a rank 16, 32 .. 128";
     if (!launch_fits(rows, w->rows, w->cols)) return "too many rows for this matrix";
     return nullptr;
