@@ -32,8 +32,8 @@ __global__ __launch_bounds__(256) void router_logits_kernel(const LogitsArgs p) 
     const int split = blockIdx.x / (p.etiles * p.ttiles);
     typedef T t8 __attribute__((ext_vector_type(8)));
     // rows past the end repeat the last; not stored
-    const T* wr = static_cast<const T*>(p.w) + min(e0 + m, p.experts - 1) * p.w_ld + 8 * g;
-    const T* xr = static_cast<const T*>(p.x) + min(t0 + m, p.tokens - 1) * p.ld + 8 * g;
+    const T* wr = static_cast<const T*>(p.w) + min(e0 + m, p.experts - 1) * p.w_ld;
+    const T* xr = static_cast<const T*>(p.x) + min(t0 + m, p.tokens - 1) * p.ld;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](t8 a, t8 b) {
         if constexpr (__is_same(T, __bf16))
@@ -41,24 +41,33 @@ __global__ __launch_bounds__(256) void router_logits_kernel(const LogitsArgs p) 
         else
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
     };
-    constexpr int kStep = 32 * 4, kBatch = 7;
+    constexpr int kStep = 32 * 4, kBatch = 8;
     const int steps = (p.hidden + 31) / 32;
     const int end = min(p.hidden, 32 * static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits));
     int h = 32 * static_cast<int>(static_cast<int64_t>(steps) * split / p.splits) + 32 * wave;
-    for (; h + (kBatch - 1) * kStep + 32 <= end; h += kBatch * kStep) {  // a batch of loads in flight
+    const t8 zero = {};
+    // The loads of a batch go out together, also of one that is not full (16 tokens and 64 or 384 experts, weights not cached: 4.9
+    // and 5.0 us at 2048 channels, 4.9 and 5.4 at 5120, 5.0 and 5.8 at 7168; one after the other in a batch that is not full 5.7
+    // and 6.3 at 5120).  Leaving out those past the end by a branch cost 96 tokens of 7168 channels 18.6 us, 17.6 so.
+    for (; h < end; h += kBatch * kStep) {
         t8 a[kBatch], b[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            a[j] = *reinterpret_cast<const t8*>(wr + h + j * kStep);
-            b[j] = *reinterpret_cast<const t8*>(xr + h + j * kStep);
+            const int at = min(h + j * kStep + 8 * g, p.hidden - 8);  // past the end: the last, which nobody takes
+            a[j] = *reinterpret_cast<const t8*>(wr + at);
+            b[j] = *reinterpret_cast<const t8*>(xr + at);
         }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) multiply(a[j], b[j]);
-    }
-    const t8 zero = {};
-    for (; h < end; h += kStep) {
-        const bool in = h + 8 * g < end;  // hidden is a multiple of 8
-        multiply(in ? *reinterpret_cast<const t8*>(wr + h) : zero, in ? *reinterpret_cast<const t8*>(xr + h) : zero);
+        for (int j = 0; j < kBatch; ++j) {
+            const int from = h + j * kStep;
+            if (from >= end) break;
+            if (from + 32 <= end) {
+                multiply(a[j], b[j]);
+            } else {
+                const bool in = from + 8 * g < end;  // hidden is a multiple of 8
+                multiply(in ? a[j] : zero, in ? b[j] : zero);
+            }
+        }
     }
     sums[wave][lane] = acc;
     __syncthreads();
@@ -72,10 +81,13 @@ __global__ __launch_bounds__(256) void router_logits_kernel(const LogitsArgs p) 
         if (e0 + 4 * g + i < p.experts) out[i] = acc[i];
 }
 
-// Splits of the channels: workgroups for every compute unit, each wave with a batch of steps at the least.
+// Splits of the channels: at most eight, whose sums the choice adds up, as many as there are compute units for, and each wave
+// with half a batch of steps at the least.  The number stands in the workspace's size, which is asked for without a device: it
+// counts on gfx950's 256 units.
 int router_splits(int64_t tokens, int64_t hidden, int64_t experts) {
+    constexpr int64_t kUnits = 256, kMost = 8, kLeast = 4 * 32 * 4;
     const int64_t tiles = ((tokens + 15) / 16) * ((experts + 15) / 16);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, std::min<int64_t>(8, hidden / 512))));
+    return static_cast<int>(std::max<int64_t>(1, std::min({kUnits / tiles, kMost, hidden / kLeast})));
 }
 
 constexpr int kMaxExperts = 1024;
