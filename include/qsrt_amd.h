@@ -518,6 +518,18 @@ int qsrt_adapter_linear(const qsrt_packed_matrix *w, const uint8_t *const *luts,
                         int64_t rows, const int32_t *ids, void *out, int64_t out_ld, void *ws, size_t ws_bytes,
                         void *stream);
 
+/*
+ * How a call would be run on the current device, for tests and profiles:
+ * plan[0] is how many rows share one decode of a label at the most (8, 16,
+ * 32 or 64: a wave's; 256 or 512: a workgroup's).  Experts: plan[1] and
+ * plan[2] are the parts that the K axes of their first and second products
+ * are cut into.  Projections: plan[1] their product's parts, plan[2] its
+ * pieces of work (rows by columns by parts).
+ */
+int qsrt_packed_moe_plan(const qsrt_packed_matrix *w1, const qsrt_packed_matrix *w3, const qsrt_packed_matrix *w2,
+                         int64_t experts, int64_t tokens, int k, int64_t *plan);
+int qsrt_adapter_linear_plan(const qsrt_packed_matrix *w, int64_t rows, int64_t adapters, int64_t rank, int64_t *plan);
+
 #ifdef __cplusplus
 }
 #endif

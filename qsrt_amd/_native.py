@@ -132,6 +132,8 @@ SIGNATURES: dict[str, tuple] = {
          ctypes.c_float, _c_void_p, _c_i64, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
          _c_size, _c_void_p],
     ),
+    "qsrt_packed_moe_plan": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_int, _c_void_p]),
+    "qsrt_adapter_linear_plan": (_c_int, [_c_void_p, _c_i64, _c_i64, _c_i64, _c_void_p]),
     "qsrt_adapter_linear_workspace_bytes": (_c_size, [_c_void_p, _c_i64, _c_i64, _c_i64]),
     "qsrt_adapter_linear": (
         _c_int,

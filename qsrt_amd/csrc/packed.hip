@@ -1593,6 +1593,20 @@ extern "C" size_t qsrt_packed_moe_workspace_bytes(const qsrt_packed_matrix* w1, 
         .bytes;
 }
 
+extern "C" int qsrt_packed_moe_plan(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
+                                    int64_t experts, int64_t tokens, int k, int64_t* plan) {
+    if (!w1 || !w3 || !w2 || !plan || tokens == 0) return fail(kBadArgument, "qsrt_packed_moe_plan: null pointer or no tokens");
+    if (const char* e = moe_size_fault(w1, w3, w2, experts, tokens, k)) return fail(kBadArgument, "qsrt_packed_moe_plan: %s", e);
+    int cus = 0;
+    if (const int rc = current_cu_count(&cus)) return rc;
+    const MoeSpace s = moe_space(nullptr, tokens, k, w1->rows, w1->cols, experts, w1->rates | w3->rates, w2->rates,
+                                 w1->suh_stride == 0, true, true, cus);
+    plan[0] = chunk_rows_of(s.groups);
+    plan[1] = s.parts[0];
+    plan[2] = s.parts[1];
+    return kOk;
+}
+
 extern "C" int qsrt_packed_moe(const qsrt_packed_matrix* w1, const qsrt_packed_matrix* w3, const qsrt_packed_matrix* w2,
                                const uint8_t* const* luts, int64_t experts, int activation, const float* pre_signs,
                                const float* post_signs, const void* x, int64_t x_ld, int dtype, int64_t tokens, int k, const int32_t* ids, const float* weights, void* out,
@@ -1682,6 +1696,19 @@ extern "C" size_t qsrt_adapter_linear_workspace_bytes(const qsrt_packed_matrix* 
     int cus = 0;
     if (!w || rows == 0 || linear_size_fault(w, rows, adapters, rank) || current_cu_count(&cus)) return 0;
     return linear_space(nullptr, rows, w->rows, w->cols, w->rates, adapters, rank, cus).bytes;
+}
+
+extern "C" int qsrt_adapter_linear_plan(const qsrt_packed_matrix* w, int64_t rows, int64_t adapters, int64_t rank,
+                                        int64_t* plan) {
+    if (!w || !plan || rows == 0) return fail(kBadArgument, "qsrt_adapter_linear_plan: null pointer or no rows");
+    if (const char* e = linear_size_fault(w, rows, adapters, rank)) return fail(kBadArgument, "qsrt_adapter_linear_plan: %s", e);
+    int cus = 0;
+    if (const int rc = current_cu_count(&cus)) return rc;
+    const LinearSpace s = linear_space(nullptr, rows, w->rows, w->cols, w->rates, adapters, rank, cus);
+    plan[0] = s.row_groups ? 16 * kRowWaves * s.row_groups : chunk_rows_of(s.groups);
+    plan[1] = s.parts;
+    plan[2] = static_cast<int64_t>(s.product_chunks) * (w->cols / 128) * s.parts;
+    return kOk;
 }
 
 extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* const* luts, const void* a, const void* b,
