@@ -219,8 +219,13 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    """The current stream of ``device`` (without a stream object: 0.1 us, not 1.9)."""
+    """The current stream of ``device`` (without a stream object: 0.1 us, not 1.9).
 
+    Every launch asks for it, so this is also where tensors in host memory are stopped: their addresses would go to a
+    kernel."""
+
+    if device.type != "cuda":
+        raise ValueError(f"the kernels take tensors on a CUDA device, not on {device}")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
