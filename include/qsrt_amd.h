@@ -456,8 +456,9 @@ typedef struct qsrt_packed_matrix {
  * falling order of key, and their scores (without bias) as weights, divided
  * by their sum where `normalize`, times `scale`.  weights f32 and ids int32
  * [tokens, k].  hidden and both leading dimensions multiples of 8, rows
- * 16-byte aligned; experts <= 1024, k <= min(64, experts).  This workspace
- * function and those below take any numbers: 0 where the call refuses them.
+ * 16-byte aligned; experts <= 1024, k <= min(64, experts).  Here and below the
+ * leading dimension of a lone row is not looked at, and workspace functions
+ * take any numbers: 0 where the call refuses them.
  */
 size_t qsrt_route_workspace_bytes(int64_t tokens, int64_t hidden, int64_t experts);
 int qsrt_route(const void *x, int64_t x_ld, const void *weight, int64_t weight_ld, int dtype, int64_t tokens,

@@ -1303,9 +1303,9 @@ const char* matrix_fault(const qsrt_packed_matrix* m, const uint8_t* const* luts
 // rotation and is looked at by itself.
 bool launch_fits(int64_t rows, int64_t a, int64_t b) { return (rows + 15) / 16 * 16 * std::max(a, b) < int64_t(1) << 32; }
 
-const char* rows_fault(const void* p, int64_t ld, int64_t cols, int align) {
+const char* rows_fault(const void* p, int64_t rows, int64_t ld, int64_t cols, int align) {
     if (!p) return "null rows";
-    if (ld < cols || ld % (align / 2) || reinterpret_cast<uintptr_t>(p) % align) return "rows are not aligned";
+    if ((rows > 1 && (ld < cols || ld % (align / 2))) || reinterpret_cast<uintptr_t>(p) % align) return "rows are not aligned";
     return nullptr;
 }
 
@@ -1452,8 +1452,8 @@ int run_moe(const char* name, const MoeCall& c, RouterArgs* router, void* ws, si
     if (coupled && c.w1->rows % 512) return fail(kBadArgument, "%s: coupled weights need a multiple of 512 hidden channels", name);
     if (c.tokens == 0) return kOk;
     const int64_t hidden = c.w1->rows, inter = c.w1->cols, pairs = c.tokens * c.k;
-    if (const char* e = rows_fault(c.x, c.x_ld, hidden, 8)) return fail(kBadArgument, "%s: x: %s", name, e);
-    if (const char* e = rows_fault(c.out, c.out_ld, hidden, 8)) return fail(kBadArgument, "%s: out: %s", name, e);
+    if (const char* e = rows_fault(c.x, c.tokens, c.x_ld, hidden, 8)) return fail(kBadArgument, "%s: x: %s", name, e);
+    if (const char* e = rows_fault(c.out, c.tokens, c.out_ld, hidden, 8)) return fail(kBadArgument, "%s: out: %s", name, e);
     if (!c.ids || !c.weights) return fail(kBadArgument, "%s: null routing", name);
     if (router) {
         if (const char* e = router_fault(*router)) return fail(kBadArgument, "%s: %s", name, e);
@@ -1722,8 +1722,8 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
         return fail(kBadArgument, "qsrt_adapter_linear: adapters need 16-byte aligned a and b, scales and ids");
     if (rows == 0) return kOk;
     const int64_t k = w->rows, n = w->cols;
-    if (const char* e = rows_fault(x, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
-    if (const char* e = rows_fault(out, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
+    if (const char* e = rows_fault(x, rows, x_ld, k, 16)) return fail(kBadArgument, "qsrt_adapter_linear: x: %s", e);
+    if (const char* e = rows_fault(out, rows, out_ld, n, 8)) return fail(kBadArgument, "qsrt_adapter_linear: out: %s", e);
     int cus = 0;
     if (const int rc = current_cu_count(&cus)) return rc;
     const LinearSpace s = linear_space(ws, rows, k, n, w->rates, adapters, rank, cus);

@@ -411,7 +411,8 @@ const char* router_fault(const RouterArgs& a) {
     if (a.experts > kMaxExperts) return "the router takes at most 1024 experts";
     if (a.k < 1 || a.k > 64 || a.k > a.experts) return "k must be 1 .. min(64, experts)";
     if (a.scoring != 0 && a.scoring != 1) return "scoring must be 0 (softmax) or 1 (sigmoid)";
-    if (a.hidden % 8 || a.x_ld % 8 || a.weight_ld % 8 || a.x_ld < a.hidden || a.weight_ld < a.hidden ||
+    const auto bad = [&](int rows, int64_t ld) { return rows > 1 && (ld % 8 || ld < a.hidden); };
+    if (a.hidden % 8 || bad(a.tokens, a.x_ld) || bad(a.experts, a.weight_ld) ||
         reinterpret_cast<uintptr_t>(a.x) % 16 || reinterpret_cast<uintptr_t>(a.weight) % 16)
         return "the router's rows must be 16-byte aligned and a multiple of 8 channels";
     return nullptr;

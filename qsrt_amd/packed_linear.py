@@ -44,8 +44,9 @@ def _records(record_bits, lead: tuple, rate_axis: str, k: int, n: int, words: in
 def refuse_gradients(*tensors) -> None:
     """Packed products have no backward pass: better no result than one that a gradient silently stops at."""
 
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("packed products have no backward pass: call them under torch.no_grad() or detach their inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("packed products have no backward pass: call them under torch.no_grad() or detach their inputs")
 
 
 def _aligned(t: torch.Tensor, size: int) -> torch.Tensor:
@@ -78,6 +79,7 @@ class PackedMatrix:
         for s in (suh, svh):
             if s.dim() not in (1, len(lead) + 1) or (s.dim() == 2 and s.shape[0] != keys):
                 raise ValueError("scales must be one vector, or one for each key")
+        refuse_gradients(suh, svh)
         k, n = suh.shape[-1], svh.shape[-1]
         if k == 0 or n == 0 or k % 128 or n % 128:
             raise ValueError("packed products need K and N multiples of 128")
@@ -124,23 +126,17 @@ def checked_rows(x: torch.Tensor, cols: int, device) -> torch.Tensor:
         raise ValueError("x must be bfloat16 or float16")
     if x.device != device:
         raise ValueError("x must be on the payload's device")
-    ld = leading(x)
-    if x.stride(1) != 1 or ld % 8 or ld < cols or x.data_ptr() % 16:
+    # (a lone row's stride says nothing: a view keeps whatever its base had)
+    if x.stride(1) != 1 or x.data_ptr() % 16 or ((x.stride(0) % 8 or x.stride(0) < cols) and x.shape[0] > 1):
         x = x.clone(memory_format=torch.contiguous_format)
     return x
-
-
-def leading(rows: torch.Tensor) -> int:
-    """Elements from row to row.  The stride of a lone row says nothing: a view keeps whatever its base had."""
-
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
 def checked_out(out: torch.Tensor | None, x: torch.Tensor, cols: int) -> torch.Tensor:
     if out is None:
         return torch.empty((x.shape[0], cols), dtype=x.dtype, device=x.device)
     if (out.shape != (x.shape[0], cols) or out.dtype != x.dtype or out.device != x.device or out.stride(1) != 1
-            or leading(out) % 4 or leading(out) < cols or out.data_ptr() % 8):
+            or out.data_ptr() % 8 or ((out.stride(0) % 4 or out.stride(0) < cols) and out.shape[0] > 1)):
         raise ValueError("out must be a row-major [rows, N] tensor of x's type, its rows 8-byte aligned")
     return out
 
@@ -203,8 +199,8 @@ def _run(x, linear, bank, ids, out):
             lib.qsrt_adapter_linear(
                 m.ref, linear.luts.ref, None if bank is None else bank.a.data_ptr(),
                 None if bank is None else bank.b.data_ptr(), None if bank is None else bank.scale.data_ptr(), adapters, rank,
-                x.data_ptr(), leading(x), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
-                leading(out), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
+                x.data_ptr(), x.stride(0), TYPES[x.dtype], rows, None if bank is None else ids.data_ptr(), out.data_ptr(),
+                out.stride(0), ws.data_ptr(), ws.numel(), _native.stream_handle(m.device)),
             "qsrt_adapter_linear",
         )
     return out
@@ -213,7 +209,7 @@ def _run(x, linear, bank, ids, out):
 def packed_linear(x: torch.Tensor, linear: PackedLinear, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``x [T, K] @ W -> [T, N]`` in ``x``'s type (bf16 or f16), FP32 sums.  No backward pass."""
 
-    refuse_gradients(x, linear.matrix.suh, linear.matrix.svh)
+    refuse_gradients(x)
     return _run(x, linear, None, None, out)
 
 
@@ -223,7 +219,7 @@ def adapter_linear(x: torch.Tensor, linear: PackedLinear, adapters: LowRankAdapt
     none.  ``ids`` int32 ``[T]``, any order; one launch sequence serves all adapters.  No backward pass."""
 
     m = linear.matrix
-    refuse_gradients(x, adapters.a, adapters.b, adapters.scale, m.suh, m.svh)
+    refuse_gradients(x, adapters.a, adapters.b, adapters.scale)
     if adapters.a.shape[2] != m.k or adapters.b.shape[1] != m.n:
         raise ValueError("the adapters do not match the projection")
     if adapters.a.dtype != x.dtype or adapters.a.device != m.device:

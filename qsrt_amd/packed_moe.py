@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows, leading, refuse_gradients
+from .packed_linear import TYPES, LabelTables, PackedMatrix, checked_out, checked_rows, refuse_gradients
 from .qsrt_coupled import CoupledHadamardSpec, rotation_signs
 
 SCORING = {"softmax": 0, "sigmoid": 1}
@@ -32,7 +32,7 @@ def _checked_router(weight: torch.Tensor, k: int, bias, scoring: str) -> tuple:
         raise ValueError(f"scoring must be one of {tuple(SCORING)}")
     if bias is not None and (bias.shape != (e,) or bias.dtype != torch.float32 or bias.device != weight.device):
         raise ValueError("bias must be float32 [experts] on the router's device")
-    if weight.stride(1) != 1 or leading(weight) % 8 or leading(weight) < h or weight.data_ptr() % 16:
+    if weight.stride(1) != 1 or weight.data_ptr() % 16 or ((weight.stride(0) % 8 or weight.stride(0) < h) and e > 1):
         weight = weight.clone(memory_format=torch.contiguous_format)
     return weight, None if bias is None else bias.contiguous()
 
@@ -51,7 +51,7 @@ def _route(x, weight, k, bias, scoring, normalize, scale):
     with _native.current(x.device):
         ws = torch.empty(lib.qsrt_route_workspace_bytes(t, h, e), dtype=torch.uint8, device=x.device)
         _native.check(
-            lib.qsrt_route(x.data_ptr(), leading(x), weight.data_ptr(), leading(weight), TYPES[x.dtype], t, h, e,
+            lib.qsrt_route(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), TYPES[x.dtype], t, h, e,
                            k, None if bias is None else bias.data_ptr(), SCORING[scoring], int(normalize), float(scale),
                            weights.data_ptr(), ids.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(x.device)),
             "qsrt_route",
@@ -102,7 +102,6 @@ class PackedExperts:
             raise ValueError("w1, w3 [hidden, inter] and w2 [inter, hidden] do not match")
         if (self.w1.suh.dim() == 1) != (self.w3.suh.dim() == 1):
             raise ValueError("w1 and w3 must both share their suh, or neither")
-        self.scales = tuple(s for m in (self.w1, self.w3, self.w2) for s in (m.suh, m.svh))
         self.luts = LabelTables(luts_by_bits, self.w1.rates | self.w3.rates | self.w2.rates, self.device)
         self.activation = ACTIVATIONS[activation]
         self.signs, self.sign_pointers = (), (None, None)
@@ -142,7 +141,7 @@ class PackedExperts:
         ``[0, experts)`` (-1) contributes nothing.  ``x [T, hidden]`` bf16 or f16, ``weights`` float32 and ``ids`` int32
         ``[T, k]``.  No backward pass."""
 
-        refuse_gradients(x, weights, *self.scales)
+        refuse_gradients(x, weights)
         x = checked_rows(x, self.hidden, self.device)
         out = checked_out(out, x, self.hidden)
         if (ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape[1] < 1 or weights.shape != ids.shape
@@ -159,8 +158,8 @@ class PackedExperts:
                              dtype=torch.uint8, device=self.device)
             _native.check(
                 lib.qsrt_packed_moe(self.w1.ref, self.w3.ref, self.w2.ref, self.luts.ref, self.experts, self.activation,
-                                    *self.sign_pointers, x.data_ptr(), leading(x), TYPES[x.dtype], t, k, ids.data_ptr(),
-                                    weights.data_ptr(), out.data_ptr(), leading(out), ws.data_ptr(), ws.numel(),
+                                    *self.sign_pointers, x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k, ids.data_ptr(),
+                                    weights.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
                                     _native.stream_handle(self.device)),
                 "qsrt_packed_moe",
             )
@@ -180,7 +179,7 @@ class PackedMoELayer:
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None):
         e = self.experts
-        refuse_gradients(x, self.router, self.bias, *e.scales)
+        refuse_gradients(x, self.router, self.bias)
         if x.dtype != self.router.dtype:
             raise ValueError("x must be of the router's type")
         x = checked_rows(x, e.hidden, e.device)
@@ -198,9 +197,9 @@ class PackedMoELayer:
                 lib.qsrt_packed_moe_layer(
                     e.w1.ref, e.w3.ref, e.w2.ref, e.luts.ref, e.experts, e.activation, *e.sign_pointers,
                     self.router.data_ptr(),
-                    leading(self.router), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
-                    int(self.normalize), float(self.scale), x.data_ptr(), leading(x), TYPES[x.dtype], t, k,
-                    weights.data_ptr(), ids.data_ptr(), out.data_ptr(), leading(out), ws.data_ptr(), ws.numel(),
+                    self.router.stride(0), None if self.bias is None else self.bias.data_ptr(), SCORING[self.scoring],
+                    int(self.normalize), float(self.scale), x.data_ptr(), x.stride(0), TYPES[x.dtype], t, k,
+                    weights.data_ptr(), ids.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
                     _native.stream_handle(e.device)),
                 "qsrt_packed_moe_layer",
             )

@@ -58,6 +58,25 @@ def test_a_layer_counts_the_threads_of_router_and_rotation_together(experts, wor
         assert rc in (-2, -3), (rc, message)
 
 
+@needs_library
+@pytest.mark.parametrize("x_ld,out_ld", [(3, 128), (256, 1), (0, 0)])
+def test_leading_dimensions_of_a_lone_row(x_ld, out_ld):
+    """Taken as they are; of two rows they are refused."""
+
+    at, lib = 1 << 12, _native.lib()
+    tables = (ctypes.c_void_p * 3)(at, at, at)
+    w = struct(words=at, records=at, suh=at, svh=at)
+    down = struct(words=at, records=at, suh=at, svh=at, rows=128, cols=256)
+    for n, codes in ((1, (-2, -3)), (2, (-1,))):
+        assert lib.qsrt_adapter_linear(w, ctypes.addressof(tables), None, None, None, 0, 0, at, x_ld, 0, n, None, at, out_ld, None, 0,
+                                       None) in codes
+        assert lib.qsrt_packed_moe(w, w, down, ctypes.addressof(tables), 4, 0, None, None, at, x_ld, 0, n, 1, at, at, at, out_ld,
+                                   None, 0, None) in codes
+        if x_ld != 256:
+            assert lib.qsrt_route(at, x_ld, at, 256, 0, n, 256, 8, 1, None, 0, 1, 1.0, at, at, None, 0, None) in codes
+            assert lib.qsrt_route(at, 256, at, x_ld, 0, 3, 256, n, 1, None, 0, 1, 1.0, at, at, None, 0, None) in codes
+
+
 @pytest.mark.gpu
 def test_product_workspaces_of_any_sizes():
     up, down, lib = struct(), struct(rows=128, cols=256), _native.lib()
