@@ -80,6 +80,45 @@ def test_rows_of_any_size(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinities_leave_the_scales_of_other_rows_alone(dtype):
+    rng = np.random.default_rng(8)
+    p = paired(rng, 256, 128, (3, 3), 8.0)
+    linear = PackedLinear(*(torch.from_numpy(v).cuda() for v in p), (3, 3), LUTS)
+    x = opposite(rng, 200, 256, dtype)
+    want = x.double() @ dense(*p, (3, 3), "k")
+    bad = [3, 64, 127, 199]
+    for row, value in zip(bad, (float("inf"), float("nan"), -float("inf"), float("nan"))):
+        x[row, (50 * row) % 256] = value
+    got = packed_linear(x.cuda(), linear).cpu()
+    keep = [i for i in range(200) if i not in bad]
+    near(got[keep], want[keep], dtype)
+    assert not bool(torch.isfinite(got[bad]).any())
+
+
+def test_scaled_rows_in_a_graph():
+    """Captured once, replayed on rows of other sizes with eager work in between."""
+
+    rng = np.random.default_rng(9)
+    p = paired(rng, 256, 128, (3, 3), 8.0)
+    linear = PackedLinear(*(torch.from_numpy(v).cuda() for v in p), (3, 3), LUTS)
+    bank = LowRankAdapters(rows(rng, 2 * 16, 256, torch.bfloat16).view(2, 16, 256).cuda(),
+                           rows(rng, 2 * 128, 16, torch.bfloat16).view(2, 128, 16).cuda())
+    x, ids = rows(rng, 150, 256, torch.bfloat16).cuda(), ((torch.arange(150) // 40) % 3 - 1).int().cuda()
+    adapter_linear(x, linear, bank, ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = adapter_linear(x, linear, bank, ids)
+    for size in (1.0, 2.0**20, 2.0**-30, 1.0):
+        x.copy_(rows(rng, 150, 256, torch.bfloat16) * size)
+        want = adapter_linear(x, linear, bank, ids)
+        packed_linear(x[:7].contiguous(), linear)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("t,run", [(2, 1), (40, 40), (200, 60)])
 def test_second_product_of_an_adapter(t, run, dtype):
     """First products that cancel in the second, where the projection itself is nothing."""
