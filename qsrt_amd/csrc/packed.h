@@ -206,7 +206,8 @@ __device__ __forceinline__ void rotate_block(const RotateArgs& p, int64_t wave, 
 }
 
 // The same by a workgroup of four waves for rows laid out by 16, two blocks of channels at once: 16 rows by 256 channels,
-// which leave in one stretch (2048 x 5120 in two pieces: 20.1 us; four blocks 23.8, one 20.9).
+// which leave in one stretch (2048 x 5120 in two pieces: 17.0 us; four blocks 24.4, one 16.4, which makes more of the stores
+// short where rows are few).
 constexpr int kRotateBlocks = 2;
 inline int64_t rotate_quads(const RotateArgs& p) { return (p.rows + 15) / 16 * p.nmat * ((p.kb + kRotateBlocks - 1) / kRotateBlocks); }
 template <typename T, int kPieces>

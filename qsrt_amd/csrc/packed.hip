@@ -358,7 +358,7 @@ __device__ __forceinline__ void lds_barrier() {
 // the product of a few rows, fall to an eighth a row and are spread over the strip's products (all at its start, with two
 // buffers of operands: 1.39 us a strip of 4 groups and 0.86 of 2, so 1.19 and 0.72).  The matrix cores take 0.95 and 0.48 of
 // that at two pieces a row and the 2.2 GHz that they leave; before and after it a workgroup waits 8 us for tables and first
-// rows and 6 to 12 for its sums' stores (2048 x 5120 x 1536: 69 us, 930 TFLOP/s of pieces).
+// rows and 6 to 12 for its sums' stores (2048 x 5120 x 1536: 70 us, 925 TFLOP/s of pieces).
 template <int G>
 __device__ __forceinline__ void multiply_rows(const char* tiles, int tile_row_bytes, int strips, int K, const char* (&x)[G],
                                               const uint8_t* lut, u32x2 (&frags)[3][8][128], int lane, int w, bool& ready,
@@ -1089,7 +1089,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs p) {
     typedef T t8 __attribute__((ext_vector_type(8)));
     if (with && !(others & ~same1)) {
         // Rows of one or two adapters, as in prompts: every wave reads 32 columns of them once for all rows (2048 rows of rank
-        // 64 in runs: 21 us, 35 on the vector units as below).
+        // 64 in runs: 22 us, 35 on the vector units as below).
         f32x4 sum[2] = {};
         for (int turn = 0; turn < (others ? 2 : 1); ++turn) {
             const uint32_t same = static_cast<uint32_t>(turn ? same1 : same0);
@@ -1169,7 +1169,8 @@ constexpr int64_t kMaxPartBytes = int64_t(128) << 20;  // part sums of one produ
 
 template <int G, bool kHalf, int kTables>
 int launch_product_g(const ProductArgs& args, int cus, hipStream_t stream) {
-    constexpr int kWaves = G == 1 ? 16 : G == 2 ? 12 : 8;  // 128, 168 and 256 registers a lane
+    // 128, 168 and 256 registers a lane; four groups keep up to five more in memory, read and written once a piece of work
+    constexpr int kWaves = G == 1 ? 16 : G == 2 ? 12 : 8;
     const int64_t items = static_cast<int64_t>(args.max_chunks) * args.nmat * args.nb * args.parts;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cus, items)));
     hipLaunchKernelGGL((product_kernel<G, kHalf, kWaves, kTables>), grid, dim3(64 * kWaves), 0, stream, args);
@@ -1251,8 +1252,8 @@ int passes_of(int rates) { return __builtin_popcount(rates & 0x1C) > 2 ? 2 : 1; 
 // The same for product_rows_kernel, with the groups of 16 rows that each of a workgroup's eight waves takes.  A workgroup is an
 // item; with 4 groups a strip takes it about 1.2 us, a part's sums (256 KB) as long as 16 strips, there and back, and its
 // set-up 3 or more.  With 2 all of it takes 0.6 of that: half the rows, at the same reads of the payload and the tables.  So few
-// rows or items go with 2 (7168 x 7168, 256 rows: 92 us, with 4 124; 5120 x 2048, 512 rows: 60 and 66), many with 4
-// (7168 x 7168, 4096 rows: 897 us, with 2 1022).
+// rows or items go with 2 (a call of 7168 x 7168, 256 rows: 80 us, with 4 114; 5120 x 2048, 512 rows: 55 and 63), many
+// with 4 (7168 x 7168, 4096 rows: 837 us, with 2 907).
 struct RowCut {
     int groups, parts;
 };
@@ -1343,8 +1344,8 @@ MoeSpace moe_space(void* ws, int64_t tokens, int k, int64_t hidden, int64_t inte
     const int64_t pairs = tokens * k;
     // An expert's rows are one chunk more often than not: 2% of experts get over 8 of 4 a head.  Larger chunks cost more a
     // strip, more chunks decode again (16 experts, 4096 x 1536 at K3, us a layer with chunks of 8, 16, 32, 64: 4 rows a head
-    // 91, 91, 94, 105; 8 rows 126, 95, 100, 112; 16 rows 182, 148, 107, 121; 24 rows 252, 164, 132, 155; 32 rows 319, 200,
-    // 177, 162).
+    // 90, 90, 94, 118; 8 rows 128, 97, 104, 132; 16 rows 184, 150, 114, 140; 24 rows 247, 165, 133, 170; 32 rows 322, 204,
+    // 211, 185).
     s.groups = pairs <= 4 * experts ? 0 : pairs <= 8 * experts ? 1 : pairs <= 24 * experts ? 2 : 4;
     const int chunk_rows = chunk_rows_of(s.groups);
     s.max_chunks = static_cast<int>(most_chunks(pairs, experts, chunk_rows));
@@ -1646,12 +1647,13 @@ LinearSpace linear_space(void* ws, int64_t rows, int64_t k, int64_t n, int rates
     LinearSpace s{};
     Carve c{static_cast<char*>(ws)};
     // Chunks of 8, 16, 32 and 64 rows, each up to two of them: more rows a wave share a decode, fewer leave more waves to
-    // share the matrix (7168 x 7168 at K3: 12 rows 36 us in one chunk of 16, 45 in two of 8; 64 rows 51 in two of 32, 54 in
-    // one of 64; 96 rows 60 in two of 64, 64 in three of 32).  Beyond 128 a workgroup shares each decode (192 rows: 85 us,
-    // 111 without; 128 rows: 82, without 64).
+    // share the matrix (7168 x 7168 at K3: 12 rows 31 us in one chunk of 16, 39 in two of 8; 64 rows 50 in two of 32, 57 in
+    // one of 64; 128 rows 66 in two of 64, 74 in four of 32; 96 rows 63 either way).  Beyond 128 a workgroup shares each
+    // decode (192 rows: 78 us, 123 without; 128 rows: 74, without 66).
     s.groups = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 64 ? 2 : 4;
-    // Rows by 16 are rotated by a quarter of the waves, which costs 2 to 3 us until the reads of the product outweigh it
-    // (7168 x 7168: 24 rows 42.7 us as rows, 45 by 16; 48 rows the same; 64 rows 58 and 56).
+    // Rows by 16 are rotated by a quarter of the waves, which costs a microsecond or two until the reads of the product
+    // outweigh it (7168 x 7168: 24 rows 42.3 us as rows, 43.5 by 16; 32 rows 43.6 and 43.9; 48 rows 48.3 and 46.4; 64 rows
+    // 50.2 and 49.7).
     s.grouped = rows > 48;
     s.passes = passes_of(rates);
     const int64_t nb = n / 128;
@@ -1759,8 +1761,8 @@ extern "C" int qsrt_adapter_linear(const qsrt_packed_matrix* w, const uint8_t* c
     int64_t shrinks = 0;
     if (adapters) {
         const auto blocks = [&](int q) { return (rows + 16 * q - 1) / (16 * q) * s.low_parts * (rank / (16 * tiles)); };
-        // Beyond four workgroups a unit 32 rows share the reads of A (2048 rows, K 5120, rank 64: 32 us for this kernel, 37
-        // with 16; 512 rows: 57 us for all with 32, 54 with 16); below, the adapters of a workgroup's rows are shared out.
+        // Beyond four workgroups a unit 32 rows share the reads of A (5120 x 1536, rank 64: 2048 rows 116 us with 32, 120 with
+        // 16; 1024 rows 76 and 74; 512 rows 58 and 55); below, the adapters of a workgroup's rows are shared out.
         if (tiles == 2 && blocks(1) > 4 * cus) sets = 2;
         shrinks = blocks(sets);
         sa.shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, rows), 4 * cus / shrinks)));

@@ -4,6 +4,9 @@
 (``qsrt_route``, ``qsrt_packed_moe`` and ``qsrt_packed_moe_layer`` in ``include/qsrt_amd.h``).  Nothing waits for the
 device: which experts are chosen is known there alone.  Workspaces come from torch's allocator on the current stream, so a
 call can be captured in a graph (after one outside it, which loads the kernels).
+
+Longer batches are taken too, but an expert's rows share a decode of its weights 64 at a time at the most: from about a
+thousand rows an expert on, decoding its matrices once (``decode``) and a library product are faster.
 """
 
 from __future__ import annotations
