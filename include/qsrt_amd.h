@@ -531,6 +531,65 @@ int qsrt_packed_moe_plan(const qsrt_packed_matrix *w1, const qsrt_packed_matrix 
                          int64_t experts, int64_t tokens, int k, int64_t *plan);
 int qsrt_adapter_linear_plan(const qsrt_packed_matrix *w, int64_t rows, int64_t adapters, int64_t rank, int64_t *plan);
 
+/*
+ * A gated feed-forward block in dense weights, bf16 (dtype 0) or f16 (1):
+ *   G = x gate^T, U = x up^T, M = act(G, U), out = M down^T
+ * x and out [tokens, hidden], gate and up [inter, hidden] (both up_ld apart),
+ * down [hidden, inter]; act as in qsrt_packed_moe.  Sums are FP32; M goes into
+ * its product in 16 bits, for a few rows as two such pieces.  hidden and inter
+ * multiples of 8 up to 2^17, at most 2^20 tokens, rows 16-byte aligned and at
+ * most 2^22 elements apart.  pre: f32 [2][tokens][inter], G and U for the
+ * backward pass, or NULL; with it out may be NULL and the call ends there.
+ */
+size_t qsrt_gated_ffn_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inter);
+int qsrt_gated_ffn(const void *x, int64_t x_ld, const void *gate, const void *up, int64_t up_ld, const void *down,
+                   int64_t down_ld, int dtype, int64_t tokens, int64_t hidden, int64_t inter, int activation, float *pre,
+                   void *out, int64_t out_ld, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * Its gradients, in x's type, from dy [tokens, hidden] and the same call's pre:
+ *   dM = dy down, dG = dM * dact/dG, dU = dM * dact/dU
+ *   dx = dG gate + dU up, d_gate = dG^T x, d_up = dU^T x, d_down = dy^T M
+ * Any of them may be NULL; d_gate, d_up, d_down are contiguous.  gate_rows,
+ * up_rows and middle (contiguous [tokens, inter], or NULL) receive dG, dU, M.
+ */
+size_t qsrt_gated_ffn_backward_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inter);
+int qsrt_gated_ffn_backward(const void *dy, int64_t dy_ld, const void *x, int64_t x_ld, const void *gate, const void *up,
+                            int64_t up_ld, const void *down, int64_t down_ld, int dtype, int64_t tokens, int64_t hidden,
+                            int64_t inter, int activation, const float *pre, void *dx, int64_t dx_ld, void *d_gate,
+                            void *d_up, void *d_down, void *gate_rows, void *up_rows, void *middle, void *ws,
+                            size_t ws_bytes, void *stream);
+
+/*
+ * What stands between two blocks, a row of [rows, hidden] at a time:
+ *   z = post y / sqrt(mean y^2 + eps)   (post NULL: z = y)
+ *   sum = scale residual + gate z       (y NULL: scale residual)
+ *   normed = weight sum / sqrt(mean sum^2 + eps)
+ * y and normed bf16 (dtype 0) or f16 (1), residual and sum f32 or y's type,
+ * weight and post [hidden] and gate ([hidden]: gate_kind 1, [rows]: 2, none:
+ * 0) all f32 or all of y's type.  normed comes from the unrounded sum.  sum
+ * may be NULL.  stats: f32 [2][rows] for the backward pass, or NULL.  hidden a
+ * multiple of 8 up to 2^14, rows and vectors 16-byte aligned.
+ */
+int qsrt_residual_norm(const void *residual, int64_t residual_ld, int residual_f32, const void *y, int64_t y_ld, int dtype,
+                       int64_t rows, int64_t hidden, const void *weight, const void *post, const void *gate, int gate_kind,
+                       int params_f32, float scale, float eps, void *sum, int64_t sum_ld, void *normed, int64_t normed_ld,
+                       float *stats, void *stream);
+
+/*
+ * Its gradients from those of sum (residual's type) and normed (y's; either
+ * may be NULL) and the same call's stats: dresidual and dy in the types of
+ * residual and y, dweight, dpost and dgate in the parameters', any of them
+ * NULL.  Sums over rows are FP32, in a fixed order.
+ */
+size_t qsrt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t hidden);
+int qsrt_residual_norm_backward(const void *dsum, int64_t dsum_ld, const void *dn, int64_t dn_ld, const void *residual,
+                                int64_t residual_ld, int residual_f32, const void *y, int64_t y_ld, int dtype,
+                                int64_t rows, int64_t hidden, const void *weight, const void *post, const void *gate,
+                                int gate_kind, int params_f32, float scale, const float *stats, void *dresidual,
+                                int64_t dresidual_ld, void *dy, int64_t dy_ld, void *dweight, void *dpost, void *dgate,
+                                void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -140,6 +140,31 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64,
          _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
     ),
+    "qsrt_gated_ffn_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "qsrt_gated_ffn": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p,
+         _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p],
+    ),
+    "qsrt_gated_ffn_backward_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "qsrt_gated_ffn_backward": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_i64,
+         _c_int, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_size, _c_void_p],
+    ),
+    "qsrt_residual_norm": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+         ctypes.c_float, ctypes.c_float, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p],
+    ),
+    "qsrt_residual_norm_backward_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "qsrt_residual_norm_backward": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_void_p,
+         _c_void_p, _c_void_p, _c_int, _c_int, ctypes.c_float, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p],
+    ),
 }
 
 

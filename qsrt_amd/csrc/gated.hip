@@ -1,0 +1,685 @@
+// A gated feed-forward block in dense 16-bit weights, forward and backward, on the matrix cores (gfx950, wave64).
+//
+//   G = x W1^T, U = x W3^T, M = act(G, U), y = M W2^T            x [T, H], W1, W3 [I, H], W2 [H, I]
+//   dM = dy W2, dG = dM act_g(G, U), dU = dM act_u(G, U)
+//   dx = dG W1 + dU W3, dW1 = dG^T x, dW3 = dU^T x, dW2 = dy^T M
+//
+// Every product is a `tile_kernel`: sums of products of two operands that each lie with the summed index innermost
+// (kRows) or outermost (kCols), so no operand is ever transposed in memory.
+#include <algorithm>
+
+#include "common.h"
+#include "qsrt_amd.h"
+
+namespace qsrt {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec4 = T __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ f32x4 multiply(vec8<T> a, vec8<T> b, f32x4 c) {
+    if constexpr (__is_same(T, __bf16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- what becomes of a product
+// The activation in FP32: silu(g) u or 4 tanh(g/4) sigmoid(g) 25 tanh(u/25), and its derivatives.
+__device__ __forceinline__ float activate(float g, float u, int activation) {
+    const float s = 1.0f / (1.0f + expf(-g));
+    return activation == 0 ? g * s * u : 4.0f * tanhf(0.25f * g) * s * (25.0f * tanhf(0.04f * u));
+}
+__device__ __forceinline__ void activate_with_slopes(float g, float u, int activation, float& m, float& by_g, float& by_u) {
+    const float s = 1.0f / (1.0f + expf(-g));
+    if (activation == 0) {
+        by_u = g * s;
+        m = by_u * u;
+        by_g = u * (s * (1.0f + g * (1.0f - s)));
+    } else {
+        const float a = tanhf(0.25f * g), b = tanhf(0.04f * u), f = 4.0f * a * s;
+        m = f * (25.0f * b);
+        by_g = 25.0f * b * ((1.0f - a * a) * s + f * (1.0f - s));
+        by_u = f * (1.0f - b * b);
+    }
+}
+
+enum Ending { kStore, kActivate, kSlopes };
+
+// A row between two products goes on in 16 bits, as the matrix cores take it: rounded once, or as two pieces (the nearest
+// 16-bit value and the nearest of what is left).
+struct Pieces {
+    void *hi, *lo;  // lo null: one
+};
+
+struct Finish {
+    // kStore: the sums, rounded once
+    void* out;
+    int64_t ld;
+    // the others: rows [rows, inter]
+    int activation;
+    float *pre_g, *pre_u;     // kActivate: G and U out, or null; kSlopes: in
+    Pieces middle, dg, du;    // kActivate: middle; kSlopes: all
+};
+
+template <typename T>
+__device__ __forceinline__ void store_pieces(const Pieces& to, int64_t at, const f32x4& v) {
+    const vec4<T> hi = __builtin_convertvector(v, vec4<T>);
+    *reinterpret_cast<vec4<T>*>(static_cast<T*>(to.hi) + at) = hi;
+    if (to.lo) {
+        f32x4 left = v - __builtin_convertvector(hi, f32x4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) left[r] = __builtin_isfinite(static_cast<float>(hi[r])) ? left[r] : 0.f;
+        *reinterpret_cast<vec4<T>*>(static_cast<T*>(to.lo) + at) = __builtin_convertvector(left, vec4<T>);
+    }
+}
+
+// Four neighbouring columns of one row: v the sums, u the second matrix's.
+template <typename T, Ending kEnding>
+__device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col, const f32x4& v, const f32x4& u) {
+    const int64_t at = row * f.ld + col;
+    if constexpr (kEnding == kStore) {
+        *reinterpret_cast<vec4<T>*>(static_cast<T*>(f.out) + at) = __builtin_convertvector(v, vec4<T>);
+    } else if constexpr (kEnding == kActivate) {
+        if (f.pre_g) {
+            *reinterpret_cast<f32x4*>(f.pre_g + at) = v;
+            *reinterpret_cast<f32x4*>(f.pre_u + at) = u;
+        }
+        f32x4 m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m[r] = activate(v[r], u[r], f.activation);
+        store_pieces<T>(f.middle, at, m);
+    } else {
+        const f32x4 g = *reinterpret_cast<const f32x4*>(f.pre_g + at), up = *reinterpret_cast<const f32x4*>(f.pre_u + at);
+        f32x4 m, dg, du;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float by_g, by_u, mid;
+            activate_with_slopes(g[r], up[r], f.activation, mid, by_g, by_u);
+            m[r] = mid;
+            dg[r] = v[r] * by_g;
+            du[r] = v[r] * by_u;
+        }
+        store_pieces<T>(f.middle, at, m);
+        store_pieces<T>(f.dg, at, dg);
+        store_pieces<T>(f.du, at, du);
+    }
+}
+
+// ---------------------------------------------------------------- the product
+enum Layout { kRows, kCols };
+
+constexpr int kDepth = 64;  // of the summed index in a stage
+constexpr int kSums = 4;    // products that one result adds up, at the most
+
+struct Product {
+    const void* a[kSums];
+    const void* b[kSums];
+    const void* b2;  // of two matrices side by side (kActivate)
+    int64_t lda, ldb;
+    int64_t m, n, k;
+    int sums;
+    int tiles_m, tiles_n;
+    Finish finish;
+};
+
+constexpr int kProducts = 3;
+struct TileArgs {
+    Product product[kProducts];
+    int products;
+    int parts;       // of the summed axis; > 1: sums go to `partial` [part][1 or 2][m][n]
+    float* partial;
+};
+
+// 16 bytes a lane from a buffer straight to LDS: lane l's go to `lds` + 16 l.  Written in assembly because the compiler,
+// which cannot see that a stage is written while another is read, waits for all of them before any read from LDS.  Nothing
+// comes back in registers; `wait_and_meet` is the wait.
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(lds)
+                 : "memory");
+}
+
+// All but the wave's last `kLeft` loads have landed, its reads from LDS are done, and so are the other waves'.
+template <int kLeft>
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
+constexpr uint32_t kNowhere = 0x80000000u;  // past the end of every buffer here: reads zero
+
+// A stage of one operand in LDS: kSize indices by 64 of the summed index, in 16-byte chunks of 8.
+//   kRows: an index's 8 chunks in a row of 128 bytes, chunk c at place c ^ (index & 7)
+//   kCols: a summed index's kSize / 8 chunks in a row, chunk c at place c ^ 2 f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2
+// so that a quarter of the wave's 16-byte reads, or half of its transposing 8-byte reads, hit distinct banks.  Loads to LDS
+// write 16 bytes a lane in lane order, so it is the address read that is permuted.
+template <Layout kLayout, int kSize, int kWaves>
+struct Loader {
+    static constexpr int kBytes = kSize * kDepth * 2;
+    static constexpr int kLoads = kBytes / 1024 / kWaves;  // a wave's
+    static constexpr int kRowBytes = kLayout == kRows ? 128 : 2 * kSize;
+    static constexpr int kChunks = kRowBytes / 16;
+    static_assert(kBytes % (1024 * kWaves) == 0 && kLoads >= 1, "a wave's loads are whole");
+    uint32_t offset[kLoads];
+    int chunk;  // kRows: of the summed index
+
+    __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+            const int row = (q * kWaves + wave) * (1024 / kRowBytes) + lane / kChunks, place = lane % kChunks;
+            int c;
+            if constexpr (kLayout == kRows) {
+                c = place ^ (row & 7);
+                chunk = c;  // 8 rows a load: the same in all
+            } else {
+                c = place ^ (((row & 3) | (row >> 3 & 1) << 2) << 1);
+            }
+            offset[q] = (static_cast<uint32_t>(row) * static_cast<uint32_t>(ld) + 8 * c) * 2;
+        }
+    }
+
+    // `p`: the operand's first element of this tile and stage; `size` and `depth`: how much of both there is
+    __device__ __forceinline__ void load(const uint16_t* p, int64_t ld, int64_t size, int64_t depth, uint32_t lds, int wave) const {
+        const int rows = static_cast<int>(kLayout == kRows ? min(size, int64_t{kSize}) : min(depth, int64_t{kDepth}));
+        const int span = static_cast<int>(kLayout == kRows ? min(depth, int64_t{kDepth}) : min(size, int64_t{kSize}));
+        const uint32_t bytes = rows > 0 ? (static_cast<uint32_t>(rows - 1) * static_cast<uint32_t>(ld) + span) * 2 : 0;
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, bytes, 0x00020000);
+        const bool past = kLayout == kRows && 8 * chunk >= span;
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q)
+            to_lds(from, past ? kNowhere : offset[q], lds + (q * kWaves + wave) * 1024);
+    }
+};
+
+// The lane's part of a 16 x 32 fragment: index lane % 16, eight summed indices from 8 (lane / 16).
+template <Layout kLayout, int kSize, typename T>
+struct Reader {
+    uint32_t base[kLayout == kRows ? 2 : 1];
+    int f;
+    __device__ __forceinline__ void init(int lane) {
+        if constexpr (kLayout == kRows) {
+            base[0] = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+            base[1] = base[0] ^ 64;
+        } else {
+            const int a = lane & 15;
+            base[0] = (8 * (lane >> 4) + (a >> 2)) * (2 * kSize) + (a & 3) * 8;
+            f = (a >> 2) | (lane >> 4 & 1) << 2;
+        }
+    }
+    // `first`: a multiple of 16; `kk`: which 32 of the stage's 64
+    __device__ __forceinline__ vec8<T> read(const char* lds, int first, int kk) const {
+        if constexpr (kLayout == kRows) {
+            return *reinterpret_cast<const vec8<T>*>(lds + first * 128 + base[kk]);
+        } else {
+            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+            const char* at = lds + kk * 32 * (2 * kSize) + (((first >> 4) ^ f) << 5) + base[0];
+            const i16x4 half[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at),
+                                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 4 * 2 * kSize))};
+            vec8<T> v;
+            __builtin_memcpy(&v, half, sizeof(v));
+            return v;
+        }
+    }
+};
+
+// Workgroup q of n runs on XCD q % 8: every XCD takes a run of the tile order.
+__device__ __forceinline__ int xcd_slot(int q, int n) {
+    const int x = q % 8, per = n / 8, rem = n % 8;
+    return x * per + (x < rem ? x : rem) + q / 8;
+}
+
+// One tile of kM rows (of a) by kN columns (of b; with kActivate half of them of b, half of b2) a workgroup of kWavesM x
+// kWavesN waves, kStages stages in LDS.  The first operand of the matrix instruction is b: a lane then holds four
+// neighbouring columns of one row.
+template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
+__global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const TileArgs args) {
+    constexpr int kWaves = kWavesM * kWavesN;
+    constexpr bool kDual = kEnding == kActivate;
+    constexpr int kNb = kDual ? kN / 2 : kN;  // of one matrix of b
+    constexpr int kWm = kM / kWavesM, kWn = kN / kWavesN, kI = kWm / 16, kJ = kWn / 16, kHalf = kDual ? kJ / 2 : kJ;
+    typedef Loader<kA, kM, kWaves> LoaderA;
+    typedef Loader<kB, kNb, kWaves> LoaderB;
+    constexpr int kStageBytes = LoaderA::kBytes + (kDual ? 2 : 1) * LoaderB::kBytes;
+    constexpr int kStageLoads = LoaderA::kLoads + (kDual ? 2 : 1) * LoaderB::kLoads;
+    extern __shared__ char lds[];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    int tile = xcd_slot(blockIdx.x, gridDim.x), which = 0, part = 0;
+    for (; which + 1 < args.products; ++which) {
+        const int tiles = args.product[which].tiles_m * args.product[which].tiles_n;
+        if (tile < tiles) break;
+        tile -= tiles;
+    }
+    const Product& p = args.product[which];
+    if (args.parts > 1) {
+        const int tiles = p.tiles_m * p.tiles_n;
+        part = tile / tiles;
+        tile %= tiles;
+    }
+    // tiles in bands of four of m: the workgroups at work on an XCD at a time share operands in its L2
+    constexpr int kBand = 4;
+    const int band = tile / (kBand * p.tiles_n), in_band = tile % (kBand * p.tiles_n);
+    const int high = min(kBand, p.tiles_m - band * kBand);
+    const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * kM, n0 = static_cast<int64_t>(in_band / high) * kNb;
+
+    const int per = static_cast<int>((p.k + kDepth - 1) / kDepth), stages = per * p.sums;
+    const int begin = static_cast<int>(static_cast<int64_t>(stages) * part / args.parts);
+    const int end = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / args.parts);
+
+    LoaderA la;
+    LoaderB lb;
+    la.init(p.lda, wave, lane);
+    lb.init(p.ldb, wave, lane);
+    Reader<kA, kM, T> ra;
+    Reader<kB, kNb, T> rb;
+    ra.init(lane);
+    rb.init(lane);
+
+    const auto load = [&](int s) {
+        const int sum = s / per;
+        const int64_t k0 = static_cast<int64_t>(s - sum * per) * kDepth, depth = p.k - k0;
+        const uint32_t to = static_cast<uint32_t>(s % kStages) * kStageBytes;
+        const uint16_t* a = static_cast<const uint16_t*>(p.a[sum]) + (kA == kRows ? m0 * p.lda + k0 : k0 * p.lda + m0);
+        const int64_t at = kB == kRows ? n0 * p.ldb + k0 : k0 * p.ldb + n0;
+        la.load(a, p.lda, p.m - m0, depth, to, wave);
+        lb.load(static_cast<const uint16_t*>(p.b[sum]) + at, p.ldb, p.n - n0, depth, to + LoaderA::kBytes, wave);
+        if constexpr (kDual)
+            lb.load(static_cast<const uint16_t*>(p.b2) + at, p.ldb, p.n - n0, depth, to + LoaderA::kBytes + LoaderB::kBytes, wave);
+    };
+
+    const int wm = wave / kWavesN * kWm, wn = wave % kWavesN * (kDual ? kWn / 2 : kWn);
+    f32x4 acc[kI][kJ];
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+        if (begin + s < end) load(begin + s);
+    for (int s = begin; s < end; ++s) {
+        // of what is on its way, the stages behind s may stay so
+        if (kStages > 2 && s + kStages - 2 < end)
+            wait_and_meet<kStageLoads*(kStages - 2)>();
+        else
+            wait_and_meet<0>();
+        if (s + kStages - 1 < end) load(s + kStages - 1);
+        const char* at = lds + static_cast<uint32_t>(s % kStages) * kStageBytes;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            vec8<T> b[kJ];
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+                b[j] = rb.read(at + LoaderA::kBytes + (j < kHalf ? 0 : LoaderB::kBytes), wn + 16 * (j % kHalf), kk);
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                const vec8<T> a = ra.read(at, wm + 16 * i, kk);
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[j], a, acc[i][j]);
+            }
+        }
+    }
+
+    const int64_t row0 = m0 + wm + (lane & 15), col0 = n0 + wn + 4 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+        const int64_t row = row0 + 16 * i;
+        if (row >= p.m) continue;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) {
+            const int64_t col = col0 + 16 * j;
+            if (col >= p.n) continue;  // n is a multiple of 8
+            if (args.parts > 1) {
+                float* to = args.partial + (part * (kDual ? 2 : 1) * p.m + row) * p.n + col;
+                *reinterpret_cast<f32x4*>(to) = acc[i][j];
+                if constexpr (kDual) *reinterpret_cast<f32x4*>(to + p.m * p.n) = acc[i][kHalf + j];
+            } else {
+                finish<T, kEnding>(p.finish, row, col, acc[i][j], acc[i][kDual ? kHalf + j : j]);
+            }
+        }
+    }
+}
+
+// Adds the parts up, in their order, four columns a thread.
+template <typename T, Ending kEnding>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int parts, int64_t m, int64_t n, const Finish f) {
+    constexpr int kPlanes = kEnding == kActivate ? 2 : 1;
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (at >= m * n) return;
+    f32x4 sum[2] = {};
+    for (int q = 0; q < parts; ++q)
+#pragma unroll
+        for (int h = 0; h < kPlanes; ++h) sum[h] += *reinterpret_cast<const f32x4*>(partial + (q * kPlanes + h) * m * n + at);
+    finish<T, kEnding>(f, at / n, at % n, sum[0], sum[1]);
+}
+
+// ---------------------------------------------------------------- host
+struct Shape {
+    int m, n, threads, stages, resident;  // of a tile; workgroups that a CU holds
+};
+constexpr Shape kShapes[] = {{256, 256, 512, 2, 1}, {128, 128, 256, 2, 2}, {32, 128, 256, 4, 2}};
+
+struct Cut {
+    int shape, parts;
+};
+
+int64_t tiles_of(const Shape& s, int64_t m, int64_t n, bool dual) {
+    const int64_t nb = dual ? s.n / 2 : s.n;
+    return (m + s.m - 1) / s.m * ((n + nb - 1) / nb);
+}
+
+Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, bool whole) {
+    int cus = 0;
+    if (current_cu_count(&cus) != kOk) cus = 256;
+    int shape = m <= 32 && !whole ? 2 : 1;
+    if (m > 32 && tiles_of(kShapes[0], m, n, dual) * 2 >= cus) shape = 0;
+    const int64_t tiles = tiles_of(kShapes[shape], m, n, dual), slots = static_cast<int64_t>(cus) * kShapes[shape].resident;
+    const int64_t stages = (k + kDepth - 1) / kDepth * sums;
+    int64_t parts = whole ? 1 : std::min(slots / tiles, stages / 4);
+    return {shape, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(parts, 32)))};
+}
+
+template <typename T, Layout kA, Layout kB, Ending kEnding>
+int launch_shape(const TileArgs& args, int shape, int64_t blocks, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(blocks));
+#define QSRT_TILE(M, N, WM, WN, STAGES)                                                                               \
+    {                                                                                                                 \
+        auto* kernel = tile_kernel<T, kA, kB, kEnding, M, N, WM, WN, STAGES>;                                         \
+        constexpr int bytes = STAGES * (M + N) * kDepth * 2;                                                          \
+        static bool raised[64] = {};                                                                                  \
+        int dev = 0;                                                                                                  \
+        QSRT_HIP_TRY(hipGetDevice(&dev));                                                                             \
+        if (dev >= 64 || !raised[dev]) {                                                                              \
+            QSRT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),                                   \
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes));                     \
+            if (dev < 64) raised[dev] = true;                                                                         \
+        }                                                                                                             \
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * WM * WN), bytes, stream, args);                                    \
+    }
+    if (shape == 0)
+        QSRT_TILE(256, 256, 2, 4, 2)
+    else if (shape == 1)
+        QSRT_TILE(128, 128, 2, 2, 2)
+    else
+        QSRT_TILE(32, 128, 1, 4, 4)
+#undef QSRT_TILE
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
+template <typename T, Layout kA, Layout kB, Ending kEnding>
+int run(TileArgs& args, Cut c, hipStream_t stream) {
+    const Shape& s = kShapes[c.shape];
+    int64_t blocks = 0;
+    for (int i = 0; i < args.products; ++i) {
+        Product& p = args.product[i];
+        const int nb = kEnding == kActivate ? s.n / 2 : s.n;
+        p.tiles_m = static_cast<int>((p.m + s.m - 1) / s.m);
+        p.tiles_n = static_cast<int>((p.n + nb - 1) / nb);
+        blocks += static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+    }
+    args.parts = c.parts;
+    blocks *= c.parts;
+    if (blocks > 1 << 30) return fail(kBadArgument, "too many tiles for one launch");
+    if (int rc = launch_shape<T, kA, kB, kEnding>(args, c.shape, blocks, stream)) return rc;
+    if (c.parts > 1) {
+        const Product& p = args.product[0];
+        hipLaunchKernelGGL((join_kernel<T, kEnding>), dim3(static_cast<unsigned>((p.m * p.n / 4 + 255) / 256)), dim3(256), 0,
+                           stream, args.partial, c.parts, p.m, p.n, p.finish);
+        QSRT_HIP_TRY(hipGetLastError());
+    }
+    return kOk;
+}
+
+constexpr int64_t kMaxTokens = 1 << 20, kMaxChannels = 1 << 17, kMaxLd = 1 << 22;
+
+bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
+    return tokens >= 0 && tokens <= kMaxTokens && hidden > 0 && hidden <= kMaxChannels && inter > 0 && inter <= kMaxChannels &&
+           hidden % 8 == 0 && inter % 8 == 0;
+}
+
+int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
+
+size_t round_up(size_t n) { return (n + 255) & ~size_t{255}; }
+size_t part_bytes(const Cut& c, int64_t m, int64_t n, int planes) {
+    return c.parts > 1 ? round_up(sizeof(float) * c.parts * planes * m * n) : 0;
+}
+
+struct Forward {
+    int pieces;
+    Cut up, down;
+    size_t middle, partial, bytes;
+};
+Forward plan_forward(int64_t tokens, int64_t hidden, int64_t inter) {
+    Forward f;
+    f.pieces = pieces_of(tokens);
+    f.up = cut(tokens, inter, hidden, 1, true, false);
+    f.down = cut(tokens, hidden, inter, f.pieces, false, false);
+    f.middle = round_up(sizeof(uint16_t) * f.pieces * tokens * inter);
+    f.partial = std::max(part_bytes(f.up, tokens, inter, 2), part_bytes(f.down, tokens, hidden, 1));
+    f.bytes = f.middle + f.partial;
+    return f;
+}
+
+struct Backward {
+    int pieces;
+    Cut middle, x, weights;
+    size_t rows, partial, bytes;
+};
+Backward plan_backward(int64_t tokens, int64_t hidden, int64_t inter) {
+    Backward b;
+    b.pieces = pieces_of(tokens);
+    b.middle = cut(tokens, inter, hidden, 1, false, false);
+    b.x = cut(tokens, hidden, inter, 2 * b.pieces, false, false);
+    b.weights = cut(inter, hidden, tokens, b.pieces, false, true);
+    b.rows = round_up(sizeof(uint16_t) * b.pieces * tokens * inter);
+    b.partial = std::max(part_bytes(b.middle, tokens, inter, 1), part_bytes(b.x, tokens, hidden, 1));
+    b.bytes = 3 * b.rows + b.partial;
+    return b;
+}
+
+struct Matrix {
+    const void* p;
+    int64_t ld, rows, cols;
+    const char* name;
+    int64_t apart() const { return rows > 1 ? ld : cols; }  // a lone row's leading dimension says nothing
+};
+int check_matrix(const char* call, const Matrix& m) {
+    if (!m.p) return fail(kBadArgument, "%s: null pointer for %s", call, m.name);
+    if (reinterpret_cast<uintptr_t>(m.p) % 16 || (m.rows > 1 && (m.ld % 8 || m.ld < m.cols || m.ld > kMaxLd)))
+        return fail(kBadArgument, "%s: rows of %s must be 16-byte aligned, whole and at most 2^22 elements apart", call, m.name);
+    return kOk;
+}
+
+struct Block {
+    Matrix x, gate, up, down;
+    int dtype, activation;
+    int64_t tokens, hidden, inter;
+};
+int check_block(const char* call, const Block& b) {
+    if (!sizes_fit(b.tokens, b.hidden, b.inter))
+        return fail(kBadArgument, "%s: at most 2^20 tokens, and channels in multiples of 8 up to 2^17", call);
+    if (b.dtype != 0 && b.dtype != 1) return fail(kBadArgument, "%s: dtype must be 0 (bf16) or 1 (f16)", call);
+    if (b.activation != 0 && b.activation != 1) return fail(kBadArgument, "%s: activation must be 0 (swiglu) or 1 (situ)", call);
+    if (b.tokens == 0) return kOk;
+    for (const Matrix* m : {&b.x, &b.gate, &b.up, &b.down})
+        if (int rc = check_matrix(call, *m)) return rc;
+    return kOk;
+}
+int check_workspace(const char* call, const void* ws, size_t given, size_t need) {
+    if (!ws || given < need) return fail(kWorkspaceTooSmall, "%s: needs %zu workspace bytes", call, need);
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return fail(kBadArgument, "%s: the workspace must be 16-byte aligned", call);
+    return kOk;
+}
+
+Pieces pieces_at(char* ws, int64_t tokens, int64_t inter, int pieces) {
+    return {ws, pieces > 1 ? ws + sizeof(uint16_t) * tokens * inter : nullptr};
+}
+
+// One product's sums: a in pieces by b, or a by b in pieces.
+void add_sums(Product& p, const Pieces& a, const void* b) {
+    for (const void* piece : {a.hi, a.lo})
+        if (piece) {
+            p.a[p.sums] = piece;
+            p.b[p.sums++] = b;
+        }
+}
+
+template <typename T>
+int forward(const Block& b, float* pre, const Matrix& out, char* ws, const Forward& f, hipStream_t stream) {
+    TileArgs args = {};
+    args.products = 1;
+    args.partial = reinterpret_cast<float*>(ws + f.middle);
+    Product& p = args.product[0];
+    const Pieces middle = pieces_at(ws, b.tokens, b.inter, f.pieces);
+    p.a[0] = b.x.p;
+    p.b[0] = b.gate.p;
+    p.b2 = b.up.p;
+    p.lda = b.x.apart();
+    p.ldb = b.gate.ld;
+    p.m = b.tokens;
+    p.n = b.inter;
+    p.k = b.hidden;
+    p.sums = 1;
+    p.finish = {nullptr, b.inter, b.activation, pre, pre ? pre + b.tokens * b.inter : nullptr, middle, {}, {}};
+    if (int rc = run<T, kRows, kRows, kActivate>(args, f.up, stream)) return rc;
+    if (!out.p) return kOk;
+    p.sums = 0;
+    add_sums(p, middle, b.down.p);
+    p.lda = b.inter;
+    p.ldb = b.down.ld;
+    p.n = b.hidden;
+    p.k = b.inter;
+    p.finish = {const_cast<void*>(out.p), out.apart()};
+    return run<T, kRows, kRows, kStore>(args, f.down, stream);
+}
+
+struct Gradients {
+    Matrix dy;
+    const float* pre;
+    Matrix dx;
+    void *gate, *up, *down;              // of the weights, in one piece each; or null
+    void *gate_rows, *up_rows, *middle;  // dG, dU and M in one piece each; or null
+};
+
+template <typename T>
+int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan, hipStream_t stream) {
+    TileArgs args = {};
+    args.products = 1;
+    args.partial = reinterpret_cast<float*>(ws + 3 * plan.rows);
+    Pieces dg = pieces_at(ws, b.tokens, b.inter, plan.pieces), du = pieces_at(ws + plan.rows, b.tokens, b.inter, plan.pieces),
+           middle = pieces_at(ws + 2 * plan.rows, b.tokens, b.inter, plan.pieces);
+    if (g.gate_rows) dg.hi = g.gate_rows;
+    if (g.up_rows) du.hi = g.up_rows;
+    if (g.middle) middle.hi = g.middle;
+    {
+        Product& p = args.product[0];
+        p.a[0] = g.dy.p;
+        p.b[0] = b.down.p;
+        p.lda = g.dy.apart();
+        p.ldb = b.down.ld;
+        p.m = b.tokens;
+        p.n = b.inter;
+        p.k = b.hidden;
+        p.sums = 1;
+        float* pre = const_cast<float*>(g.pre);
+        p.finish = {nullptr, b.inter, b.activation, pre, pre + b.tokens * b.inter, middle, dg, du};
+        if (int rc = run<T, kRows, kCols, kSlopes>(args, plan.middle, stream)) return rc;
+    }
+    if (g.dx.p) {
+        Product& p = args.product[0];
+        p.sums = 0;
+        add_sums(p, dg, b.gate.p);
+        add_sums(p, du, b.up.p);
+        p.lda = b.inter;
+        p.ldb = b.gate.ld;
+        p.n = b.hidden;
+        p.k = b.inter;
+        p.finish = {const_cast<void*>(g.dx.p), g.dx.apart()};
+        if (int rc = run<T, kRows, kCols, kStore>(args, plan.x, stream)) return rc;
+    }
+    args.products = 0;
+    const auto add = [&](const Pieces& rows, const Matrix& other, void* out, bool rows_first) {
+        if (!out) return;
+        Product& p = args.product[args.products++];
+        p = {};
+        add_sums(p, rows, other.p);
+        p.lda = b.inter;
+        p.ldb = other.apart();
+        p.m = b.inter;
+        p.n = b.hidden;
+        if (!rows_first) {
+            std::swap_ranges(p.a, p.a + kSums, p.b);
+            std::swap(p.lda, p.ldb);
+            std::swap(p.m, p.n);
+        }
+        p.k = b.tokens;
+        p.finish = {out, p.n};
+    };
+    add(dg, b.x, g.gate, true);
+    add(du, b.x, g.up, true);
+    add(middle, g.dy, g.down, false);
+    return args.products ? run<T, kCols, kCols, kStore>(args, plan.weights, stream) : kOk;
+}
+
+}  // namespace
+}  // namespace qsrt
+
+using namespace qsrt;
+
+extern "C" size_t qsrt_gated_ffn_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inter) {
+    if (tokens == 0 || !sizes_fit(tokens, hidden, inter)) return 0;
+    return plan_forward(tokens, hidden, inter).bytes;
+}
+
+extern "C" int qsrt_gated_ffn(const void* x, int64_t x_ld, const void* gate, const void* up, int64_t up_ld, const void* down,
+                              int64_t down_ld, int dtype, int64_t tokens, int64_t hidden, int64_t inter, int activation,
+                              float* pre, void* out, int64_t out_ld, void* ws, size_t ws_bytes, void* stream) {
+    constexpr const char* kCall = "qsrt_gated_ffn";
+    const Block b{{x, x_ld, tokens, hidden, "x"}, {gate, up_ld, inter, hidden, "gate"}, {up, up_ld, inter, hidden, "up"},
+                  {down, down_ld, hidden, inter, "down"}, dtype, activation, tokens, hidden, inter};
+    if (int rc = check_block(kCall, b)) return rc;
+    if (tokens == 0) return kOk;
+    const Matrix y{out, out_ld, tokens, hidden, "out"};
+    if (out || !pre)
+        if (int rc = check_matrix(kCall, y)) return rc;
+    if (reinterpret_cast<uintptr_t>(pre) % 16) return fail(kBadArgument, "%s: pre must be 16-byte aligned", kCall);
+    const Forward f = plan_forward(tokens, hidden, inter);
+    if (int rc = check_workspace(kCall, ws, ws_bytes, f.bytes)) return rc;
+    return (dtype == 0 ? forward<__bf16> : forward<_Float16>)(b, pre, y, static_cast<char*>(ws), f, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t qsrt_gated_ffn_backward_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inter) {
+    if (tokens == 0 || !sizes_fit(tokens, hidden, inter)) return 0;
+    return plan_backward(tokens, hidden, inter).bytes;
+}
+
+extern "C" int qsrt_gated_ffn_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* gate, const void* up,
+                                       int64_t up_ld, const void* down, int64_t down_ld, int dtype, int64_t tokens, int64_t hidden,
+                                       int64_t inter, int activation, const float* pre, void* dx, int64_t dx_ld, void* d_gate,
+                                       void* d_up, void* d_down, void* gate_rows, void* up_rows, void* middle, void* ws,
+                                       size_t ws_bytes, void* stream) {
+    constexpr const char* kCall = "qsrt_gated_ffn_backward";
+    const Block b{{x, x_ld, tokens, hidden, "x"}, {gate, up_ld, inter, hidden, "gate"}, {up, up_ld, inter, hidden, "up"},
+                  {down, down_ld, hidden, inter, "down"}, dtype, activation, tokens, hidden, inter};
+    if (int rc = check_block(kCall, b)) return rc;
+    if (tokens == 0) return kOk;
+    const Gradients g{{dy, dy_ld, tokens, hidden, "dy"}, pre, {dx, dx_ld, tokens, hidden, "dx"}, d_gate, d_up, d_down,
+                      gate_rows, up_rows, middle};
+    if (int rc = check_matrix(kCall, g.dy)) return rc;
+    if (dx)
+        if (int rc = check_matrix(kCall, g.dx)) return rc;
+    if (!pre) return fail(kBadArgument, "%s: null pointer for pre", kCall);
+    for (const void* p : {static_cast<const void*>(pre), static_cast<const void*>(d_gate), static_cast<const void*>(d_up),
+                          static_cast<const void*>(d_down), static_cast<const void*>(gate_rows),
+                          static_cast<const void*>(up_rows), static_cast<const void*>(middle)})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kBadArgument, "%s: pre, gradients and rows must be 16-byte aligned", kCall);
+    const Backward plan = plan_backward(tokens, hidden, inter);
+    if (int rc = check_workspace(kCall, ws, ws_bytes, plan.bytes)) return rc;
+    return (dtype == 0 ? backward<__bf16> : backward<_Float16>)(b, g, static_cast<char*>(ws), plan, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,376 @@
+// What stands between two blocks of a model: the norm behind the first, its gate, the residual with its scale and the norm
+// before the second, in one pass over the rows; and its gradients in another (gfx950, wave64).
+//
+//   z = post * y sy, sy = (mean y^2 + eps)^-1/2   (without post: z = y)
+//   h = scale * residual + gate * z
+//   n = weight * h sh, sh = (mean h^2 + eps)^-1/2
+//
+// Bound by memory: a row stays in registers between its loads and its stores, sums and statistics are FP32, n comes from h
+// before h is rounded.  The gradients, with e = weight * dn and p = post * gate:
+//   dh = dsum + sh (e - h sh^2 mean(e h)),  dresidual = scale dh,  dz = gate dh
+//   dy = sy (post dz - yhat mean(post dz yhat)),  yhat = y sy
+//   dweight = sum over rows of dn h sh,  dpost of dz yhat,  dgate of dh z (a row's own gate: over its channels)
+// mean(post dz yhat) is put together from sums that do not wait for mean(e h), so a row meets once:
+//   sum p yhat dh = sum p yhat (dsum + sh e) - sh^3 mean(e h) sum p yhat h
+#include <algorithm>
+
+#include "common.h"
+#include "qsrt_amd.h"
+
+namespace qsrt {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+
+constexpr int64_t kMaxRows = 1 << 22, kMaxHidden = 1 << 14;
+enum Gate { kNone, kChannel, kRow };
+
+struct NormArgs {
+    const void *residual, *y, *weight, *post, *gate;
+    int64_t residual_ld, y_ld, rows;
+    int hidden, gate_kind;
+    bool residual_f32, params_f32;
+    float scale, eps;
+    void *sum, *normed;  // sum may be null
+    int64_t sum_ld, normed_ld;
+    float* stats;  // [2][rows]: sy (1 without post) and sh; null where no gradient is to follow
+    // backward
+    const void *dsum, *dn;  // one may be null
+    int64_t dsum_ld, dn_ld;
+    void *dresidual, *dy;  // either may be null
+    int64_t dresidual_ld, dy_ld;
+    float* partial;       // [workgroup][3][hidden]
+    void* drow;           // [rows], of a row's own gate; or null
+};
+
+__device__ __forceinline__ f32x8 load_f32(const void* p, int64_t at) {
+    const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+    const f32x4 a = q[0], b = q[1];
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const void* p, int64_t at, bool f32) {
+    if (f32) return load_f32(p, at);
+    return __builtin_convertvector(*reinterpret_cast<const vec8<T>*>(static_cast<const T*>(p) + at), f32x8);
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* p, int64_t at, const f32x8& v, bool f32) {
+    if (f32) {
+        f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + at);
+        q[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+        q[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    } else {
+        *reinterpret_cast<vec8<T>*>(static_cast<T*>(p) + at) = __builtin_convertvector(v, vec8<T>);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float load1(const void* p, int64_t at, bool f32) {
+    return f32 ? static_cast<const float*>(p)[at] : static_cast<float>(static_cast<const T*>(p)[at]);
+}
+__device__ __forceinline__ float total(const f32x8& v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
+
+// The sums of kSums values over a workgroup, in every thread.  `room`: two sets, used in turn, so one barrier a call is enough.
+template <int kThreads, int kSums>
+__device__ __forceinline__ void meet(float (&v)[kSums], float (*room)[kSums], int lane, int wave) {
+#pragma unroll
+    for (int s = 0; s < kSums; ++s)
+#pragma unroll
+        for (int step = 32; step; step >>= 1) v[s] += __shfl_xor(v[s], step);
+    if (lane == 0)
+#pragma unroll
+        for (int s = 0; s < kSums; ++s) room[wave][s] = v[s];
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSums; ++s) {
+        v[s] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) v[s] += room[w][s];
+    }
+}
+
+template <typename T, int kThreads, int kSteps>
+__global__ __launch_bounds__(kThreads) void norm_kernel(const NormArgs p) {
+    __shared__ float room[2][kThreads / 64][1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x;
+    const f32x8 zero = {};
+    f32x8 r[kSteps], y[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+        const bool in = c < p.hidden;
+        r[s] = in ? load8<T>(p.residual, row * p.residual_ld + c, p.residual_f32) : zero;
+        y[s] = in && p.y ? load8<T>(p.y, row * p.y_ld + c, false) : zero;
+    }
+    float sy = 1.f;
+    if (p.post) {
+        float v[1] = {0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[0] += total(y[s] * y[s]);
+        meet<kThreads, 1>(v, room[0], lane, wave);
+        sy = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
+    }
+    const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
+    float v[1] = {0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+        if (c >= p.hidden) continue;
+        f32x8 z = y[s];
+        if (p.post) z = z * sy * load8<T>(p.post, c, p.params_f32);
+        if (p.gate_kind == kChannel) z = z * load8<T>(p.gate, c, p.params_f32);
+        r[s] = p.scale * r[s] + row_gate * z;
+        if (p.sum) store8<T>(p.sum, row * p.sum_ld + c, r[s], p.residual_f32);
+        v[0] += total(r[s] * r[s]);
+    }
+    meet<kThreads, 1>(v, room[1], lane, wave);
+    const float sh = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+        if (c < p.hidden) store8<T>(p.normed, row * p.normed_ld + c, r[s] * sh * load8<T>(p.weight, c, p.params_f32), false);
+    }
+    if (p.stats && threadIdx.x == 0) {
+        p.stats[row] = sy;
+        p.stats[p.rows + row] = sh;
+    }
+}
+
+template <typename T, int kThreads, int kSteps>
+__global__ __launch_bounds__(kThreads) void norm_gradients_kernel(const NormArgs p) {
+    __shared__ float room[2][kThreads / 64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const f32x8 zero = {};
+    f32x8 by_weight[kSteps], by_post[kSteps], by_gate[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) by_weight[s] = by_post[s] = by_gate[s] = zero;
+    const float mean = 1.0f / static_cast<float>(p.hidden);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const float sy = p.stats[row], sh = p.stats[p.rows + row];
+        const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
+        // yhat (y without post), h, e sh + dsum
+        f32x8 yhat[kSteps], h[kSteps], d[kSteps];
+        float v[4] = {0.f, 0.f, 0.f, 0.f};  // e h, p yhat (dsum + sh e), p yhat h; a row's gate: z's of both
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+            yhat[s] = h[s] = d[s] = zero;
+            if (c >= p.hidden) continue;
+            if (p.y) yhat[s] = load8<T>(p.y, row * p.y_ld + c, false) * sy;
+            h[s] = load8<T>(p.residual, row * p.residual_ld + c, p.residual_f32);
+            const f32x8 dn = p.dn ? load8<T>(p.dn, row * p.dn_ld + c, false) : zero;
+            if (p.dsum) d[s] = load8<T>(p.dsum, row * p.dsum_ld + c, p.residual_f32);
+            f32x8 post = zero + 1.f, gate = zero + row_gate;
+            if (p.post) post = load8<T>(p.post, c, p.params_f32);
+            if (p.gate_kind == kChannel) gate = load8<T>(p.gate, c, p.params_f32);
+            const f32x8 z = yhat[s] * post;
+            h[s] = p.scale * h[s] + gate * z;
+            by_weight[s] += dn * (h[s] * sh);
+            const f32x8 e = dn * load8<T>(p.weight, c, p.params_f32);
+            d[s] += e * sh;
+            v[0] += total(e * h[s]);
+            const f32x8 zg = p.gate_kind == kRow ? z : z * gate;  // without a row's gate: its gradient needs the same sums
+            v[1] += total(zg * d[s]);
+            v[2] += total(zg * h[s]);
+        }
+        meet<kThreads, 4>(v, room[turn], lane, wave);
+        const float back = sh * sh * sh * (v[0] * mean);
+        const float by_z = v[1] - back * v[2];  // sum of zg dh
+        const float shared = by_z * row_gate * mean;
+        if (p.drow && threadIdx.x == 0) {
+            if (p.params_f32)
+                static_cast<float*>(p.drow)[row] = by_z;
+            else
+                static_cast<T*>(p.drow)[row] = static_cast<T>(by_z);
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+            if (c >= p.hidden) continue;
+            const f32x8 dh = d[s] - h[s] * back;
+            if (p.dresidual) store8<T>(p.dresidual, row * p.dresidual_ld + c, p.scale * dh, p.residual_f32);
+            if (!p.y) continue;
+            f32x8 post = zero + 1.f, gate = zero + row_gate;
+            if (p.post) post = load8<T>(p.post, c, p.params_f32);
+            if (p.gate_kind == kChannel) gate = load8<T>(p.gate, c, p.params_f32);
+            f32x8 dy = gate * dh;
+            by_post[s] += dy * yhat[s];
+            by_gate[s] += dh * (yhat[s] * post);
+            if (p.post) dy = sy * (dy * post - yhat[s] * shared);
+            if (p.dy) store8<T>(p.dy, row * p.dy_ld + c, dy, false);
+        }
+    }
+    float* to = p.partial + static_cast<int64_t>(blockIdx.x) * 3 * p.hidden;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+        if (c >= p.hidden) continue;
+        store8<T>(to, c, by_weight[s], true);
+        if (p.post) store8<T>(to, p.hidden + c, by_post[s], true);
+        if (p.gate_kind == kChannel) store8<T>(to, 2 * static_cast<int64_t>(p.hidden) + c, by_gate[s], true);
+    }
+}
+
+// Adds the workgroups' sums, 32 channels a workgroup: thread (c, q) every eighth from q, then the eight in order.
+struct JoinArgs {
+    const float* partial;
+    int64_t groups;
+    int hidden;
+    void* out[3];
+    bool f32;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void norm_join_kernel(const JoinArgs p) {
+    __shared__ float sums[8][32];
+    const int c = threadIdx.x & 31, q = threadIdx.x >> 5, which = blockIdx.y;
+    const int64_t channel = static_cast<int64_t>(blockIdx.x) * 32 + c;
+    void* const out = which == 0 ? p.out[0] : which == 1 ? p.out[1] : p.out[2];
+    if (!out) return;
+    float v = 0.f;
+    if (channel < p.hidden)
+        for (int64_t g = q; g < p.groups; g += 8) v += p.partial[(g * 3 + which) * p.hidden + channel];
+    sums[q][c] = v;
+    __syncthreads();
+    if (q || channel >= p.hidden) return;
+    v = ((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) + ((sums[4][c] + sums[5][c]) + (sums[6][c] + sums[7][c]));
+    if (p.f32)
+        static_cast<float*>(out)[channel] = v;
+    else
+        static_cast<T*>(out)[channel] = static_cast<T>(v);
+}
+
+// ---------------------------------------------------------------- host
+int64_t gradient_groups(int64_t rows) {
+    int cus = 0;
+    if (current_cu_count(&cus) != kOk) cus = 256;
+    return std::min<int64_t>(rows, 2 * cus);
+}
+
+int check_rows(const char* call, const void* p, int64_t ld, int64_t rows, int64_t hidden, const char* name) {
+    if (!p) return fail(kBadArgument, "%s: null pointer for %s", call, name);
+    if (reinterpret_cast<uintptr_t>(p) % 16 || (rows > 1 && (ld % 8 || ld < hidden)))
+        return fail(kBadArgument, "%s: rows of %s must be whole and 16-byte aligned", call, name);
+    return kOk;
+}
+int check_norm(const char* call, const NormArgs& a, int dtype) {
+    if (a.rows < 0 || a.rows > kMaxRows || a.hidden <= 0 || a.hidden % 8)
+        return fail(kBadArgument, "%s: at most 2^22 rows, and channels in multiples of 8 up to 2^14", call);
+    if (dtype != 0 && dtype != 1) return fail(kBadArgument, "%s: dtype must be 0 (bf16) or 1 (f16)", call);
+    if (a.gate_kind < kNone || a.gate_kind > kRow) return fail(kBadArgument, "%s: gate must be 0 (none), 1 (channels) or 2 (rows)", call);
+    if ((a.gate_kind != kNone) != (a.gate != nullptr)) return fail(kBadArgument, "%s: a gate needs its kind and its values", call);
+    if (!a.y && (a.post || a.gate)) return fail(kBadArgument, "%s: without y there is nothing to norm or gate before the sum", call);
+    if (!(a.eps >= 0.f)) return fail(kBadArgument, "%s: eps must not be negative", call);
+    if (a.rows == 0) return kOk;
+    if (int rc = check_rows(call, a.residual, a.residual_ld, a.rows, a.hidden, "residual")) return rc;
+    if (a.y)
+        if (int rc = check_rows(call, a.y, a.y_ld, a.rows, a.hidden, "y")) return rc;
+    for (const void* v : {a.weight, a.post, a.gate_kind == kChannel ? a.gate : nullptr})
+        if (reinterpret_cast<uintptr_t>(v) % 16) return fail(kBadArgument, "%s: weights must be 16-byte aligned", call);
+    if (!a.weight) return fail(kBadArgument, "%s: null pointer for weight", call);
+    return kOk;
+}
+
+}  // namespace
+}  // namespace qsrt
+
+using namespace qsrt;
+
+extern "C" int qsrt_residual_norm(const void* residual, int64_t residual_ld, int residual_f32, const void* y, int64_t y_ld, int dtype,
+                                  int64_t rows, int64_t hidden, const void* weight, const void* post, const void* gate,
+                                  int gate_kind, int params_f32, float scale, float eps, void* sum, int64_t sum_ld, void* normed,
+                                  int64_t normed_ld, float* stats, void* stream) {
+    constexpr const char* kCall = "qsrt_residual_norm";
+    NormArgs a = {};
+    a.residual = residual, a.residual_ld = residual_ld, a.residual_f32 = residual_f32 != 0;
+    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
+    a.weight = weight, a.post = post, a.gate = gate, a.gate_kind = gate_kind, a.params_f32 = params_f32 != 0;
+    a.scale = scale, a.eps = eps, a.sum = sum, a.sum_ld = sum_ld, a.normed = normed, a.normed_ld = normed_ld, a.stats = stats;
+    if (int rc = check_norm(kCall, a, dtype)) return rc;
+    if (rows == 0) return kOk;
+    if (sum)
+        if (int rc = check_rows(kCall, sum, sum_ld, rows, hidden, "sum")) return rc;
+    if (int rc = check_rows(kCall, normed, normed_ld, rows, hidden, "normed")) return rc;
+    const dim3 grid(static_cast<unsigned>(rows));
+    const auto s = static_cast<hipStream_t>(stream);
+#define QSRT_NORM(THREADS, STEPS)                                                                                \
+    if (dtype == 0)                                                                                              \
+        hipLaunchKernelGGL((norm_kernel<__bf16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a);                 \
+    else                                                                                                         \
+        hipLaunchKernelGGL((norm_kernel<_Float16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a)
+    if (hidden <= 2048) {
+        QSRT_NORM(256, 1);
+    } else if (hidden <= 8192) {
+        QSRT_NORM(512, 2);
+    } else {
+        QSRT_NORM(512, 4);
+    }
+#undef QSRT_NORM
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
+extern "C" size_t qsrt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t hidden) {
+    if (rows <= 0 || rows > kMaxRows || hidden <= 0 || hidden > kMaxHidden || hidden % 8) return 0;
+    return sizeof(float) * 3 * static_cast<size_t>(gradient_groups(rows) * hidden);
+}
+
+extern "C" int qsrt_residual_norm_backward(const void* dsum, int64_t dsum_ld, const void* dn, int64_t dn_ld, const void* residual,
+                                           int64_t residual_ld, int residual_f32, const void* y, int64_t y_ld, int dtype,
+                                           int64_t rows, int64_t hidden, const void* weight, const void* post, const void* gate,
+                                           int gate_kind, int params_f32, float scale, const float* stats, void* dresidual,
+                                           int64_t dresidual_ld, void* dy, int64_t dy_ld, void* dweight, void* dpost, void* dgate,
+                                           void* ws, size_t ws_bytes, void* stream) {
+    constexpr const char* kCall = "qsrt_residual_norm_backward";
+    NormArgs a = {};
+    a.residual = residual, a.residual_ld = residual_ld, a.residual_f32 = residual_f32 != 0;
+    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
+    a.weight = weight, a.post = post, a.gate = gate, a.gate_kind = gate_kind, a.params_f32 = params_f32 != 0;
+    a.scale = scale, a.stats = const_cast<float*>(stats);
+    a.dsum = dsum, a.dsum_ld = dsum_ld, a.dn = dn, a.dn_ld = dn_ld;
+    a.dresidual = dresidual, a.dresidual_ld = dresidual_ld, a.dy = dy, a.dy_ld = dy_ld;
+    a.drow = gate_kind == kRow ? dgate : nullptr;
+    if (int rc = check_norm(kCall, a, dtype)) return rc;
+    if (rows == 0) return kOk;
+    if (!stats) return fail(kBadArgument, "%s: null pointer for stats", kCall);
+    if (!y && (dy || dpost || dgate)) return fail(kBadArgument, "%s: no gradients of y, post or gate without y", kCall);
+    if ((dpost && !post) || (dgate && !gate)) return fail(kBadArgument, "%s: no gradient of what is not there", kCall);
+    const struct { const void* p; int64_t ld; const char* name; } given[] = {
+        {dsum, dsum_ld, "dsum"}, {dn, dn_ld, "dn"}, {dresidual, dresidual_ld, "dresidual"}, {dy, dy_ld, "dy"}};
+    for (const auto& g : given)
+        if (g.p)
+            if (int rc = check_rows(kCall, g.p, g.ld, rows, hidden, g.name)) return rc;
+    const size_t need = qsrt_residual_norm_backward_workspace_bytes(rows, hidden);
+    if (!ws || ws_bytes < need) return fail(kWorkspaceTooSmall, "%s: needs %zu workspace bytes", kCall, need);
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return fail(kBadArgument, "%s: the workspace must be 16-byte aligned", kCall);
+    a.partial = static_cast<float*>(ws);
+    const int64_t groups = gradient_groups(rows);
+    const dim3 grid(static_cast<unsigned>(groups));
+    const auto s = static_cast<hipStream_t>(stream);
+#define QSRT_NORM(THREADS, STEPS)                                                                                \
+    if (dtype == 0)                                                                                              \
+        hipLaunchKernelGGL((norm_gradients_kernel<__bf16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a);       \
+    else                                                                                                         \
+        hipLaunchKernelGGL((norm_gradients_kernel<_Float16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a)
+    if (hidden <= 4096) {
+        QSRT_NORM(512, 1);
+    } else if (hidden <= 8192) {
+        QSRT_NORM(512, 2);
+    } else {
+        QSRT_NORM(1024, 2);
+    }
+#undef QSRT_NORM
+    QSRT_HIP_TRY(hipGetLastError());
+    const JoinArgs j{a.partial, groups, a.hidden, {dweight, dpost, gate_kind == kChannel ? dgate : nullptr}, a.params_f32};
+    if (!j.out[0] && !j.out[1] && !j.out[2]) return kOk;
+    const dim3 columns(static_cast<unsigned>((hidden + 31) / 32), 3);
+    if (dtype == 0)
+        hipLaunchKernelGGL(norm_join_kernel<__bf16>, columns, dim3(256), 0, s, j);
+    else
+        hipLaunchKernelGGL(norm_join_kernel<_Float16>, columns, dim3(256), 0, s, j);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}

@@ -1,0 +1,179 @@
+"""A gated feed-forward block in dense weights on MI355X, with its gradients: the expert before it is encoded, a shared expert
+beside packed ones, a layer that is trained.
+
+``gated_ffn`` is differentiable; ``gated_ffn_gradients`` returns, beside the gradients, the rows they are products of
+(``qsrt_gated_ffn`` and ``qsrt_gated_ffn_backward`` in ``include/qsrt_amd.h``).  Nothing waits for the device, workspaces come
+from torch's allocator on the current stream.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _native
+from .packed_linear import TYPES, checked_out, checked_rows
+
+ACTIVATIONS = {"swiglu": 0, "situ": 1}
+MAX_CHANNELS = 1 << 17
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with 16-byte aligned rows (copied where they are not)."""
+
+    if t.stride(1) != 1 or t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(0) < t.shape[1]:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _checked(x, gate, up, down, activation):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+    if gate.dim() != 2 or up.shape != gate.shape or down.shape != (gate.shape[1], gate.shape[0]):
+        raise ValueError("gate and up must be [inter, hidden] and down [hidden, inter]")
+    if gate.dtype not in TYPES or not gate.is_cuda:
+        raise ValueError("the weights must be bfloat16 or float16 on a CUDA device")
+    if any(w.dtype != gate.dtype or w.device != gate.device for w in (up, down)):
+        raise ValueError("the weights must be of one type and on one device")
+    inter, hidden = gate.shape
+    if not 0 < hidden <= MAX_CHANNELS or not 0 < inter <= MAX_CHANNELS or hidden % 8 or inter % 8:
+        raise ValueError(f"hidden and inter must be multiples of 8 up to {MAX_CHANNELS}")
+    if x.device != gate.device or x.dtype != gate.dtype:
+        raise ValueError("x must be of the weights' type and on their device")
+    return checked_rows(x, hidden, gate.device), *_checked_weights(gate, up, down)
+
+
+def _checked_weights(gate, up, down):
+    gate, up, down = _rows(gate), _rows(up), _rows(down)
+    if gate.stride(0) != up.stride(0):  # one leading dimension serves both
+        gate, up = gate.contiguous(), up.contiguous()
+    return gate, up, down
+
+
+def _forward(x, gate, up, down, activation, out, pre):
+    t, hidden = x.shape
+    inter = gate.shape[0]
+    lib = _native.lib()
+    with _native.current(x.device):
+        ws = torch.empty(lib.qsrt_gated_ffn_workspace_bytes(t, hidden, inter), dtype=torch.uint8, device=x.device)
+        _native.check(
+            lib.qsrt_gated_ffn(
+                x.data_ptr(), x.stride(0), gate.data_ptr(), up.data_ptr(), gate.stride(0), down.data_ptr(), down.stride(0),
+                TYPES[x.dtype], t, hidden, inter, ACTIVATIONS[activation], None if pre is None else pre.data_ptr(),
+                None if out is None else out.data_ptr(), 0 if out is None else out.stride(0), ws.data_ptr(), ws.numel(),
+                _native.stream_handle(x.device)),
+            "qsrt_gated_ffn",
+        )
+
+
+def _backward(dy, x, gate, up, down, activation, pre, dx, weights, rows):
+    t, hidden = x.shape
+    inter = gate.shape[0]
+    lib = _native.lib()
+    with _native.current(x.device):
+        ws = torch.empty(lib.qsrt_gated_ffn_backward_workspace_bytes(t, hidden, inter), dtype=torch.uint8, device=x.device)
+        _native.check(
+            lib.qsrt_gated_ffn_backward(
+                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), gate.data_ptr(), up.data_ptr(), gate.stride(0),
+                down.data_ptr(), down.stride(0), TYPES[x.dtype], t, hidden, inter, ACTIVATIONS[activation], pre.data_ptr(),
+                None if dx is None else dx.data_ptr(), hidden, *(None if w is None else w.data_ptr() for w in weights),
+                *(None if r is None else r.data_ptr() for r in rows), ws.data_ptr(), ws.numel(),
+                _native.stream_handle(x.device)),
+            "qsrt_gated_ffn_backward",
+        )
+
+
+def _like(t: torch.Tensor, needed: bool = True) -> torch.Tensor | None:
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device) if needed else None
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, activation):
+        x, gate, up, down = _checked(x, gate, up, down, activation)
+        y = _like(x)
+        pre = torch.empty((2, x.shape[0], gate.shape[0]), dtype=torch.float32, device=x.device)
+        if x.shape[0]:
+            _forward(x, gate, up, down, activation, y, pre)
+        ctx.save_for_backward(x, gate, up, down, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gate, up, down, pre = ctx.saved_tensors
+        grads = [_like(t, needed) for t, needed in zip((x, gate, up, down), ctx.needs_input_grad)]
+        if x.shape[0]:
+            _backward(checked_rows(dy, x.shape[1], x.device), x, gate, up, down, ctx.activation, pre, grads[0], grads[1:],
+                      (None, None, None))
+        else:
+            for g in grads[1:]:
+                if g is not None:
+                    g.zero_()
+        return *grads, None
+
+
+def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *, activation: str = "swiglu",
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x gate^T, x up^T) down^T -> [T, hidden]`` in ``x``'s type.
+
+    ``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]``, all bf16 or all f16, hidden and inter
+    multiples of 8.  ``activation``: ``"swiglu"`` (``silu(g) u``) or ``"situ"``.  Sums are FP32; the rows between the two
+    products are held in ``x``'s type (f16 ends at 65504), of 64 rows or less as two values each.  Differentiable in all four;
+    the backward pass keeps the rows before the activation in FP32 (``8 T inter`` bytes).  ``out``: where the result goes, of a
+    call without gradients."""
+
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
+        if out is not None:
+            raise ValueError("out is for calls without gradients")
+        return _GatedFFN.apply(x, gate, up, down, activation)
+    x, gate, up, down = _checked(x, gate, up, down, activation)
+    out = checked_out(out, x, x.shape[1])
+    if out.data_ptr() % 16 or (out.stride(0) % 8 and out.shape[0] > 1):
+        raise ValueError("out's rows must be 16-byte aligned")
+    if x.shape[0]:
+        _forward(x, gate, up, down, activation, out, None)
+    return out
+
+
+@dataclass(frozen=True)
+class GatedFFNGradients:
+    """``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]`` (None where not asked for), and the rows
+    ``gate_rows`` (dG), ``up_rows`` (dU) and ``middle`` (M), ``[T, inter]``:  ``gate = gate_rows^T x``, ``up = up_rows^T x``,
+    ``down = dy^T middle``."""
+
+    x: torch.Tensor | None
+    gate: torch.Tensor | None
+    up: torch.Tensor | None
+    down: torch.Tensor | None
+    gate_rows: torch.Tensor
+    up_rows: torch.Tensor
+    middle: torch.Tensor
+
+
+@torch.no_grad()
+def gated_ffn_gradients(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *,
+                        activation: str = "swiglu", inputs: bool = True, weights: bool = True) -> GatedFFNGradients:
+    """Gradients of ``sum(dy * gated_ffn(x, gate, up, down))`` without the graph: of ``x`` where ``inputs``, of the weights
+    where ``weights``, and always the rows that a weight's gradient is the product of.  ``dy [T, hidden]`` in ``x``'s type."""
+
+    x, gate, up, down = _checked(x, gate, up, down, activation)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and type")
+    dy = checked_rows(dy, x.shape[1], x.device)
+    t, inter = x.shape[0], gate.shape[0]
+    grads = [_like(x, inputs), *(_like(w, weights) for w in (gate, up, down))]
+    rows = [torch.empty((t, inter), dtype=x.dtype, device=x.device) for _ in range(3)]
+    if t:
+        pre = torch.empty((2, t, inter), dtype=torch.float32, device=x.device)
+        _forward(x, gate, up, down, activation, None, pre)
+        _backward(dy, x, gate, up, down, activation, pre, grads[0], grads[1:], rows)
+    elif weights:
+        for g in grads[1:]:
+            g.zero_()
+    return GatedFFNGradients(*grads, *rows)
+
+
+__all__ = ["GatedFFNGradients", "gated_ffn", "gated_ffn_gradients"]
