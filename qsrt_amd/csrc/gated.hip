@@ -183,17 +183,30 @@ struct Loader {
         }
     }
 
-    // `p`: the operand's first element of this tile and stage; `size` and `depth`: how much of both there is
-    __device__ __forceinline__ void load(const uint16_t* p, int64_t ld, int64_t size, int64_t depth, uint32_t lds, int wave) const {
-        const int rows = static_cast<int>(kLayout == kRows ? min(size, int64_t{kSize}) : min(depth, int64_t{kDepth}));
-        const int span = static_cast<int>(kLayout == kRows ? min(depth, int64_t{kDepth}) : min(size, int64_t{kSize}));
-        const uint32_t bytes = rows > 0 ? (static_cast<uint32_t>(rows - 1) * static_cast<uint32_t>(ld) + span) * 2 : 0;
-        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, bytes, 0x00020000);
-        const bool past = kLayout == kRows && 8 * chunk >= span;
-#pragma unroll
-        for (int q = 0; q < kLoads; ++q)
-            to_lds(from, past ? kNowhere : offset[q], lds + (q * kWaves + wave) * 1024);
+    // The wave's q-th load of a stage from `from`, of which `depth` summed indices are left.
+    __device__ __forceinline__ void load(int q, __amdgpu_buffer_rsrc_t from, int depth, uint32_t lds, int wave) const {
+        const bool past = kLayout == kRows && 8 * chunk >= depth;
+        to_lds(from, past ? kNowhere : offset[q], lds + (q * kWaves + wave) * 1024);
     }
+};
+
+// Where an operand's next stage lies: a buffer that ends with the last of its values, so that reads past the tile's end of
+// either index are zero or feed results that are not stored.
+template <Layout kLayout>
+struct Feed {
+    const char* p;
+    uint32_t ld, span;  // bytes between rows; kRows: in the tile's rows but the last, kCols: of a row
+    __device__ __forceinline__ void init(int64_t stride, int64_t size, int tile) {
+        ld = static_cast<uint32_t>(stride) * 2;
+        const uint32_t n = static_cast<uint32_t>(min(size, static_cast<int64_t>(tile)));
+        span = kLayout == kRows ? (n - 1) * ld : n * 2;
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int depth) const {
+        const uint32_t k = static_cast<uint32_t>(min(depth, kDepth));
+        const uint32_t bytes = kLayout == kRows ? span + 2 * k : (k - 1) * ld + span;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, 0x00020000);
+    }
+    __device__ __forceinline__ void advance() { p += kLayout == kRows ? 2 * kDepth : static_cast<int64_t>(ld) * kDepth; }
 };
 
 // The lane's part of a 16 x 32 fragment: index lane % 16, eight summed indices from 8 (lane / 16).
@@ -267,7 +280,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     const int high = min(kBand, p.tiles_m - band * kBand);
     const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * kM, n0 = static_cast<int64_t>(in_band / high) * kNb;
 
-    const int per = static_cast<int>((p.k + kDepth - 1) / kDepth), stages = per * p.sums;
+    const int k = static_cast<int>(p.k), per = (k + kDepth - 1) / kDepth, stages = per * p.sums;
     const int begin = static_cast<int>(static_cast<int64_t>(stages) * part / args.parts);
     const int end = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / args.parts);
 
@@ -280,16 +293,45 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     ra.init(lane);
     rb.init(lane);
 
-    const auto load = [&](int s) {
-        const int sum = s / per;
-        const int64_t k0 = static_cast<int64_t>(s - sum * per) * kDepth, depth = p.k - k0;
-        const uint32_t to = static_cast<uint32_t>(s % kStages) * kStageBytes;
-        const uint16_t* a = static_cast<const uint16_t*>(p.a[sum]) + (kA == kRows ? m0 * p.lda + k0 : k0 * p.lda + m0);
+    // the stage to be loaded next
+    Feed<kA> fa;
+    Feed<kB> fb, fb2;
+    fa.init(p.lda, p.m - m0, kM);
+    fb.init(p.ldb, p.n - n0, kNb);
+    if constexpr (kDual) fb2 = fb;
+    int sum = begin / per, depth = k - (begin - sum * per) * kDepth;
+    uint32_t to = 0;
+    const auto enter = [&]() {  // the operands of `sum`, `depth` before their end
+        const int64_t k0 = k - depth;
         const int64_t at = kB == kRows ? n0 * p.ldb + k0 : k0 * p.ldb + n0;
-        la.load(a, p.lda, p.m - m0, depth, to, wave);
-        lb.load(static_cast<const uint16_t*>(p.b[sum]) + at, p.ldb, p.n - n0, depth, to + LoaderA::kBytes, wave);
-        if constexpr (kDual)
-            lb.load(static_cast<const uint16_t*>(p.b2) + at, p.ldb, p.n - n0, depth, to + LoaderA::kBytes + LoaderB::kBytes, wave);
+        fa.p = static_cast<const char*>(p.a[sum]) + 2 * (kA == kRows ? m0 * p.lda + k0 : k0 * p.lda + m0);
+        fb.p = static_cast<const char*>(p.b[sum]) + 2 * at;
+        if constexpr (kDual) fb2.p = static_cast<const char*>(p.b2) + 2 * at;
+    };
+    const auto load_one = [&](int q) {  // of the wave's loads of a stage
+        if (q < LoaderA::kLoads)
+            la.load(q, fa.buffer(depth), depth, to, wave);
+        else if (q < LoaderA::kLoads + LoaderB::kLoads)
+            lb.load(q - LoaderA::kLoads, fb.buffer(depth), depth, to + LoaderA::kBytes, wave);
+        else
+            lb.load(q - LoaderA::kLoads - LoaderB::kLoads, fb2.buffer(depth), depth, to + LoaderA::kBytes + LoaderB::kBytes, wave);
+    };
+    const auto loaded = [&]() {
+        to = to + kStageBytes == kStages * kStageBytes ? 0 : to + kStageBytes;
+        depth -= kDepth;
+        if (depth > 0) {
+            fa.advance();
+            fb.advance();
+            if constexpr (kDual) fb2.advance();
+        } else if (++sum < p.sums) {
+            depth = k;
+            enter();
+        }
+    };
+    const auto load = [&]() {
+#pragma unroll
+        for (int q = 0; q < kStageLoads; ++q) load_one(q);
+        loaded();
     };
 
     const int wm = wave / kWavesN * kWm, wn = wave % kWavesN * (kDual ? kWn / 2 : kWn);
@@ -298,30 +340,96 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     for (int i = 0; i < kI; ++i)
 #pragma unroll
         for (int j = 0; j < kJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto read_a = [&](const char* at, int i, int kk) { return ra.read(at, wm + 16 * i, kk); };
+    const auto read_b = [&](const char* at, int j, int kk) {
+        return rb.read(at + LoaderA::kBytes + (j < kHalf ? 0 : LoaderB::kBytes), wn + 16 * (j % kHalf), kk);
+    };
 
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s)
-        if (begin + s < end) load(begin + s);
-    for (int s = begin; s < end; ++s) {
-        // of what is on its way, the stages behind s may stay so
-        if (kStages > 2 && s + kStages - 2 < end)
-            wait_and_meet<kStageLoads*(kStages - 2)>();
-        else
+    enter();
+    if constexpr (kI >= 4) {
+        // A stage is 2 kI steps of kJ products: fragment i of a by all of b.  Before a step's products go the reads of what
+        // is used kI steps later (a's fragments in place of those just used, b's in turn), from the middle of the second
+        // half on those of the next stage: then every wave has read all of this one, the next has landed, and its buffer
+        // takes the stage after that.  One wait and barrier a stage, with products before and behind it.
+        static_assert(kStages == 2, "two stages");
+        vec8<T> a[kI], b[2][kJ];
+        load();
+        if (begin + 1 < end) {
+            load();
+            wait_and_meet<kStageLoads>();
+        } else {
             wait_and_meet<0>();
-        if (s + kStages - 1 < end) load(s + kStages - 1);
-        const char* at = lds + static_cast<uint32_t>(s % kStages) * kStageBytes;
+        }
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            vec8<T> b[kJ];
+        for (int j = 0; j < kJ; ++j) b[0][j] = read_b(lds, j, 0);
 #pragma unroll
-            for (int j = 0; j < kJ; ++j)
-                b[j] = rb.read(at + LoaderA::kBytes + (j < kHalf ? 0 : LoaderB::kBytes), wn + 16 * (j % kHalf), kk);
+        for (int i = 0; i < kI; ++i) a[i] = read_a(lds, i, 0);
+        uint32_t now = 0;
+        for (int s = begin; s < end; ++s) {
+            const char *at = lds + now, *next = lds + (now ^ kStageBytes);
+            const bool more = s + 2 < end;
 #pragma unroll
             for (int i = 0; i < kI; ++i) {
-                const vec8<T> a = ra.read(at, wm + 16 * i, kk);
+                if (i > 0) a[i - 1] = read_a(at, i - 1, 1);
 #pragma unroll
-                for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[j], a, acc[i][j]);
+                for (int j = i * kJ / (kI - 1); j < (i + 1) * kJ / (kI - 1) && j < kJ; ++j) b[1][j] = read_b(at, j, 1);
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[0][j], a[i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                if (i == 0) a[kI - 1] = read_a(at, kI - 1, 1);
+                if (i >= 2) {
+                    if (i == 2) a[0] = read_a(next, 0, 0);
+                    a[i - 1] = read_a(next, i - 1, 0);
+#pragma unroll
+                    for (int j = (i - 2) * kJ / (kI - 2); j < (i - 1) * kJ / (kI - 2); ++j) b[0][j] = read_b(next, j, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[1][j], a[i], acc[i][j]);
+                if (i >= 2 && more) {
+#pragma unroll
+                    for (int q = (i - 2) * kStageLoads / (kI - 2); q < (i - 1) * kStageLoads / (kI - 2); ++q) load_one(q);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (i == 1) {
+                    wait_and_meet<0>();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (more) loaded();
+            a[kI - 1] = read_a(next, kI - 1, 0);
+            now ^= kStageBytes;
+        }
+    } else {
+        uint32_t now = 0;
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s)
+            if (begin + s < end) load();
+        for (int s = begin; s < end; ++s) {
+            // of what is on its way, the stages behind s may stay so
+            if (kStages > 2 && s + kStages - 2 < end)
+                wait_and_meet<kStageLoads*(kStages - 2)>();
+            else
+                wait_and_meet<0>();
+            if (s + kStages - 1 < end) load();
+            const char* at = lds + now;
+            now = now + kStageBytes == kStages * kStageBytes ? 0 : now + kStageBytes;
+            vec8<T> a[2][kI], b[2][kJ];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) b[kk][j] = read_b(at, j, kk);
+#pragma unroll
+                for (int i = 0; i < kI; ++i) a[kk][i] = read_a(at, i, kk);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int i = 0; i < kI; ++i)
+#pragma unroll
+                    for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[kk][j], a[kk][i], acc[i][j]);
         }
     }
 
