@@ -299,7 +299,11 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     fa.init(p.lda, p.m - m0, kM);
     fb.init(p.ldb, p.n - n0, kNb);
     if constexpr (kDual) fb2 = fb;
-    int sum = begin / per, depth = k - (begin - sum * per) * kDepth;
+    // Neighbouring tiles walk the sum from stages of their own, around its end: rows whose distance has a high power of two
+    // would come from the same few channels of the L2 in every workgroup at once (4096 rows of 7168 x 2048 with gradients: 972
+    // us from the first stage, 961 so).
+    int coming = begin + tile % 8 % (end - begin);
+    int sum = coming / per, depth = k - (coming - sum * per) * kDepth;
     uint32_t to = 0;
     const auto enter = [&]() {  // the operands of `sum`, `depth` before their end
         const int64_t k0 = k - depth;
@@ -319,11 +323,17 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     const auto loaded = [&]() {
         to = to + kStageBytes == kStages * kStageBytes ? 0 : to + kStageBytes;
         depth -= kDepth;
-        if (depth > 0) {
+        if (++coming == end) {
+            coming = begin;
+            sum = coming / per;
+            depth = k - (coming - sum * per) * kDepth;
+            enter();
+        } else if (depth > 0) {
             fa.advance();
             fb.advance();
             if constexpr (kDual) fb2.advance();
-        } else if (++sum < p.sums) {
+        } else {
+            ++sum;
             depth = k;
             enter();
         }
