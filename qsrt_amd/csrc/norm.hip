@@ -12,6 +12,7 @@
 //   dweight = sum over rows of dn h sh,  dpost of dz yhat,  dgate of dh z (a row's own gate: over its channels)
 // mean(post dz yhat) is put together from sums that do not wait for mean(e h), so a row meets once:
 //   sum p yhat dh = sum p yhat (dsum + sh e) - sh^3 mean(e h) sum p yhat h
+// and a gate for each channel shares its sum over the rows with post: dpost = gate S, dgate = post S, S = sum of dh yhat.
 #include <algorithm>
 
 #include "common.h"
@@ -42,7 +43,7 @@ struct NormArgs {
     int64_t dsum_ld, dn_ld;
     void *dresidual, *dy;  // either may be null
     int64_t dresidual_ld, dy_ld;
-    float* partial;       // [workgroup][3][hidden]
+    float* partial;       // [workgroup][2][hidden]: dweight, S
     void* drow;           // [rows], of a row's own gate; or null
 };
 
@@ -72,115 +73,198 @@ __device__ __forceinline__ float load1(const void* p, int64_t at, bool f32) {
 }
 __device__ __forceinline__ float total(const f32x8& v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
 
-// The sums of kSums values over a workgroup, in every thread.  `room`: two sets, used in turn, so one barrier a call is enough.
-template <int kThreads, int kSums>
-__device__ __forceinline__ void meet(float (&v)[kSums], float (*room)[kSums], int lane, int wave) {
-#pragma unroll
-    for (int s = 0; s < kSums; ++s)
-#pragma unroll
-        for (int step = 32; step; step >>= 1) v[s] += __shfl_xor(v[s], step);
-    if (lane == 0)
-#pragma unroll
-        for (int s = 0; s < kSums; ++s) room[wave][s] = v[s];
-    __syncthreads();
+template <int kControl>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, 0xF, 0xF, true));
+}
+// The sum over 16 lanes, in each of them: neighbours, pairs, then mirrors of 8 and 16.
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    return v + dpp<0x140>(v);
+}
+__device__ __forceinline__ float sum64(float v) {
+    v = sum16(v);
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, static_cast<uint32_t>(rows[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(rows[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(halves[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(halves[1]));
+}
+
+constexpr int kMaxWaves = 16;
+// The sums of kSums values over a workgroup, in every thread.  `room` starts at zero (the waves that are not there) and has
+// two sets that are used in turn, so one barrier a call is enough.
+template <int kSums>
+__device__ __forceinline__ void meet(float (&v)[kSums], float (*room)[kMaxWaves], int lane, int wave) {
 #pragma unroll
     for (int s = 0; s < kSums; ++s) {
-        v[s] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) v[s] += room[w][s];
+        v[s] = sum64(v[s]);
+        if (lane == 0) room[s][wave] = v[s];
     }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSums; ++s) v[s] = sum16(room[s][lane & 15]);
 }
 
-template <typename T, int kThreads, int kSteps>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const NormArgs p) {
-    __shared__ float room[2][kThreads / 64][1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
-    const f32x8 zero = {};
-    f32x8 r[kSteps], y[kSteps];
+// Eight values as they lie in memory: the next row's are on their way while a row is computed.
+template <typename T, bool kF32>
+struct Packed {
+    vec8<T> v;
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        v = *reinterpret_cast<const vec8<T>*>(static_cast<const T*>(p) + at);
+    }
+    __device__ __forceinline__ f32x8 get() const { return __builtin_convertvector(v, f32x8); }
+};
+template <typename T>
+struct Packed<T, true> {
+    f32x8 v;
+    __device__ __forceinline__ void load(const void* p, int64_t at) { v = load_f32(p, at); }
+    __device__ __forceinline__ f32x8 get() const { return v; }
+};
+
+// A workgroup walks the rows in strides, eight channels a thread and step, in as many waves as a row needs.
+template <typename T, int kSteps, bool kF32>
+__global__ __launch_bounds__(1024) void norm_kernel(const NormArgs p) {
+    __shared__ float room[2][1][kMaxWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x;
+    if (threadIdx.x < 2 * kMaxWaves) room[0][0][threadIdx.x] = 0.f;
+    Packed<T, false> y[kSteps];
+    Packed<T, kF32> residual[kSteps];
+    const auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
+            if (c >= p.hidden) continue;
+            residual[s].load(p.residual, row * p.residual_ld + c);
+            if (p.y) y[s].load(p.y, row * p.y_ld + c);
+        }
+    };
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
-        const bool in = c < p.hidden;
-        r[s] = in ? load8<T>(p.residual, row * p.residual_ld + c, p.residual_f32) : zero;
-        y[s] = in && p.y ? load8<T>(p.y, row * p.y_ld + c, false) : zero;
+        residual[s] = {};
+        y[s] = {};
     }
-    float sy = 1.f;
-    if (p.post) {
+    fetch(blockIdx.x);
+    __syncthreads();
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        f32x8 r[kSteps], z[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            r[s] = residual[s].get();
+            z[s] = y[s].get();
+        }
+        if (row + gridDim.x < p.rows) fetch(row + gridDim.x);
+        float sy = 1.f;
+        if (p.post) {
+            float v[1] = {0.f};
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) v[0] += total(z[s] * z[s]);
+            meet(v, room[turn], lane, wave);
+            turn ^= 1;
+            sy = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
+        }
+        const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
         float v[1] = {0.f};
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[0] += total(y[s] * y[s]);
-        meet<kThreads, 1>(v, room[0], lane, wave);
-        sy = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
-    }
-    const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
-    float v[1] = {0.f};
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
+            if (c >= p.hidden) continue;
+            if (p.post) z[s] = z[s] * sy * load8<T>(p.post, c, p.params_f32);
+            if (p.gate_kind == kChannel) z[s] = z[s] * load8<T>(p.gate, c, p.params_f32);
+            r[s] = p.scale * r[s] + row_gate * z[s];
+            if (p.sum) store8<T>(p.sum, row * p.sum_ld + c, r[s], kF32);
+            v[0] += total(r[s] * r[s]);
+        }
+        meet(v, room[turn], lane, wave);
+        turn ^= 1;
+        const float sh = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
-        if (c >= p.hidden) continue;
-        f32x8 z = y[s];
-        if (p.post) z = z * sy * load8<T>(p.post, c, p.params_f32);
-        if (p.gate_kind == kChannel) z = z * load8<T>(p.gate, c, p.params_f32);
-        r[s] = p.scale * r[s] + row_gate * z;
-        if (p.sum) store8<T>(p.sum, row * p.sum_ld + c, r[s], p.residual_f32);
-        v[0] += total(r[s] * r[s]);
-    }
-    meet<kThreads, 1>(v, room[1], lane, wave);
-    const float sh = 1.0f / sqrtf(v[0] / static_cast<float>(p.hidden) + p.eps);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
-        if (c < p.hidden) store8<T>(p.normed, row * p.normed_ld + c, r[s] * sh * load8<T>(p.weight, c, p.params_f32), false);
-    }
-    if (p.stats && threadIdx.x == 0) {
-        p.stats[row] = sy;
-        p.stats[p.rows + row] = sh;
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
+            if (c < p.hidden) store8<T>(p.normed, row * p.normed_ld + c, r[s] * sh * load8<T>(p.weight, c, p.params_f32), false);
+        }
+        if (p.stats && threadIdx.x == 0) {
+            p.stats[row] = sy;
+            p.stats[p.rows + row] = sh;
+        }
     }
 }
 
-template <typename T, int kThreads, int kSteps>
-__global__ __launch_bounds__(kThreads) void norm_gradients_kernel(const NormArgs p) {
-    __shared__ float room[2][kThreads / 64][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The same walk; sums over rows stay in registers until the end.  Of rows that take two steps neither the parameters nor the
+// next row fit the 128 registers that 16 waves leave a thread: both are loaded where they are used.
+template <typename T, int kSteps, bool kF32>
+__global__ __launch_bounds__(1024) void norm_gradients_kernel(const NormArgs p) {
+    __shared__ float room[2][3][kMaxWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x;
+    if (threadIdx.x < 64)
+        for (int i = lane; i < 2 * 3 * kMaxWaves; i += 64) room[0][0][i] = 0.f;
     const f32x8 zero = {};
-    f32x8 by_weight[kSteps], by_post[kSteps], by_gate[kSteps];
+    constexpr bool kKeep = kSteps == 1;
+    f32x8 by_weight[kSteps], by_scale[kSteps], kept_weight, kept_pz;
+    const auto weight_at = [&](int c) { return load8<T>(p.weight, c, p.params_f32); };
+    const auto pz_at = [&](int c) {  // what z is yhat's multiple by, the row's gate apart
+        f32x8 v = zero + 1.f;
+        if (p.post) v = load8<T>(p.post, c, p.params_f32);
+        return p.gate_kind == kChannel ? v * load8<T>(p.gate, c, p.params_f32) : v;
+    };
+    Packed<T, false> y[kSteps], dn[kSteps];
+    Packed<T, kF32> residual[kSteps], dsum[kSteps];
+    const auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) by_weight[s] = by_post[s] = by_gate[s] = zero;
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
+            if (c >= p.hidden) continue;
+            residual[s].load(p.residual, row * p.residual_ld + c);
+            if (p.y) y[s].load(p.y, row * p.y_ld + c);
+            if (p.dn) dn[s].load(p.dn, row * p.dn_ld + c);
+            if (p.dsum) dsum[s].load(p.dsum, row * p.dsum_ld + c);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
+        by_weight[s] = by_scale[s] = kept_weight = kept_pz = zero;
+        residual[s] = dsum[s] = {};
+        y[s] = dn[s] = {};
+        if (!kKeep || c >= p.hidden) continue;
+        kept_weight = weight_at(c);
+        kept_pz = pz_at(c);
+    }
+    if (kKeep) fetch(blockIdx.x);
+    __syncthreads();
     const float mean = 1.0f / static_cast<float>(p.hidden);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const float sy = p.stats[row], sh = p.stats[p.rows + row];
         const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
-        // yhat (y without post), h, e sh + dsum
-        f32x8 yhat[kSteps], h[kSteps], d[kSteps];
-        float v[4] = {0.f, 0.f, 0.f, 0.f};  // e h, p yhat (dsum + sh e), p yhat h; a row's gate: z's of both
+        if (!kKeep) fetch(row);
+        f32x8 yhat[kSteps], h[kSteps], d[kSteps];  // d: dsum + sh e, dh but for the row's mean
+        float v[3] = {0.f, 0.f, 0.f};              // e h, z d, z h, without a row's gate: its gradient needs the same sums
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
             yhat[s] = h[s] = d[s] = zero;
             if (c >= p.hidden) continue;
-            if (p.y) yhat[s] = load8<T>(p.y, row * p.y_ld + c, false) * sy;
-            h[s] = load8<T>(p.residual, row * p.residual_ld + c, p.residual_f32);
-            const f32x8 dn = p.dn ? load8<T>(p.dn, row * p.dn_ld + c, false) : zero;
-            if (p.dsum) d[s] = load8<T>(p.dsum, row * p.dsum_ld + c, p.residual_f32);
-            f32x8 post = zero + 1.f, gate = zero + row_gate;
-            if (p.post) post = load8<T>(p.post, c, p.params_f32);
-            if (p.gate_kind == kChannel) gate = load8<T>(p.gate, c, p.params_f32);
-            const f32x8 z = yhat[s] * post;
-            h[s] = p.scale * h[s] + gate * z;
-            by_weight[s] += dn * (h[s] * sh);
-            const f32x8 e = dn * load8<T>(p.weight, c, p.params_f32);
-            d[s] += e * sh;
+            const f32x8 weight = kKeep ? kept_weight : weight_at(c), pz = kKeep ? kept_pz : pz_at(c);
+            yhat[s] = y[s].get() * sy;
+            const f32x8 z = yhat[s] * pz;
+            h[s] = p.scale * residual[s].get() + row_gate * z;
+            const f32x8 n = dn[s].get(), e = n * weight;
+            by_weight[s] += n * (h[s] * sh);
+            d[s] = dsum[s].get() + e * sh;
             v[0] += total(e * h[s]);
-            const f32x8 zg = p.gate_kind == kRow ? z : z * gate;  // without a row's gate: its gradient needs the same sums
-            v[1] += total(zg * d[s]);
-            v[2] += total(zg * h[s]);
+            v[1] += total(z * d[s]);
+            v[2] += total(z * h[s]);
         }
-        meet<kThreads, 4>(v, room[turn], lane, wave);
+        if (kKeep && row + gridDim.x < p.rows) fetch(row + gridDim.x);
+        meet(v, room[turn], lane, wave);
         const float back = sh * sh * sh * (v[0] * mean);
-        const float by_z = v[1] - back * v[2];  // sum of zg dh
-        const float shared = by_z * row_gate * mean;
+        const float by_z = v[1] - back * v[2];  // the sum of z dh
+        const float shared = p.post ? by_z * row_gate * mean : 0.f;
         if (p.drow && threadIdx.x == 0) {
             if (p.params_f32)
                 static_cast<float*>(p.drow)[row] = by_z;
@@ -189,58 +273,65 @@ __global__ __launch_bounds__(kThreads) void norm_gradients_kernel(const NormArgs
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+            const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
             if (c >= p.hidden) continue;
             const f32x8 dh = d[s] - h[s] * back;
-            if (p.dresidual) store8<T>(p.dresidual, row * p.dresidual_ld + c, p.scale * dh, p.residual_f32);
-            if (!p.y) continue;
-            f32x8 post = zero + 1.f, gate = zero + row_gate;
-            if (p.post) post = load8<T>(p.post, c, p.params_f32);
-            if (p.gate_kind == kChannel) gate = load8<T>(p.gate, c, p.params_f32);
-            f32x8 dy = gate * dh;
-            by_post[s] += dy * yhat[s];
-            by_gate[s] += dh * (yhat[s] * post);
-            if (p.post) dy = sy * (dy * post - yhat[s] * shared);
-            if (p.dy) store8<T>(p.dy, row * p.dy_ld + c, dy, false);
+            if (p.dresidual) store8<T>(p.dresidual, row * p.dresidual_ld + c, p.scale * dh, kF32);
+            const f32x8 dz = row_gate * dh;
+            by_scale[s] += dz * yhat[s];
+            if (p.dy) store8<T>(p.dy, row * p.dy_ld + c, sy * (dz * (kKeep ? kept_pz : pz_at(c)) - yhat[s] * shared), false);
         }
     }
-    float* to = p.partial + static_cast<int64_t>(blockIdx.x) * 3 * p.hidden;
+    float* to = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.hidden;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * kThreads + static_cast<int>(threadIdx.x)) * 8;
+        const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
         if (c >= p.hidden) continue;
         store8<T>(to, c, by_weight[s], true);
-        if (p.post) store8<T>(to, p.hidden + c, by_post[s], true);
-        if (p.gate_kind == kChannel) store8<T>(to, 2 * static_cast<int64_t>(p.hidden) + c, by_gate[s], true);
+        store8<T>(to, p.hidden + c, by_scale[s], true);
     }
 }
 
-// Adds the workgroups' sums, 32 channels a workgroup: thread (c, q) every eighth from q, then the eight in order.
+// Adds the workgroups' sums, 32 channels a workgroup: thread (c, q) every 32nd from q, then those in pairs.
 struct JoinArgs {
     const float* partial;
     int64_t groups;
     int hidden;
-    void* out[3];
+    const void *post, *gate;
+    void *dweight, *dpost, *dgate;  // any may be null
     bool f32;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void norm_join_kernel(const JoinArgs p) {
-    __shared__ float sums[8][32];
+__global__ __launch_bounds__(1024) void norm_join_kernel(const JoinArgs p) {
+    __shared__ float sums[32][33];
     const int c = threadIdx.x & 31, q = threadIdx.x >> 5, which = blockIdx.y;
     const int64_t channel = static_cast<int64_t>(blockIdx.x) * 32 + c;
-    void* const out = which == 0 ? p.out[0] : which == 1 ? p.out[1] : p.out[2];
-    if (!out) return;
     float v = 0.f;
     if (channel < p.hidden)
-        for (int64_t g = q; g < p.groups; g += 8) v += p.partial[(g * 3 + which) * p.hidden + channel];
+#pragma unroll 4
+        for (int64_t g = q; g < p.groups; g += 32) v += p.partial[(g * 2 + which) * p.hidden + channel];
     sums[q][c] = v;
     __syncthreads();
-    if (q || channel >= p.hidden) return;
-    v = ((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) + ((sums[4][c] + sums[5][c]) + (sums[6][c] + sums[7][c]));
-    if (p.f32)
-        static_cast<float*>(out)[channel] = v;
-    else
-        static_cast<T*>(out)[channel] = static_cast<T>(v);
+    // the transposed pair: thread (q, c) now holds part c of channel q
+    v = sum16(sums[c][q]);
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, static_cast<uint32_t>(rows[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(rows[1]));
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + q;
+    if (c || at >= p.hidden) return;
+    const auto put = [&](void* out, float value) {
+        if (!out) return;
+        if (p.f32)
+            static_cast<float*>(out)[at] = value;
+        else
+            static_cast<T*>(out)[at] = static_cast<T>(value);
+    };
+    if (which == 0) {
+        put(p.dweight, v);
+    } else {
+        put(p.dpost, p.gate ? load1<T>(p.gate, at, p.f32) * v : v);
+        put(p.dgate, p.post ? load1<T>(p.post, at, p.f32) * v : v);
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -248,6 +339,19 @@ int64_t gradient_groups(int64_t rows) {
     int cus = 0;
     if (current_cu_count(&cus) != kOk) cus = 256;
     return std::min<int64_t>(rows, 2 * cus);
+}
+
+// Eight channels a thread, in whole waves; over 8192 channels twice.
+unsigned row_threads(int hidden) {
+    const int each = hidden <= 8192 ? 512 : 1024;  // channels of a wave
+    return 64 * static_cast<unsigned>((hidden + each - 1) / each);
+}
+
+// Workgroups that the chip holds at a time: 32 waves a compute unit.
+int64_t row_groups(int hidden) {
+    int cus = 0;
+    if (current_cu_count(&cus) != kOk) cus = 256;
+    return static_cast<int64_t>(cus) * (2048 / row_threads(hidden));
 }
 
 int check_rows(const char* call, const void* p, int64_t ld, int64_t rows, int64_t hidden, const char* name) {
@@ -294,19 +398,24 @@ extern "C" int qsrt_residual_norm(const void* residual, int64_t residual_ld, int
     if (sum)
         if (int rc = check_rows(kCall, sum, sum_ld, rows, hidden, "sum")) return rc;
     if (int rc = check_rows(kCall, normed, normed_ld, rows, hidden, "normed")) return rc;
-    const dim3 grid(static_cast<unsigned>(rows));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, row_groups(a.hidden))));
     const auto s = static_cast<hipStream_t>(stream);
-#define QSRT_NORM(THREADS, STEPS)                                                                                \
+    const dim3 threads(row_threads(a.hidden));
+#define QSRT_NORM(STEPS, F32)                                                                                    \
     if (dtype == 0)                                                                                              \
-        hipLaunchKernelGGL((norm_kernel<__bf16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a);                 \
+        hipLaunchKernelGGL((norm_kernel<__bf16, STEPS, F32>), grid, threads, 0, s, a);                           \
     else                                                                                                         \
-        hipLaunchKernelGGL((norm_kernel<_Float16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a)
-    if (hidden <= 2048) {
-        QSRT_NORM(256, 1);
-    } else if (hidden <= 8192) {
-        QSRT_NORM(512, 2);
+        hipLaunchKernelGGL((norm_kernel<_Float16, STEPS, F32>), grid, threads, 0, s, a)
+    if (hidden <= 8192) {
+        if (a.residual_f32) {
+            QSRT_NORM(1, true);
+        } else {
+            QSRT_NORM(1, false);
+        }
+    } else if (a.residual_f32) {
+        QSRT_NORM(2, true);
     } else {
-        QSRT_NORM(512, 4);
+        QSRT_NORM(2, false);
     }
 #undef QSRT_NORM
     QSRT_HIP_TRY(hipGetLastError());
@@ -315,7 +424,7 @@ extern "C" int qsrt_residual_norm(const void* residual, int64_t residual_ld, int
 
 extern "C" size_t qsrt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t hidden) {
     if (rows <= 0 || rows > kMaxRows || hidden <= 0 || hidden > kMaxHidden || hidden % 8) return 0;
-    return sizeof(float) * 3 * static_cast<size_t>(gradient_groups(rows) * hidden);
+    return sizeof(float) * 2 * static_cast<size_t>(gradient_groups(rows) * hidden);
 }
 
 extern "C" int qsrt_residual_norm_backward(const void* dsum, int64_t dsum_ld, const void* dn, int64_t dn_ld, const void* residual,
@@ -350,27 +459,34 @@ extern "C" int qsrt_residual_norm_backward(const void* dsum, int64_t dsum_ld, co
     const int64_t groups = gradient_groups(rows);
     const dim3 grid(static_cast<unsigned>(groups));
     const auto s = static_cast<hipStream_t>(stream);
-#define QSRT_NORM(THREADS, STEPS)                                                                                \
+    const dim3 threads(row_threads(a.hidden));
+#define QSRT_NORM(STEPS, F32)                                                                                    \
     if (dtype == 0)                                                                                              \
-        hipLaunchKernelGGL((norm_gradients_kernel<__bf16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a);       \
+        hipLaunchKernelGGL((norm_gradients_kernel<__bf16, STEPS, F32>), grid, threads, 0, s, a);                 \
     else                                                                                                         \
-        hipLaunchKernelGGL((norm_gradients_kernel<_Float16, THREADS, STEPS>), grid, dim3(THREADS), 0, s, a)
-    if (hidden <= 4096) {
-        QSRT_NORM(512, 1);
-    } else if (hidden <= 8192) {
-        QSRT_NORM(512, 2);
+        hipLaunchKernelGGL((norm_gradients_kernel<_Float16, STEPS, F32>), grid, threads, 0, s, a)
+    if (hidden <= 8192) {
+        if (a.residual_f32) {
+            QSRT_NORM(1, true);
+        } else {
+            QSRT_NORM(1, false);
+        }
+    } else if (a.residual_f32) {
+        QSRT_NORM(2, true);
     } else {
-        QSRT_NORM(1024, 2);
+        QSRT_NORM(2, false);
     }
 #undef QSRT_NORM
     QSRT_HIP_TRY(hipGetLastError());
-    const JoinArgs j{a.partial, groups, a.hidden, {dweight, dpost, gate_kind == kChannel ? dgate : nullptr}, a.params_f32};
-    if (!j.out[0] && !j.out[1] && !j.out[2]) return kOk;
-    const dim3 columns(static_cast<unsigned>((hidden + 31) / 32), 3);
+    const bool channels = gate_kind == kChannel;
+    const JoinArgs j{a.partial, groups, a.hidden, post, channels ? gate : nullptr, dweight, dpost, channels ? dgate : nullptr,
+                     a.params_f32};
+    if (!j.dweight && !j.dpost && !j.dgate) return kOk;
+    const dim3 columns(static_cast<unsigned>((hidden + 31) / 32), 2);
     if (dtype == 0)
-        hipLaunchKernelGGL(norm_join_kernel<__bf16>, columns, dim3(256), 0, s, j);
+        hipLaunchKernelGGL(norm_join_kernel<__bf16>, columns, dim3(1024), 0, s, j);
     else
-        hipLaunchKernelGGL(norm_join_kernel<_Float16>, columns, dim3(256), 0, s, j);
+        hipLaunchKernelGGL(norm_join_kernel<_Float16>, columns, dim3(1024), 0, s, j);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
