@@ -355,29 +355,31 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
         return rb.read(at + LoaderA::kBytes + (j < kHalf ? 0 : LoaderB::kBytes), wn + 16 * (j % kHalf), kk);
     };
 
+    const auto after = [](uint32_t at) { return at + kStageBytes == kStages * kStageBytes ? 0 : at + kStageBytes; };
+
     enter();
     if constexpr (kI >= 4) {
         // A stage is 2 kI steps of kJ products: fragment i of a by all of b.  Before a step's products go the reads of what
         // is used kI steps later (a's fragments in place of those just used, b's in turn), from the middle of the second
         // half on those of the next stage: then every wave has read all of this one, the next has landed, and its buffer
         // takes the stage after that.  One wait and barrier a stage, with products before and behind it.
-        static_assert(kStages == 2, "two stages");
         vec8<T> a[kI], b[2][kJ];
-        load();
-        if (begin + 1 < end) {
-            load();
-            wait_and_meet<kStageLoads>();
-        } else {
+#pragma unroll
+        for (int s = 0; s < kStages; ++s)
+            if (begin + s < end) load();
+        if (begin + kStages <= end)
+            wait_and_meet<kStageLoads*(kStages - 1)>();
+        else
             wait_and_meet<0>();
-        }
 #pragma unroll
         for (int j = 0; j < kJ; ++j) b[0][j] = read_b(lds, j, 0);
 #pragma unroll
         for (int i = 0; i < kI; ++i) a[i] = read_a(lds, i, 0);
         uint32_t now = 0;
         for (int s = begin; s < end; ++s) {
-            const char *at = lds + now, *next = lds + (now ^ kStageBytes);
-            const bool more = s + 2 < end;
+            const uint32_t then = after(now);
+            const char *at = lds + now, *next = lds + then;
+            const bool more = s + kStages < end;
 #pragma unroll
             for (int i = 0; i < kI; ++i) {
                 if (i > 0) a[i - 1] = read_a(at, i - 1, 1);
@@ -404,13 +406,16 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 if (i == 1) {
-                    wait_and_meet<0>();
+                    if (kStages > 2 && s + kStages - 1 < end)  // what is on its way behind the next stage may stay so
+                        wait_and_meet<kStageLoads*(kStages - 2)>();
+                    else
+                        wait_and_meet<0>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (more) loaded();
             a[kI - 1] = read_a(next, kI - 1, 0);
-            now ^= kStageBytes;
+            now = then;
         }
     } else {
         uint32_t now = 0;
@@ -425,7 +430,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
                 wait_and_meet<0>();
             if (s + kStages - 1 < end) load();
             const char* at = lds + now;
-            now = now + kStageBytes == kStages * kStageBytes ? 0 : now + kStageBytes;
+            now = after(now);
             vec8<T> a[2][kI], b[2][kJ];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
@@ -447,11 +452,29 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
 #pragma unroll
     for (int i = 0; i < kI; ++i) {
         const int64_t row = row0 + 16 * i;
+        if (kEnding == kStore && args.parts == 1) {
+            // Two tiles' columns exchanged between neighbouring groups of 16 lanes: a lane then stores eight in a row of one.
+            const int odd = lane >> 4 & 1;
+            const int64_t col = n0 + wn + 8 * (lane >> 5) + 16 * odd;
+#pragma unroll
+            for (int j = 0; j + 1 < kJ; j += 2) {
+                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                const u32x2 a = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j], vec4<T>));
+                const u32x2 b = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j + 1], vec4<T>));
+                const auto low = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+                const auto high = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+                const u32x4 v = {low[0], high[0], low[1], high[1]};
+                if (row < p.m && col + 16 * j < p.n)  // n is a multiple of 8
+                    *reinterpret_cast<u32x4*>(static_cast<T*>(p.finish.out) + row * p.finish.ld + col + 16 * j) = v;
+            }
+            continue;
+        }
         if (row >= p.m) continue;
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) {
             const int64_t col = col0 + 16 * j;
-            if (col >= p.n) continue;  // n is a multiple of 8
+            if (col >= p.n) continue;
             if (args.parts > 1) {
                 float* to = args.partial + (part * (kDual ? 2 : 1) * p.m + row) * p.n + col;
                 *reinterpret_cast<f32x4*>(to) = acc[i][j];
@@ -470,17 +493,104 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
     if (at >= m * n) return;
     f32x4 sum[2] = {};
-    for (int q = 0; q < parts; ++q)
+    const int64_t plane = m * n;
+    int q = 0;
+    // eight parts' loads go out together: few columns leave nothing else to hide them behind
+    for (; q + 8 <= parts; q += 8) {
+        f32x4 v[8][kPlanes];
 #pragma unroll
-        for (int h = 0; h < kPlanes; ++h) sum[h] += *reinterpret_cast<const f32x4*>(partial + (q * kPlanes + h) * m * n + at);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int h = 0; h < kPlanes; ++h) v[i][h] = *reinterpret_cast<const f32x4*>(partial + ((q + i) * kPlanes + h) * plane + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int h = 0; h < kPlanes; ++h) sum[h] += v[i][h];
+    }
+    for (; q < parts; ++q)
+#pragma unroll
+        for (int h = 0; h < kPlanes; ++h) sum[h] += *reinterpret_cast<const f32x4*>(partial + (q * kPlanes + h) * plane + at);
     finish<T, kEnding>(f, at / n, at % n, sum[0], sum[1]);
 }
 
-// ---------------------------------------------------------------- host
-struct Shape {
-    int m, n, threads, stages, resident;  // of a tile; workgroups that a CU holds
+// ---------------------------------------------------------------- a few rows
+// Up to 64 rows of activations by a matrix whose rows lie with the summed index innermost: bound by reading the matrix once.
+// A workgroup takes 16 of its rows (kActivate: eight of gate and the same eight of up), its waves a part of the sum each,
+// weights straight to registers in the matrix instruction's order, kBatch loads of 64 bytes a row at a time; the parts are
+// added in LDS, in wave order, so there is no second kernel.
+struct RowsArgs {
+    const void* a[2];  // rows of activations, in pieces
+    int pieces;
+    const void *b, *b2;
+    int64_t lda, ldb;
+    int m, n, k;
+    Finish finish;
 };
-constexpr Shape kShapes[] = {{256, 256, 512, 2, 1}, {128, 128, 256, 2, 2}, {32, 128, 256, 4, 2}};
+
+template <typename T, Ending kEnding, int kTiles, int kWaves, int kBatch>
+__global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowsArgs p) {
+    static_assert(kTiles <= kWaves, "a wave adds up a tile");
+    __shared__ f32x4 sums[kWaves][kTiles][64];
+    constexpr bool kDual = kEnding == kActivate;
+    constexpr int kPieces = kDual ? 1 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * (kDual ? 8 : 16);
+    // rows past the end repeat the last; not stored
+    const T* weights = kDual ? static_cast<const T*>(r < 8 ? p.b : p.b2) + (n0 + (r & 7)) * p.ldb
+                             : static_cast<const T*>(p.b) + min(n0 + r, p.n - 1) * p.ldb;
+    int64_t row[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) row[i] = min(16 * i + r, p.m - 1) * p.lda;
+    const int steps = (p.k + 31) / 32, begin = steps * wave / kWaves, end = steps * (wave + 1) / kWaves;
+    const vec8<T> zero = {};
+    f32x4 acc[kTiles] = {};
+    for (int s = begin; s < end; s += kBatch) {
+        vec8<T> w[kBatch], x[kPieces][kTiles][kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int at = min((s + j) * 32 + 8 * g, p.k - 8);  // past the end: the last, set to zero below
+            w[j] = *reinterpret_cast<const vec8<T>*>(weights + at);
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+                    x[q][i][j] = *reinterpret_cast<const vec8<T>*>(static_cast<const T*>(p.a[q]) + row[i] + at);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const bool in = s + j < end && (s + j) * 32 + 8 * g < p.k;
+            w[j] = in ? w[j] : zero;
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) acc[i] = multiply<T>(w[j], in ? x[q][i][j] : zero, acc[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= kTiles) return;
+    f32x4 sum = sums[0][wave][lane];
+#pragma unroll
+    for (int q = 1; q < kWaves; ++q) sum += sums[q][wave][lane];
+    f32x4 up = sum;
+    if constexpr (kDual)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) up[q] = __shfl_xor(sum[q], 32);
+    const int t = 16 * wave + r, col = n0 + 4 * g;
+    if (t < p.m && col < p.n && !(kDual && g >= 2)) finish<T, kEnding>(p.finish, t, col, sum, up);
+}
+
+// ---------------------------------------------------------------- host
+// The tiles, and what one takes on MI355X in microseconds: before and behind the sum, and for each stage of 64 while the chip
+// is full (fits to 128 .. 4096 rows of 5120 x 1536 and 7168 x 2048).  A tile of 256 x 256 has two stages in LDS, one of 128 x
+// 256 three, one of 128 x 128 five: the smaller it is, the more a stage's loads count, which take 1.4 us to land.
+struct Shape {
+    int m, n, resident;  // rows, columns; workgroups that a compute unit holds
+    float fixed, stage;
+};
+enum { kSquare, kWide, kSmall, kFlat, kFewRows };
+constexpr Shape kShapes[] = {{256, 256, 1, 6.f, 1.66f}, {128, 256, 1, 4.f, 1.15f}, {128, 128, 1, 3.f, 0.68f}, {32, 128, 2, 3.f, 0.7f}};
 
 struct Cut {
     int shape, parts;
@@ -491,15 +601,30 @@ int64_t tiles_of(const Shape& s, int64_t m, int64_t n, bool dual) {
     return (m + s.m - 1) / s.m * ((n + nb - 1) / nb);
 }
 
-Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, bool whole) {
+// The tile, and the parts that the sum is cut into, with the least time to expect; `products` of this size go together and
+// are not cut.  Parts cost their sums' way to memory and back and a launch.
+Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
     int cus = 0;
     if (current_cu_count(&cus) != kOk) cus = 256;
-    int shape = m <= 32 && !whole ? 2 : 1;
-    if (m > 32 && tiles_of(kShapes[0], m, n, dual) * 2 >= cus) shape = 0;
-    const int64_t tiles = tiles_of(kShapes[shape], m, n, dual), slots = static_cast<int64_t>(cus) * kShapes[shape].resident;
     const int64_t stages = (k + kDepth - 1) / kDepth * sums;
-    int64_t parts = whole ? 1 : std::min(slots / tiles, stages / 4);
-    return {shape, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(parts, 32)))};
+    Cut best{kSquare, 1};
+    float least = 0.f;
+    for (int i = kSquare; i <= kFlat; ++i) {
+        const Shape& s = kShapes[i];
+        if ((i == kFlat) != (m <= 32 && products == 1)) continue;
+        const int64_t tiles = tiles_of(s, m, n, dual) * products, slots = static_cast<int64_t>(cus) * s.resident;
+        const int64_t most = products > 1 ? 1 : std::min<int64_t>(32, stages / 2);
+        for (int64_t parts = 1; parts == 1 || (parts <= most && tiles * parts <= slots); ++parts) {
+            float time = static_cast<float>((tiles * parts + slots - 1) / slots) *
+                         (s.fixed + s.stage * static_cast<float>((stages + parts - 1) / parts));
+            if (parts > 1) time += 3.f + static_cast<float>(parts * (dual ? 2 : 1) * m * n) * 8.f / 4.6e6f;
+            if (least == 0.f || time < least) {
+                least = time;
+                best = {i, static_cast<int>(parts)};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T, Layout kA, Layout kB, Ending kEnding>
@@ -519,10 +644,12 @@ int launch_shape(const TileArgs& args, int shape, int64_t blocks, hipStream_t st
         }                                                                                                             \
         hipLaunchKernelGGL(kernel, grid, dim3(64 * WM * WN), bytes, stream, args);                                    \
     }
-    if (shape == 0)
+    if (shape == kSquare)
         QSRT_TILE(256, 256, 2, 4, 2)
-    else if (shape == 1)
-        QSRT_TILE(128, 128, 2, 2, 2)
+    else if (shape == kWide)
+        QSRT_TILE(128, 256, 2, 4, 3)
+    else if (shape == kSmall)
+        QSRT_TILE(128, 128, 2, 4, 5)
     else
         QSRT_TILE(32, 128, 1, 4, 4)
 #undef QSRT_TILE
@@ -530,8 +657,35 @@ int launch_shape(const TileArgs& args, int shape, int64_t blocks, hipStream_t st
     return kOk;
 }
 
+template <typename T, Ending kEnding, int kTiles, int kBatch>
+void launch_rows(const RowsArgs& r, hipStream_t stream) {
+    constexpr bool kDual = kEnding == kActivate;
+    constexpr int kMost = kTiles > 1 ? 8 : kDual ? 16 : 8, kFewer = kDual ? 8 : 4;
+    const dim3 grid(static_cast<unsigned>((r.n + (kDual ? 7 : 15)) / (kDual ? 8 : 16)));
+    if (r.k > 4096)
+        hipLaunchKernelGGL((rows_kernel<T, kEnding, kTiles, kMost, kBatch>), grid, dim3(64 * kMost), 0, stream, r);
+    else
+        hipLaunchKernelGGL((rows_kernel<T, kEnding, kTiles, kFewer, kBatch>), grid, dim3(64 * kFewer), 0, stream, r);
+}
+
+template <typename T, Ending kEnding>
+int run_rows(const Product& p, hipStream_t stream) {
+    const RowsArgs r{{p.a[0], p.a[1]}, p.sums, p.b[0], p.b2, p.lda, p.ldb, static_cast<int>(p.m), static_cast<int>(p.n),
+                     static_cast<int>(p.k), p.finish};
+    if (p.m <= 16)
+        launch_rows<T, kEnding, 1, kEnding == kActivate ? 7 : 16>(r, stream);
+    else if (p.m <= 32)
+        launch_rows<T, kEnding, 2, 8>(r, stream);
+    else
+        launch_rows<T, kEnding, 4, 4>(r, stream);
+    QSRT_HIP_TRY(hipGetLastError());
+    return kOk;
+}
+
 template <typename T, Layout kA, Layout kB, Ending kEnding>
 int run(TileArgs& args, Cut c, hipStream_t stream) {
+    if constexpr (kB == kRows)
+        if (c.shape == kFewRows) return run_rows<T, kEnding>(args.product[0], stream);
     const Shape& s = kShapes[c.shape];
     int64_t blocks = 0;
     for (int i = 0; i < args.products; ++i) {
@@ -576,8 +730,9 @@ struct Forward {
 Forward plan_forward(int64_t tokens, int64_t hidden, int64_t inter) {
     Forward f;
     f.pieces = pieces_of(tokens);
-    f.up = cut(tokens, inter, hidden, 1, true, false);
-    f.down = cut(tokens, hidden, inter, f.pieces, false, false);
+    const Cut few{kFewRows, 1};
+    f.up = tokens <= 8 ? few : cut(tokens, inter, hidden, 1, true, 1);
+    f.down = tokens <= 8 ? few : cut(tokens, hidden, inter, f.pieces, false, 1);
     f.middle = round_up(sizeof(uint16_t) * f.pieces * tokens * inter);
     f.partial = std::max(part_bytes(f.up, tokens, inter, 2), part_bytes(f.down, tokens, hidden, 1));
     f.bytes = f.middle + f.partial;
@@ -592,9 +747,9 @@ struct Backward {
 Backward plan_backward(int64_t tokens, int64_t hidden, int64_t inter) {
     Backward b;
     b.pieces = pieces_of(tokens);
-    b.middle = cut(tokens, inter, hidden, 1, false, false);
-    b.x = cut(tokens, hidden, inter, 2 * b.pieces, false, false);
-    b.weights = cut(inter, hidden, tokens, b.pieces, false, true);
+    b.middle = cut(tokens, inter, hidden, 1, false, 1);
+    b.x = cut(tokens, hidden, inter, 2 * b.pieces, false, 1);
+    b.weights = cut(inter, hidden, tokens, b.pieces, false, 3);
     b.rows = round_up(sizeof(uint16_t) * b.pieces * tokens * inter);
     b.partial = std::max(part_bytes(b.middle, tokens, inter, 1), part_bytes(b.x, tokens, hidden, 1));
     b.bytes = 3 * b.rows + b.partial;
