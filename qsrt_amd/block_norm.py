@@ -19,7 +19,8 @@ _NONE, _CHANNEL, _ROW = range(3)
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with 16-byte aligned rows (copied where they are not)."""
 
-    if t.stride(1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+    apart, step = t.stride()
+    if step != 1 or t.data_ptr() % 16 or ((apart % 8 or apart < t.shape[1]) and t.shape[0] > 1):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -27,8 +28,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _vector(v: torch.Tensor | None) -> torch.Tensor | None:
     if v is None:
         return None
-    v = v.contiguous()
-    return v.clone() if v.data_ptr() % 16 else v
+    return v.clone(memory_format=torch.contiguous_format) if v.data_ptr() % 16 or not v.is_contiguous() else v
 
 
 def _checked(residual, y, weight, post, gate, dtype, eps):

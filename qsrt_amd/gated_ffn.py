@@ -22,7 +22,8 @@ MAX_CHANNELS = 1 << 17
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with 16-byte aligned rows (copied where they are not)."""
 
-    if t.stride(1) != 1 or t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(0) < t.shape[1]:
+    apart, step = t.stride()
+    if step != 1 or t.data_ptr() % 16 or apart % 8 or apart < t.shape[1]:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -30,25 +31,22 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _checked(x, gate, up, down, activation):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
-    if gate.dim() != 2 or up.shape != gate.shape or down.shape != (gate.shape[1], gate.shape[0]):
+    shape, dtype, device = gate.shape, gate.dtype, gate.device
+    if len(shape) != 2 or up.shape != shape or down.shape != shape[::-1]:
         raise ValueError("gate and up must be [inter, hidden] and down [hidden, inter]")
-    if gate.dtype not in TYPES or not gate.is_cuda:
+    if dtype not in TYPES or device.type != "cuda":
         raise ValueError("the weights must be bfloat16 or float16 on a CUDA device")
-    if any(w.dtype != gate.dtype or w.device != gate.device for w in (up, down)):
+    if up.dtype != dtype or down.dtype != dtype or up.device != device or down.device != device:
         raise ValueError("the weights must be of one type and on one device")
-    inter, hidden = gate.shape
+    inter, hidden = shape
     if not 0 < hidden <= MAX_CHANNELS or not 0 < inter <= MAX_CHANNELS or hidden % 8 or inter % 8:
         raise ValueError(f"hidden and inter must be multiples of 8 up to {MAX_CHANNELS}")
-    if x.device != gate.device or x.dtype != gate.dtype:
+    if x.dtype != dtype or x.device != device:
         raise ValueError("x must be of the weights' type and on their device")
-    return checked_rows(x, hidden, gate.device), *_checked_weights(gate, up, down)
-
-
-def _checked_weights(gate, up, down):
-    gate, up, down = _rows(gate), _rows(up), _rows(down)
+    x, gate, up, down = checked_rows(x, hidden, device), _rows(gate), _rows(up), _rows(down)
     if gate.stride(0) != up.stride(0):  # one leading dimension serves both
         gate, up = gate.contiguous(), up.contiguous()
-    return gate, up, down
+    return x, gate, up, down
 
 
 def _forward(x, gate, up, down, activation, out, pre):
@@ -85,7 +83,7 @@ def _backward(dy, x, gate, up, down, activation, pre, dx, weights, rows):
 
 
 def _like(t: torch.Tensor, needed: bool = True) -> torch.Tensor | None:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device) if needed else None
+    return torch.empty_like(t, memory_format=torch.contiguous_format) if needed else None
 
 
 class _GatedFFN(torch.autograd.Function):
