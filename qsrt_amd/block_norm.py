@@ -9,7 +9,7 @@ import math
 import torch
 
 from . import _native
-from .packed_linear import TYPES
+from .packed_linear import TYPES, refuse_second_derivatives
 
 MAX_CHANNELS = 1 << 14
 MAX_ROWS = 1 << 22
@@ -99,8 +99,8 @@ class _ResidualNorm(torch.autograd.Function):
         return total, normed
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dsum, dn):
+        refuse_second_derivatives()
         residual, y, weight, post, gate, stats = ctx.saved_tensors
         t, hidden = residual.shape
         if dsum is None and dn is None:
@@ -142,14 +142,14 @@ def residual_norm(residual: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
 
     ``y [T, hidden]``, a block's result, and ``n``, the next block's input, are bf16 or f16; ``residual`` and ``h`` float32 or
     of that type.  ``weight`` and ``post_weight [hidden]`` and ``gate`` (``[hidden]``, or ``[T, 1]``: each row its own) are all
-    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors."""
+    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors, once."""
 
     return _run(residual, y, weight, post_weight, gate, float(scale), float(eps), y.dtype, True)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, dtype: torch.dtype | None = None) -> torch.Tensor:
     """``weight * x / rms(x)``, what stands before the first block.  ``x [T, hidden]`` bf16, f16, or float32 with the result's
-    ``dtype`` (bf16 or f16) named.  Differentiable in both."""
+    ``dtype`` (bf16 or f16) named.  Differentiable in both, once."""
 
     return _run(x, None, weight, None, None, 1.0, float(eps), x.dtype if dtype is None else dtype, False)[1]
 

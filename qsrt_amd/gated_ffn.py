@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .packed_linear import TYPES, checked_out, checked_rows
+from .packed_linear import TYPES, checked_out, checked_rows, refuse_second_derivatives
 
 ACTIVATIONS = {"swiglu": 0, "situ": 1}
 MAX_CHANNELS = 1 << 17
@@ -99,8 +99,8 @@ class _GatedFFN(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_second_derivatives()
         x, gate, up, down, pre = ctx.saved_tensors
         grads = [_like(t, needed) for t, needed in zip((x, gate, up, down), ctx.needs_input_grad)]
         if x.shape[0]:
@@ -119,7 +119,7 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
 
     ``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]``, all bf16 or all f16, hidden and inter
     multiples of 8.  ``activation``: ``"swiglu"`` (``silu(g) u``) or ``"situ"``.  Sums are FP32; the rows between the two
-    products are held in ``x``'s type (f16 ends at 65504), of 64 rows or less as two values each.  Differentiable in all four;
+    products are held in ``x``'s type (f16 ends at 65504), of 64 rows or less as two values each.  Differentiable in all four, once;
     the backward pass keeps the rows before the activation in FP32 (``8 T inter`` bytes).  ``out``: where the result goes, of a
     call without gradients."""
 

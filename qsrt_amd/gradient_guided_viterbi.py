@@ -19,6 +19,8 @@ from dataclasses import dataclass
 
 import torch
 
+from .gated_ffn import gated_ffn_gradients
+
 
 def _check_strength(strength: float) -> None:
     if not math.isfinite(float(strength)) or float(strength) < 0.0:
@@ -114,6 +116,24 @@ class LowRankViterbiGradientGuidance:
         return float(self.strength) * float(torch.sum((left.T @ delta) * right))
 
 
+def expert_guidance(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *,
+                    anchor_id: str, objective_id: str, strength: float = 1.0,
+                    activation: str = "situ") -> dict[str, LowRankViterbiGradientGuidance]:
+    """Guidance for the three matrices of an expert from its routed rows ``x [T, hidden]`` and the objective's gradients of
+    its output ``dy [T, hidden]`` (both bf16 or f16, on the GPU): ``{"w1", "w3", "w2"}`` in the encoder's ``[K, N]``
+    orientation, their gradients held as the rows that they are products of.  ``gate``, ``up [inter, hidden]`` and ``down
+    [hidden, inter]`` are the reconstruction that the gradients belong to, and the anchor.  ``dy`` carries the route weights."""
+
+    _check_strength(strength)
+    _check_identities(anchor_id, objective_id)
+    g = gated_ffn_gradients(x, dy, gate, up, down, activation=activation, inputs=False, weights=False)
+
+    def low_rank(left, right, anchor):
+        return LowRankViterbiGradientGuidance(left.T.float(), right.float(), anchor.T.float(), anchor_id, objective_id, strength)
+
+    return {"w1": low_rank(x, g.gate_rows, gate), "w3": low_rank(x, g.up_rows, up), "w2": low_rank(g.middle, dy, down)}
+
+
 def shift_elementwise_target(target: torch.Tensor, gradient: torch.Tensor, *, strength: float,
                              quadratic_weight=1.0) -> torch.Tensor:
     """Target with the same minimiser under ``a (q - target')^2`` as
@@ -175,6 +195,7 @@ def two_sided_guided_objective(target: torch.Tensor, candidate: torch.Tensor, an
 __all__ = [
     "LowRankViterbiGradientGuidance",
     "ViterbiGradientGuidance",
+    "expert_guidance",
     "shift_elementwise_target",
     "shift_two_sided_target",
     "two_sided_guided_objective",

@@ -49,6 +49,13 @@ def refuse_gradients(*tensors) -> None:
             raise ValueError("packed products have no backward pass: call them under torch.no_grad() or detach their inputs")
 
 
+def refuse_second_derivatives() -> None:
+    """For a backward pass that is not differentiable itself: better no gradient than one that a graph silently stops at."""
+
+    if torch.is_grad_enabled():  # create_graph=True
+        raise RuntimeError("there are no second derivatives here: call the backward pass without create_graph")
+
+
 def _aligned(t: torch.Tensor, size: int) -> torch.Tensor:
     """``t`` in one piece at a multiple of ``size`` bytes, copied where it is not."""
 
