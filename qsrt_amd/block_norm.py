@@ -105,7 +105,7 @@ class _ResidualNorm(torch.autograd.Function):
         t, hidden = residual.shape
         if dsum is None and dn is None:
             return (None,) * 10
-        grads = [torch.empty(v.shape, dtype=v.dtype, device=v.device) if needed else None
+        grads = [torch.empty_like(v, memory_format=torch.contiguous_format) if needed else None
                  for v, needed in zip((residual, y, weight, post, gate), ctx.needs_input_grad)]
         if t == 0:
             return *(None if g is None else g.zero_() for g in grads), *(None,) * 5

@@ -7,6 +7,7 @@
 // Every product is a `tile_kernel`: sums of products of two operands that each lie with the summed index innermost
 // (kRows) or outermost (kCols), so no operand is ever transposed in memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "qsrt_amd.h"
@@ -137,12 +138,24 @@ struct TileArgs {
     float* partial;
 };
 
+// f of every number from kFrom on, before kTo, as a constant.
+template <int kFrom, int kTo, typename F>
+__device__ __forceinline__ void count(const F& f) {
+    if constexpr (kFrom < kTo) {
+        f(std::integral_constant<int, kFrom>{});
+        count<kFrom + 1, kTo>(f);
+    }
+}
+
 // 16 bytes a lane from a buffer straight to LDS: lane l's go to `lds` + 16 l.  Written in assembly because the compiler,
 // which cannot see that a stage is written while another is read, waits for all of them before any read from LDS.  Nothing
 // comes back in registers; `wait_and_meet` is the wait.
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(lds)
-                 : "memory");
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int kAt>
+__device__ __forceinline__ void to_lds(u32x4 from, uint32_t offset, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(lds),
+                 "n"(kAt)
+                 : "memory", "scc");
 }
 
 // All but the wave's last `kLeft` loads have landed, its reads from LDS are done, and so are the other waves'.
@@ -183,30 +196,46 @@ struct Loader {
         }
     }
 
-    // The wave's q-th load of a stage from `from`, of which `depth` summed indices are left.
-    __device__ __forceinline__ void load(int q, __amdgpu_buffer_rsrc_t from, int depth, uint32_t lds, int wave) const {
+    // The wave's q-th load of a stage from `from`, of which `depth` summed indices are left, to kAt behind `lds` (its place of
+    // the wave's first load).
+    template <int kAt, int q>
+    __device__ __forceinline__ void load(u32x4 from, int depth, uint32_t lds) const {
         const bool past = kLayout == kRows && 8 * chunk >= depth;
-        to_lds(from, past ? kNowhere : offset[q], lds + (q * kWaves + wave) * 1024);
+        to_lds<kAt + q * kWaves * 1024>(from, past ? kNowhere : offset[q], lds);
     }
 };
 
-// Where an operand's next stage lies: a buffer that ends with the last of its values, so that reads past the tile's end of
-// either index are zero or feed results that are not stored.
+// Where an operand's next stage lies: a buffer resource that ends with the last of its values, so that reads past the tile's
+// end of either index are zero or feed results that are not stored.  Kept as the instruction takes it: a small tile's stage is
+// short enough for scalar instructions to count.
 template <Layout kLayout>
 struct Feed {
-    const char* p;
+    u32x4 buffer;
     uint32_t ld, span;  // bytes between rows; kRows: in the tile's rows but the last, kCols: of a row
     __device__ __forceinline__ void init(int64_t stride, int64_t size, int tile) {
         ld = static_cast<uint32_t>(stride) * 2;
         const uint32_t n = static_cast<uint32_t>(min(size, static_cast<int64_t>(tile)));
         span = kLayout == kRows ? (n - 1) * ld : n * 2;
+        buffer[3] = 0x00020000;
     }
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int depth) const {
-        const uint32_t k = static_cast<uint32_t>(min(depth, kDepth));
-        const uint32_t bytes = kLayout == kRows ? span + 2 * k : (k - 1) * ld + span;
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, 0x00020000);
+    __device__ __forceinline__ void end(int depth) {  // nothing at depth 0 and below
+        const int bytes = kLayout == kRows ? static_cast<int>(span) + 2 * depth
+                                           : (min(depth, kDepth) - 1) * static_cast<int>(ld) + static_cast<int>(span);
+        buffer[2] = static_cast<uint32_t>(max(bytes, 0));
     }
-    __device__ __forceinline__ void advance() { p += kLayout == kRows ? 2 * kDepth : static_cast<int64_t>(ld) * kDepth; }
+    __device__ __forceinline__ void enter(const char* p, int depth) {
+        const uint64_t at = reinterpret_cast<uint64_t>(p);
+        buffer[0] = static_cast<uint32_t>(at);
+        buffer[1] = static_cast<uint32_t>(at >> 32);
+        end(depth);
+    }
+    __device__ __forceinline__ void advance(int depth) {
+        const uint64_t at = (static_cast<uint64_t>(buffer[1]) << 32 | buffer[0]) +
+                            (kLayout == kRows ? 2 * kDepth : static_cast<uint64_t>(ld) * kDepth);
+        buffer[0] = static_cast<uint32_t>(at);
+        buffer[1] = static_cast<uint32_t>(at >> 32);
+        end(depth);
+    }
 };
 
 // The lane's part of a 16 x 32 fragment: index lane % 16, eight summed indices from 8 (lane / 16).
@@ -293,54 +322,61 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     ra.init(lane);
     rb.init(lane);
 
-    // the stage to be loaded next
+    // The stage to be loaded next.  Neighbouring tiles walk the sum from stages of their own, around its end: rows whose
+    // distance has a high power of two would come from the same few channels of the L2 in every workgroup at once (4096 rows of
+    // 7168 x 2048 with gradients: 972 us from the first stage, 961 so).  Behind the last stage come empty ones, so that what
+    // is on its way is always the same number of loads.
     Feed<kA> fa;
     Feed<kB> fb, fb2;
     fa.init(p.lda, p.m - m0, kM);
     fb.init(p.ldb, p.n - n0, kNb);
     if constexpr (kDual) fb2 = fb;
-    // Neighbouring tiles walk the sum from stages of their own, around its end: rows whose distance has a high power of two
-    // would come from the same few channels of the L2 in every workgroup at once (4096 rows of 7168 x 2048 with gradients: 972
-    // us from the first stage, 961 so).
-    int coming = begin + tile % 8 % (end - begin);
-    int sum = coming / per, depth = k - (coming - sum * per) * kDepth;
+    int coming = begin + tile % 8 % (end - begin), remaining = end - begin, run = 0, left, sum, depth;
     uint32_t to = 0;
     const auto enter = [&]() {  // the operands of `sum`, `depth` before their end
         const int64_t k0 = k - depth;
         const int64_t at = kB == kRows ? n0 * p.ldb + k0 : k0 * p.ldb + n0;
-        fa.p = static_cast<const char*>(p.a[sum]) + 2 * (kA == kRows ? m0 * p.lda + k0 : k0 * p.lda + m0);
-        fb.p = static_cast<const char*>(p.b[sum]) + 2 * at;
-        if constexpr (kDual) fb2.p = static_cast<const char*>(p.b2) + 2 * at;
+        fa.enter(static_cast<const char*>(p.a[sum]) + 2 * (kA == kRows ? m0 * p.lda + k0 : k0 * p.lda + m0), depth);
+        fb.enter(static_cast<const char*>(p.b[sum]) + 2 * at, depth);
+        if constexpr (kDual) fb2.enter(static_cast<const char*>(p.b2) + 2 * at, depth);
     };
-    const auto load_one = [&](int q) {  // of the wave's loads of a stage
-        if (q < LoaderA::kLoads)
-            la.load(q, fa.buffer(depth), depth, to, wave);
-        else if (q < LoaderA::kLoads + LoaderB::kLoads)
-            lb.load(q - LoaderA::kLoads, fb.buffer(depth), depth, to + LoaderA::kBytes, wave);
+    const uint32_t own = 1024 * static_cast<uint32_t>(wave);
+    const auto load_one = [&](auto number) {  // of the wave's loads of a stage
+        constexpr int q = decltype(number)::value, qb = q - LoaderA::kLoads, qb2 = qb - LoaderB::kLoads;
+        if constexpr (qb < 0)
+            la.template load<0, q>(fa.buffer, depth, to + own);
+        else if constexpr (qb2 < 0)
+            lb.template load<LoaderA::kBytes, qb>(fb.buffer, depth, to + own);
         else
-            lb.load(q - LoaderA::kLoads - LoaderB::kLoads, fb2.buffer(depth), depth, to + LoaderA::kBytes + LoaderB::kBytes, wave);
+            lb.template load<LoaderA::kBytes + LoaderB::kBytes, qb2>(fb2.buffer, depth, to + own);
+    };
+    const auto enter_run = [&]() {  // stages of one sum, one behind another
+        remaining -= run;
+        coming += run;
+        if (remaining == 0) {
+            depth = 0;
+            fa.end(0);
+            fb.end(0);
+            if constexpr (kDual) fb2.end(0);
+            left = 1 << 30;
+            return;
+        }
+        if (coming == end) coming = begin;
+        sum = coming / per;
+        depth = k - (coming - sum * per) * kDepth;
+        left = run = min(min(per * (sum + 1), end) - coming, remaining);
+        enter();
     };
     const auto loaded = [&]() {
         to = to + kStageBytes == kStages * kStageBytes ? 0 : to + kStageBytes;
         depth -= kDepth;
-        if (++coming == end) {
-            coming = begin;
-            sum = coming / per;
-            depth = k - (coming - sum * per) * kDepth;
-            enter();
-        } else if (depth > 0) {
-            fa.advance();
-            fb.advance();
-            if constexpr (kDual) fb2.advance();
-        } else {
-            ++sum;
-            depth = k;
-            enter();
-        }
+        fa.advance(depth);
+        fb.advance(depth);
+        if constexpr (kDual) fb2.advance(depth);
+        if (--left == 0) enter_run();
     };
     const auto load = [&]() {
-#pragma unroll
-        for (int q = 0; q < kStageLoads; ++q) load_one(q);
+        count<0, kStageLoads>(load_one);
         loaded();
     };
 
@@ -357,29 +393,23 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
 
     const auto after = [](uint32_t at) { return at + kStageBytes == kStages * kStageBytes ? 0 : at + kStageBytes; };
 
-    enter();
+    enter_run();
+    uint32_t now = 0;
     if constexpr (kI >= 4) {
         // A stage is 2 kI steps of kJ products: fragment i of a by all of b.  Before a step's products go the reads of what
         // is used kI steps later (a's fragments in place of those just used, b's in turn), from the middle of the second
         // half on those of the next stage: then every wave has read all of this one, the next has landed, and its buffer
-        // takes the stage after that.  One wait and barrier a stage, with products before and behind it.
+        // takes the one kStages on.  One wait and barrier a stage, with products before and behind it.
         vec8<T> a[kI], b[2][kJ];
 #pragma unroll
-        for (int s = 0; s < kStages; ++s)
-            if (begin + s < end) load();
-        if (begin + kStages <= end)
-            wait_and_meet<kStageLoads*(kStages - 1)>();
-        else
-            wait_and_meet<0>();
+        for (int s = 0; s < kStages; ++s) load();
+        wait_and_meet<kStageLoads*(kStages - 1)>();
 #pragma unroll
         for (int j = 0; j < kJ; ++j) b[0][j] = read_b(lds, j, 0);
 #pragma unroll
         for (int i = 0; i < kI; ++i) a[i] = read_a(lds, i, 0);
-        uint32_t now = 0;
         for (int s = begin; s < end; ++s) {
-            const uint32_t then = after(now);
-            const char *at = lds + now, *next = lds + then;
-            const bool more = s + kStages < end;
+            const char *at = lds + now, *next = lds + (now = after(now));
 #pragma unroll
             for (int i = 0; i < kI; ++i) {
                 if (i > 0) a[i - 1] = read_a(at, i - 1, 1);
@@ -389,8 +419,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
                 for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[0][j], a[i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int i = 0; i < kI; ++i) {
+            count<0, kI>([&](auto step) {
+                constexpr int i = decltype(step)::value;
                 if (i == 0) a[kI - 1] = read_a(at, kI - 1, 1);
                 if (i >= 2) {
                     if (i == 2) a[0] = read_a(next, 0, 0);
@@ -400,35 +430,23 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
                 }
 #pragma unroll
                 for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[1][j], a[i], acc[i][j]);
-                if (i >= 2 && more) {
-#pragma unroll
-                    for (int q = (i - 2) * kStageLoads / (kI - 2); q < (i - 1) * kStageLoads / (kI - 2); ++q) load_one(q);
-                }
+                if constexpr (i >= 2) count<(i - 2) * kStageLoads / (kI - 2), (i - 1) * kStageLoads / (kI - 2)>(load_one);
                 __builtin_amdgcn_sched_barrier(0);
-                if (i == 1) {
-                    if (kStages > 2 && s + kStages - 1 < end)  // what is on its way behind the next stage may stay so
-                        wait_and_meet<kStageLoads*(kStages - 2)>();
-                    else
-                        wait_and_meet<0>();
+                if constexpr (i == 1) {
+                    wait_and_meet<kStageLoads*(kStages - 2)>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-            if (more) loaded();
+            });
+            loaded();
             a[kI - 1] = read_a(next, kI - 1, 0);
-            now = then;
         }
     } else {
-        uint32_t now = 0;
+        // few rows: bound by reading b, with a stage on its way less
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s)
-            if (begin + s < end) load();
+        for (int s = 0; s < kStages - 1; ++s) load();
         for (int s = begin; s < end; ++s) {
-            // of what is on its way, the stages behind s may stay so
-            if (kStages > 2 && s + kStages - 2 < end)
-                wait_and_meet<kStageLoads*(kStages - 2)>();
-            else
-                wait_and_meet<0>();
-            if (s + kStages - 1 < end) load();
+            wait_and_meet<kStageLoads*(kStages - 2)>();  // this stage has landed, the one before has been read
+            load();
             const char* at = lds + now;
             now = after(now);
             vec8<T> a[2][kI], b[2][kJ];
@@ -447,6 +465,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
                     for (int j = 0; j < kJ; ++j) acc[i][j] = multiply<T>(b[kk][j], a[kk][i], acc[i][j]);
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
     const int64_t row0 = m0 + wm + (lane & 15), col0 = n0 + wn + 4 * (lane >> 4);
 #pragma unroll
