@@ -131,12 +131,15 @@ struct Product {
 };
 
 constexpr int kProducts = 3;
+template <int kMost>
 struct TileArgs {
-    Product product[kProducts];
+    Product product[kMost];
     int products;
     int parts;       // of the summed axis; > 1: sums go to `partial` [part][1 or 2][m][n]
     float* partial;
 };
+template <Layout kA>
+using ArgsOf = TileArgs<kA == kCols ? kProducts : 1>;  // the weights' gradients go together
 
 // f of every number from kFrom on, before kTo, as a constant.
 template <int kFrom, int kTo, typename F>
@@ -279,7 +282,7 @@ __device__ __forceinline__ int xcd_slot(int q, int n) {
 // kWavesN waves, kStages stages in LDS.  The first operand of the matrix instruction is b: a lane then holds four
 // neighbouring columns of one row.
 template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
-__global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const TileArgs args) {
+__global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const ArgsOf<kA> args) {
     constexpr int kWaves = kWavesM * kWavesN;
     constexpr bool kDual = kEnding == kActivate;
     constexpr int kNb = kDual ? kN / 2 : kN;  // of one matrix of b
@@ -292,13 +295,15 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     int tile = xcd_slot(blockIdx.x, gridDim.x), which = 0, part = 0;
-    for (; which + 1 < args.products; ++which) {
-        const int tiles = args.product[which].tiles_m * args.product[which].tiles_n;
-        if (tile < tiles) break;
-        tile -= tiles;
-    }
-    const Product& p = args.product[which];
-    if (args.parts > 1) {
+    const int parts = args.parts;
+    if constexpr (kA == kCols)
+        for (; which + 1 < args.products; ++which) {
+            const int tiles = args.product[which].tiles_m * args.product[which].tiles_n;
+            if (tile < tiles) break;
+            tile -= tiles;
+        }
+    const Product& p = args.product[kA == kCols ? which : 0];
+    if (parts > 1) {
         const int tiles = p.tiles_m * p.tiles_n;
         part = tile / tiles;
         tile %= tiles;
@@ -310,8 +315,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
     const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % high) * kM, n0 = static_cast<int64_t>(in_band / high) * kNb;
 
     const int k = static_cast<int>(p.k), per = (k + kDepth - 1) / kDepth, stages = per * p.sums;
-    const int begin = static_cast<int>(static_cast<int64_t>(stages) * part / args.parts);
-    const int end = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / args.parts);
+    const int begin = static_cast<int>(static_cast<int64_t>(stages) * part / parts);
+    const int end = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / parts);
 
     LoaderA la;
     LoaderB lb;
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
 #pragma unroll
     for (int i = 0; i < kI; ++i) {
         const int64_t row = row0 + 16 * i;
-        if (kEnding == kStore && args.parts == 1) {
+        if (kEnding == kStore && parts == 1) {
             // Two tiles' columns exchanged between neighbouring groups of 16 lanes: a lane then stores eight in a row of one.
             const int odd = lane >> 4 & 1;
             const int64_t col = n0 + wn + 8 * (lane >> 5) + 16 * odd;
@@ -494,7 +499,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Tile
         for (int j = 0; j < kHalf; ++j) {
             const int64_t col = col0 + 16 * j;
             if (col >= p.n) continue;
-            if (args.parts > 1) {
+            if (parts > 1) {
                 float* to = args.partial + (part * (kDual ? 2 : 1) * p.m + row) * p.n + col;
                 *reinterpret_cast<f32x4*>(to) = acc[i][j];
                 if constexpr (kDual) *reinterpret_cast<f32x4*>(to + p.m * p.n) = acc[i][kHalf + j];
@@ -647,7 +652,7 @@ Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
 }
 
 template <typename T, Layout kA, Layout kB, Ending kEnding>
-int launch_shape(const TileArgs& args, int shape, int64_t blocks, hipStream_t stream) {
+int launch_shape(const ArgsOf<kA>& args, int shape, int64_t blocks, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(blocks));
 #define QSRT_TILE(M, N, WM, WN, STAGES)                                                                               \
     {                                                                                                                 \
@@ -702,7 +707,7 @@ int run_rows(const Product& p, hipStream_t stream) {
 }
 
 template <typename T, Layout kA, Layout kB, Ending kEnding>
-int run(TileArgs& args, Cut c, hipStream_t stream) {
+int run(ArgsOf<kA>& args, Cut c, hipStream_t stream) {
     if constexpr (kB == kRows)
         if (c.shape == kFewRows) return run_rows<T, kEnding>(args.product[0], stream);
     const Shape& s = kShapes[c.shape];
@@ -824,7 +829,7 @@ void add_sums(Product& p, const Pieces& a, const void* b) {
 
 template <typename T>
 int forward(const Block& b, float* pre, const Matrix& out, char* ws, const Forward& f, hipStream_t stream) {
-    TileArgs args = {};
+    TileArgs<1> args = {};
     args.products = 1;
     args.partial = reinterpret_cast<float*>(ws + f.middle);
     Product& p = args.product[0];
@@ -861,7 +866,7 @@ struct Gradients {
 
 template <typename T>
 int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan, hipStream_t stream) {
-    TileArgs args = {};
+    TileArgs<1> args = {};
     args.products = 1;
     args.partial = reinterpret_cast<float*>(ws + 3 * plan.rows);
     Pieces dg = pieces_at(ws, b.tokens, b.inter, plan.pieces), du = pieces_at(ws + plan.rows, b.tokens, b.inter, plan.pieces),
@@ -895,10 +900,10 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
         p.finish = {const_cast<void*>(g.dx.p), g.dx.apart()};
         if (int rc = run<T, kRows, kCols, kStore>(args, plan.x, stream)) return rc;
     }
-    args.products = 0;
+    TileArgs<kProducts> three = {};
     const auto add = [&](const Pieces& rows, const Matrix& other, void* out, bool rows_first) {
         if (!out) return;
-        Product& p = args.product[args.products++];
+        Product& p = three.product[three.products++];
         p = {};
         add_sums(p, rows, other.p);
         p.lda = b.inter;
@@ -916,7 +921,7 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
     add(dg, b.x, g.gate, true);
     add(du, b.x, g.up, true);
     add(middle, g.dy, g.down, false);
-    return args.products ? run<T, kCols, kCols, kStore>(args, plan.weights, stream) : kOk;
+    return three.products ? run<T, kCols, kCols, kStore>(three, plan.weights, stream) : kOk;
 }
 
 }  // namespace
