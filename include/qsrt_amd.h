@@ -561,6 +561,14 @@ int qsrt_gated_ffn_backward(const void *dy, int64_t dy_ld, const void *x, int64_
                             size_t ws_bytes, void *stream);
 
 /*
+ * Which kernels calls of these sizes take: for gate and up's product, down's,
+ * dM, dx and the weights' gradients the tile (0: 256 x 256, 1: 128 x 256, 2:
+ * 128 x 128, 3: 32 x 128, 4: a few whole rows) and the parts that the sum is
+ * cut into, then the pieces of a row between products: 11 values.
+ */
+int qsrt_gated_ffn_plan(int64_t tokens, int64_t hidden, int64_t inter, int64_t *plan);
+
+/*
  * What stands between two blocks, a row of [rows, hidden] at a time:
  *   z = post y / sqrt(mean y^2 + eps)   (post NULL: z = y)
  *   sum = scale residual + gate z       (y NULL: scale residual)

@@ -153,6 +153,7 @@ SIGNATURES: dict[str, tuple] = {
          _c_int, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
          _c_size, _c_void_p],
     ),
+    "qsrt_gated_ffn_plan": (_c_int, [_c_i64, _c_i64, _c_i64, _c_void_p]),
     "qsrt_residual_norm": (
         _c_int,
         [_c_void_p, _c_i64, _c_int, _c_void_p, _c_i64, _c_int, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,

@@ -7,6 +7,7 @@
 // Every product is a `tile_kernel`: sums of products of two operands that each lie with the summed index innermost
 // (kRows) or outermost (kCols), so no operand is ever transposed in memory.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     int tile = xcd_slot(blockIdx.x, gridDim.x), which = 0, part = 0;
-    const int parts = args.parts;
+    const int parts = kA == kCols ? 1 : args.parts;  // the weights' gradients are not cut
     if constexpr (kA == kCols)
         for (; which + 1 < args.products; ++which) {
             const int tiles = args.product[which].tiles_m * args.product[which].tiles_n;
@@ -483,7 +484,6 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
 #pragma unroll
             for (int j = 0; j + 1 < kJ; j += 2) {
                 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
                 const u32x2 a = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j], vec4<T>));
                 const u32x2 b = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j + 1], vec4<T>));
                 const auto low = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
@@ -538,23 +538,26 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 }
 
 // ---------------------------------------------------------------- a few rows
-// Up to 64 rows of activations by a matrix whose rows lie with the summed index innermost: bound by reading the matrix once.
+// Up to 16 rows of activations by a matrix whose rows lie with the summed index innermost: bound by reading the matrix once.
 // A workgroup takes 16 of its rows (kActivate: eight of gate and the same eight of up), its waves a part of the sum each,
-// weights straight to registers in the matrix instruction's order, kBatch loads of 64 bytes a row at a time; the parts are
-// added in LDS, in wave order, so there is no second kernel.
+// weights straight to registers in the matrix instruction's order, the next kAhead steps of 32 always on their way; the parts
+// are added in LDS, in wave order, so there is no second kernel.
+//
+// 7168 x 2048, one row: both products in 21.5 us, 4.1 TB/s of weights (a large copy moves 4.6).  Eight waves a workgroup for
+// gate and up, whose workgroups are fewer, four for down, four steps ahead (waves, steps of the one, then the other; us at 1
+// row of 7168 x 2048, 5120 x 1536, 2048 x 1024): 8, 4, 4, 4: 21.5, 15.9, 8.7; 8, 4, 8, 4: 22.0, 17.3, 8.5; 8, 7, 4, 6: 24.2,
+// 17.9, 11.0; 16, 4, 8, 4: 23.0, 18.9, 8.7.  More steps ahead leave fewer waves room and reach past the end of short sums.
 struct RowsArgs {
-    const void* a[2];  // rows of activations, in pieces
-    int pieces;
+    const void* a[2];  // rows of activations; kStore: in two pieces
     const void *b, *b2;
     int64_t lda, ldb;
     int m, n, k;
     Finish finish;
 };
 
-template <typename T, Ending kEnding, int kTiles, int kWaves, int kBatch>
+template <typename T, Ending kEnding, int kWaves, int kAhead>
 __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowsArgs p) {
-    static_assert(kTiles <= kWaves, "a wave adds up a tile");
-    __shared__ f32x4 sums[kWaves][kTiles][64];
+    __shared__ f32x4 sums[kWaves][64];
     constexpr bool kDual = kEnding == kActivate;
     constexpr int kPieces = kDual ? 1 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -562,47 +565,48 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowsArgs p) {
     // rows past the end repeat the last; not stored
     const T* weights = kDual ? static_cast<const T*>(r < 8 ? p.b : p.b2) + (n0 + (r & 7)) * p.ldb
                              : static_cast<const T*>(p.b) + min(n0 + r, p.n - 1) * p.ldb;
-    int64_t row[kTiles];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) row[i] = min(16 * i + r, p.m - 1) * p.lda;
+    const int64_t row = min(r, p.m - 1) * p.lda;
     const int steps = (p.k + 31) / 32, begin = steps * wave / kWaves, end = steps * (wave + 1) / kWaves;
-    const vec8<T> zero = {};
-    f32x4 acc[kTiles] = {};
-    for (int s = begin; s < end; s += kBatch) {
-        vec8<T> w[kBatch], x[kPieces][kTiles][kBatch];
+    f32x4 acc = {};
+    vec8<T> w[kAhead], x[kPieces][kAhead];
+    const auto fetch = [&](int j, int step) {
+        const int at = min(step * 32 + 8 * g, p.k - 8);
+        w[j] = *reinterpret_cast<const vec8<T>*>(weights + at);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int at = min((s + j) * 32 + 8 * g, p.k - 8);  // past the end: the last, set to zero below
-            w[j] = *reinterpret_cast<const vec8<T>*>(weights + at);
+        for (int q = 0; q < kPieces; ++q) x[q][j] = *reinterpret_cast<const vec8<T>*>(static_cast<const T*>(p.a[q]) + row + at);
+    };
+    if (begin < end) {
 #pragma unroll
-            for (int q = 0; q < kPieces; ++q)
+        for (int j = 0; j < kAhead; ++j) fetch(j, min(begin + j, end - 1));
+        int s = begin;
+        for (; s + kAhead < end; s += kAhead)
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i)
-                    x[q][i][j] = *reinterpret_cast<const vec8<T>*>(static_cast<const T*>(p.a[q]) + row[i] + at);
-        }
+            for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+                for (int q = 0; q < kPieces; ++q) acc = multiply<T>(w[j], x[q][j], acc);
+                fetch(j, min(s + kAhead + j, end - 1));
+            }
+        const vec8<T> zero = {};
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
             const bool in = s + j < end && (s + j) * 32 + 8 * g < p.k;
             w[j] = in ? w[j] : zero;
 #pragma unroll
-            for (int q = 0; q < kPieces; ++q)
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) acc[i] = multiply<T>(w[j], in ? x[q][i][j] : zero, acc[i]);
+            for (int q = 0; q < kPieces; ++q) acc = multiply<T>(w[j], in ? x[q][j] : zero, acc);
         }
     }
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) sums[wave][i][lane] = acc[i];
+    sums[wave][lane] = acc;
     __syncthreads();
-    if (wave >= kTiles) return;
-    f32x4 sum = sums[0][wave][lane];
+    if (wave > 0) return;
+    f32x4 sum = sums[0][lane];
 #pragma unroll
-    for (int q = 1; q < kWaves; ++q) sum += sums[q][wave][lane];
+    for (int q = 1; q < kWaves; ++q) sum += sums[q][lane];
     f32x4 up = sum;
     if constexpr (kDual)
 #pragma unroll
         for (int q = 0; q < 4; ++q) up[q] = __shfl_xor(sum[q], 32);
-    const int t = 16 * wave + r, col = n0 + 4 * g;
-    if (t < p.m && col < p.n && !(kDual && g >= 2)) finish<T, kEnding>(p.finish, t, col, sum, up);
+    const int col = n0 + 4 * g;
+    if (r < p.m && col < p.n && !(kDual && g >= 2)) finish<T, kEnding>(p.finish, r, col, sum, up);
 }
 
 // ---------------------------------------------------------------- host
@@ -651,64 +655,47 @@ Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
     return best;
 }
 
-template <typename T, Layout kA, Layout kB, Ending kEnding>
-int launch_shape(const ArgsOf<kA>& args, int shape, int64_t blocks, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(blocks));
-#define QSRT_TILE(M, N, WM, WN, STAGES)                                                                               \
-    {                                                                                                                 \
-        auto* kernel = tile_kernel<T, kA, kB, kEnding, M, N, WM, WN, STAGES>;                                         \
-        constexpr int bytes = STAGES * (M + N) * kDepth * 2;                                                          \
-        static bool raised[64] = {};                                                                                  \
-        int dev = 0;                                                                                                  \
-        QSRT_HIP_TRY(hipGetDevice(&dev));                                                                             \
-        if (dev >= 64 || !raised[dev]) {                                                                              \
-            QSRT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),                                   \
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes));                     \
-            if (dev < 64) raised[dev] = true;                                                                         \
-        }                                                                                                             \
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * WM * WN), bytes, stream, args);                                    \
+template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
+int launch_tiles(const ArgsOf<kA>& args, int64_t blocks, hipStream_t stream) {
+    auto* kernel = tile_kernel<T, kA, kB, kEnding, kM, kN, kWavesM, kWavesN, kStages>;
+    constexpr int kBytes = kStages * (kM + kN) * kDepth * 2;
+    static std::atomic<uint64_t> raised{0};  // devices on which the kernel has been given its LDS
+    int dev = 0;
+    QSRT_HIP_TRY(hipGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (!(raised.load(std::memory_order_relaxed) & bit)) {
+        QSRT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+        raised.fetch_or(bit, std::memory_order_relaxed);
     }
-    if (shape == kSquare)
-        QSRT_TILE(256, 256, 2, 4, 2)
-    else if (shape == kWide)
-        QSRT_TILE(128, 256, 2, 4, 3)
-    else if (shape == kSmall)
-        QSRT_TILE(128, 128, 2, 4, 5)
-    else
-        QSRT_TILE(32, 128, 1, 4, 4)
-#undef QSRT_TILE
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWavesM * kWavesN), kBytes, stream, args);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
 
-template <typename T, Ending kEnding, int kTiles, int kBatch>
-void launch_rows(const RowsArgs& r, hipStream_t stream) {
-    constexpr bool kDual = kEnding == kActivate;
-    constexpr int kMost = kTiles > 1 ? 8 : kDual ? 16 : 8, kFewer = kDual ? 8 : 4;
-    const dim3 grid(static_cast<unsigned>((r.n + (kDual ? 7 : 15)) / (kDual ? 8 : 16)));
-    if (r.k > 4096)
-        hipLaunchKernelGGL((rows_kernel<T, kEnding, kTiles, kMost, kBatch>), grid, dim3(64 * kMost), 0, stream, r);
-    else
-        hipLaunchKernelGGL((rows_kernel<T, kEnding, kTiles, kFewer, kBatch>), grid, dim3(64 * kFewer), 0, stream, r);
+template <typename T, Layout kA, Layout kB, Ending kEnding>
+int launch_shape(const ArgsOf<kA>& args, int shape, int64_t blocks, hipStream_t stream) {
+    if constexpr (kA == kRows)  // the weights' gradients go together
+        if (shape == kFlat) return launch_tiles<T, kA, kB, kEnding, 32, 128, 1, 4, 4>(args, blocks, stream);
+    if (shape == kSquare) return launch_tiles<T, kA, kB, kEnding, 256, 256, 2, 4, 2>(args, blocks, stream);
+    if (shape == kWide) return launch_tiles<T, kA, kB, kEnding, 128, 256, 2, 4, 3>(args, blocks, stream);
+    return launch_tiles<T, kA, kB, kEnding, 128, 128, 2, 4, 5>(args, blocks, stream);
 }
 
 template <typename T, Ending kEnding>
 int run_rows(const Product& p, hipStream_t stream) {
-    const RowsArgs r{{p.a[0], p.a[1]}, p.sums, p.b[0], p.b2, p.lda, p.ldb, static_cast<int>(p.m), static_cast<int>(p.n),
+    constexpr bool kDual = kEnding == kActivate;
+    const RowsArgs r{{p.a[0], p.a[1]}, p.b[0], p.b2, p.lda, p.ldb, static_cast<int>(p.m), static_cast<int>(p.n),
                      static_cast<int>(p.k), p.finish};
-    if (p.m <= 16)
-        launch_rows<T, kEnding, 1, kEnding == kActivate ? 7 : 16>(r, stream);
-    else if (p.m <= 32)
-        launch_rows<T, kEnding, 2, 8>(r, stream);
-    else
-        launch_rows<T, kEnding, 4, 4>(r, stream);
+    constexpr int kWaves = kDual ? 8 : 4, kColumns = kDual ? 8 : 16;
+    const dim3 grid(static_cast<unsigned>((r.n + kColumns - 1) / kColumns));
+    hipLaunchKernelGGL((rows_kernel<T, kEnding, kWaves, 4>), grid, dim3(64 * kWaves), 0, stream, r);
     QSRT_HIP_TRY(hipGetLastError());
     return kOk;
 }
 
 template <typename T, Layout kA, Layout kB, Ending kEnding>
 int run(ArgsOf<kA>& args, Cut c, hipStream_t stream) {
-    if constexpr (kB == kRows)
+    if constexpr (kA == kRows && kB == kRows)
         if (c.shape == kFewRows) return run_rows<T, kEnding>(args.product[0], stream);
     const Shape& s = kShapes[c.shape];
     int64_t blocks = 0;
@@ -721,9 +708,9 @@ int run(ArgsOf<kA>& args, Cut c, hipStream_t stream) {
     }
     args.parts = c.parts;
     blocks *= c.parts;
-    if (blocks > 1 << 30) return fail(kBadArgument, "too many tiles for one launch");
+    if (blocks >= 1 << 23) return fail(kBadArgument, "qsrt_gated_ffn: too many tiles for one launch");  // of 512 threads, 2^32 in all
     if (int rc = launch_shape<T, kA, kB, kEnding>(args, c.shape, blocks, stream)) return rc;
-    if (c.parts > 1) {
+    if (kA == kRows && c.parts > 1) {
         const Product& p = args.product[0];
         hipLaunchKernelGGL((join_kernel<T, kEnding>), dim3(static_cast<unsigned>((p.m * p.n / 4 + 255) / 256)), dim3(256), 0,
                            stream, args.partial, c.parts, p.m, p.n, p.finish);
@@ -741,6 +728,11 @@ bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
 
 int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
 
+// Up to 16 rows, one side of a matrix instruction, meet a kernel of their own.  Against tiles with parts, in us at 8, 12 and 16
+// rows: 2048 x 1024 10.0, 10.6, 11.3 for 16.9, 17.2, 17.8; 5120 x 1536 21, 23.6, 26.7 for 27.3, 27.6, 28.0; 7168 x 2048 27,
+// 30.5, 33.7 for 32.3, 32.6, 33.2.  With 17 to 32 the rows of activations would be read twice as often as the weights.
+bool few_rows(int64_t tokens) { return tokens <= 16; }
+
 size_t round_up(size_t n) { return (n + 255) & ~size_t{255}; }
 size_t part_bytes(const Cut& c, int64_t m, int64_t n, int planes) {
     return c.parts > 1 ? round_up(sizeof(float) * c.parts * planes * m * n) : 0;
@@ -755,8 +747,8 @@ Forward plan_forward(int64_t tokens, int64_t hidden, int64_t inter) {
     Forward f;
     f.pieces = pieces_of(tokens);
     const Cut few{kFewRows, 1};
-    f.up = tokens <= 8 ? few : cut(tokens, inter, hidden, 1, true, 1);
-    f.down = tokens <= 8 ? few : cut(tokens, hidden, inter, f.pieces, false, 1);
+    f.up = few_rows(tokens) ? few : cut(tokens, inter, hidden, 1, true, 1);
+    f.down = few_rows(tokens) ? few : cut(tokens, hidden, inter, f.pieces, false, 1);
     f.middle = round_up(sizeof(uint16_t) * f.pieces * tokens * inter);
     f.partial = std::max(part_bytes(f.up, tokens, inter, 2), part_bytes(f.down, tokens, hidden, 1));
     f.bytes = f.middle + f.partial;
@@ -979,4 +971,17 @@ extern "C" int qsrt_gated_ffn_backward(const void* dy, int64_t dy_ld, const void
     const Backward plan = plan_backward(tokens, hidden, inter);
     if (int rc = check_workspace(kCall, ws, ws_bytes, plan.bytes)) return rc;
     return (dtype == 0 ? backward<__bf16> : backward<_Float16>)(b, g, static_cast<char*>(ws), plan, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int qsrt_gated_ffn_plan(int64_t tokens, int64_t hidden, int64_t inter, int64_t* plan) {
+    constexpr const char* kCall = "qsrt_gated_ffn_plan";
+    if (tokens == 0 || !sizes_fit(tokens, hidden, inter) || !plan) return fail(kBadArgument, "%s: bad sizes or no plan", kCall);
+    const Forward f = plan_forward(tokens, hidden, inter);
+    const Backward b = plan_backward(tokens, hidden, inter);
+    for (const Cut& c : {f.up, f.down, b.middle, b.x, b.weights}) {
+        *plan++ = c.shape;
+        *plan++ = c.parts;
+    }
+    *plan = f.pieces;
+    return kOk;
 }

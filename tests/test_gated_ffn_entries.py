@@ -154,3 +154,10 @@ def test_python_calls_refuse_shapes_before_anything_else():
     for bad in ((w, w[:4], d), (w, w, d.T), (w[0], w[0], d)):
         with pytest.raises(ValueError, match="inter, hidden"):
             gated_ffn(x, *bad)
+
+
+@native
+@pytest.mark.parametrize("t,hidden,inter", [(0, 64, 64), (-1, 64, 64), (1, 60, 64), (1, 64, 1 << 18)])
+def test_plan_refuses(t, hidden, inter):
+    refused(_native.lib().qsrt_gated_ffn_plan(t, hidden, inter, (ctypes.c_int64 * 11)()), "sizes")
+    refused(_native.lib().qsrt_gated_ffn_plan(1, 64, 64, None), "plan")
