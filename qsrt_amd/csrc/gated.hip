@@ -55,7 +55,7 @@ __device__ __forceinline__ void activate_with_slopes(float g, float u, int activ
 enum Ending { kStore, kActivate, kSlopes };
 
 // A row between two products goes on in 16 bits, as the matrix cores take it: rounded once, or as two pieces (the nearest
-// 16-bit value and the nearest of what is left).
+// 16-bit value and the nearest of what is left; `pieces_of` says when).
 struct Pieces {
     void *hi, *lo;  // lo null: one
 };
@@ -282,6 +282,13 @@ __device__ __forceinline__ int xcd_slot(int q, int n) {
 // One tile of kM rows (of a) by kN columns (of b; with kActivate half of them of b, half of b2) a workgroup of kWavesM x
 // kWavesN waves, kStages stages in LDS.  The first operand of the matrix instruction is b: a lane then holds four
 // neighbouring columns of one row.
+//
+// Many rows are bound by the operands' way from L2 to LDS, with the matrix cores close behind: a stage of a 256 x 256 tile
+// brings 64 KB to each compute unit in 1.66 us, 10 TB/s on the chip, 79% of it out of L2.  4096 rows of 7168 x 2048 take 187 to
+// 202 us for gate and up (1.2 to 1.3 PFLOP/s; 164 with the loads alone, 148 with the products and their reads from LDS alone,
+// at 1.8 GHz), 110 for down, 104 for dM, 196 for dx, 313 for the weights' gradients.  64 deep: stages of 32 in rings of four or
+// five cost 10%, having twice the barriers.  Eight waves of 128 x 64: four of 128 x 128 have nobody to load while they wait
+// (25% slower), 32 x 32 x 16 instructions 5%.
 template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const ArgsOf<kA> args) {
     constexpr int kWaves = kWavesM * kWavesN;
@@ -510,7 +517,9 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
     }
 }
 
-// Adds the parts up, in their order, four columns a thread.
+// Adds the parts up, in their order, four columns a thread.  Bound by memory (dM of 4096 rows of 2048 in two parts, with G and
+// U read and three rows written: 184 MB in 31 us), of few rows by its launch and two round trips (45 rows of 1536, ten parts:
+// 4.2).
 template <typename T, Ending kEnding>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int parts, int64_t m, int64_t n, const Finish f) {
     constexpr int kPlanes = kEnding == kActivate ? 2 : 1;
@@ -726,6 +735,9 @@ bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
            hidden % 8 == 0 && inter % 8 == 0;
 }
 
+// Up to 64 rows, where reading the weights bounds a product, rows between products go on in two pieces: the result is then
+// off by its own rounding alone.  In one, it is off by 1.4 times as much (two roundings of one size); in two, 64 rows of 7168 x
+// 2048 take 39.4 us, not 35.5, 32 of 5120 x 1536 31.1, not 28.9, and 500 rows 89 us, not 73.
 int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
 
 // Up to 16 rows, one side of a matrix instruction, meet a kernel of their own.  Against tiles with parts, in us at 8, 12 and 16
