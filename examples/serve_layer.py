@@ -1,4 +1,7 @@
-"""Serve tokens through a packed layer: a projection with low-rank adapters, then a router and its experts.
+"""Serve tokens through a packed layer.
+
+A norm, a projection with low-rank adapters, a router and its experts beside a shared expert in dense weights, then the
+residual and the next layer's norm.
 
     python examples/serve_layer.py [--file qsrt-layer-00024.safetensors] [--tokens 4] [--steps 64]
 
@@ -21,7 +24,9 @@ if __package__ in (None, ""):
 import torch
 
 from qsrt_amd import exl3_encoder_backend as backend
+from qsrt_amd.block_norm import residual_norm, rms_norm
 from qsrt_amd.decode import DecodePlan, decode_words
+from qsrt_amd.gated_ffn import gated_ffn
 from qsrt_amd.ldlq import make_shared_h
 from qsrt_amd.packed_linear import LowRankAdapters, PackedLinear, adapter_linear
 from qsrt_amd.packed_moe import PackedExperts, PackedMoELayer
@@ -135,39 +140,57 @@ def main(argv=None) -> dict:
     adapters = LowRankAdapters(rand(3, 16, hidden) * hidden**-0.5, rand(3, hidden, 16) * 0.25)
     ids = (torch.arange(args.tokens, dtype=torch.int32) % 4 - 1).to(device)  # every fourth token has no adapter
     layer = PackedMoELayer(rand(experts, hidden) * hidden**-0.5, packed, min(args.k, experts), scoring="sigmoid")
-    x = rand(args.tokens, hidden)
+    inter = packed.inter
+    shared = [rand(inter, hidden) * hidden**-0.5, rand(inter, hidden) * hidden**-0.5, rand(hidden, inter) * inter**-0.5]
+    stream, first, last = rand(args.tokens, hidden).float(), 1 + 0.1 * rand(hidden).float(), 1 + 0.1 * rand(hidden).float()
 
     def step():
+        x = rms_norm(stream, first, dtype=torch.bfloat16)
         h = adapter_linear(x, linear, adapters, ids)
         y, weights, chosen = layer(h)
-        return h, y, weights, chosen
+        beside = gated_ffn(h, *shared, activation=args.activation)
+        return x, h, y, weights, chosen, beside, *residual_norm(stream, y + beside, last)
 
-    h, y, weights, chosen = step()
+    def act(g, u):
+        return situ(g, u) if args.activation == "situ" else torch.nn.functional.silu(g) * u
+
+    def normed(v, weight):
+        return weight * v * (v.square().mean(1, keepdim=True) + 1e-6).rsqrt()
+
+    def off(got, want):
+        return float((got.float() - want).norm() / want.norm())
+
+    x, h, y, weights, chosen, beside, after, following = step()
+    errors = {"norm": off(x, normed(stream, first))}
     want = x.float() @ dense
     for i, a in enumerate(ids.tolist()):
         if a >= 0:
             want[i] += (x[i].float() @ adapters.a[a].float().T) @ adapters.b[a].float().T
-    errors = {"projection": float((h.float() - want).norm() / want.norm())}
+    errors["projection"] = off(h, want)
     matrices, want = decoded(payloads, schedule, coupled, device), torch.zeros((args.tokens, hidden), device=device)
     for i in range(args.tokens):
         for w, e in zip(weights[i].tolist(), chosen[i].tolist()):
             g, u = h[i].float() @ matrices[e]["w1"], h[i].float() @ matrices[e]["w3"]
-            middle = situ(g, u) if args.activation == "situ" else torch.nn.functional.silu(g) * u
-            want[i] += w * (middle @ matrices[e]["w2"])
-    errors["layer"] = float((y.float() - want).norm() / want.norm())
+            want[i] += w * (act(g, u) @ matrices[e]["w2"])
+    errors["layer"] = off(y, want)
+    gate, up, down = (w.float() for w in shared)
+    errors["shared expert"] = off(beside, act(h.float() @ gate.T, h.float() @ up.T) @ down.T)
+    want = stream + y.float() + beside.float()
+    errors["residual"] = off(after, want)
+    errors["next norm"] = off(following, normed(want, last))
     del matrices
 
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        h, y, weights, chosen = step()
+        step()
     graph.replay()
     torch.cuda.synchronize()
     start = time.perf_counter()
     for _ in range(args.steps):
         graph.replay()
     torch.cuda.synchronize()
-    result = {"experts": experts, "hidden": hidden, "inter": packed.inter, "tokens": args.tokens, "errors": errors,
+    result = {"experts": experts, "hidden": hidden, "inter": inter, "tokens": args.tokens, "errors": errors,
               "us_per_step": (time.perf_counter() - start) / args.steps * 1e6}
     print(result, flush=True)
     return result

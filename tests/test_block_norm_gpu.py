@@ -83,7 +83,8 @@ def call(v, dsum, dn, scale):
     return {"h": h.detach(), "n": n.detach()} | {"d" + k: g for k, g in zip(leaf, grads)}
 
 
-SIZES = [(1, 8), (1, 7168), (3, 2048), (7, 2056), (300, 520), (513, 4104), (33, 8200), (5, 16384), (1100, 5120)]
+SIZES = [(1, 8), (1, 7168), (3, 2048), (7, 2056), (300, 520), (513, 4104), (33, 8200), (5, 16384), (1100, 5120),
+         (8200, 264)]
 
 
 @pytest.mark.parametrize("gate", ["none", "channel", "row"])
