@@ -61,6 +61,10 @@ def _checked(residual, y, weight, post, gate, dtype, eps):
     return kind
 
 
+def _like(t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _at(t):
     return (None, 0) if t is None else (t.data_ptr(), t.stride(0))
 
@@ -70,7 +74,7 @@ def _ptr(t):
 
 
 def _forward(residual, y, weight, post, gate, kind, scale, eps, dtype, total, stats):
-    normed = torch.empty(residual.shape, dtype=dtype, device=residual.device)
+    normed = _like(residual, dtype)
     t, hidden = residual.shape
     if t == 0:
         return normed
@@ -91,7 +95,7 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         residual, y, weight = _rows(residual), None if y is None else _rows(y), _vector(weight)
         post, gate = _vector(post), _vector(gate)
-        total = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device) if with_sum else None
+        total = _like(residual) if with_sum else None
         stats = torch.empty((2, residual.shape[0]), dtype=torch.float32, device=residual.device)
         normed = _forward(residual, y, weight, post, gate, kind, scale, eps, dtype, total, stats)
         ctx.save_for_backward(residual, y, weight, post, gate, stats)
@@ -105,8 +109,7 @@ class _ResidualNorm(torch.autograd.Function):
         t, hidden = residual.shape
         if dsum is None and dn is None:
             return (None,) * 10
-        grads = [torch.empty_like(v, memory_format=torch.contiguous_format) if needed else None
-                 for v, needed in zip((residual, y, weight, post, gate), ctx.needs_input_grad)]
+        grads = [_like(v) if needed else None for v, needed in zip((residual, y, weight, post, gate), ctx.needs_input_grad)]
         if t == 0:
             return *(None if g is None else g.zero_() for g in grads), *(None,) * 5
         dsum, dn = (None if d is None else _rows(d) for d in (dsum, dn))
@@ -131,7 +134,7 @@ def _run(residual, y, weight, post, gate, scale, eps, dtype, with_sum):
     if torch.is_grad_enabled() and any(v.requires_grad for v in leaves):
         return _ResidualNorm.apply(residual, y, weight, post, gate, kind, scale, eps, dtype, with_sum)
     residual, y = _rows(residual), None if y is None else _rows(y)
-    total = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device) if with_sum else None
+    total = _like(residual) if with_sum else None
     return total, _forward(residual, y, _vector(weight), _vector(post), _vector(gate), kind, scale, eps, dtype, total, None)
 
 

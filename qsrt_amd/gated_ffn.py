@@ -128,7 +128,7 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
             raise ValueError("out is for calls without gradients")
         return _GatedFFN.apply(x, gate, up, down, activation)
     x, gate, up, down = _checked(x, gate, up, down, activation)
-    out = checked_out(out, x, x.shape[1])
+    out = _like(x) if out is None else checked_out(out, x, x.shape[1])
     if out.data_ptr() % 16 or (out.stride(0) % 8 and out.shape[0] > 1):
         raise ValueError("out's rows must be 16-byte aligned")
     if x.shape[0]:
