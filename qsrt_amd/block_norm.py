@@ -1,6 +1,7 @@
 """What stands between two blocks of a model on MI355X: the norm behind the first, its gate, the residual with its scale and
 the norm before the second, in one pass over the rows, with gradients (``qsrt_residual_norm`` and
-``qsrt_residual_norm_backward`` in ``include/qsrt_amd.h``).  Norms are by the root of the mean square."""
+``qsrt_residual_norm_backward`` in ``include/qsrt_amd.h``).  Norms are by the root of the mean square.  Forward and backward can
+be captured in a graph; graphs that eager calls built of the same leaves have to be freed before that."""
 
 from __future__ import annotations
 

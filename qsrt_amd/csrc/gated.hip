@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
 
     // The stage to be loaded next.  Neighbouring tiles walk the sum from stages of their own, around its end: rows whose
     // distance has a high power of two would come from the same few channels of the L2 in every workgroup at once (4096 rows of
-    // 7168 x 2048 with gradients: 972 us from the first stage, 961 so).  Behind the last stage come empty ones, so that what
+    // 7168 x 2048 with gradients: 943 us from the first stage, 933 so).  Behind the last stage come empty ones, so that what
     // is on its way is always the same number of loads.
     Feed<kA> fa;
     Feed<kB> fb, fb2;

@@ -3,7 +3,8 @@ beside packed ones, a layer that is trained.
 
 ``gated_ffn`` is differentiable; ``gated_ffn_gradients`` returns, beside the gradients, the rows they are products of
 (``qsrt_gated_ffn`` and ``qsrt_gated_ffn_backward`` in ``include/qsrt_amd.h``).  Nothing waits for the device, workspaces come
-from torch's allocator on the current stream.
+from torch's allocator on the current stream.  Forward and backward can be captured in a graph; graphs that eager calls built of
+the same leaves have to be freed before that.
 """
 
 from __future__ import annotations
