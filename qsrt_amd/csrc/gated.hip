@@ -382,7 +382,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
     };
     const auto loaded = [&]() {
         to = to + kStageBytes == kStages * kStageBytes ? 0 : to + kStageBytes;
-        depth -= kDepth;
+        depth = max(depth - kDepth, 0);  // times the bytes between rows: five empty stages of rows far apart would pass 2^31
         fa.advance(depth);
         fb.advance(depth);
         if constexpr (kDual) fb2.advance(depth);

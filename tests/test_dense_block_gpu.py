@@ -373,3 +373,107 @@ def test_guidance_holds_the_gradients_of_an_expert(activation):
         candidate = weight.T.float() + 0.01
         assert abs(one.linear_term(candidate, dtype=torch.float64) - 0.5 * 0.01 * float((left.T @ right).sum())) <= \
             0.5 * 0.011 * float(bound.sum()) + 1e-6
+
+
+def test_gradients_given_in_another_type():
+    """The engine casts them to the result's type before they come here."""
+
+    x, gate, up, down, dy = draw(12, 20, 72, 136, BF16)
+    leaves = [v.requires_grad_() for v in (x, gate, up, down)]
+    for got, expected in zip(torch.autograd.grad(gated_ffn(*leaves), leaves, dy.float()),
+                             torch.autograd.grad(gated_ffn(*leaves), leaves, dy)):
+        assert torch.equal(got, expected)
+    v, dsum, dn = draw_norm(1, 6, 72, BF16, torch.float32, True, "row", BF16)
+    leaves = [u.requires_grad_() for u in v.values()]
+
+    def run(dsum, dn):
+        h, n = residual_norm(*leaves[:3], post_weight=leaves[3], gate=leaves[4])
+        return torch.autograd.grad((h, n), leaves, (dsum, dn))
+
+    for got, expected in zip(run(dsum.to(BF16).double(), dn.float()), run(dsum.to(BF16).float(), dn)):
+        assert torch.equal(got, expected)
+
+
+def test_result_in_place_of_the_input():
+    for t in (2, 30, 100):
+        x, gate, up, down, _ = draw(t, t, 136, 72, BF16)
+        expected = gated_ffn(x, gate, up, down)
+        assert torch.equal(gated_ffn(x, gate, up, down, out=x), expected)
+
+
+def test_one_matrix_as_both():
+    x, gate, _, down, dy = draw(13, 33, 72, 136, F16)
+    leaf = gate.requires_grad_()
+    both = gated_ffn_gradients(x, dy, gate, gate, down)
+    got = torch.autograd.grad(gated_ffn(x, leaf, leaf, down), leaf, dy)[0]
+    assert torch.equal(got, both.gate + both.up)
+
+
+@pytest.mark.parametrize("t,hidden,inter", [(3, 1 << 17, 8), (20, 8, 1 << 17), (70, 1 << 17, 16), (130, 24, 1 << 17)])
+def test_the_most_channels(t, hidden, inter):
+    x, gate, up, down, dy = draw(t, t, hidden, inter, BF16)
+    expected = want(x, gate, up, down, dy, "swiglu", 2 if t <= 64 else 1)
+    check({"y": gated_ffn(x, gate, up, down)}, expected, ["y"])
+    check(vars(gated_ffn_gradients(x, dy, gate, up, down)), expected, ["middle", "gate_rows", "up_rows", "x", "gate", "up", "down"])
+
+
+def test_rows_far_apart():
+    """2^22 elements: offsets inside a tile nearly reach 2^31 bytes.  More is refused."""
+
+    far, t, hidden, inter = 1 << 22, 260, 72, 264
+    x, gate, up, down, dy = draw(14, t, hidden, inter, BF16)
+    plain = gated_ffn_gradients(x, dy, gate, up, down)
+    y = gated_ffn(x, gate, up, down)
+    room = torch.full(((t + 4) * far,), float("nan"), dtype=BF16, device="cuda")
+
+    def spread(v):
+        view = room[:v.shape[0] * far].view(-1, far)[:, :v.shape[1]]
+        return view.copy_(v)
+
+    assert torch.equal(gated_ffn(spread(x), gate, up, down), y)
+    for got, expected in zip(vars(gated_ffn_gradients(spread(x), dy, gate, up, down)).values(), vars(plain).values()):
+        assert torch.equal(got, expected)
+    for got, expected in zip(vars(gated_ffn_gradients(x, dy, gate, up, spread(down))).values(), vars(plain).values()):
+        assert torch.equal(got, expected)
+    wide = torch.empty((2 * (far + 8),), dtype=BF16, device="cuda").view(2, far + 8)[:, :hidden]
+    with pytest.raises(ValueError, match="2\\^22"):
+        gated_ffn(wide, gate, up, down)
+
+
+def test_offsets_over_32_bits():
+    """Rows whose elements number more than 2^31: the last ones are what they are in a small call."""
+
+    t, hidden, inter, last = 1 << 20, 16, 2056, 128
+    x, gate, up, down, _ = draw(15, t, hidden, inter, BF16)
+    dy = torch.zeros_like(x)
+    dy[-last:] = draw(16, last, hidden, inter, BF16)[4]
+    few = gated_ffn_gradients(x[-last:], dy[-last:], gate, up, down)
+    got = gated_ffn_gradients(x, dy, gate, up, down)
+    assert got.middle.numel() > 1 << 31
+    # sums of 16 and 2056 products, in other parts: (K + 1) 2^-24 each of values of order one, and half a step of bf16 on top
+    for name in ("middle", "gate_rows", "up_rows", "x"):
+        a, b = getattr(got, name)[-last:].double(), getattr(few, name).double()
+        assert bool(((a - b).abs() <= 2.0**-7 * b.abs() + 2.0**-10 * b.abs().max()).all()), name
+    for name in ("gate", "up", "down"):
+        a, b = getattr(got, name).double(), getattr(few, name).double()
+        assert bool(((a - b).abs() <= 2.0**-7 * b.abs() + 2.0**-10 * b.abs().max()).all()), name
+    y = gated_ffn(x, gate, up, down)[-last:].double()
+    b = gated_ffn(x[-last:], gate, up, down).double()
+    assert bool(((y - b).abs() <= 2.0**-7 * b.abs() + 2.0**-10 * b.abs().max()).all())
+
+
+def test_norm_offsets_over_32_bits():
+    t, hidden, last = (1 << 21) + 5, 1032, 64
+    residual = torch.zeros((t, hidden), dtype=BF16, device="cuda")
+    y, dn = torch.zeros_like(residual), torch.zeros_like(residual)
+    v, dsum, dlast = draw_norm(17, last, hidden, BF16, BF16, True, "channel", BF16)
+    residual[-last:], y[-last:], dn[-last:] = v["residual"], v["y"], dlast
+    assert residual.numel() > 1 << 31
+
+    def run(r, y, dn):
+        r, y = r.detach().requires_grad_(), y.detach().requires_grad_()
+        h, n = residual_norm(r, y, v["weight"], post_weight=v["post"], gate=v["gate"])
+        return [u[-last:] for u in (h.detach(), n.detach(), *torch.autograd.grad(n, (r, y), dn))]
+
+    for got, expected in zip(run(residual, y, dn), run(v["residual"], v["y"], dlast)):
+        assert torch.equal(got, expected)  # rows are alone
