@@ -356,7 +356,8 @@ int64_t gradient_groups(int64_t rows, int64_t hidden) {
     return std::min<int64_t>(rows, cus * std::min(fit, most));
 }
 
-// Workgroups that the chip holds at a time: 32 waves a compute unit.
+// Workgroups that the chip holds at a time: 32 waves a compute unit.  With half or twice as many, 4096 rows of 7168 take 73 and
+// 79 us for 75, 8192 of 5120 91 and 81 for 84.
 int64_t row_groups(int hidden) {
     int cus = 0;
     if (current_cu_count(&cus) != kOk) cus = 256;
