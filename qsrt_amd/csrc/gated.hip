@@ -623,11 +623,11 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowsArgs p) {
 // is full (fits to 128 .. 4096 rows of 5120 x 1536 and 7168 x 2048).  A tile of 256 x 256 has two stages in LDS, one of 128 x
 // 256 three, one of 128 x 128 five: the smaller it is, the more a stage's loads count, which take 1.4 us to land.
 struct Shape {
-    int m, n, resident;  // rows, columns; workgroups that a compute unit holds
+    int m, n;  // rows, columns
     float fixed, stage;
 };
 enum { kSquare, kWide, kSmall, kFlat, kFewRows };
-constexpr Shape kShapes[] = {{256, 256, 1, 6.f, 1.66f}, {128, 256, 1, 4.f, 1.15f}, {128, 128, 1, 3.f, 0.68f}, {32, 128, 2, 3.f, 0.7f}};
+constexpr Shape kShapes[] = {{256, 256, 6.f, 1.66f}, {128, 256, 4.f, 1.15f}, {128, 128, 3.f, 0.68f}, {32, 128, 3.f, 0.7f}};
 
 struct Cut {
     int shape, parts;
@@ -639,7 +639,9 @@ int64_t tiles_of(const Shape& s, int64_t m, int64_t n, bool dual) {
 }
 
 // The tile, and the parts that the sum is cut into, with the least time to expect; `products` of this size go together and
-// are not cut.  Parts cost their sums' way to memory and back and a launch.
+// are not cut.  Parts cost a launch, a round trip for every eight and their sums' way to memory and back.  Against 3 us and 4.6
+// TB/s for that, with two workgroups of 32 rows a compute unit, in us: 24 rows of 5120 x 1536 24.6 (28.6), 333 of 2048 x 1024
+// 31.2 (34.9), 200 of 5120 x 1536 36.8 (40.5); nothing more than 1% slower.
 Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
     int cus = 0;
     if (current_cu_count(&cus) != kOk) cus = 256;
@@ -649,12 +651,14 @@ Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
     for (int i = kSquare; i <= kFlat; ++i) {
         const Shape& s = kShapes[i];
         if ((i == kFlat) != (m <= 32 && products == 1)) continue;
-        const int64_t tiles = tiles_of(s, m, n, dual) * products, slots = static_cast<int64_t>(cus) * s.resident;
+        const int64_t tiles = tiles_of(s, m, n, dual) * products, slots = cus;
         const int64_t most = products > 1 ? 1 : std::min<int64_t>(32, stages / 2);
         for (int64_t parts = 1; parts == 1 || (parts <= most && tiles * parts <= slots); ++parts) {
             float time = static_cast<float>((tiles * parts + slots - 1) / slots) *
                          (s.fixed + s.stage * static_cast<float>((stages + parts - 1) / parts));
-            if (parts > 1) time += 3.f + static_cast<float>(parts * (dual ? 2 : 1) * m * n) * 8.f / 4.6e6f;
+            if (parts > 1)
+                time += 4.f + 1.2f * static_cast<float>((parts - 1) / 8) +
+                        static_cast<float>(parts * (dual ? 2 : 1) * m * n) * 8.f / 3.5e6f;
             if (least == 0.f || time < least) {
                 least = time;
                 best = {i, static_cast<int>(parts)};
@@ -741,8 +745,8 @@ bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
 int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
 
 // Up to 16 rows, one side of a matrix instruction, meet a kernel of their own.  Against tiles with parts, in us at 8, 12 and 16
-// rows: 2048 x 1024 10.0, 10.6, 11.3 for 16.9, 17.2, 17.8; 5120 x 1536 21, 23.6, 26.7 for 27.3, 27.6, 28.0; 7168 x 2048 27,
-// 30.5, 33.7 for 32.3, 32.6, 33.2.  With 17 to 32 the rows of activations would be read twice as often as the weights.
+// rows: 2048 x 1024 10.1, 10.7, 11.3 for 15.5, 15.8, 16.0; 5120 x 1536 20.9, 23.2, 26.2 for 24.8, 25.3, 25.3; 7168 x 2048 27.1,
+// 30.3, 33.4 for 31.3, 31.6, 32.1.  With 17 to 32 the rows of activations would be read twice as often as the weights.
 bool few_rows(int64_t tokens) { return tokens <= 16; }
 
 size_t round_up(size_t n) { return (n + 255) & ~size_t{255}; }

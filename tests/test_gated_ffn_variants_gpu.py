@@ -21,23 +21,25 @@ SQUARE, WIDE, SMALL, FLAT, ROWS = range(5)
 CASES = {
     (1, 72, 72): ((ROWS, 0), (ROWS, 0), (FLAT, 0), (FLAT, 1), (SMALL, 0)),
     (7, 4104, 2056): ((ROWS, 0), (ROWS, 0), (FLAT, 1), (FLAT, 1), (SQUARE, 0)),  # waves' parts of 16 and 17 steps
-    (16, 4096, 520): ((ROWS, 0), (ROWS, 0), (FLAT, 1), (FLAT, 1), (WIDE, 0)),     # of 16, of four and five
+    (16, 4096, 520): ((ROWS, 0), (ROWS, 0), (FLAT, 1), (FLAT, 1), (WIDE, 0)),  # of 16, of four and five
     (17, 72, 72): ((FLAT, 0), (FLAT, 0), (FLAT, 0), (FLAT, 1), (SMALL, 0)),
     (24, 520, 264): ((FLAT, 1), (FLAT, 1), (FLAT, 1), (FLAT, 1), (SMALL, 0)),
+    (24, 520, 72): ((FLAT, 1), (FLAT, 0), (FLAT, 1), (FLAT, 1), (SMALL, 0)),
     (32, 6152, 72): ((FLAT, 1), (FLAT, 0), (FLAT, 1), (FLAT, 0), (SMALL, 0)),
     (33, 72, 264): ((SMALL, 0), (SMALL, 1), (SMALL, 0), (SMALL, 1), (SMALL, 0)),
-    (33, 520, 72): ((SMALL, 1), (SMALL, 0), (SMALL, 1), (SMALL, 1), (SMALL, 0)),
-    (65, 72, 72): ((SMALL, 0),) * 5,
-    (33, 2056, 6152): ((WIDE, 1), (SMALL, 1), (SMALL, 1), (SMALL, 1), (SQUARE, 0)),
-    (33, 4104, 8200): ((WIDE, 1),) * 4 + ((SQUARE, 0),),
-    (33, 8200, 2056): ((SMALL, 1), (WIDE, 1), (SMALL, 1), (WIDE, 1), (SQUARE, 0)),
+    (33, 520, 72): ((SMALL, 1), (SMALL, 0), (SMALL, 1), (SMALL, 0), (SMALL, 0)),
+    (65, 72, 72): ((SMALL, 0), (SMALL, 0), (SMALL, 0), (SMALL, 0), (SMALL, 0)),
+    (33, 2568, 6152): ((WIDE, 1), (SMALL, 1), (SMALL, 1), (SMALL, 1), (SQUARE, 0)),
+    (33, 5128, 8200): ((WIDE, 1), (SMALL, 1), (WIDE, 1), (WIDE, 1), (SQUARE, 0)),
+    (33, 8200, 2568): ((SMALL, 1), (WIDE, 1), (SMALL, 1), (WIDE, 1), (SQUARE, 0)),
     (130, 72, 8200): ((WIDE, 0), (SMALL, 1), (SMALL, 0), (SMALL, 1), (SMALL, 0)),
     (390, 72, 8200): ((SQUARE, 0), (SMALL, 1), (WIDE, 0), (SMALL, 1), (SMALL, 0)),
     (390, 8200, 72): ((SMALL, 1), (WIDE, 0), (SMALL, 1), (WIDE, 0), (SMALL, 0)),
     (900, 72, 8200): ((SQUARE, 0), (SMALL, 1), (SQUARE, 0), (SMALL, 1), (SMALL, 0)),
     (900, 8200, 72): ((SMALL, 1), (SQUARE, 0), (SMALL, 1), (SQUARE, 0), (SMALL, 0)),
-    (130, 8200, 5128): ((SQUARE, 1), (SQUARE, 1), (SMALL, 1), (SQUARE, 1), (SQUARE, 0)),
-    (130, 5128, 8200): ((SQUARE, 1), (SMALL, 1), (SQUARE, 1), (SQUARE, 1), (SQUARE, 0)),
+    (130, 8200, 6152): ((SQUARE, 1), (SQUARE, 1), (WIDE, 1), (SQUARE, 1), (SQUARE, 0)),
+    (130, 6152, 8200): ((SQUARE, 1), (WIDE, 1), (SQUARE, 1), (SQUARE, 1), (SQUARE, 0)),
+    (130, 2568, 8200): ((SQUARE, 1), (SMALL, 1), (SMALL, 0), (SMALL, 1), (SQUARE, 0)),
 }
 
 
