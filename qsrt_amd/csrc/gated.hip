@@ -286,7 +286,7 @@ __device__ __forceinline__ int xcd_slot(int q, int n) {
 // Many rows are bound by the operands' way from L2 to LDS, with the matrix cores close behind: a stage of a 256 x 256 tile
 // brings 64 KB to each compute unit in 1.66 us, 10 TB/s on the chip, 79% of it out of L2.  4096 rows of 7168 x 2048 take 187 to
 // 202 us for gate and up (1.2 to 1.3 PFLOP/s; 164 with the loads alone, 148 with the products and their reads from LDS alone,
-// at 1.8 GHz), 110 for down, 104 for dM, 196 for dx, 313 for the weights' gradients.  64 deep: stages of 32 in rings of four or
+// at 1.8 GHz), 110 for down, 196 for dx, 313 for the weights' gradients, and dM, in tiles of 128 x 256, 144.  64 deep: stages of 32 in rings of four or
 // five cost 10%, having twice the barriers.  Eight waves of 128 x 64: four of 128 x 128 have nobody to load while they wait
 // (25% slower), 32 x 32 x 16 instructions 5%.
 template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
@@ -517,9 +517,9 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
     }
 }
 
-// Adds the parts up, in their order, four columns a thread.  Bound by memory (dM of 4096 rows of 2048 in two parts, with G and
-// U read and three rows written: 184 MB in 31 us), of few rows by its launch and two round trips (45 rows of 1536, ten parts:
-// 4.2).
+// Adds the parts up, in their order, four columns a thread.  Bound by its launch and round trips (45 rows of 1536 in eight parts
+// 3.2 to 4.2 us, 500 in two 4.7), of many rows by memory (4096 rows of 2048 in two parts, with G and U read and three rows
+// written: 184 MB in 31).
 template <typename T, Ending kEnding>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int parts, int64_t m, int64_t n, const Finish f) {
     constexpr int kPlanes = kEnding == kActivate ? 2 : 1;
@@ -641,7 +641,7 @@ int64_t tiles_of(const Shape& s, int64_t m, int64_t n, bool dual) {
 // The tile, and the parts that the sum is cut into, with the least time to expect; `products` of this size go together and
 // are not cut.  Parts cost a launch, a round trip for every eight and their sums' way to memory and back.  Against 3 us and 4.6
 // TB/s for that, with two workgroups of 32 rows a compute unit, in us: 24 rows of 5120 x 1536 24.6 (28.6), 333 of 2048 x 1024
-// 31.2 (34.9), 200 of 5120 x 1536 36.8 (40.5); nothing more than 1% slower.
+// 31.2 (34.9), 200 of 5120 x 1536 36.8 (40.5); at worst 1.5% slower (4096 of 7168 x 2048 with gradients).
 Cut cut(int64_t m, int64_t n, int64_t k, int sums, bool dual, int products) {
     int cus = 0;
     if (current_cu_count(&cus) != kOk) cus = 256;
