@@ -284,11 +284,11 @@ __device__ __forceinline__ int xcd_slot(int q, int n) {
 // neighbouring columns of one row.
 //
 // Many rows are bound by the operands' way from L2 to LDS, with the matrix cores close behind: a stage of a 256 x 256 tile
-// brings 64 KB to each compute unit in 1.66 us, 10 TB/s on the chip, 79% of it out of L2.  4096 rows of 7168 x 2048 take 187 to
-// 202 us for gate and up (1.2 to 1.3 PFLOP/s; 164 with the loads alone, 148 with the products and their reads from LDS alone,
-// at 1.8 GHz), 110 for down, 196 for dx, 313 for the weights' gradients, and dM, in tiles of 128 x 256, 144.  64 deep: stages of 32 in rings of four or
-// five cost 10%, having twice the barriers.  Eight waves of 128 x 64: four of 128 x 128 have nobody to load while they wait
-// (25% slower), 32 x 32 x 16 instructions 5%.
+// brings 64 KB to each compute unit in 1.66 us, 10 TB/s on the chip, 79% of it out of L2.  4096 rows of 7168 x 2048 take 187
+// to 202 us for gate and up (1.2 to 1.3 PFLOP/s; 164 with the loads alone, 148 with the products and their reads from LDS
+// alone, at 1.8 GHz), 110 for down, 196 for dx, 313 for the weights' gradients, and dM, in tiles of 128 x 256, 144.  64 deep:
+// stages of 32 in rings of four or five cost 10%, having twice the barriers.  Eight waves of 128 x 64: four of 128 x 128 have
+// nobody to load while they wait (25% slower), 32 x 32 x 16 instructions 5%.
 template <typename T, Layout kA, Layout kB, Ending kEnding, int kM, int kN, int kWavesM, int kWavesN, int kStages>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const ArgsOf<kA> args) {
     constexpr int kWaves = kWavesM * kWavesN;
@@ -316,7 +316,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
         part = tile / tiles;
         tile %= tiles;
     }
-    // tiles in bands of four of m: the workgroups at work on an XCD at a time share operands in its L2
+    // tiles in bands of four of m: the workgroups at work on an XCD at a time share operands in its L2 (bands of six: 1% less at
+    // 4096 rows of 7168 x 2048 with gradients, 2% more at 4096 of 2056 x 1400; of 16 1% more)
     constexpr int kBand = 4;
     const int band = tile / (kBand * p.tiles_n), in_band = tile % (kBand * p.tiles_n);
     const int high = min(kBand, p.tiles_m - band * kBand);

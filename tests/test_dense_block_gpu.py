@@ -267,6 +267,44 @@ def test_captured_forward_and_backward(t):
             assert torch.equal(a, b)
 
 
+def test_captured_backward_into_the_leaves():
+    """A training step's own form, on the side stream that its eager steps ran on; those left no graph behind."""
+
+    x, gate, up, down, dy = draw(18, 40, 136, 72, BF16)
+    leaves = [v.requires_grad_() for v in (gate, up, down)]
+    weight = torch.ones(136, device="cuda", requires_grad=True)
+
+    def step():
+        n = rms_norm(x, weight)
+        h, n = residual_norm(x, gated_ffn(n, *leaves), weight)
+        torch.autograd.backward((h, n), (dy, dy))
+
+    params = [*leaves, weight]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        for p in params:
+            p.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    captured = [p.grad for p in params]
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(draw(30 + k, 40, 136, 72, BF16)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [g.clone() for g in captured]
+        for p in params:
+            p.grad = None
+        step()
+        for a, p in zip(got, params):
+            assert torch.equal(a, p.grad)
+            p.grad = None
+
+
 def test_gradients_against_differences():
     """Directional differences of the block in 64 bits at the kernel's own inputs: the gradients are those of its formula."""
 
