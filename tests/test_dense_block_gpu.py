@@ -50,6 +50,23 @@ def test_views(t, ld, offset):
         assert torch.equal(got, expected)
 
 
+@pytest.mark.parametrize("ld,offset", [(8, 0), (3, 0), (0, 1), (16, 5)])
+def test_views_of_the_norms(ld, offset):
+    v, dsum, dn = draw_norm(5, 37, 264, BF16, torch.float32, True, "row", torch.float32)
+    views = {k: embed(t, t.shape[1] + ld, offset) if t.dim() == 2 else embed(t[:, None], 1 + ld, offset)[:, 0] for k, t in v.items()}
+
+    def run(v, dsum, dn):
+        leaves = [t.detach().requires_grad_() for t in v.values()]
+        h, n = residual_norm(*leaves[:3], post_weight=leaves[3], gate=leaves[4], scale=0.5)
+        return [h, n, *torch.autograd.grad((h, n), leaves, (dsum, dn))]
+
+    for got, expected in zip(run(views, embed(dsum, 264 + ld, offset), dn.T.contiguous().T), run(v, dsum, dn)):
+        assert torch.equal(got, expected)
+    one = torch.ones((1, 1), dtype=BF16, device="cuda").expand(37, 264)
+    for got, expected in zip(run(views, one.float(), one), run(v, one.float().contiguous(), one.contiguous())):
+        assert torch.equal(got, expected)
+
+
 def test_lone_row_of_any_stride():
     x, gate, up, down, dy = draw(9, 1, 64, 72, BF16)
     odd = x.as_strided((1, 64), (3, 1))
