@@ -146,7 +146,8 @@ def residual_norm(residual: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
 
     ``y [T, hidden]``, a block's result, and ``n``, the next block's input, are bf16 or f16; ``residual`` and ``h`` float32 or
     of that type.  ``weight`` and ``post_weight [hidden]`` and ``gate`` (``[hidden]``, or ``[T, 1]``: each row its own) are all
-    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors, once."""
+    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors, once.
+    Squares are summed in FP32: a row's rms may be up to 1e17 and, with an eps of 0, down to 1e-18."""
 
     return _run(residual, y, weight, post_weight, gate, float(scale), float(eps), y.dtype, True)
 

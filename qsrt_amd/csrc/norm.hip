@@ -6,12 +6,13 @@
 //   n = weight * h sh, sh = (mean h^2 + eps)^-1/2
 //
 // Bound by memory: a row stays in registers between its loads and its stores, sums and statistics are FP32, n comes from h
-// before h is rounded.  The gradients, with e = weight * dn and p = post * gate:
-//   dh = dsum + sh (e - h sh^2 mean(e h)),  dresidual = scale dh,  dz = gate dh
+// before h is rounded.  The gradients, with e = weight * dn, p = post * gate and hhat = h sh (no higher power of sh stands alone:
+// rows of 1e13 or, with a small eps, 1e-13 would end FP32's range there, where their gradients do not):
+//   dh = dsum + sh (e - hhat mean(e hhat)),  dresidual = scale dh,  dz = gate dh
 //   dy = sy (post dz - yhat mean(post dz yhat)),  yhat = y sy
-//   dweight = sum over rows of dn h sh,  dpost of dz yhat,  dgate of dh z (a row's own gate: over its channels)
-// mean(post dz yhat) is put together from sums that do not wait for mean(e h), so a row meets once:
-//   sum p yhat dh = sum p yhat (dsum + sh e) - sh^3 mean(e h) sum p yhat h
+//   dweight = sum over rows of dn hhat,  dpost of dz yhat,  dgate of dh z (a row's own gate: over its channels)
+// mean(post dz yhat) is put together from sums that do not wait for mean(e hhat), so a row meets once:
+//   sum p yhat dh = sum p yhat (dsum + sh e) - sh mean(e hhat) sum p yhat hhat
 // and a gate for each channel shares its sum over the rows with post: dpost = gate S, dgate = post S, S = sum of dh yhat.
 #include <algorithm>
 
@@ -245,27 +246,27 @@ __global__ __launch_bounds__(1024) void norm_gradients_kernel(const NormArgs p) 
         const float sy = p.stats[row], sh = p.stats[p.rows + row];
         const float row_gate = p.gate_kind == kRow ? load1<T>(p.gate, row, p.params_f32) : 1.f;
         if (!kKeep) fetch(row);
-        f32x8 yhat[kSteps], h[kSteps], d[kSteps];  // d: dsum + sh e, dh but for the row's mean
-        float v[3] = {0.f, 0.f, 0.f};              // e h, z d, z h, without a row's gate: its gradient needs the same sums
+        f32x8 yhat[kSteps], hhat[kSteps], d[kSteps];  // d: dsum + sh e, dh but for the row's mean
+        float v[3] = {0.f, 0.f, 0.f};  // e hhat, z d, z hhat, without a row's gate: its gradient needs the same sums
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
-            yhat[s] = h[s] = d[s] = zero;
+            yhat[s] = hhat[s] = d[s] = zero;
             if (c >= p.hidden) continue;
             const f32x8 weight = kKeep ? kept_weight : weight_at(c), pz = kKeep ? kept_pz : pz_at(c);
             yhat[s] = y[s].get() * sy;
             const f32x8 z = yhat[s] * pz;
-            h[s] = p.scale * residual[s].get() + row_gate * z;
+            hhat[s] = (p.scale * residual[s].get() + row_gate * z) * sh;
             const f32x8 n = dn[s].get(), e = n * weight;
-            by_weight[s] += n * (h[s] * sh);
+            by_weight[s] += n * hhat[s];
             d[s] = dsum[s].get() + e * sh;
-            v[0] += total(e * h[s]);
+            v[0] += total(e * hhat[s]);
             v[1] += total(z * d[s]);
-            v[2] += total(z * h[s]);
+            v[2] += total(z * hhat[s]);
         }
         if (kKeep && row + gridDim.x < p.rows) fetch(row + gridDim.x);
         meet(v, room[turn], lane, wave);
-        const float back = sh * sh * sh * (v[0] * mean);
+        const float back = sh * (v[0] * mean);
         const float by_z = v[1] - back * v[2];  // the sum of z dh
         const float shared = p.post ? by_z * row_gate * mean : 0.f;
         if (p.drow && threadIdx.x == 0) {
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(1024) void norm_gradients_kernel(const NormArgs p) 
         for (int s = 0; s < kSteps; ++s) {
             const int c = (s * threads + static_cast<int>(threadIdx.x)) * 8;
             if (c >= p.hidden) continue;
-            const f32x8 dh = d[s] - h[s] * back;
+            const f32x8 dh = d[s] - hhat[s] * back;
             if (p.dresidual) store8<T>(p.dresidual, row * p.dresidual_ld + c, p.scale * dh, kF32);
             const f32x8 dz = row_gate * dh;
             by_scale[s] += dz * yhat[s];
