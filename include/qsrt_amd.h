@@ -552,6 +552,8 @@ int qsrt_gated_ffn(const void *x, int64_t x_ld, const void *gate, const void *up
  *   dx = dG gate + dU up, d_gate = dG^T x, d_up = dU^T x, d_down = dy^T M
  * Any of them may be NULL; d_gate, d_up, d_down are contiguous.  gate_rows,
  * up_rows and middle (contiguous [tokens, inter], or NULL) receive dG, dU, M.
+ * For their products f16 rows are scaled by powers of two, so that gradients
+ * under 2^-14 keep their bits; the rows handed out are not.
  */
 size_t qsrt_gated_ffn_backward_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inter);
 int qsrt_gated_ffn_backward(const void *dy, int64_t dy_ld, const void *x, int64_t x_ld, const void *gate, const void *up,

@@ -8,6 +8,7 @@
 // (kRows) or outermost (kCols), so no operand is ever transposed in memory.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.h"
@@ -31,6 +32,9 @@ __device__ __forceinline__ f32x4 multiply(vec8<T> a, vec8<T> b, f32x4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+
+template <typename T>
+constexpr bool kScaled = std::is_same<T, _Float16>::value;  // its rows between products, in the backward pass
 
 // ---------------------------------------------------------------- what becomes of a product
 // The activation in FP32: silu(g) u or 4 tanh(g/4) sigmoid(g) 25 tanh(u/25), and its derivatives.
@@ -76,6 +80,12 @@ enum Ending { kStore, kActivate, kSlopes };
 // 16-bit value and the nearest of what is left; `pieces_of` says when).
 struct Pieces {
     void *hi, *lo;  // lo null: one
+    void* plain;    // where the rows go as they are, beside the scaled ones; or null
+};
+
+// What scaled rows between products are multiplied by: dG and dU, and M.  kStore: `rows`, what the sums are.
+struct Scales {
+    float rows, middle;
 };
 
 struct Finish {
@@ -86,10 +96,17 @@ struct Finish {
     int activation;
     float *pre_g, *pre_u;     // kActivate: G and U out, or null; kSlopes: in
     Pieces middle, dg, du;    // kActivate: middle; kSlopes: all
+    // f16 in the backward pass, or null
+    const f32x4* bounds;  // kSlopes: of `bounds_kernel`
+    float* unscale;       // kSlopes: one over each of the scales, out; kStore: the one for these sums
 };
 
 template <typename T>
-__device__ __forceinline__ void store_pieces(const Pieces& to, int64_t at, const f32x4& v) {
+__device__ __forceinline__ void store_pieces(const Pieces& to, int64_t at, f32x4 v, float scale) {
+    if constexpr (kScaled<T>) {
+        if (to.plain) *reinterpret_cast<vec4<T>*>(static_cast<T*>(to.plain) + at) = __builtin_convertvector(v, vec4<T>);
+        v *= scale;
+    }
     const vec4<T> hi = __builtin_convertvector(v, vec4<T>);
     *reinterpret_cast<vec4<T>*>(static_cast<T*>(to.hi) + at) = hi;
     if (to.lo) {
@@ -102,10 +119,10 @@ __device__ __forceinline__ void store_pieces(const Pieces& to, int64_t at, const
 
 // Four neighbouring columns of one row: v the sums, u the second matrix's.
 template <typename T, Ending kEnding>
-__device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col, const f32x4& v, const f32x4& u) {
+__device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col, const f32x4& v, const f32x4& u, const Scales& by) {
     const int64_t at = row * f.ld + col;
     if constexpr (kEnding == kStore) {
-        *reinterpret_cast<vec4<T>*>(static_cast<T*>(f.out) + at) = __builtin_convertvector(v, vec4<T>);
+        *reinterpret_cast<vec4<T>*>(static_cast<T*>(f.out) + at) = __builtin_convertvector(kScaled<T> ? v * by.rows : v, vec4<T>);
     } else if constexpr (kEnding == kActivate) {
         if (f.pre_g) {
             *reinterpret_cast<f32x4*>(f.pre_g + at) = v;
@@ -114,7 +131,7 @@ __device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col
         f32x4 m;
 #pragma unroll
         for (int r = 0; r < 4; ++r) m[r] = activate(v[r], u[r], f.activation);
-        store_pieces<T>(f.middle, at, m);
+        store_pieces<T>(f.middle, at, m, 1.f);
     } else {
         const f32x4 g = *reinterpret_cast<const f32x4*>(f.pre_g + at), up = *reinterpret_cast<const f32x4*>(f.pre_u + at);
         f32x4 m, dg, du;
@@ -126,10 +143,114 @@ __device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col
             dg[r] = v[r] * by_g;
             du[r] = v[r] * by_u;
         }
-        store_pieces<T>(f.middle, at, m);
-        store_pieces<T>(f.dg, at, dg);
-        store_pieces<T>(f.du, at, du);
+        store_pieces<T>(f.middle, at, m, by.middle);
+        store_pieces<T>(f.dg, at, dg, by.rows);
+        store_pieces<T>(f.du, at, du, by.rows);
     }
+}
+
+// The steps of f16 stop shrinking at 2^-24: of gradients of 1e-5 seven bits would be left, in two pieces no more.  So in the
+// backward pass f16 rows between products are scaled by powers of two, dG and dU by one, M by another, which are divided out of
+// the FP32 sums again.  Which: what takes a bound on all of them to 2^14 .. 2^15, so that none ends at 65504 for being scaled,
+// but never less than 1.  The bound of M is its largest value; |dG| and |dU| are at most
+//   max over rows |dy| * sqrt(H) max |W2| * the largest slope
+// as no column of W2 is longer than sqrt(H) max |W2|.  That is some 2^6 to 2^12 above their usual size, of the 2^29 from 2^15 down
+// to the least f16 that has all its bits.  Values that are not finite do not count.
+//
+// The forward pass does without: its bound would need gate and up read once more.  `bounds_kernel` is bound by memory (dy, W2, G
+// and U of 4096 rows of 7168 x 2048, 154 MB, in 36 to 46 us); a call with gradients takes 1012 to 1025 us, not 980 to 992, of 500
+// rows of 5120 x 1536 155, not 150.
+constexpr int kBoundGroups = 256, kBoundWaves = 16;
+struct BoundArgs {
+    const void *dy, *down;
+    int64_t dy_ld, down_ld, tokens, hidden, inter;
+    int activation;
+    const float* pre;
+    f32x4* bounds;  // a workgroup's: sqrt(H) |dy| of a row, |W2|, slopes, |M|
+};
+
+__device__ __forceinline__ f32x4 most_of(f32x4 v) {  // of the wave, in each lane
+#pragma unroll
+    for (int apart = 32; apart > 0; apart >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaxf(v[i], __shfl_xor(v[i], apart));
+    return v;
+}
+
+__global__ __launch_bounds__(64 * kBoundWaves) void bounds_kernel(const BoundArgs p) {
+    __shared__ f32x4 room[kBoundWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = blockIdx.x * kBoundWaves + wave, waves = kBoundGroups * kBoundWaves;
+    f32x4 most = {};
+    const auto see = [&](int i, float v) { most[i] = v <= FLT_MAX ? fmaxf(most[i], v) : most[i]; };
+    for (int64_t row = first; row < p.tokens; row += waves) {
+        float sum = 0.f;
+        for (int64_t c = 8 * lane; c < p.hidden; c += 512) {
+            const vec8<_Float16> v = *reinterpret_cast<const vec8<_Float16>*>(static_cast<const _Float16*>(p.dy) + row * p.dy_ld + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = static_cast<float>(v[i]);
+                sum += fabsf(f) <= FLT_MAX ? f * f : 0.f;
+            }
+        }
+#pragma unroll
+        for (int apart = 32; apart > 0; apart >>= 1) sum += __shfl_xor(sum, apart);
+        see(0, sqrtf(sum * static_cast<float>(p.hidden)));
+    }
+    for (int64_t row = first; row < p.hidden; row += waves)
+        for (int64_t c = 8 * lane; c < p.inter; c += 512) {
+            const vec8<_Float16> v = *reinterpret_cast<const vec8<_Float16>*>(static_cast<const _Float16*>(p.down) + row * p.down_ld + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) see(1, fabsf(static_cast<float>(v[i])));
+        }
+    const int64_t plane = p.tokens * p.inter;
+    for (int64_t at = (first * 64 + lane) * 4; at < plane; at += waves * 64 * 4) {
+        const f32x4 g = *reinterpret_cast<const f32x4*>(p.pre + at), u = *reinterpret_cast<const f32x4*>(p.pre + plane + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float m, by_g, by_u;
+            activate_with_slopes(g[i], u[i], p.activation, m, by_g, by_u);
+            see(2, fabsf(by_g));
+            see(2, fabsf(by_u));
+            see(3, fabsf(m));
+        }
+    }
+    most = most_of(most);
+    if (lane == 0) room[wave] = most;
+    __syncthreads();
+    if (wave > 0) return;
+    most = most_of(room[lane % kBoundWaves]);
+    if (lane == 0) p.bounds[blockIdx.x] = most;
+}
+
+// The power of two, 1 at the least, that takes `bound` to 2^14 .. 2^15.
+__device__ __forceinline__ float scale_to(float bound) {
+    const int exponent = static_cast<int>(__builtin_bit_cast(uint32_t, bound) >> 23) - 127;  // (bound is not negative)
+    const int up = min(max(14 - exponent, 0), 60);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(127 + up) << 23);
+}
+
+// For all threads of a workgroup, at its end; `first`: of the launch.
+template <typename T, Ending kEnding>
+__device__ __forceinline__ Scales scales_of(const Finish& f, bool first) {
+    Scales by = {1.f, 1.f};
+    if constexpr (kScaled<T> && kEnding == kStore) {
+        if (f.unscale) by.rows = *f.unscale;
+    } else if constexpr (kScaled<T> && kEnding == kSlopes) {
+        if (f.bounds) {
+            f32x4 most = {};
+#pragma unroll
+            for (int q = 0; q < kBoundGroups; q += 64) {
+                const f32x4 v = f.bounds[q + (threadIdx.x & 63)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], v[i]);
+            }
+            most = most_of(most);
+            by = {scale_to(most[0] * most[1] * most[2]), scale_to(most[3])};
+            if (first && threadIdx.x == 0) f.unscale[0] = 1.f / by.rows, f.unscale[1] = 1.f / by.middle;
+        }
+    }
+    return by;
 }
 
 // ---------------------------------------------------------------- the product
@@ -499,6 +620,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
+    Scales by = {1.f, 1.f};
+    if (parts == 1) by = scales_of<T, kEnding>(p.finish, blockIdx.x == 0);
     const int64_t row0 = m0 + wm + (lane & 15), col0 = n0 + wn + 4 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < kI; ++i) {
@@ -510,6 +633,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
 #pragma unroll
             for (int j = 0; j + 1 < kJ; j += 2) {
                 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                if constexpr (kScaled<T>) acc[i][j] *= by.rows, acc[i][j + 1] *= by.rows;
                 const u32x2 a = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j], vec4<T>));
                 const u32x2 b = __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j + 1], vec4<T>));
                 const auto low = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
@@ -530,7 +654,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
                 *reinterpret_cast<f32x4*>(to) = acc[i][j];
                 if constexpr (kDual) *reinterpret_cast<f32x4*>(to + p.m * p.n) = acc[i][kHalf + j];
             } else {
-                finish<T, kEnding>(p.finish, row, col, acc[i][j], acc[i][kDual ? kHalf + j : j]);
+                finish<T, kEnding>(p.finish, row, col, acc[i][j], acc[i][kDual ? kHalf + j : j], by);
             }
         }
     }
@@ -542,6 +666,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void tile_kernel(const Args
 template <typename T, Ending kEnding>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int parts, int64_t m, int64_t n, const Finish f) {
     constexpr int kPlanes = kEnding == kActivate ? 2 : 1;
+    const Scales by = scales_of<T, kEnding>(f, blockIdx.x == 0);
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
     if (at >= m * n) return;
     f32x4 sum[2] = {};
@@ -562,7 +687,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     for (; q < parts; ++q)
 #pragma unroll
         for (int h = 0; h < kPlanes; ++h) sum[h] += *reinterpret_cast<const f32x4*>(partial + (q * kPlanes + h) * plane + at);
-    finish<T, kEnding>(f, at / n, at % n, sum[0], sum[1]);
+    finish<T, kEnding>(f, at / n, at % n, sum[0], sum[1], by);
 }
 
 // ---------------------------------------------------------------- a few rows
@@ -634,7 +759,7 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowsArgs p) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) up[q] = __shfl_xor(sum[q], 32);
     const int col = n0 + 4 * g;
-    if (r < p.m && col < p.n && !(kDual && g >= 2)) finish<T, kEnding>(p.finish, r, col, sum, up);
+    if (r < p.m && col < p.n && !(kDual && g >= 2)) finish<T, kEnding>(p.finish, r, col, sum, up, Scales{1.f, 1.f});
 }
 
 // ---------------------------------------------------------------- host
@@ -759,7 +884,8 @@ bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
 }
 
 // Up to 64 rows, where reading the weights bounds a product, rows between products go on in two pieces: the result is then
-// off by its own rounding alone.  In one, it is off by 1.4 times as much (two roundings of one size); in two, 64 rows of 7168 x
+// off by its own rounding alone (forward in f16 while M is over 2^-10 or so: under 2^-14 both pieces end at 2^-24, as the result
+// itself does).  In one, it is off by 1.4 times as much (two roundings of one size); in two, 64 rows of 7168 x
 // 2048 take 39.4 us, not 35.5, 32 of 5120 x 1536 31.1, not 28.9, and 500 rows 89 us, not 73.
 int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
 
@@ -793,7 +919,7 @@ Forward plan_forward(int64_t tokens, int64_t hidden, int64_t inter) {
 struct Backward {
     int pieces;
     Cut middle, x, weights;
-    size_t rows, partial, bytes;
+    size_t rows, partial, scales, bytes;
 };
 Backward plan_backward(int64_t tokens, int64_t hidden, int64_t inter) {
     Backward b;
@@ -803,7 +929,8 @@ Backward plan_backward(int64_t tokens, int64_t hidden, int64_t inter) {
     b.weights = cut(inter, hidden, tokens, b.pieces, false, 3);
     b.rows = round_up(sizeof(uint16_t) * b.pieces * tokens * inter);
     b.partial = std::max(part_bytes(b.middle, tokens, inter, 1), part_bytes(b.x, tokens, hidden, 1));
-    b.bytes = 3 * b.rows + b.partial;
+    b.scales = round_up(sizeof(f32x4) * kBoundGroups + sizeof(Scales));  // of f16
+    b.bytes = 3 * b.rows + b.partial + b.scales;
     return b;
 }
 
@@ -842,7 +969,7 @@ int check_workspace(const char* call, const void* ws, size_t given, size_t need)
 }
 
 Pieces pieces_at(char* ws, int64_t tokens, int64_t inter, int pieces) {
-    return {ws, pieces > 1 ? ws + sizeof(uint16_t) * tokens * inter : nullptr};
+    return {ws, pieces > 1 ? ws + sizeof(uint16_t) * tokens * inter : nullptr, nullptr};
 }
 
 // One product's sums: a in pieces by b, or a by b in pieces.
@@ -898,9 +1025,21 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
     args.partial = reinterpret_cast<float*>(ws + 3 * plan.rows);
     Pieces dg = pieces_at(ws, b.tokens, b.inter, plan.pieces), du = pieces_at(ws + plan.rows, b.tokens, b.inter, plan.pieces),
            middle = pieces_at(ws + 2 * plan.rows, b.tokens, b.inter, plan.pieces);
-    if (g.gate_rows) dg.hi = g.gate_rows;
-    if (g.up_rows) du.hi = g.up_rows;
-    if (g.middle) middle.hi = g.middle;
+    const bool scaled = kScaled<T> && (g.dx.p || g.gate || g.up || g.down);
+    const auto hand_out = [&](Pieces& rows, void* to) {
+        if (to) (scaled ? rows.plain : rows.hi) = to;
+    };
+    hand_out(dg, g.gate_rows);
+    hand_out(du, g.up_rows);
+    hand_out(middle, g.middle);
+    f32x4* const bounds = scaled ? reinterpret_cast<f32x4*>(ws + 3 * plan.rows + plan.partial) : nullptr;
+    float* const unscale = scaled ? reinterpret_cast<float*>(bounds + kBoundGroups) : nullptr;
+    if constexpr (kScaled<T>)
+        if (scaled) {
+            const BoundArgs a{g.dy.p, b.down.p, g.dy.apart(), b.down.ld, b.tokens, b.hidden, b.inter, b.activation, g.pre, bounds};
+            hipLaunchKernelGGL(bounds_kernel, dim3(kBoundGroups), dim3(64 * kBoundWaves), 0, stream, a);
+            QSRT_HIP_TRY(hipGetLastError());
+        }
     {
         Product& p = args.product[0];
         p.a[0] = g.dy.p;
@@ -912,7 +1051,7 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
         p.k = b.hidden;
         p.sums = 1;
         float* pre = const_cast<float*>(g.pre);
-        p.finish = {nullptr, b.inter, b.activation, pre, pre + b.tokens * b.inter, middle, dg, du};
+        p.finish = {nullptr, b.inter, b.activation, pre, pre + b.tokens * b.inter, middle, dg, du, bounds, unscale};
         if (int rc = run<T, kRows, kCols, kSlopes>(args, plan.middle, stream)) return rc;
     }
     if (g.dx.p) {
@@ -925,10 +1064,11 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
         p.n = b.hidden;
         p.k = b.inter;
         p.finish = {const_cast<void*>(g.dx.p), g.dx.apart()};
+        p.finish.unscale = unscale;
         if (int rc = run<T, kRows, kCols, kStore>(args, plan.x, stream)) return rc;
     }
     TileArgs<kProducts> three = {};
-    const auto add = [&](const Pieces& rows, const Matrix& other, void* out, bool rows_first) {
+    const auto add = [&](const Pieces& rows, const Matrix& other, void* out, bool rows_first, float* sums_by) {
         if (!out) return;
         Product& p = three.product[three.products++];
         p = {};
@@ -944,10 +1084,11 @@ int backward(const Block& b, const Gradients& g, char* ws, const Backward& plan,
         }
         p.k = b.tokens;
         p.finish = {out, p.n};
+        p.finish.unscale = sums_by;
     };
-    add(dg, b.x, g.gate, true);
-    add(du, b.x, g.up, true);
-    add(middle, g.dy, g.down, false);
+    add(dg, b.x, g.gate, true, unscale);
+    add(du, b.x, g.up, true, unscale);
+    add(middle, g.dy, g.down, false, scaled ? unscale + 1 : nullptr);
     return three.products ? run<T, kCols, kCols, kStore>(three, plan.weights, stream) : kOk;
 }
 

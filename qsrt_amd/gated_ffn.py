@@ -120,8 +120,9 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
 
     ``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]``, all bf16 or all f16, hidden and inter
     multiples of 8.  ``activation``: ``"swiglu"`` (``silu(g) u``) or ``"situ"``.  Sums are FP32; the rows between the two
-    products are held in ``x``'s type (f16 ends at 65504), of 64 rows or less as two values each.  Differentiable in all four, once;
-    the backward pass keeps the rows before the activation in FP32 (``8 T inter`` bytes).  ``out``: where the result goes, of a
+    products are held in ``x``'s type (f16: infinite over 65504, off by up to 2^-25 each under 2^-14), of 64 rows or less as two
+    values each.  Differentiable in all four, once; the backward pass keeps the rows before the activation in FP32 (``8 T inter``
+    bytes) and scales f16 rows between its products by powers of two, so that small gradients keep their bits.  ``out``: where the result goes, of a
     call without gradients."""
 
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
@@ -141,7 +142,7 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
 class GatedFFNGradients:
     """``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]`` (None where not asked for), and the rows
     ``gate_rows`` (dG), ``up_rows`` (dU) and ``middle`` (M), ``[T, inter]``:  ``gate = gate_rows^T x``, ``up = up_rows^T x``,
-    ``down = dy^T middle``."""
+    ``down = dy^T middle``, but for the rows' rounding to ``x``'s type (f16: 2^-25 each under 2^-14)."""
 
     x: torch.Tensor | None
     gate: torch.Tensor | None
