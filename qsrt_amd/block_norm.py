@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import _native
-from .packed_linear import TYPES, refuse_second_derivatives
+from .packed_linear import TYPES, refuse_second_derivatives, refuse_tangents
 
 MAX_CHANNELS = 1 << 14
 MAX_ROWS = 1 << 22
@@ -106,6 +106,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dsum, dn):
         refuse_second_derivatives()
+        refuse_tangents(dsum, dn)
         residual, y, weight, post, gate, stats = ctx.saved_tensors
         t, hidden = residual.shape
         if dsum is None and dn is None:
@@ -130,6 +131,7 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def _run(residual, y, weight, post, gate, scale, eps, dtype, with_sum):
+    refuse_tangents(residual, y, weight, post, gate)
     kind = _checked(residual, y, weight, post, gate, dtype, eps)
     leaves = [v for v in (residual, y, weight, post, gate) if v is not None]
     if torch.is_grad_enabled() and any(v.requires_grad for v in leaves):
@@ -146,15 +148,15 @@ def residual_norm(residual: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
 
     ``y [T, hidden]``, a block's result, and ``n``, the next block's input, are bf16 or f16; ``residual`` and ``h`` float32 or
     of that type.  ``weight`` and ``post_weight [hidden]`` and ``gate`` (``[hidden]``, or ``[T, 1]``: each row its own) are all
-    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors, once.
-    Squares are summed in FP32: a row's rms may be up to 1e17 and, with an eps of 0, down to 1e-18."""
+    float32 or all of ``y``'s type.  ``n`` comes from ``h`` before it is rounded.  Differentiable in all five tensors, once and
+    backward.  Squares are summed in FP32: a row's rms may be up to 1e17 and, with an eps of 0, down to 1e-18."""
 
     return _run(residual, y, weight, post_weight, gate, float(scale), float(eps), y.dtype, True)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, dtype: torch.dtype | None = None) -> torch.Tensor:
     """``weight * x / rms(x)``, what stands before the first block.  ``x [T, hidden]`` bf16, f16, or float32 with the result's
-    ``dtype`` (bf16 or f16) named.  Differentiable in both, once."""
+    ``dtype`` (bf16 or f16) named.  Differentiable in both, once and backward."""
 
     return _run(x, None, weight, None, None, 1.0, float(eps), x.dtype if dtype is None else dtype, False)[1]
 

@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .packed_linear import TYPES, checked_out, checked_rows, refuse_second_derivatives
+from .packed_linear import TYPES, checked_out, checked_rows, refuse_second_derivatives, refuse_tangents
 
 ACTIVATIONS = {"swiglu": 0, "situ": 1}
 MAX_CHANNELS = 1 << 17
@@ -30,6 +30,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _checked(x, gate, up, down, activation):
+    refuse_tangents(x, gate, up, down)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
     shape, dtype, device = gate.shape, gate.dtype, gate.device
@@ -102,6 +103,7 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         refuse_second_derivatives()
+        refuse_tangents(dy)
         x, gate, up, down, pre = ctx.saved_tensors
         grads = [_like(t, needed) for t, needed in zip((x, gate, up, down), ctx.needs_input_grad)]
         if x.shape[0]:
@@ -121,7 +123,7 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
     ``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]``, all bf16 or all f16, hidden and inter
     multiples of 8.  ``activation``: ``"swiglu"`` (``silu(g) u``) or ``"situ"``.  Sums are FP32; the rows between the two
     products are held in ``x``'s type (f16: infinite over 65504, off by up to 2^-25 each under 2^-14), of 64 rows or less as two
-    values each.  Differentiable in all four, once; the backward pass keeps the rows before the activation in FP32 (``8 T inter``
+    values each.  Differentiable in all four, once and backward; the backward pass keeps the rows before the activation in FP32 (``8 T inter``
     bytes) and scales f16 rows between its products by powers of two, so that small gradients keep their bits.  ``out``: where the result goes, of a
     call without gradients."""
 
@@ -159,6 +161,7 @@ def gated_ffn_gradients(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, u
     """Gradients of ``sum(dy * gated_ffn(x, gate, up, down))`` without the graph: of ``x`` where ``inputs``, of the weights
     where ``weights``, and always the rows that a weight's gradient is the product of.  ``dy [T, hidden]`` in ``x``'s type."""
 
+    refuse_tangents(dy)
     x, gate, up, down = _checked(x, gate, up, down, activation)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("dy must have x's shape and type")

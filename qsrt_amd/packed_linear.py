@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .decode import _check_lut
@@ -41,9 +42,21 @@ def _records(record_bits, lead: tuple, rate_axis: str, k: int, n: int, words: in
     return tables, rates
 
 
+def refuse_tangents(*tensors) -> None:
+    """For calls without forward-mode derivatives: a tensor with a tangent does not require a gradient, and the tangent would be
+    dropped."""
+
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no tensor has one: 0.1 us, where asking each takes 0.6
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("there are no forward-mode derivatives here: an argument has a tangent")
+
+
 def refuse_gradients(*tensors) -> None:
     """Packed products have no backward pass: better no result than one that a gradient silently stops at."""
 
+    refuse_tangents(*tensors)
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError("packed products have no backward pass: call them under torch.no_grad() or detach their inputs")
