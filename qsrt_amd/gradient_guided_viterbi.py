@@ -116,6 +116,7 @@ class LowRankViterbiGradientGuidance:
         return float(self.strength) * float(torch.sum((left.T @ delta) * right))
 
 
+@torch.no_grad()
 def expert_guidance(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *,
                     anchor_id: str, objective_id: str, strength: float = 1.0,
                     activation: str = "situ") -> dict[str, LowRankViterbiGradientGuidance]:
