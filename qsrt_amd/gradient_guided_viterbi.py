@@ -116,6 +116,17 @@ class LowRankViterbiGradientGuidance:
         return float(self.strength) * float(torch.sum((left.T @ delta) * right))
 
 
+def _raised(dy: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor | float]:
+    """``dy`` times a power of two, and that: in f16 what brings its largest value to 2^-4 .. 2^-3, but not less than 1.  Rows that
+    are linear in it then have all their bits down to 2^-10 of that value, and 2^18 of room above it."""
+
+    if dy.dtype != torch.float16 or dy.numel() == 0:
+        return dy, 1.0
+    exponent = torch.frexp(dy.abs().amax().float()).exponent
+    by = (((-3 - exponent).clamp(0, 24) + 127) << 23).view(torch.float32)
+    return (dy.float() * by).to(dy.dtype), by
+
+
 @torch.no_grad()
 def expert_guidance(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *,
                     anchor_id: str, objective_id: str, strength: float = 1.0,
@@ -127,12 +138,14 @@ def expert_guidance(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, up: t
 
     _check_strength(strength)
     _check_identities(anchor_id, objective_id)
-    g = gated_ffn_gradients(x, dy, gate, up, down, activation=activation, inputs=False, weights=False)
+    raised, by = _raised(dy)
+    g = gated_ffn_gradients(x, raised, gate, up, down, activation=activation, inputs=False, weights=False)
 
     def low_rank(left, right, anchor):
-        return LowRankViterbiGradientGuidance(left.T.float(), right.float(), anchor.T.float(), anchor_id, objective_id, strength)
+        return LowRankViterbiGradientGuidance(left.T.float(), right, anchor.T.float(), anchor_id, objective_id, strength)
 
-    return {"w1": low_rank(x, g.gate_rows, gate), "w3": low_rank(x, g.up_rows, up), "w2": low_rank(g.middle, dy, down)}
+    return {"w1": low_rank(x, g.gate_rows.float() / by, gate), "w3": low_rank(x, g.up_rows.float() / by, up),
+            "w2": low_rank(g.middle, dy.float(), down)}
 
 
 def shift_elementwise_target(target: torch.Tensor, gradient: torch.Tensor, *, strength: float,

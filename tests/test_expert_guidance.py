@@ -51,3 +51,36 @@ def test_no_graph_is_kept(dtype, stand_in):
         out = torch.zeros(16, shape[1])
         out.copy_(g.rows(slice(0, 16), device="cpu", dtype=torch.float32))
         out.numpy()
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6, 2.0**-24])
+def test_small_f16_gradients_keep_their_bits(size, stand_in):
+    """dG and dU are f16, off by 2^-11 of themselves or 2^-25, half the type's last step.  dy's largest value is brought to 2^-4 or
+    more for them: 2^-25 there is 2^-21 of it here."""
+
+    x, dy, gate, up, down = draw(torch.float16, size)
+    guidance = call(x, dy, gate, up, down)
+    X, Y, G, U, D = (t.double() for t in (x, dy, gate, up, down))
+    g, u = X @ G.T, X @ U.T
+    s = torch.sigmoid(g)
+    most = float(Y.abs().max())
+    for name, by in (("w1", u * s * (1 + g * (1 - s))), ("w3", g * s)):
+        rows = (Y @ D) * by
+        off = (guidance[name].right.double() - rows).abs()
+        assert bool((off <= 2.0**-11 * rows.abs() + 2.0**-21 * most).all()), name
+    assert torch.equal(guidance["w2"].right, dy.float())
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_gradients_that_are_not_finite_are_found(value, stand_in):
+    x, dy, gate, up, down = draw(torch.float16)
+    dy[3, 5] = value
+    for g, shape in zip(call(x, dy, gate, up, down).values(), ((64, 40), (64, 40), (40, 64))):
+        with pytest.raises(ValueError, match="finite"):
+            g.validate(shape)
+
+
+def test_a_gradient_of_zeros(stand_in):
+    x, dy, gate, up, down = draw(torch.float16, 0.0)
+    for name, g in call(x, dy, gate, up, down).items():
+        assert bool((g.left @ g.right == 0).all())

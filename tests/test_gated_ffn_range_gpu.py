@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from qsrt_amd.gated_ffn import gated_ffn, gated_ffn_gradients
+from qsrt_amd.gradient_guided_viterbi import expert_guidance
 from test_gated_ffn_gpu import V, check, draw, slopes
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +177,26 @@ def test_views_and_a_lone_row(t):
         assert torch.equal(a, b)
     one = gated_ffn_gradients(x[:1], dy[:1].as_strided((1, 264), (3, 1)), gate, up, down)
     check(vars(one), want(x[:1], gate, up, down, dy[:1], "swiglu"), ["x", "gate", "up", "down"])
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6])
+@pytest.mark.parametrize("t", [5, 100])
+def test_guidance_of_small_gradients(t, size):
+    """The factors dG and dU: FP32 sums of ``hidden`` products, times a slope, rounded to f16 once, or off by 2^-25 of dy's largest
+    over 2^-4."""
+
+    x, gate, up, down, dy = draw(t, t, 264, 136, F16)
+    dy = (dy.float() * size).half()
+    guidance = expert_guidance(x, dy, gate, up, down, anchor_id="a", objective_id="o", activation="swiglu")
+    X, G, U, D, Y = (v.double() for v in (x, gate, up, down, dy))
+    g, u = X @ G.T, X @ U.T
+    _, by_g, by_u = slopes(g, u, "swiglu")
+    dg, du = (265 * V * (X.abs() @ w.abs().T) for w in (G, U))
+    slope_g, slope_u = 1.1 * u.abs() * dg + 1.1 * du + 32 * V * 1.1 * u.abs(), 1.1 * (dg + du) + 32 * V * 1.1 * g.abs()
+    rows, rows_off = Y @ D, 265 * V * (Y.abs() @ D.abs())
+    for name, by, slope in (("w1", by_g, slope_g), ("w3", by_u, slope_u)):
+        value = rows * by
+        off = rows_off * by.abs() + (rows.abs() + rows_off) * slope + 4 * V * value.abs()
+        bound = off + 2.0**-11 * (value.abs() + off) + 2.0**-21 * float(Y.abs().max())
+        assert float(((guidance[name].right.double() - value).abs() / bound).max()) <= 1, name
+        assert torch.equal(guidance[name].left, x.T.float())
