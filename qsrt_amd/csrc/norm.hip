@@ -401,7 +401,7 @@ extern "C" int qsrt_residual_norm(const void* residual, int64_t residual_ld, int
     constexpr const char* kCall = "qsrt_residual_norm";
     NormArgs a = {};
     a.residual = residual, a.residual_ld = residual_ld, a.residual_f32 = residual_f32 != 0;
-    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
+    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden < 0 || hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
     a.weight = weight, a.post = post, a.gate = gate, a.gate_kind = gate_kind, a.params_f32 = params_f32 != 0;
     a.scale = scale, a.eps = eps, a.sum = sum, a.sum_ld = sum_ld, a.normed = normed, a.normed_ld = normed_ld, a.stats = stats;
     if (int rc = check_norm(kCall, a, dtype)) return rc;
@@ -447,7 +447,7 @@ extern "C" int qsrt_residual_norm_backward(const void* dsum, int64_t dsum_ld, co
     constexpr const char* kCall = "qsrt_residual_norm_backward";
     NormArgs a = {};
     a.residual = residual, a.residual_ld = residual_ld, a.residual_f32 = residual_f32 != 0;
-    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
+    a.y = y, a.y_ld = y_ld, a.rows = rows, a.hidden = hidden < 0 || hidden > kMaxHidden ? -1 : static_cast<int>(hidden);
     a.weight = weight, a.post = post, a.gate = gate, a.gate_kind = gate_kind, a.params_f32 = params_f32 != 0;
     a.scale = scale, a.stats = const_cast<float*>(stats);
     a.dsum = dsum, a.dsum_ld = dsum_ld, a.dn = dn, a.dn_ld = dn_ld;
