@@ -292,14 +292,18 @@ __device__ __forceinline__ void count(const F& f) {
 
 // 16 bytes a lane from a buffer straight to LDS: lane l's go to `lds` + 16 l.  Written in assembly because the compiler,
 // which cannot see that a stage is written while another is read, waits for all of them before any read from LDS.  Nothing
-// comes back in registers; `wait_and_meet` is the wait.
+// comes back in registers; `wait_and_meet` is the wait.  m0, the LDS address, is named as written: the compiler remarks that it
+// never allocates it, but it does merge its own writes of it.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int kAt>
 __device__ __forceinline__ void to_lds(u32x4 from, uint32_t offset, uint32_t lds) {
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(lds),
                  "n"(kAt)
-                 : "memory", "scc");
+                 : "memory", "scc", "m0");
 }
+#pragma clang diagnostic pop
 
 // All but the wave's last `kLeft` loads have landed, its reads from LDS are done, and so are the other waves'.
 template <int kLeft>
