@@ -163,8 +163,8 @@ def gated_ffn_gradients(x: torch.Tensor, dy: torch.Tensor, gate: torch.Tensor, u
 
     refuse_tangents(dy)
     x, gate, up, down = _checked(x, gate, up, down, activation)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError("dy must have x's shape and type")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("dy must have x's shape and type, on its device")
     dy = checked_rows(dy, x.shape[1], x.device)
     t, inter = x.shape[0], gate.shape[0]
     grads = [_like(x, inputs), *(_like(w, weights) for w in (gate, up, down))]
