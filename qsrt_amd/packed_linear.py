@@ -153,11 +153,18 @@ def checked_rows(x: torch.Tensor, cols: int, device) -> torch.Tensor:
 
 
 def checked_out(out: torch.Tensor | None, x: torch.Tensor, cols: int) -> torch.Tensor:
+    """``out``, or a new tensor.  A kernel writes it behind autograd's back: one that is part of a graph is refused, and a graph
+    that has kept its values is told that they change, as it would be of torch's own calls."""
+
     if out is None:
         return torch.empty((x.shape[0], cols), dtype=x.dtype, device=x.device)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out requires a gradient, and the call has no backward pass: detach it, or call under torch.no_grad()")
+    refuse_tangents(out)
     if (out.shape != (x.shape[0], cols) or out.dtype != x.dtype or out.device != x.device or out.stride(1) != 1
             or out.data_ptr() % 8 or ((out.stride(0) % 4 or out.stride(0) < cols) and out.shape[0] > 1)):
         raise ValueError("out must be a row-major [rows, N] tensor of x's type, its rows 8-byte aligned")
+    torch.autograd.graph.increment_version(out)
     return out
 
 
