@@ -122,8 +122,8 @@ def _raised(dy: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor | float]:
 
     if dy.dtype != torch.float16 or dy.numel() == 0:
         return dy, 1.0
-    exponent = torch.frexp(dy.abs().amax().float()).exponent
-    by = (((-3 - exponent).clamp(0, 24) + 127) << 23).view(torch.float32)
+    largest = torch.linalg.vector_norm(dy, math.inf, dtype=torch.float32)
+    by = ((124 - torch.frexp(largest).exponent).clamp(127, 151) << 23).view(torch.float32)  # its bits
     return (dy.float() * by).to(dy.dtype), by
 
 
