@@ -10,20 +10,11 @@ import math
 import torch
 
 from . import _native
-from .packed_linear import TYPES, refuse_second_derivatives, refuse_tangents
+from .packed_linear import TYPES, aligned_rows, refuse_second_derivatives, refuse_tangents
 
 MAX_CHANNELS = 1 << 14
 MAX_ROWS = 1 << 22
 _NONE, _CHANNEL, _ROW = range(3)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with 16-byte aligned rows (copied where they are not)."""
-
-    apart, step = t.stride()
-    if step != 1 or t.data_ptr() % 16 or ((apart % 8 or apart < t.shape[1]) and t.shape[0] > 1):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
 
 
 def _vector(v: torch.Tensor | None) -> torch.Tensor | None:
@@ -94,7 +85,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, y, weight, post, gate, kind, scale, eps, dtype, with_sum):
         ctx.set_materialize_grads(False)
-        residual, y, weight = _rows(residual), None if y is None else _rows(y), _vector(weight)
+        residual, y, weight = aligned_rows(residual), None if y is None else aligned_rows(y), _vector(weight)
         post, gate = _vector(post), _vector(gate)
         total = _like(residual) if with_sum else None
         stats = torch.empty((2, residual.shape[0]), dtype=torch.float32, device=residual.device)
@@ -114,7 +105,7 @@ class _ResidualNorm(torch.autograd.Function):
         grads = [_like(v) if needed else None for v, needed in zip((residual, y, weight, post, gate), ctx.needs_input_grad)]
         if t == 0:
             return *(None if g is None else g.zero_() for g in grads), *(None,) * 5
-        dsum, dn = (None if d is None else _rows(d) for d in (dsum, dn))
+        dsum, dn = (None if d is None else aligned_rows(d) for d in (dsum, dn))
         lib = _native.lib()
         with _native.current(residual.device):
             ws = torch.empty(lib.qsrt_residual_norm_backward_workspace_bytes(t, hidden), dtype=torch.uint8,
@@ -136,7 +127,7 @@ def _run(residual, y, weight, post, gate, scale, eps, dtype, with_sum):
     leaves = [v for v in (residual, y, weight, post, gate) if v is not None]
     if torch.is_grad_enabled() and any(v.requires_grad for v in leaves):
         return _ResidualNorm.apply(residual, y, weight, post, gate, kind, scale, eps, dtype, with_sum)
-    residual, y = _rows(residual), None if y is None else _rows(y)
+    residual, y = aligned_rows(residual), None if y is None else aligned_rows(y)
     total = _like(residual) if with_sum else None
     return total, _forward(residual, y, _vector(weight), _vector(post), _vector(gate), kind, scale, eps, dtype, total, None)
 

@@ -14,19 +14,10 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .packed_linear import TYPES, checked_out, checked_rows, refuse_second_derivatives, refuse_tangents
+from .packed_linear import TYPES, aligned_rows, checked_out, checked_rows, refuse_second_derivatives, refuse_tangents
 
 ACTIVATIONS = {"swiglu": 0, "situ": 1}
 MAX_CHANNELS = 1 << 17
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with 16-byte aligned rows (copied where they are not)."""
-
-    apart, step = t.stride()
-    if step != 1 or t.data_ptr() % 16 or apart % 8 or apart < t.shape[1]:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
 
 
 def _checked(x, gate, up, down, activation):
@@ -45,7 +36,7 @@ def _checked(x, gate, up, down, activation):
         raise ValueError(f"hidden and inter must be multiples of 8 up to {MAX_CHANNELS}")
     if x.dtype != dtype or x.device != device:
         raise ValueError("x must be of the weights' type and on their device")
-    x, gate, up, down = checked_rows(x, hidden, device), _rows(gate), _rows(up), _rows(down)
+    x, gate, up, down = checked_rows(x, hidden, device), *(aligned_rows(w) for w in (gate, up, down))
     if gate.stride(0) != up.stride(0):  # one leading dimension serves both
         gate, up = gate.contiguous(), up.contiguous()
     return x, gate, up, down
@@ -123,9 +114,9 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
     ``x [T, hidden]``, ``gate``, ``up [inter, hidden]``, ``down [hidden, inter]``, all bf16 or all f16, hidden and inter
     multiples of 8.  ``activation``: ``"swiglu"`` (``silu(g) u``) or ``"situ"``.  Sums are FP32; the rows between the two
     products are held in ``x``'s type (f16: infinite over 65504, off by up to 2^-25 each under 2^-14), of 64 rows or less as two
-    values each.  Differentiable in all four, once and backward; the backward pass keeps the rows before the activation in FP32 (``8 T inter``
-    bytes) and scales f16 rows between its products by powers of two, so that small gradients keep their bits.  ``out``: where the result goes, of a
-    call without gradients."""
+    values each.  Differentiable in all four, once and backward; the backward pass keeps the rows before the activation in FP32
+    (``8 T inter`` bytes) and scales f16 rows between its products by powers of two, so that small gradients keep their bits.
+    ``out``: where the result goes, of a call without gradients."""
 
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
         if out is not None:

@@ -137,6 +137,16 @@ class LabelTables:
         self.ref = ctypes.addressof(self.array)
 
 
+def aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [rows, cols]`` with whole rows at multiples of 16 bytes (copied where they are not)."""
+
+    apart, step = t.stride()
+    # (a lone row's stride says nothing: a view keeps whatever its base had)
+    if step != 1 or t.data_ptr() % 16 or ((apart % 8 or apart < t.shape[1]) and t.shape[0] > 1):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def checked_rows(x: torch.Tensor, cols: int, device) -> torch.Tensor:
     """``x`` as rows the kernels read: ``[rows, cols]``, rows 16-byte aligned (copied where they are not)."""
 
@@ -146,10 +156,7 @@ def checked_rows(x: torch.Tensor, cols: int, device) -> torch.Tensor:
         raise ValueError("x must be bfloat16 or float16")
     if x.device != device:
         raise ValueError("x must be on the payload's device")
-    # (a lone row's stride says nothing: a view keeps whatever its base had)
-    if x.stride(1) != 1 or x.data_ptr() % 16 or ((x.stride(0) % 8 or x.stride(0) < cols) and x.shape[0] > 1):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return aligned_rows(x)
 
 
 def checked_out(out: torch.Tensor | None, x: torch.Tensor, cols: int) -> torch.Tensor:
