@@ -200,3 +200,11 @@ def test_guidance_of_small_gradients(t, size):
         bound = off + 2.0**-11 * (value.abs() + off) + 2.0**-21 * float(Y.abs().max())
         assert float(((guidance[name].right.double() - value).abs() / bound).max()) <= 1, name
         assert torch.equal(guidance[name].left, x.T.float())
+
+
+@pytest.mark.parametrize("t", [12, 90])
+def test_large_gradients_are_not_scaled(t):
+    """The bound is over 2^15, the rows are not: they go as they are."""
+
+    x, gate, up, down, dy = spread(t, t, 264, 136, 128.0, 1.0)
+    check(vars(gated_ffn_gradients(x, dy, gate, up, down)), want(x, gate, up, down, dy, "swiglu"), ["x", "gate", "up", "down"])
