@@ -158,8 +158,8 @@ __device__ __forceinline__ void finish(const Finish& f, int64_t row, int64_t col
 // to the least f16 that has all its bits.  Values that are not finite do not count.
 //
 // The forward pass does without: its bound would need gate and up read once more.  `bounds_kernel` is bound by memory (dy, W2, G
-// and U of 4096 rows of 7168 x 2048, 154 MB, in 36 to 46 us); a call with gradients takes 1012 to 1025 us, not 980 to 992, of 500
-// rows of 5120 x 1536 155, not 150.
+// and U of 4096 rows of 7168 x 2048, 154 MB, in 33 to 37 us, 4.2 to 4.7 TB/s), of few rows by its loads' way (27 rows of 5120 x
+// 1536: 11).  4096 rows with gradients take 978 to 987 us, where they took 953 to 961 unscaled, 500 of 5120 x 1536 132 for 118.
 constexpr int kBoundGroups = 256, kBoundWaves = 16;
 struct BoundArgs {
     const void *dy, *down;
@@ -179,41 +179,64 @@ __device__ __forceinline__ f32x4 most_of(f32x4 v) {  // of the wave, in each lan
 
 __global__ __launch_bounds__(64 * kBoundWaves) void bounds_kernel(const BoundArgs p) {
     __shared__ f32x4 room[kBoundWaves];
+    typedef vec8<_Float16> f16x8;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t first = blockIdx.x * kBoundWaves + wave, waves = kBoundGroups * kBoundWaves;
+    const uint32_t first = blockIdx.x * kBoundWaves + wave, waves = kBoundGroups * kBoundWaves;
     f32x4 most = {};
     const auto see = [&](int i, float v) { most[i] = v <= FLT_MAX ? fmaxf(most[i], v) : most[i]; };
+    // Four loads a lane on their way at a time; those past an end repeat the last.
     for (int64_t row = first; row < p.tokens; row += waves) {
+        const _Float16* at = static_cast<const _Float16*>(p.dy) + row * p.dy_ld;
         float sum = 0.f;
-        for (int64_t c = 8 * lane; c < p.hidden; c += 512) {
-            const vec8<_Float16> v = *reinterpret_cast<const vec8<_Float16>*>(static_cast<const _Float16*>(p.dy) + row * p.dy_ld + c);
+        for (int64_t c = 8 * lane; c < p.hidden; c += 4 * 512) {
+            f16x8 v[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float f = static_cast<float>(v[i]);
-                sum += fabsf(f) <= FLT_MAX ? f * f : 0.f;
-            }
+            for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const f16x8*>(at + min(c + 512 * q, p.hidden - 8));
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float f = static_cast<float>(v[q][i]);
+                    sum += c + 512 * q < p.hidden && fabsf(f) <= FLT_MAX ? f * f : 0.f;
+                }
         }
 #pragma unroll
         for (int apart = 32; apart > 0; apart >>= 1) sum += __shfl_xor(sum, apart);
         see(0, sqrtf(sum * static_cast<float>(p.hidden)));
     }
-    for (int64_t row = first; row < p.hidden; row += waves)
-        for (int64_t c = 8 * lane; c < p.inter; c += 512) {
-            const vec8<_Float16> v = *reinterpret_cast<const vec8<_Float16>*>(static_cast<const _Float16*>(p.down) + row * p.down_ld + c);
+    const uint32_t thread = first * 64 + lane, threads = waves * 64;
+    const uint32_t across = static_cast<uint32_t>(p.inter / 8), chunks = static_cast<uint32_t>(p.hidden) * across;  // 2^31 at most
+    for (uint32_t n = thread; n < chunks; n += 4 * threads) {
+        f16x8 v[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) see(1, fabsf(static_cast<float>(v[i])));
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t k = min(n + q * threads, chunks - 1), row = k / across;
+            v[q] = *reinterpret_cast<const f16x8*>(static_cast<const _Float16*>(p.down) + row * p.down_ld + 8 * (k - row * across));
         }
-    const int64_t plane = p.tokens * p.inter;
-    for (int64_t at = (first * 64 + lane) * 4; at < plane; at += waves * 64 * 4) {
-        const f32x4 g = *reinterpret_cast<const f32x4*>(p.pre + at), u = *reinterpret_cast<const f32x4*>(p.pre + plane + at);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float m, by_g, by_u;
-            activate_with_slopes(g[i], u[i], p.activation, m, by_g, by_u);
-            see(2, fabsf(by_g));
-            see(2, fabsf(by_u));
-            see(3, fabsf(m));
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) see(1, fabsf(static_cast<float>(v[q][i])));
+    }
+    const int64_t plane = p.tokens * p.inter, step = static_cast<int64_t>(threads) * 4;
+    for (int64_t n = static_cast<int64_t>(thread) * 4; n < plane; n += 2 * step) {
+        f32x4 g[2], u[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int64_t at = min(n + q * step, plane - 4);
+            g[q] = *reinterpret_cast<const f32x4*>(p.pre + at);
+            u[q] = *reinterpret_cast<const f32x4*>(p.pre + plane + at);
         }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float m, by_g, by_u;
+                activate_with_slopes(g[q][i], u[q][i], p.activation, m, by_g, by_u);
+                see(2, fabsf(by_g));
+                see(2, fabsf(by_u));
+                see(3, fabsf(m));
+            }
     }
     most = most_of(most);
     if (lane == 0) room[wave] = most;
@@ -889,8 +912,9 @@ bool sizes_fit(int64_t tokens, int64_t hidden, int64_t inter) {
 
 // Up to 64 rows, where reading the weights bounds a product, rows between products go on in two pieces: the result is then
 // off by its own rounding alone (forward in f16 while M is over 2^-10 or so: under 2^-14 both pieces end at 2^-24, as the result
-// itself does).  In one, it is off by 1.4 times as much (two roundings of one size); in two, 64 rows of 7168 x
-// 2048 take 39.4 us, not 35.5, 32 of 5120 x 1536 31.1, not 28.9, and 500 rows 89 us, not 73.
+// itself does).  In one, it is off by 1.4 times as much (two roundings of one size); in two, 64 rows of 7168 x 2048 take 39.4
+// us, not 35.5, 32 of 5120 x 1536 31.1, not 28.9, and 500 rows 89 us, not 73; 4096 of 7168 x 2048 395, not 304, and with
+// gradients 1468, not 932.
 int pieces_of(int64_t tokens) { return tokens <= 64 ? 2 : 1; }
 
 // Up to 16 rows, one side of a matrix instruction, meet a kernel of their own.  Against tiles with parts, in us at 8, 12 and 16

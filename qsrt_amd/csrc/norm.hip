@@ -197,9 +197,10 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs p) {
     }
 }
 
-// The same walk; sums over rows stay in registers until the end.  8192 rows of 5120: 109 us, 4.6 TB/s.  Of rows that take two
-// steps neither the parameters nor the next row fit the 128 registers that 16 waves leave a thread: both are loaded where they
-// are used (2048 rows of 16384: 200 us, 2.0 TB/s).
+// The same walk; sums over rows stay in registers until the end.  8192 rows of 5120: 109 us, 4.6 TB/s; without y (a first norm)
+// 78, 3.2 TB/s.  Rows over 8192 channels take two steps, which do not fit the 128 registers that 16 waves leave a thread: the
+// parameters and the next row are loaded where they are used, and of the sums, yhat, hhat and d 248 bytes a thread are spilled to
+// scratch (328 with a residual in 32 bits).  2048 rows of 16384: 195 to 200 us, 2.0 TB/s; 270 in 32 bits, 2.2.
 template <typename T, int kSteps, bool kF32>
 __global__ __launch_bounds__(1024) void norm_gradients_kernel(const NormArgs p) {
     __shared__ float room[2][3][kMaxWaves];
